@@ -197,7 +197,7 @@ def prepare(case, seed):
     slots = np.concatenate([bt[b, p // block] * block + p % block for b, p in enumerate(pos)])
     cu = np.concatenate([[0], np.cumsum(ends)])
     return {"case": case, "new_k": qkv[:, 0], "new_v": qkv[:, 1], "k": k, "ks": ks, "v": v, "vs": vs, "bt": _dev(bt),
-            "slots": _dev(slots), "cu": _dev(cu), "total": int(cu[-1]), "longest": max(ends)}
+            "slots": _dev(slots), "cu": _dev(cu), "total": int(cu[-1])}
 
 
 # ---------------------------------------------------------------- the plain forms
@@ -280,7 +280,7 @@ def run(state):
         if c["kind"] == "attn":
             return f["decode"](state["q"], k, v, state["bt"], state["lens"], c["hq"], c["hkv"], D, k_block_scale=ks, v_block_scale=vs)
         f["store"](state["new_k"], state["new_v"], k, v, state["slots"], k_block_scale=ks, v_block_scale=vs)
-        return f["gather"](k, v, state["bt"], state["cu"], state["total"], state["longest"], k_block_scale=ks, v_block_scale=vs)
+        return f["gather"](k, v, state["bt"], state["cu"], state["total"], k_block_scale=ks, v_block_scale=vs)
     return {"kv": _plain_kv, "attn": _plain_attn, "linear": _plain_linear}[c["kind"]](state)
 
 
