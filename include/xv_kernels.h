@@ -144,6 +144,47 @@ int xv_gather_kv_fp8(const void* k_cache, const void* v_cache, int64_t cache_pag
                      void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream);
 
 /*
+ * KV store into a 4-bit cache (OCP MXFP4).  No counterpart in the reference,
+ * whose pool holds the model dtype (src/compute/kv_pool.py:49-51): an optional
+ * on-HBM format of 4.25 bits a value.  As xv_store_kvcache, with every run of 32
+ * values of a head row stored as 32 e2m1 codes and one e8m0 scale byte s; code
+ * c stands for c * 2^(s - 127).
+ *   s: the exponent of the run's largest magnitude (carried up where its
+ *   mantissa is 1.75 or more) minus 2, kept within -126 .. 125, plus 127; each
+ *   value x becomes the code nearest to x / 2^(s - 127), ties to even, past 6
+ *   to 6.  A run that holds an infinity or NaN is stored as s = 255 and zero
+ *   codes and stands for NaN.
+ * Codes: row of (page, t, h) at page*cache_page_stride + t*cache_tok_stride +
+ * h*cache_head_stride bytes, head_dim / 2 bytes, value 2i in the low half of
+ * byte i; scales likewise at the scale strides, head_dim / 32 bytes.  head_dim
+ * a multiple of 32; key and value rows as xv_store_kvcache; code rows 4-byte
+ * aligned.  Slots other than -1 are distinct.
+ */
+int xv_store_kvcache_fp4(const void* key, int64_t key_stride_tok, int64_t key_stride_head,
+                         const void* value, int64_t value_stride_tok, int64_t value_stride_head,
+                         void* k_cache, void* v_cache, int64_t cache_page_stride, int64_t cache_tok_stride,
+                         int64_t cache_head_stride, void* k_scale, void* v_scale, int64_t scale_page_stride,
+                         int64_t scale_tok_stride, int64_t scale_head_stride, int block_size,
+                         const int32_t* slot_mapping, int64_t num_tokens, int num_kv_heads, int head_dim,
+                         hipStream_t stream);
+
+/*
+ * Read back of a 4-bit cache: row r < total_tokens of k_out / v_out ([T, Hkv,
+ * head_dim] bf16 at out_stride_tok) is token r - cu_seqlens_k[b] of the sequence
+ * b with cu_seqlens_k[b] <= r < cu_seqlens_k[b + 1], through its block table:
+ * the varlen k/v that xv_prefill_attention reads.  Every code times its scale
+ * is an exact bf16.  Rows from cu_seqlens_k[batch] on, and tokens past the
+ * table's max_blocks_per_seq blocks, are left as they are.  Layouts as
+ * xv_store_kvcache_fp4; outputs 16-byte aligned, out_stride_tok a multiple of 8.
+ */
+int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
+                     int64_t cache_tok_stride, int64_t cache_head_stride, const void* k_scale, const void* v_scale,
+                     int64_t scale_page_stride, int64_t scale_tok_stride, int64_t scale_head_stride, int block_size,
+                     const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                     const int32_t* cu_seqlens_k, int batch, int64_t total_tokens, int num_kv_heads, int head_dim,
+                     void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream);
+
+/*
  * Shared-prefix (cascade) decode attention: xv_paged_decode_attention for a
  * batch whose rows may share their first tokens' cache blocks, as a radix
  * prefix cache maps them (the reference's prefix index,

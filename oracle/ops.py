@@ -199,3 +199,42 @@ def quantize_fp8(x, inv_scale: float) -> np.ndarray:
 def dequantize_fp8(codes, scale: float) -> np.ndarray:
     """float64 values the decode attends to: value(code) * scale."""
     return fp8_e4m3fn_values()[np.asarray(codes, np.uint8)].astype(np.float64) * float(scale)
+
+
+# ---------------------------------------------------------------- MXFP4 (this build's optional 4-bit formats)
+FP4_BLOCK = 32
+FP4_MAGNITUDES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def quantize_fp4(x) -> tuple[np.ndarray, np.ndarray]:
+    """MXFP4 of x [..., n] (n a multiple of 32): (codes [..., n / 2] uint8, value
+    2i in the low half of byte i; e8m0 scale bytes [..., n / 32]).  All in 64
+    bits: the block's exponent is that of its largest magnitude (one more where
+    its mantissa is at least 1.75) minus 2, within -126 .. 125; each value goes
+    to the nearest of the eight magnitudes, ties to the even code, 6 at most.
+    A block with an infinity or NaN: scale 255, codes 0."""
+    b = np.asarray(x, np.float64).reshape(*np.shape(x)[:-1], -1, FP4_BLOCK)
+    bad = ~np.isfinite(b).all(-1)
+    b = np.where(bad[..., None], 0.0, b)
+    top = np.abs(b).max(-1)
+    m, e = np.frexp(top)  # top = m * 2^e, m in [0.5, 1)
+    e = np.where(top > 0, e - 1 + (m >= 0.875) - 2, -126)
+    e = np.clip(e, -126, 125)
+    a = np.ldexp(np.abs(b), -e[..., None])
+    hi = np.clip(np.searchsorted(FP4_MAGNITUDES, a, side="left"), 0, 7)  # first magnitude >= a, 7 past the end
+    lo = np.clip(hi - 1, 0, 7)
+    d_lo, d_hi = a - FP4_MAGNITUDES[lo], FP4_MAGNITUDES[hi] - a
+    code = np.where(a >= 6.0, 7, np.where(d_lo < d_hi, lo, np.where(d_hi < d_lo, hi, np.where(lo % 2 == 0, lo, hi))))
+    code = (code | np.where(np.signbit(b), 8, 0)).astype(np.uint8)
+    code = code.reshape(*code.shape[:-2], -1)
+    return code[..., 0::2] | (code[..., 1::2] << 4), np.where(bad, 255, e + 127).astype(np.uint8)
+
+
+def dequantize_fp4(codes, scales) -> np.ndarray:
+    """float64 values of MXFP4 codes [..., n / 2] and scale bytes [..., n / 32] (scale 255: NaN)."""
+    c = np.asarray(codes, np.uint8)
+    c = np.stack((c & 15, c >> 4), axis=-1).reshape(*c.shape[:-1], -1)
+    v = np.where(c & 8, -1.0, 1.0) * FP4_MAGNITUDES[c & 7]
+    s = np.asarray(scales, np.uint8)
+    unit = np.where(s == 255, np.nan, np.ldexp(1.0, s.astype(np.int64) - 127))
+    return v * np.repeat(unit, FP4_BLOCK, axis=-1)

@@ -1,0 +1,119 @@
+"""4-bit (MXFP4) formats without a GPU: the oracle's quantiser against the
+definition by exhaustive search, and the refusals of the C ABI (fake pointers,
+never dereferenced) and of the Python entry points."""
+import numpy as np
+import pytest
+import torch
+
+import oracle.ops as O
+from fp4_cases import codes, scales
+
+INVALID = 1  # hipErrorInvalidValue
+A = 0x10000
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from xvllm import _C
+
+    if not _C.lib_path().exists():
+        pytest.fail("libxv_kernels.so is not built (run __graft_entry__.build())")
+    return _C.lib()
+
+
+def test_oracle_quantiser_is_nearest_and_even():
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((500, 32)) * np.exp2(rng.integers(-130, 127, (500, 1)).astype(np.float64))
+    x = torch.from_numpy(x).to(torch.bfloat16).double().numpy()
+    x = np.where(np.isfinite(x), x, 0.0)
+    x[0] = 0.0
+    x[1] = 2.0 ** np.arange(-20, 12)
+    x[2] = np.linspace(-6, 6, 32)
+    q, s = O.quantize_fp4(x)
+    v = O.dequantize_fp4(q, s)
+    assert s.min() >= 1 and s.max() <= 252
+    unit = np.exp2(s.astype(np.float64) - 127)[:, 0]
+    for i in range(x.shape[0]):
+        grid = np.concatenate([O.FP4_MAGNITUDES, -O.FP4_MAGNITUDES]) * unit[i]
+        best = np.abs(grid[None, :] - x[i][:, None]).min(1)
+        assert (np.abs(v[i] - x[i]) == best).all()
+        top = np.abs(x[i]).max()
+        if top > 0 and 1 < s[i, 0] < 252:
+            assert 3.5 <= top / unit[i] < 7  # 1.75 .. 3.5 times two: the codes reach their largest or the one below
+    # ties: to the even code
+    ties = np.zeros((1, 32))
+    ties[0, :8] = [6, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]
+    got = O.dequantize_fp4(*O.quantize_fp4(ties))[0, :8]
+    assert got.tolist() == [6, 0, 1, 1, 2, 2, 4, 4]
+
+
+def test_oracle_blocks_with_infinities_read_back_as_nan():
+    x = np.ones((2, 64))
+    x[0, 3], x[1, 40] = np.inf, np.nan
+    v = O.dequantize_fp4(*O.quantize_fp4(x))
+    assert np.isnan(v[0, :32]).all() and (v[0, 32:] == 1).all()
+    assert (v[1, :32] == 1).all() and np.isnan(v[1, 32:]).all()
+
+
+def _store(lib, **kw):
+    a = dict(k=A, kst=1024, ksh=128, v=A, vst=1024, vsh=128, kc=A, vc=A, ps=8192, ts=512, hs=64, ks=A, vs=A, sps=512,
+             sts=32, shs=4, BS=16, sl=A, n=4, H=8, D=128)
+    a.update(kw)
+    return lib.xv_store_kvcache_fp4(*a.values(), None)
+
+
+def test_store_rejects_bad_arguments(lib):
+    for kw in (dict(k=A + 8), dict(v=A + 2), dict(kst=1020), dict(vsh=132), dict(kc=A + 2), dict(kc=None), dict(ks=None),
+               dict(ts=510), dict(hs=66), dict(BS=0), dict(BS=-16), dict(D=100), dict(D=16), dict(D=0), dict(H=0),
+               dict(n=-1), dict(n=1 << 25)):
+        assert _store(lib, **kw) == INVALID, kw
+    assert _store(lib, n=0) == 0
+
+
+def _gather(lib, **kw):
+    a = dict(kc=A, vc=A, ps=8192, ts=512, hs=64, ks=A, vs=A, sps=512, sts=32, shs=4, BS=16, bt=A, bts=8, maxb=8, cu=A,
+             B=4, T=100, H=8, D=128, ko=A, vo=A, ost=1024)
+    a.update(kw)
+    return lib.xv_gather_kv_fp4(*a.values(), None)
+
+
+def test_gather_rejects_bad_arguments(lib):
+    for kw in (dict(kc=None), dict(vc=A + 1), dict(ts=510), dict(BS=0), dict(D=48), dict(H=0), dict(B=-1), dict(T=-1),
+               dict(T=1 << 31), dict(ko=A + 8), dict(ost=1020), dict(ost=512), dict(maxb=-1), dict(vs=None)):
+        assert _gather(lib, **kw) == INVALID, kw
+    assert _gather(lib, T=0) == 0 and _gather(lib, B=0) == 0
+
+
+def test_python_entry_points_refuse_cpu_tensors_and_wrong_types():
+    from xvllm.kv_ops import gather_kvcache, store_kvcache
+
+    q = codes(np.zeros((4, 16, 2, 64), np.uint8))
+    s = scales(np.zeros((4, 16, 2, 4), np.uint8))
+    bt, cu = torch.zeros(1, 4, dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32)
+    kv = torch.zeros(5, 2, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        store_kvcache(kv, kv, q, q, torch.arange(5, dtype=torch.int32), k_block_scale=s, v_block_scale=s)
+    with pytest.raises(RuntimeError, match="GPU"):
+        gather_kvcache(q, q, bt, cu, 5, k_block_scale=s, v_block_scale=s)
+
+
+def test_cache_checks():
+    from xvllm.kv_ops import fp4_pages
+
+    q = codes(np.zeros((4, 16, 2, 64), np.uint8))
+    s = scales(np.zeros((4, 16, 2, 4), np.uint8))
+    with pytest.raises(ValueError, match="needs k_block_scale"):
+        fp4_pages(q, q, None, None)
+    with pytest.raises(TypeError, match="scales"):
+        fp4_pages(q, q, s.view(torch.uint8), s)
+    with pytest.raises(TypeError, match="codes"):
+        fp4_pages(q, q.view(torch.uint8), s, s)
+    with pytest.raises(ValueError, match="layout"):
+        fp4_pages(q, q[:3], s, s)
+    with pytest.raises(ValueError, match="layout"):
+        fp4_pages(q, q.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(q.dtype), s, s)
+    for bad in (s[:, :, :, :3], s[:, :8]):
+        with pytest.raises(ValueError, match="D/32"):
+            fp4_pages(q, q, bad, bad)
+    with pytest.raises(RuntimeError, match="GPU"):
+        fp4_pages(q, q, s, s)
