@@ -185,6 +185,28 @@ int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_pag
                      void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream);
 
 /*
+ * xv_paged_decode_attention over a 4-bit (MXFP4) cache written by
+ * xv_store_kvcache_fp4.  No counterpart in the reference (its pool holds the
+ * model dtype).  K and V are the codes times their block scales, exactly;
+ * strides of the codes and of the scales in bytes as there, the codes' base and
+ * strides multiples of 16, the scales' of 4, head_dim 128.  A sequence is read
+ * up to max_blocks_per_seq * block_size tokens at most (256M at most).
+ * workspace: xv_paged_decode_fp4_workspace_size(...) bytes, 16-byte aligned, no
+ * initial contents; it grows neither with the table nor, past 256 sequences,
+ * with the batch, and never decreases with either.  Calls sharing one must be ordered on one stream.
+ */
+size_t xv_paged_decode_fp4_workspace_size(int batch, int num_q_heads, int num_kv_heads);
+int xv_paged_decode_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                  const void* k_cache, const void* v_cache,
+                                  int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                                  const void* k_scale, const void* v_scale, int64_t scale_page_stride,
+                                  int64_t scale_tok_stride, int64_t scale_head_stride,
+                                  const int32_t* block_tables, int64_t bt_stride, const int32_t* cache_seqlens,
+                                  void* out, int64_t out_stride_tok, void* workspace, size_t workspace_bytes,
+                                  int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                  int block_size, int max_blocks_per_seq, float scale, hipStream_t stream);
+
+/*
  * Shared-prefix (cascade) decode attention: xv_paged_decode_attention for a
  * batch whose rows may share their first tokens' cache blocks, as a radix
  * prefix cache maps them (the reference's prefix index,
@@ -511,6 +533,24 @@ int xv_dense_gemm(const void* x, int64_t x_stride, const void* w_packed, void* o
 int xv_stream_gemm_parts(int m, int n, int k, int mode);
 int xv_stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_stride, void* out, int64_t out_stride,
                    int64_t part_stride, int m, int n, int k, int mode, int parts, hipStream_t stream);
+
+/*
+ * Product with a 4-bit (OCP MXFP4) weight: out[m, n] = x[m, k] . W[n, k]^T, W[i][j] =
+ * code[i][j] * 2^(scale[i][j / 32] - 127) (scale 255: NaN), bf16 x, fp32
+ * accumulate, one rounding to bf16.  No counterpart in the reference, whose
+ * linears hold the model dtype (src/compute/layers/linear.py:141,306).
+ *   x         row i at i * x_stride (a multiple of 8, >= k), 16-byte aligned.
+ *   w         codes, row i at i * w_stride bytes (a multiple of 16, >= k / 2), two to
+ *             a byte, value 2j in the low half; 16-byte aligned.
+ *   w_scale   e8m0 bytes, row i at i * scale_stride (>= k / 32).
+ *   out       row i at i * out_stride, 2-byte aligned.
+ *   silu_mul  nonzero: W is the gate / up weight [2I, k] (n = 2I, gate rows first)
+ *             and out[m, I] = silu(g) * u of the two fp32 products.
+ * k a multiple of 32; any m >= 0 and n > 0.
+ */
+int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* w_scale,
+                  int64_t scale_stride, void* out, int64_t out_stride, int m, int n, int k, int silu_mul,
+                  hipStream_t stream);
 
 /*
  * Streaming copy of `bytes` (a multiple of 16; both pointers 16-byte aligned)

@@ -117,3 +117,39 @@ def test_cache_checks():
             fp4_pages(q, q, bad, bad)
     with pytest.raises(RuntimeError, match="GPU"):
         fp4_pages(q, q, s, s)
+
+
+def _decode(lib, **kw):
+    a = dict(q=A, qst=4096, qsh=128, kc=A, vc=A, ps=8192, ts=64, hs=1024, ks=A, vs=A, sps=512, sts=4, shs=64, bt=A, bts=256,
+             sl=A, out=A, ost=4096, ws=A, wsb=1 << 30, B=64, Hq=32, Hkv=8, D=128, BS=16, maxb=256, scale=0.088)
+    a.update(kw)
+    return lib.xv_paged_decode_attention_fp4(*a.values(), None)
+
+
+def test_decode_rejects_bad_arguments(lib):
+    for kw in (dict(D=64), dict(BS=24), dict(BS=0), dict(Hq=24), dict(Hq=128), dict(Hq=12), dict(Hq=0), dict(Hkv=0), dict(q=A + 8),
+               dict(kc=A + 8), dict(vc=A + 4), dict(qst=4100), dict(ts=72), dict(ts=48), dict(ts=0), dict(hs=1028), dict(ks=A + 2), dict(sts=6),
+               dict(sts=0), dict(shs=66), dict(out=A + 2), dict(ost=4097), dict(ws=None), dict(ws=A + 8), dict(wsb=1024),
+               dict(maxb=0), dict(maxb=1 << 25), dict(bts=255), dict(bts=1 << 24, maxb=256), dict(B=-1)):
+        assert _decode(lib, **kw) == INVALID, kw
+    assert _decode(lib, B=0) == 0
+
+
+def test_decode_workspace_never_shrinks(lib):
+    for hq, hkv in ((32, 8), (8, 8), (64, 8), (8, 1)):
+        sizes = [lib.xv_paged_decode_fp4_workspace_size(b, hq, hkv) for b in range(0, 600)]
+        assert sizes == sorted(sizes) and sizes[256] == sizes[-1]
+
+
+def _gemm(lib, **kw):
+    a = dict(x=A, xst=4096, w=A, wst=2048, s=A, sst=128, out=A, ost=1024, m=4, n=1024, k=4096, silu=0)
+    a.update(kw)
+    return lib.xv_mxfp4_gemm(*a.values(), None)
+
+
+def test_gemm_rejects_bad_arguments(lib):
+    for kw in (dict(x=None), dict(x=A + 8), dict(xst=4092), dict(xst=4088), dict(w=A + 8), dict(w=None), dict(wst=2040),
+               dict(wst=2032), dict(s=None), dict(sst=127), dict(out=None), dict(out=A + 1), dict(ost=1023), dict(m=-1),
+               dict(n=0), dict(k=0), dict(k=4080), dict(n=1023, silu=1), dict(m=1 << 21)):
+        assert _gemm(lib, **kw) == INVALID, kw
+    assert _gemm(lib, m=0) == 0

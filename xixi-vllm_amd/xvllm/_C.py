@@ -80,6 +80,13 @@ SIGNATURES: dict[str, tuple] = {
     "xv_gather_kv_fp4": (
         i32, [vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i32, vp, i64, i32, vp, i32, i64, i32, i32, vp, vp, i64, vp]
     ),
+    "xv_paged_decode_fp4_workspace_size": (sz, [i32, i32, i32]),
+    "xv_paged_decode_attention_fp4": (
+        i32,
+        [vp, i64, i64, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, vp, i64, vp, sz,
+         i32, i32, i32, i32, i32, i32, f32, vp],
+    ),
+    "xv_mxfp4_gemm": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp]),
     "xv_silu_and_mul": (i32, [vp, i64, vp, i64, i64, i32, vp]),
     "xv_dense_gemm": (i32, [vp, i64, vp, vp, i64, i64, i32, i32, i32, i32, i32, i32, i32, vp]),
     "xv_stream_gemm_parts": (i32, [i32, i32, i32, i32]),

@@ -15,8 +15,8 @@ import torch
 import torch.nn as nn
 
 from .. import _C
-from .._torch_glue import aligned16, ptr, require_bf16, require_cuda, stream_of
-from ..kv_ops import store_kvcache
+from .._torch_glue import aligned16, call, ptr, require_bf16, require_cuda, stream_of
+from ..kv_ops import FP4_PAGES, fp4_pages, store_kvcache
 
 
 @dataclass
@@ -118,6 +118,39 @@ def _q_view(q: torch.Tensor, num_heads: int, head_dim: int) -> tuple[torch.Tenso
     return q3, q3.stride(0), q3.stride(1)
 
 
+def _paged_decode_fp4(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, softmax_scale, out,
+                      k_block_scale, v_block_scale) -> torch.Tensor:
+    require_bf16(q)
+    codes, scales, (_, bs, heads, dim) = fp4_pages(k_cache, v_cache, k_block_scale, v_block_scale)
+    if k_cache.dim() != 4 or heads != hkv or dim != d:
+        raise ValueError(f"cache {tuple(k_cache.shape)} is not 4-bit pages [NB, BS, {hkv}, {d} / 2]")
+    q3, qs0, qs1 = _q_view(q, hq, d)
+    bsz = q3.shape[0]
+    if q3.shape[1:] != (hq, d) or block_tables.dim() != 2 or block_tables.shape[0] < bsz or cache_seqlens.numel() < bsz:
+        raise ValueError(f"q {tuple(q.shape)}, block_tables {tuple(block_tables.shape)}, cache_seqlens "
+                         f"{tuple(cache_seqlens.shape)}: not {hq} heads of {d} with a table row and a length each")
+    dev = k_cache.device
+    if q.device != dev or block_tables.device != dev or cache_seqlens.device != dev:
+        raise RuntimeError("q, the cache, block_tables and cache_seqlens must be on one device")
+    bt = block_tables.to(torch.int32)
+    if bt.stride(-1) != 1 or (bsz > 1 and bt.stride(0) < bt.shape[1]):
+        bt = bt.contiguous()
+    sl = cache_seqlens.to(torch.int32).contiguous()
+    if out is None:
+        out = torch.empty((bsz, hq * d), dtype=q.dtype, device=dev)
+    elif out.shape != (bsz, hq * d) or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
+        raise ValueError(f"out must be bf16 [{bsz}, {hq * d}] of unit last stride")
+    if bsz == 0:
+        return out
+    max_blocks = bt.shape[1]
+    # a workspace of the call's own, from the caching allocator: calls on several streams and captured graphs share none
+    ws = torch.empty(_C.lib().xv_paged_decode_fp4_workspace_size(bsz, hq, hkv), dtype=torch.uint8, device=dev)
+    scale = 1.0 / math.sqrt(d) if softmax_scale is None else softmax_scale
+    call("xv_paged_decode_attention_fp4", q3, ptr(q3), qs0, qs1, *codes, *scales, ptr(bt), max(bt.stride(0), max_blocks),
+         ptr(sl), ptr(out), out.stride(0), ptr(ws), ws.numel(), bsz, hq, hkv, d, bs, max_blocks, float(scale))
+    return out
+
+
 def paged_decode_attention(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -132,13 +165,22 @@ def paged_decode_attention(
     *,
     k_scale: float = 1.0,
     v_scale: float = 1.0,
+    k_block_scale: torch.Tensor | None = None,
+    v_block_scale: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Causal decode over the paged cache: q [B, Hq*D] (or [B, Hq, D]),
     k_cache/v_cache [NB, BS, Hkv, D], block_tables int32 [B, max_blocks],
     cache_seqlens int32 [B] (0 = padding row) -> [B, Hq*D].  An fp8 cache
     (torch.float8_e4m3fn, written by store_kvcache with the same scales)
-    attends to k_cache * k_scale and v_cache * v_scale."""
+    attends to k_cache * k_scale and v_cache * v_scale; a 4-bit cache
+    (torch.float4_e2m1fn_x2 [NB, BS, Hkv, D/2]) to its codes times the block
+    scales k_block_scale / v_block_scale [NB, BS, Hkv, D/32].  The 4-bit form
+    takes a workspace of its own per call; the others share one per device
+    (decode_workspace)."""
     require_cuda(q, k_cache, v_cache, block_tables, cache_seqlens)
+    if k_cache.dtype == FP4_PAGES:
+        return _paged_decode_fp4(q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim,
+                                 softmax_scale, out, k_block_scale, v_block_scale)
     fp8 = k_cache.dtype == torch.float8_e4m3fn
     require_bf16(q, *(() if fp8 else (k_cache, v_cache)))
     if fp8 and v_cache.dtype != torch.float8_e4m3fn:

@@ -351,3 +351,58 @@ def streamed_into_norm(x: torch.Tensor, w) -> PartialSums:
         return dense_gemm(x, w, GEMM_PARTS, col_tiles=1, waves=8, parts=p)
     p = in_place_parts(x.shape[0], w.shape[0], x.shape[1], GEMM_PARTS)
     return PartialSums(torch.ops.xv.stream_gemm(x, w, GEMM_PARTS, p))
+
+
+@torch.library.custom_op("xv::mxfp4_linear", mutates_args=())
+def _mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
+    """mxfp4_linear on x [M, K] with codes and scales as bytes."""
+    from .._torch_glue import aligned16, call, ptr
+
+    m, k = x.shape
+    n = w.shape[0]
+    if x.stride(1) != 1 or x.stride(0) % 8 or (m > 1 and x.stride(0) < k) or not aligned16(x):
+        x = x.clone(memory_format=torch.contiguous_format)
+    out = torch.empty((m, n // 2 if silu_mul else n), dtype=torch.bfloat16, device=x.device)
+    if out.numel():
+        call("xv_mxfp4_gemm", x, ptr(x), x.stride(0), ptr(w), w.stride(0), ptr(w_scale), w_scale.stride(0), ptr(out),
+             out.shape[1], m, n, k, int(silu_mul))
+    return out
+
+
+@_mxfp4_linear.register_fake
+def _mxfp4_linear_fake(x, w, w_scale, silu_mul):
+    return x.new_empty((x.shape[0], w.shape[0] // 2 if silu_mul else w.shape[0]))
+
+
+def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, silu_mul: bool = False) -> torch.Tensor:
+    """x [..., K] @ w^T with a 4-bit weight (OCP MXFP4, read in place): w
+    torch.float4_e2m1fn_x2 [N, K/2], two e2m1 codes a byte, the lower index in
+    the low half; w_scale torch.float8_e8m0fnu [N, K/32]; bf16 x and result,
+    fp32 sums, one rounding.  silu_mul: w is a gate/up weight [2I, K], gate rows
+    first, and the result is silu(x w_gate^T) * (x w_up^T), [..., I].
+
+    K is a multiple of 32, N any (even with silu_mul).  w's rows start 16-byte
+    aligned and have unit stride, as w_scale's have; x of any layout.  For
+    inference: it has no backward."""
+    from .._torch_glue import aligned16, require_bf16, require_cuda
+
+    require_cuda(x, w, w_scale)
+    require_bf16(x)
+    if w.dtype != torch.float4_e2m1fn_x2 or w_scale.dtype != torch.float8_e8m0fnu:
+        raise TypeError(f"mxfp4_linear takes float4_e2m1fn_x2 codes and float8_e8m0fnu scales, got {w.dtype} and "
+                        f"{w_scale.dtype}")
+    k = x.shape[-1]
+    if w.dim() != 2 or w_scale.dim() != 2 or k % 32 or k == 0 or w.shape[1] * 2 != k or w_scale.shape != (w.shape[0], k // 32):
+        raise ValueError(f"mxfp4_linear: x {tuple(x.shape)}, codes {tuple(w.shape)}, scales {tuple(w_scale.shape)} are not "
+                         "[..., K], [N, K/2] and [N, K/32], K a multiple of 32")
+    if silu_mul and w.shape[0] % 2:
+        raise ValueError(f"mxfp4_linear: a gate/up weight has an even number of rows, got {w.shape[0]}")
+    if x.device != w.device or x.device != w_scale.device:
+        raise RuntimeError("mxfp4_linear: x, w and w_scale must be on one device")
+    if (w.stride(1) != 1 or w_scale.stride(1) != 1 or w.stride(0) % 16 or w.stride(0) < k // 2 or w_scale.stride(0) < k // 32
+            or not aligned16(w)):
+        raise ValueError("mxfp4_linear reads w in place: rows of unit stride, whole and 16-byte aligned")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("mxfp4_linear has no backward: call it under torch.no_grad()")
+    y = torch.ops.xv.mxfp4_linear(x.reshape(-1, k), w.view(torch.uint8), w_scale.view(torch.uint8), silu_mul)
+    return y.view(*x.shape[:-1], y.shape[1])
