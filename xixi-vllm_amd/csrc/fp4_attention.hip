@@ -4,24 +4,24 @@
 // e2m1 codes (64 bytes a row of one kv head) and one e8m0 scale per 32 values
 // (4 bytes a row).
 //
-// Work split, as the bf16 kernel's: the (sequence, kv head, 64-token unit)
-// space is flattened in that order and cut into equal contiguous ranges, one
-// per resident single-wave workgroup; segments cut by a range boundary leave
-// partials (normalised bf16 rows and their log2-sum-exp) for a merge kernel.
-// A range holds at most two cut segments (its first and its last), so a wave has two
-// partial slots and the workspace does not grow with the table's width.
+// Work split: the (sequence, kv head, 64-token unit) space is flattened in
+// that order and cut into equal contiguous ranges, one per wave, eight waves a
+// CU; segments cut by a range boundary leave partials (normalised bf16 rows and
+// their log2-sum-exp) for a merge kernel.  A range holds at most two cut
+// segments (its first and its last), so a wave has two partial slots and the
+// workspace does not grow with the table's width.
 //
 // A unit is 64 tokens: per lane that is one full set of operands.
 //   K and V codes (4 KB each) and their scales (256 B each) go HBM -> LDS by
-//   LDS-DMA.
-//   S^T = K Q^T, v_mfma_f32_16x16x32_bf16, one product chain per 16-token row
-//   block p: lane (g, i) reads the 16 bytes of token 16p + i's values 32g ..
-//   32g + 31: exactly one scale block, so the conversion to bf16 (one
-//   instruction per pair) applies the scale and is exact.
+//   LDS-DMA, one unit ahead of the one in work.
+//   S^T = K Q^T on v_mfma_scale_f32_16x16x128_f8f6f4, one 16-token row block p
+//   per product: operand A is K as it is stored, lane (g, i) the 16 bytes of
+//   token 16p + i's values 32g .. 32g + 31 with that block's own scale byte.
+//   Operand B is q as the sum of two e4m3 terms (see split_q): no conversion of K.
 //   The scores land as acc[p][r] = head c % G, token 16p + 4g + r: the 16
 //   tokens of lane group g, which are the k indices that group supplies to
-//   O = P V.  V comes out of LDS by ds_read_b64_tr_b4, which gives a lane one
-//   column of 16 rows: lane (g, i), tile n holds column 16n + i of those 16
+//   O = P V (bf16).  V comes out of LDS by ds_read_b64_tr_b4, which gives a lane
+//   one column of 16 rows: lane (g, i), tile n holds column 16n + i of those 16
 //   tokens.  Its scale varies along the 16 rows and is folded into P, and P is
 //   one operand for the columns of one scale block only.  The G heads fill G
 //   of the 16 operand rows, so row rep * G + h takes head h scaled for block
@@ -38,19 +38,21 @@ constexpr int kD = 128;
 constexpr int kRow = kD / 2;      // bytes of a head row's codes
 constexpr int kUnit = 64;         // tokens of a unit
 constexpr int kMaxBatch = 256;    // sequences per launch (larger batches are launched in chunks)
-constexpr int kMaxWaves = 1024;   // workgroups of the main kernel at most
-constexpr int kWavesPerCu = 4;    // one wave per SIMD
-constexpr int kRing = 3;          // units in LDS per wave, kRing - 1 of them in flight
+constexpr int kWaves = 8;         // waves of a workgroup, one workgroup per CU
+constexpr int kMaxGroups = 256;   // workgroups at most
+constexpr int kMaxWaves = kWaves * kMaxGroups;
 constexpr int kUnitOps = 10;      // LDS-DMA instructions a unit: 4 + 4 of codes, 1 + 1 of scales
-// LDS of one unit: K codes, V codes, K scales, V scales, then the q rows of a segment that starts with it
-constexpr int kVOff = 4096, kKsOff = 8192, kVsOff = 8448, kQOff = 8704;
-template <int G> constexpr int kSlot = kQOff + (G <= 4 ? 1024 : G * 256);
-constexpr int kIdWindow = 32;     // units per half of the block-id table (4 ids each)
+// LDS of one unit: K codes, V codes, K scales, V scales
+constexpr int kVOff = 4096, kKsOff = 8192, kVsOff = 8448, kUnitLds = 8704;
+constexpr int kIdWindow = 16;     // units per half of the block-id table (4 ids each)
+// LDS of one wave: two units, the q rows of a segment, the block-id table
+template <int G> constexpr int kQBytes = G <= 4 ? 1024 : G * 256;
+template <int G> constexpr int kWaveLds = 2 * kUnitLds + kQBytes<G> + 2 * kIdWindow * 16;
 
 struct Fp4DecodeArgs {
   const bf16_t* q; int64_t q_st, q_sh;
-  const uint8_t* kc; const uint8_t* vc; int64_t ps, ts, hs;
-  const uint8_t* ks; const uint8_t* vs; int64_t sps, sts, shs;
+  const uint8_t* kc; const uint8_t* vc; uint32_t ps, ts, hs;
+  const uint8_t* ks; const uint8_t* vs; uint32_t sps, sts, shs;
   const int32_t* bt; int64_t bt_stride;
   const int32_t* seqlens;
   bf16_t* out; int64_t out_st;
@@ -60,9 +62,12 @@ struct Fp4DecodeArgs {
   int batch, hq, hkv, group;
   int nsub;         // 16-token pages per cache block
   int max_ctx;      // tokens the block table has room for
-  int nwaves;
-  float scale_log2;
+  float scale_log2; // not negative: q_sign carries the sign of the scale
+  float q_sign;
 };
+
+typedef int v8i_t __attribute__((ext_vector_type(8)));
+typedef const __attribute__((address_space(1))) void* global_cptr;
 
 XV_INLINE int lds_int(const int* p) {
   int v;
@@ -71,6 +76,14 @@ XV_INLINE int lds_int(const int* p) {
                        : "v"((uint32_t)reinterpret_cast<uintptr_t>(p))
                        : "memory");
   return __builtin_amdgcn_readfirstlane(v);
+}
+XV_INLINE u32x4_t lds_ids(const char* p) {
+  u32x4_t v;
+  __asm__ __volatile__("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)"
+                       : "=&v"(v)
+                       : "v"((uint32_t)reinterpret_cast<uintptr_t>(p))
+                       : "memory");
+  return v;
 }
 
 struct Fp4Cursor {
@@ -98,20 +111,21 @@ XV_INLINE void advance(Fp4Cursor& c, const int* pref, const int* sl, int hkv, in
   c.ctx = lds_int(sl + c.b);
 }
 
+// LDS offsets of a lane within a unit, and of its 16-byte piece within a page
+// of codes.  Piece j of a row sits in piece j ^ (row / 4) of the row's 64
+// bytes: the 16 rows of a K read (one piece) then cover all banks once.
 struct Fp4Lane {
-  int g;           // global byte offset of this lane's piece of a 16-token page of codes
-  uint32_t k;      // LDS offset of its K operand (row block 0)
-  uint32_t v[4];   // LDS offsets of its transposed V reads of tiles 2m (tile 2m + 1: 8 bytes on)
-  uint32_t ks, vs; // LDS offsets of its scales
+  uint32_t g;      // global byte offset of this lane's piece of a 16-token page
+  uint32_t k;      // K operand, row block 0 (block p: + 1024 p)
+  uint32_t v[4];   // transposed V reads of tiles 2m (tile 2m + 1: 8 bytes on)
+  uint32_t ks, vs; // scales
 };
 
-// The 16-byte piece of a row sits in piece ^ (row / 4) of the row's 64 bytes:
-// the 16 rows of a K read (one piece) then cover all banks once.
-XV_INLINE Fp4Lane lane_offsets(int64_t tok_stride, int lane) {
+XV_INLINE Fp4Lane lane_offsets(uint32_t tok_stride, int lane) {
   Fp4Lane o;
   const int i = lane & 15, g = lane >> 4;
   const int row = lane >> 2;
-  o.g = (int)(row * tok_stride) + (((lane & 3) ^ (row >> 2)) << 4);
+  o.g = row * tok_stride + (((lane & 3) ^ (row >> 2)) << 4);
   o.k = (uint32_t)(64 * i + ((g ^ (i >> 2)) << 4));
   // input lane L of group g addresses token 16 (L / 4) + 4g + L % 4: output nibble L
 #pragma unroll
@@ -123,47 +137,46 @@ XV_INLINE Fp4Lane lane_offsets(int64_t tok_stride, int lane) {
 }
 
 struct UnitRegs {
-  u32x4_t k[4];                                          // K codes of row blocks 0..3
-  uint32_t ks[4];                                        // the scale bytes of those tokens
-  uint32_t v[8][2];                                      // V codes of column tiles 0..7, 16 tokens each
-  u32x4_t vs[4];                                         // scale bytes of tokens 16p + 4g .. + 3
+  u32x4_t k[4];      // K codes of row blocks 0..3
+  uint32_t ks[4];    // the scale bytes of those tokens
+  uint32_t v[8][2];  // V codes of column tiles 0..7, 16 tokens each
+  u32x4_t vs[4];     // scale bytes of tokens 16p + 4g .. + 3
+  u32x4_t ids;       // block ids of a later unit
 };
 
-// A unit's operands out of its LDS image once at most VM vector-memory
-// operations are outstanding, in one asm block with one wait.
-template <int VM>
-XV_INLINE void read_unit(UnitRegs& u, const char* buf, const Fp4Lane& lo) {
+// A unit's operands out of its LDS image (its loads have arrived) in one asm block with one wait.
+XV_INLINE void read_unit(UnitRegs& u, const char* buf, const Fp4Lane& lo, const char* ids) {
   typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
   const uint32_t b = (uint32_t)reinterpret_cast<uintptr_t>(buf);
   u32x2_t v[8];
   __asm__ __volatile__(
-      "s_waitcnt vmcnt(%27)\n\t"
-      "ds_read_b128 %0, %20\n\t"
-      "ds_read_b128 %1, %20 offset:1024\n\t"
-      "ds_read_b128 %2, %20 offset:2048\n\t"
-      "ds_read_b128 %3, %20 offset:3072\n\t"
-      "ds_read_b32 %4, %25\n\t"
-      "ds_read_b32 %5, %25 offset:64\n\t"
-      "ds_read_b32 %6, %25 offset:128\n\t"
-      "ds_read_b32 %7, %25 offset:192\n\t"
-      "ds_read_b64_tr_b4 %8, %21\n\t"
-      "ds_read_b64_tr_b4 %9, %21 offset:8\n\t"
-      "ds_read_b64_tr_b4 %10, %22\n\t"
-      "ds_read_b64_tr_b4 %11, %22 offset:8\n\t"
-      "ds_read_b64_tr_b4 %12, %23\n\t"
-      "ds_read_b64_tr_b4 %13, %23 offset:8\n\t"
-      "ds_read_b64_tr_b4 %14, %24\n\t"
-      "ds_read_b64_tr_b4 %15, %24 offset:8\n\t"
-      "ds_read_b128 %16, %26\n\t"
-      "ds_read_b128 %17, %26 offset:64\n\t"
-      "ds_read_b128 %18, %26 offset:128\n\t"
-      "ds_read_b128 %19, %26 offset:192\n\t"
+      "ds_read_b128 %0, %21\n\t"
+      "ds_read_b128 %1, %21 offset:1024\n\t"
+      "ds_read_b128 %2, %21 offset:2048\n\t"
+      "ds_read_b128 %3, %21 offset:3072\n\t"
+      "ds_read_b32 %4, %26\n\t"
+      "ds_read_b32 %5, %26 offset:64\n\t"
+      "ds_read_b32 %6, %26 offset:128\n\t"
+      "ds_read_b32 %7, %26 offset:192\n\t"
+      "ds_read_b64_tr_b4 %8, %22\n\t"
+      "ds_read_b64_tr_b4 %9, %22 offset:8\n\t"
+      "ds_read_b64_tr_b4 %10, %23\n\t"
+      "ds_read_b64_tr_b4 %11, %23 offset:8\n\t"
+      "ds_read_b64_tr_b4 %12, %24\n\t"
+      "ds_read_b64_tr_b4 %13, %24 offset:8\n\t"
+      "ds_read_b64_tr_b4 %14, %25\n\t"
+      "ds_read_b64_tr_b4 %15, %25 offset:8\n\t"
+      "ds_read_b128 %16, %27\n\t"
+      "ds_read_b128 %17, %27 offset:64\n\t"
+      "ds_read_b128 %18, %27 offset:128\n\t"
+      "ds_read_b128 %19, %27 offset:192\n\t"
+      "ds_read_b128 %20, %28\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(u.k[0]), "=&v"(u.k[1]), "=&v"(u.k[2]), "=&v"(u.k[3]), "=&v"(u.ks[0]), "=&v"(u.ks[1]), "=&v"(u.ks[2]),
         "=&v"(u.ks[3]), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]),
-        "=&v"(v[7]), "=&v"(u.vs[0]), "=&v"(u.vs[1]), "=&v"(u.vs[2]), "=&v"(u.vs[3])
+        "=&v"(v[7]), "=&v"(u.vs[0]), "=&v"(u.vs[1]), "=&v"(u.vs[2]), "=&v"(u.vs[3]), "=&v"(u.ids)
       : "v"(b + lo.k), "v"(b + lo.v[0]), "v"(b + lo.v[1]), "v"(b + lo.v[2]), "v"(b + lo.v[3]), "v"(b + lo.ks),
-        "v"(b + lo.vs), "n"(VM)
+        "v"(b + lo.vs), "v"((uint32_t)reinterpret_cast<uintptr_t>(ids))
       : "memory");
 #pragma unroll
   for (int n = 0; n < 8; ++n) { u.v[n][0] = v[n][0]; u.v[n][1] = v[n][1]; }
@@ -182,9 +195,66 @@ XV_INLINE void reset(Fp4State& st) {
   for (int n = 0; n < 8; ++n) st.o[n] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 }
 
-XV_INLINE bf16x8_t widen8(uint32_t w, float scale) {
+// q as two e4m3 terms with power-of-two scales per 32 values.  The first is
+// scaled to a largest magnitude of 128 .. 256 and rounds to 4 significant
+// bits; the rest (at most 8, and at most 2^-4 of the value) is exact in 4 more
+// bits for values within 2^-10 of the block's largest, and within 2^-21 of the
+// largest otherwise: far below the fp32 rounding of a 128-term product of
+// values of that size.  An infinity or NaN converts to NaN.
+struct QSplit {
+  v8i_t hi, lo;       // operand B of 128 values: lane (g, c) holds values 16g .. + 15 and 64 + 16g .. + 15 of head c % G
+  int s_hi, s_lo;     // the scale bytes of block g (values 32g .. 32g + 31)
+};
+
+XV_INLINE void split_q(QSplit& o, const u32x4_t (&raw)[4], float sign, int lane) {
+  typedef short v2s_t __attribute__((ext_vector_type(2)));
+  int byte[2];
+  uint32_t hi[8], lo[8];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float f[16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t w = raw[2 * half + e / 4][e % 4];
+      top = max(top, max((w >> 16) & 0x7fffu, w & 0x7fffu));
+      f[2 * e] = bf16lo(w) * sign;
+      f[2 * e + 1] = bf16hi(w) * sign;
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));  // the block's other 16 values: lane group g ^ 1
+    byte[half] = max((int)(top >> 7) - 7, 5);
+    const float inv = __uint_as_float((uint32_t)(254 - byte[half]) << 23), s4 = 0.0625f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v2s_t h = {0, 0}, l = {0, 0};
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = f[4 * e + j] * inv;
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[0], x[1], 1.0f, false);
+      h = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(h, x[2], x[3], 1.0f, true);
+      uint32_t hb, lb;
+      __builtin_memcpy(&hb, &h, 4);
+      const auto b0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hb, 1.0f, false);
+      const auto b1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hb, 1.0f, true);
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, x[0] - b0[0], x[1] - b0[1], s4, false);
+      l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, x[2] - b1[0], x[3] - b1[1], s4, true);
+      __builtin_memcpy(&lb, &l, 4);
+      hi[4 * half + e] = hb;
+      lo[4 * half + e] = lb;
+    }
+  }
+  __builtin_memcpy(&o.hi, hi, 32);
+  __builtin_memcpy(&o.lo, lo, 32);
+  // lane group g holds blocks g / 2 and 2 + g / 2; block b's scale comes from group 2 (b % 2)
+  const int g = lane >> 4, c = lane & 15;
+  const int b0 = __shfl(byte[0], 32 * (g & 1) + c), b1 = __shfl(byte[1], 32 * (g & 1) + c);
+  o.s_hi = g < 2 ? b0 : b1;
+  o.s_lo = o.s_hi - 4;
+}
+
+XV_INLINE bf16x8_t widen8(uint32_t w) {
   uint32_t o[4];
-  fp4x8_to_bf16(w, scale, o);
+  fp4x8_to_bf16(w, 1.0f, o);
   bf16x8_t r;
   __builtin_memcpy(&r, o, 16);
   return r;
@@ -199,30 +269,29 @@ XV_INLINE void rescale_row(Fp4State& st, float alpha, int g) {
 
 // Scores, softmax update and O += P V of one unit; tokens ntok .. 63 are masked.
 template <int G>
-XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const bf16x8_t (&qb)[4], int ntok, float scale_log2, int lane) {
+XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const QSplit& q, int ntok, float scale_log2, int lane) {
   const int g = lane >> 4, c = lane & 15;
-  float sc[4][4];
+  floatx4_t acc[4];
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    const float s = fp4_scale(__builtin_amdgcn_ubfe(u.ks[p], 8 * g, 8));
-    floatx4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(u.k[p][j], s), qb[j], acc, 0, 0, 0);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) sc[p][r] = acc[r] * scale_log2;
+    const v8i_t k = {(int)u.k[p][0], (int)u.k[p][1], (int)u.k[p][2], (int)u.k[p][3], 0, 0, 0, 0};
+    const int s = (int)(u.ks[p] >> (8 * g));  // byte 0: the scale of this lane's block
+    acc[p] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+    acc[p] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.lo, acc[p], 4, 0, 0, s, 0, q.s_lo);
+    acc[p] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q.hi, acc[p], 4, 0, 0, s, 0, q.s_hi);
   }
-  if (ntok < kUnit) {
+  const bool tail = ntok < kUnit;
+  if (tail) {
 #pragma unroll
     for (int p = 0; p < 4; ++p)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (16 * p + 4 * g + r >= ntok) sc[p][r] = -INFINITY;
+        if (16 * p + 4 * g + r >= ntok) acc[p][r] = -INFINITY;
   }
   float mx = -INFINITY;
 #pragma unroll
-  for (int p = 0; p < 4; ++p) mx = fmaxf(mx, fmaxf(fmaxf(sc[p][0], sc[p][1]), fmaxf(sc[p][2], sc[p][3])));
-  mx = xor32_max(xor16_max(mx));
+  for (int p = 0; p < 4; ++p) mx = fmaxf(mx, fmaxf(fmaxf(acc[p][0], acc[p][1]), fmaxf(acc[p][2], acc[p][3])));
+  mx = xor32_max(xor16_max(mx)) * scale_log2;
   // the maximum in use moves only when some head's grew by more than kLazy
   const float m_new = fmaxf(st.m, mx);
   if (__any(m_new > st.m + kLazy)) {
@@ -234,6 +303,18 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const bf16x8_t (&qb)[4
     rescale_row<G, 2>(st, alpha, g);
     rescale_row<G, 3>(st, alpha, g);
   }
+  float pr[4][4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) pr[p][r] = __builtin_amdgcn_exp2f(fmaf(acc[p][r], scale_log2, -st.m));
+  if (tail) {  // also where a scale of 0 makes -inf * scale a NaN
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * p + 4 * g + r >= ntok) pr[p][r] = 0.f;
+  }
   // p in fp32 for the sum; times the V scale and rounded to bf16 as the operand
   constexpr int NV = G == 8 ? 2 : 1;
   bf16x8_t pa[NV][2];
@@ -244,14 +325,13 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const bf16x8_t (&qb)[4
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       const int p = 2 * j + e / 4, r = e % 4;
-      const float p0 = __builtin_amdgcn_exp2f(sc[p][r] - st.m), p1 = __builtin_amdgcn_exp2f(sc[p][r + 1] - st.m);
-      st.l += p0 + p1;
+      st.l += pr[p][r] + pr[p][r + 1];
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         // the low mantissa bit turns scale 255 into a NaN and moves the others by 2^-23 of themselves
         const float f0 = __uint_as_float((__builtin_amdgcn_ubfe(u.vs[p][r], shift + 16 * v, 8) << 23) | 1u);
         const float f1 = __uint_as_float((__builtin_amdgcn_ubfe(u.vs[p][r + 1], shift + 16 * v, 8) << 23) | 1u);
-        w[v][e / 2] = pack_bf16x2(p0 * f0, p1 * f1);
+        w[v][e / 2] = pack_bf16x2(pr[p][r] * f0, pr[p][r + 1] * f1);
       }
     }
 #pragma unroll
@@ -260,8 +340,8 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const bf16x8_t (&qb)[4
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
     const int v = NV == 2 ? n / 4 : 0;
-    st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[v][0], widen8(u.v[n][0], 1.0f), st.o[n], 0, 0, 0);
-    st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[v][1], widen8(u.v[n][1], 1.0f), st.o[n], 0, 0, 0);
+    st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[v][0], widen8(u.v[n][0]), st.o[n], 0, 0, 0);
+    st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[v][1], widen8(u.v[n][1]), st.o[n], 0, 0, 0);
   }
 }
 
@@ -277,25 +357,24 @@ XV_INLINE void issue_q(char* slot, const Fp4DecodeArgs& a, int b, int kvh, int l
   }
 }
 
-// Q^T operand of step j: column c holds head c % G, its values 32g + 8j .. + 7.
-template <int G, int VM>
-XV_INLINE void read_q(bf16x8_t (&qb)[4], const char* slot, int lane) {
-  const uint32_t a0 = (uint32_t)reinterpret_cast<uintptr_t>(slot) + ((lane & 15) % G) * 256 + (lane >> 4) * 64;
+// This lane's 32 values of head c % G out of the q slot: 16g .. + 15 and 64 + 16g .. + 15.
+template <int G>
+XV_INLINE void read_q(u32x4_t (&raw)[4], const char* slot, int lane) {
+  const uint32_t a0 = (uint32_t)reinterpret_cast<uintptr_t>(slot) + ((lane & 15) % G) * 256 + (lane >> 4) * 32;
   __asm__ __volatile__(
-      "s_waitcnt vmcnt(%5)\n\t"
       "ds_read_b128 %0, %4\n\t"
       "ds_read_b128 %1, %4 offset:16\n\t"
-      "ds_read_b128 %2, %4 offset:32\n\t"
-      "ds_read_b128 %3, %4 offset:48\n\t"
+      "ds_read_b128 %2, %4 offset:128\n\t"
+      "ds_read_b128 %3, %4 offset:144\n\t"
       "s_waitcnt lgkmcnt(0)"
-      : "=&v"(qb[0]), "=&v"(qb[1]), "=&v"(qb[2]), "=&v"(qb[3])
-      : "v"(a0), "n"(VM)
+      : "=&v"(raw[0]), "=&v"(raw[1]), "=&v"(raw[2]), "=&v"(raw[3])
+      : "v"(a0)
       : "memory");
 }
 
 // The finished segment's G rows: the bf16 output if the wave covered the whole
 // segment (part < 0), else partial slot `part`.  They go through `stage` (the
-// q slot in hand, its q in registers) and leave in 16-byte pieces; LDS access in asm.
+// q slot, its q in registers) and leave in 16-byte pieces; LDS access in asm.
 template <int G>
 XV_INLINE void finish_segment(const Fp4DecodeArgs& a, const Fp4State& st, int b, int kvh, int part, int lane, char* stage) {
   const int c = lane & 15, g = lane >> 4;
@@ -339,58 +418,61 @@ XV_INLINE void finish_segment(const Fp4DecodeArgs& a, const Fp4State& st, int b,
 // pages past a sequence's end, fetch an entry that exists.
 XV_INLINE void load_window(char* half, const Fp4DecodeArgs& a, __amdgpu_buffer_rsrc_t rbt, const int* pref, const int* sl,
                            int64_t f0, int base, int n, int lane) {
-#pragma unroll
-  for (int j = 0; j < kIdWindow * 4 / 64; ++j) {
-    const int y = base + 16 * j + (lane >> 2);
-    int off = 0;
-    if (y < n) {
-      const int64_t f = f0 + y;
-      const int b = seq_of(pref, a.batch, a.hkv, f);
-      const int nu = pref[b + 1] - pref[b];
-      const int r = (int)(f - (int64_t)a.hkv * pref[b]);
-      const int page = min(4 * (r % nu) + (lane & 3), (sl[b] - 1) / 16);
-      off = (int)(((int64_t)b * a.bt_stride + page / a.nsub) * 4);
-    }
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rbt, (lds_void*)(half + 256 * j), 4, off, 0, 0, 0);
+  static_assert(kIdWindow * 4 == 64, "one id per lane");
+  const int y = base + (lane >> 2);
+  int off = 0;
+  if (y < n) {
+    const int64_t f = f0 + y;
+    const int b = seq_of(pref, a.batch, a.hkv, f);
+    const int nu = pref[b + 1] - pref[b];
+    const int r = (int)(f - (int64_t)a.hkv * pref[b]);
+    const int page = min(4 * (r % nu) + (lane & 3), (sl[b] - 1) / 16);
+    off = (int)(((int64_t)b * a.bt_stride + page / a.nsub) * 4);
   }
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rbt, (lds_void*)half, 4, off, 0, 0, 0);
 }
 
 template <int G>
-__global__ __launch_bounds__(64) void fp4_decode_kernel(Fp4DecodeArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[kRing * kSlot<G>];
-  __shared__ __attribute__((aligned(16))) char idtab[2 * kIdWindow * 16];
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_decode_kernel(Fp4DecodeArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * kWaveLds<G>];
   __shared__ int pref[kMaxBatch + 1];  // units of sequences 0 .. b - 1
   __shared__ int sl[kMaxBatch];        // their tokens
-  const int lane = threadIdx.x;
-  int carry = 0, max_nu = 0;
-  for (int c = 0; c < a.batch; c += 64) {
-    const int b = c + lane;
-    const int ctx = b < a.batch ? min(max(a.seqlens[b], 0), a.max_ctx) : 0;
-    const int nu = (ctx + kUnit - 1) / kUnit;
-    max_nu = max(max_nu, nu);
-    int inc = nu;
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xf, 0xf, true);  // inclusive scan: row_shr 1, 2, 4, 8,
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xf, 0xf, true);  // then the row sums across rows
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xf, 0xf, true);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x118, 0xf, 0xf, true);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x142, 0xa, 0xf, true);
-    inc += __builtin_amdgcn_update_dpp(0, inc, 0x143, 0xc, 0xf, true);
-    if (b < a.batch) {
-      pref[b + 1] = carry + inc;
-      sl[b] = ctx;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave == 0) {
+    int carry = 0;
+    for (int c = 0; c < a.batch; c += 64) {
+      const int b = c + lane;
+      const int ctx = b < a.batch ? min(max(a.seqlens[b], 0), a.max_ctx) : 0;
+      int inc = (ctx + kUnit - 1) / kUnit;
+      inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xf, 0xf, true);  // inclusive scan: row_shr 1, 2, 4, 8,
+      inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xf, 0xf, true);  // then the row sums across rows
+      inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xf, 0xf, true);
+      inc += __builtin_amdgcn_update_dpp(0, inc, 0x118, 0xf, 0xf, true);
+      inc += __builtin_amdgcn_update_dpp(0, inc, 0x142, 0xa, 0xf, true);
+      inc += __builtin_amdgcn_update_dpp(0, inc, 0x143, 0xc, 0xf, true);
+      if (b < a.batch) {
+        pref[b + 1] = carry + inc;
+        sl[b] = ctx;
+      }
+      carry += __builtin_amdgcn_readlane(inc, 63);
     }
-    carry += __builtin_amdgcn_readlane(inc, 63);
+    if (lane == 0) pref[0] = 0;
   }
-  if (lane == 0) pref[0] = 0;
   __syncthreads();
-  max_nu = (int)wave_max((float)max_nu);  // exact in fp32 (below 2^24)
-  const int64_t total = (int64_t)a.hkv * carry;
+  int longest = 0;
+  for (int b = lane; b < a.batch; b += 64) longest = max(longest, sl[b]);
+  const int max_nu = ((int)wave_max((float)((longest + kUnit - 1) / kUnit)));  // exact in fp32 (below 2^24)
+  const int64_t total = (int64_t)a.hkv * __builtin_amdgcn_readfirstlane(pref[a.batch]);
   // units per range: every wave the same, and no segment in more than kMergeMaxParts ranges
-  const int L = (int)max((int64_t)max(1, (max_nu + kMergeMaxParts - 2) / (kMergeMaxParts - 1)),
-                         (total + a.nwaves - 1) / a.nwaves);
-  const int64_t f0 = (int64_t)blockIdx.x * L;
+  const int nwaves = gridDim.x * kWaves;
+  const int L = (int)max((int64_t)max(1, (max_nu + kMergeMaxParts - 2) / (kMergeMaxParts - 1)), (total + nwaves - 1) / nwaves);
+  const int id = wave * gridDim.x + blockIdx.x;  // short launches spread over the CUs first
+  const int64_t f0 = (int64_t)id * L;
   const int n = (int)max((int64_t)0, min(f0 + L, total) - f0);
   if (n == 0) return;
+  char* const mine = lds + wave * kWaveLds<G>;
+  char* const qslot = mine + 2 * kUnitLds;
+  char* const idtab = qslot + kQBytes<G>;
   const Fp4Lane offs = lane_offsets(a.ts, lane);
 
   Fp4Cursor c0;
@@ -407,93 +489,88 @@ __global__ __launch_bounds__(64) void fp4_decode_kernel(Fp4DecodeArgs a) {
   const __amdgpu_buffer_rsrc_t rbt =
       page_rsrc(reinterpret_cast<const bf16_t*>(a.bt), (uint32_t)((int64_t)a.batch * a.bt_stride * 4));
   load_window(idtab, a, rbt, pref, sl, f0, 0, n, lane);
-  load_window(idtab + kIdWindow * 16, a, rbt, pref, sl, f0, kIdWindow, n, lane);
+  if (n > kIdWindow) load_window(idtab + kIdWindow * 16, a, rbt, pref, sl, f0, kIdWindow, n, lane);
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
-  int issued = -1;
 
-  // Unit y (clamped to the range's last: a harmless re-read, so that every
-  // call issues the same kUnitOps loads) into ring slot `slot`.
-  auto issue = [&](int y, int slot) {
-    char* buf = lds + slot * kSlot<G>;
-    if (y > issued) {
-      const bool newseg = issued < 0 || (advance(ic, pref, sl, a.hkv, a.batch, a.nsub), ic.u == 0);
-      issued = y;
-      if (y % kIdWindow == 0 && y > 0)  // entering window k (in place since window k - 1 began): request window k + 1
-        load_window(idtab + ((y / kIdWindow + 1) & 1) * (kIdWindow * 16), a, rbt, pref, sl, f0, y + kIdWindow, n, lane);
-      if (newseg) issue_q<G>(buf + kQOff, a, ic.b, ic.kvh, lane);
-    }
-    u32x4_t idv;
-    __asm__ __volatile__("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)"
-                         : "=&v"(idv)
-                         : "v"((uint32_t)reinterpret_cast<uintptr_t>(idtab) + ((y / kIdWindow) & 1) * (kIdWindow * 16) +
-                               (y % kIdWindow) * 16)
-                         : "memory");
-    const int ntok = min(kUnit, ic.ctx - ic.u * kUnit);
-    const int t = min(lane, ntok - 1);  // whose scales this lane fetches
-    int64_t soff = 0;
+  // Unit y, whose cursor is ic and whose block ids are idv, into its ring
+  // slot.  A page's rows past the sequence's end are read as they are (they are
+  // masked, and every code is finite); their scales are those of the last token.
+  auto issue = [&](int y, const u32x4_t& idv) {
+    char* buf = mine + (y & 1) * kUnitLds;
+    if (y % kIdWindow == 0 && y > 0)  // entering window k (in place since window k - 1 began): request window k + 1
+      load_window(idtab + ((y / kIdWindow + 1) & 1) * (kIdWindow * 16), a, rbt, pref, sl, f0, y + kIdWindow, n, lane);
+    const int t = min(lane, ic.ctx - ic.u * kUnit - 1);  // whose scales this lane fetches
+    const uint64_t hoff = (uint64_t)(uint32_t)ic.kvh * a.hs;
+    uint32_t id_t = 0, row_t = 0;
     int sub = ic.sub;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t page = __builtin_amdgcn_readfirstlane(idv[j]);
-      const int64_t base = page * a.ps + (int64_t)sub * (16 * a.ts) + (int64_t)ic.kvh * a.hs;
-      const int rows = min(16, ntok - 16 * j);
-      const uint32_t bytes = rows > 0 ? (uint32_t)((int64_t)(rows - 1) * a.ts + kRow) : 0u;  // rows past the end read as zeros
-      const __amdgpu_buffer_rsrc_t rk = page_rsrc(reinterpret_cast<const bf16_t*>(a.kc + base), bytes);
-      const __amdgpu_buffer_rsrc_t rv = page_rsrc(reinterpret_cast<const bf16_t*>(a.vc + base), bytes);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(buf + 1024 * j), 16, offs.g, 0, 0, kNontemporal);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(buf + kVOff + 1024 * j), 16, offs.g, 0, 0, kNontemporal);
-      const int64_t sbase = page * a.sps + (int64_t)sub * (16 * a.sts) + (int64_t)ic.kvh * a.shs;
-      if ((t >> 4) == j) soff = sbase;
+      const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)idv[j]);
+      const uint64_t base = (uint64_t)page * a.ps + hoff + (uint64_t)(uint32_t)(16 * sub) * a.ts;
+      __builtin_amdgcn_global_load_lds((global_cptr)(a.kc + base + offs.g), (lds_void*)(buf + 1024 * j), 16, 0, kNontemporal);
+      __builtin_amdgcn_global_load_lds((global_cptr)(a.vc + base + offs.g), (lds_void*)(buf + kVOff + 1024 * j), 16, 0,
+                                       kNontemporal);
+      if ((t >> 4) == j) {
+        id_t = page;
+        row_t = 16 * sub;
+      }
       if (++sub == a.nsub) sub = 0;
     }
-    soff += (int64_t)(t & 15) * a.sts;
-    typedef const __attribute__((address_space(1))) void* gptr;
-    __builtin_amdgcn_global_load_lds((gptr)(uintptr_t)(a.ks + soff), (lds_void*)(buf + kKsOff), 4, 0, 0);
-    __builtin_amdgcn_global_load_lds((gptr)(uintptr_t)(a.vs + soff), (lds_void*)(buf + kVsOff), 4, 0, 0);
+    const uint64_t soff = (uint64_t)id_t * a.sps + (uint64_t)(row_t + (t & 15)) * a.sts + (uint64_t)(uint32_t)ic.kvh * a.shs;
+    __builtin_amdgcn_global_load_lds((global_cptr)(a.ks + soff), (lds_void*)(buf + kKsOff), 4, 0, 0);
+    __builtin_amdgcn_global_load_lds((global_cptr)(a.vs + soff), (lds_void*)(buf + kVsOff), 4, 0, 0);
   };
+  auto ids_at = [&](int y) { return idtab + ((y / kIdWindow) & 1) * (kIdWindow * 16) + (y % kIdWindow) * 16; };
 
   Fp4State st;
-  reset(st);
-  bf16x8_t qb[4];
-  constexpr int kVm = kUnitOps * (kRing - 1);
-  auto finish = [&](const Fp4Cursor& c, char* stage) {
+  QSplit q;
+  auto finish = [&](const Fp4Cursor& c) {
     const int64_t seg0 = (int64_t)a.hkv * lds_int(pref + c.b) + (int64_t)c.kvh * c.nu;
     const bool first = seg0 >= f0, last = seg0 + c.nu <= f0 + n;
     // a segment that starts in this range and ends after it: slot 1 of the wave, one that started before: slot 0
-    finish_segment<G>(a, st, c.b, c.kvh, first && last ? -1 : 2 * (int)blockIdx.x + (first ? 1 : 0), lane, stage);
+    finish_segment<G>(a, st, c.b, c.kvh, first && last ? -1 : 2 * id + (first ? 1 : 0), lane, qslot);
     if (lane == 0 && last) {
       const int w0 = (int)(seg0 / L);
-      a.ws_seg[c.b * a.hkv + c.kvh] = make_int2(w0, (int)blockIdx.x - w0 + 1);
+      a.ws_seg[c.b * a.hkv + c.kvh] = make_int2(w0, id - w0 + 1);
     }
   };
-  auto process = [&](int x, int slot) {
-    char* buf = lds + slot * kSlot<G>;
-    if (x > 0) {
-      const Fp4Cursor prev = pc;
-      advance(pc, pref, sl, a.hkv, a.batch, a.nsub);
-      if (pc.u == 0) {
-        read_q<G, kVm>(qb, buf + kQOff, lane);  // the new segment's q first: its slot then stages the finished one
-        finish(prev, buf + kQOff);
-        reset(st);
-      }
+  // Unit x begins a segment (or the range): take its q, then write out the segment before through the q slot.
+  auto begin_segment = [&](int x, const Fp4Cursor& prev) {
+    u32x4_t raw[4];
+    read_q<G>(raw, qslot, lane);
+    if (x > 0) finish(prev);
+    reset(st);
+    split_q(q, raw, a.q_sign, lane);
+  };
+  issue_q<G>(qslot, a, ic.b, ic.kvh, lane);
+  issue(0, lds_ids(ids_at(0)));
+  UnitRegs u;
+  u.ids = lds_ids(ids_at(1));
+  for (int x = 0; x < n; ++x) {
+    const Fp4Cursor prev = pc;
+    if (x > 0) pc = ic;
+    const bool seg = x == 0 || pc.u == 0;
+    const bool next = x + 1 < n;
+    // where the next unit begins a segment too, its q would overwrite this one's before it is read
+    const bool early = seg && next && pc.u + 1 == pc.nu;
+    if (early) {
+      __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
+      begin_segment(x, prev);
+    }
+    if (next) {
+      advance(ic, pref, sl, a.hkv, a.batch, a.nsub);
+      if (ic.u == 0) issue_q<G>(qslot, a, ic.b, ic.kvh, lane);
+      issue(x + 1, u.ids);
+      static_assert(kUnitOps == 10, "the wait below");
+      __asm__ __volatile__("s_waitcnt vmcnt(10)" ::: "memory");
     } else {
-      read_q<G, kVm>(qb, buf + kQOff, lane);
+      __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    UnitRegs u;
-    read_unit<kVm>(u, buf, offs);
-    unit_math<G>(st, u, qb, min(kUnit, pc.ctx - pc.u * kUnit), a.scale_log2, lane);
-  };
-#pragma unroll
-  for (int k = 0; k < kRing - 1; ++k) issue(min(k, n - 1), k);
-  for (int x0 = 0; x0 < n; x0 += kRing) {
-#pragma unroll
-    for (int u = 0; u < kRing; ++u) {
-      issue(min(x0 + u + kRing - 1, n - 1), (u + kRing - 1) % kRing);
-      if (x0 + u < n) process(x0 + u, u);
-    }
+    if (seg && !early) begin_segment(x, prev);
+    read_unit(u, mine + (x & 1) * kUnitLds, offs, ids_at(x + 2));
+    unit_math<G>(st, u, q, min(kUnit, pc.ctx - pc.u * kUnit), a.scale_log2, lane);
   }
-  __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");  // nothing still writes this wave's LDS when it ends
-  finish(pc, lds + ((n - 1) % kRing) * kSlot<G> + kQOff);
+  finish(pc);
 }
 
 // One wave per (sequence, query head): zeros for an empty sequence, else the
@@ -521,14 +598,14 @@ __global__ __launch_bounds__(64) void fp4_merge_kernel(Fp4DecodeArgs a) {
       [&](int j) { return a.ws_lse[slot(j)]; }, 0.f, orow, lane);
 }
 
-int fp4_waves() {
+int fp4_groups() {
   static int cached = 0;  // one GPU model per process
   if (!cached) {
     int dev = 0, cus = 0;
     if (hipGetDevice(&dev) != hipSuccess ||
         hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-      cus = 256;
-    cached = min(kMaxWaves, max(1, cus) * kWavesPerCu);
+      cus = kMaxGroups;
+    cached = max(1, min(kMaxGroups, cus));
   }
   return cached;
 }
@@ -565,7 +642,8 @@ extern "C" int xv_paged_decode_attention_fp4(
       (scale_page_stride | scale_tok_stride | scale_head_stride) & 3)
     return (int)hipErrorInvalidValue;
   if (tok_stride < kRow || tok_stride > (1 << 26) || scale_tok_stride < 4 || scale_tok_stride > (1 << 26) ||
-      q_stride_head < 0 || q_stride_head > (1 << 26) || bt_stride < max_blocks_per_seq ||
+      page_stride < 0 || page_stride > INT32_MAX || head_stride < 0 || head_stride > INT32_MAX || scale_page_stride < 0 ||
+      scale_page_stride > INT32_MAX || scale_head_stride < 0 || scale_head_stride > INT32_MAX || q_stride_head < 0 || q_stride_head > (1 << 26) || bt_stride < max_blocks_per_seq ||
       (int64_t)kMaxBatch * bt_stride * 4 > INT32_MAX)
     return (int)hipErrorInvalidValue;
   if ((uintptr_t)out & 3 || out_stride_tok & 1) return (int)hipErrorInvalidValue;
@@ -575,28 +653,31 @@ extern "C" int xv_paged_decode_attention_fp4(
     return (int)hipErrorInvalidValue;
   Fp4DecodeArgs a;
   a.q_st = q_stride_tok; a.q_sh = q_stride_head;
-  a.kc = (const uint8_t*)k_cache; a.vc = (const uint8_t*)v_cache; a.ps = page_stride; a.ts = tok_stride; a.hs = head_stride;
+  a.kc = (const uint8_t*)k_cache; a.vc = (const uint8_t*)v_cache;
+  a.ps = (uint32_t)page_stride; a.ts = (uint32_t)tok_stride; a.hs = (uint32_t)head_stride;
   a.ks = (const uint8_t*)k_scale; a.vs = (const uint8_t*)v_scale;
-  a.sps = scale_page_stride; a.sts = scale_tok_stride; a.shs = scale_head_stride;
+  a.sps = (uint32_t)scale_page_stride; a.sts = (uint32_t)scale_tok_stride; a.shs = (uint32_t)scale_head_stride;
   a.bt_stride = bt_stride; a.out_st = out_stride_tok;
   a.ws_seg = (int2*)workspace;
   a.ws_lse = (float*)((char*)workspace + seg_bytes(batch, num_kv_heads));
   a.ws_o = (bf16_t*)((char*)a.ws_lse + lse_bytes(group));
   a.hq = num_q_heads; a.hkv = num_kv_heads; a.group = group;
   a.nsub = block_size / 16; a.max_ctx = (int)max_ctx;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  a.q_sign = scale < 0.f ? -1.f : 1.f;
   for (int b0 = 0; b0 < batch; b0 += kMaxBatch) {
     a.batch = min(kMaxBatch, batch - b0);
     a.q = (const bf16_t*)q + (int64_t)b0 * q_stride_tok;
     a.bt = block_tables + (int64_t)b0 * bt_stride;
     a.seqlens = cache_seqlens + b0;
     a.out = (bf16_t*)out + (int64_t)b0 * out_stride_tok;
-    a.nwaves = (int)min((int64_t)fp4_waves(), (int64_t)a.batch * num_kv_heads * ((max_ctx + kUnit - 1) / kUnit));
+    const int64_t units = (int64_t)a.batch * num_kv_heads * ((max_ctx + kUnit - 1) / kUnit);
+    const unsigned groups = (unsigned)min((int64_t)fp4_groups(), units);
     switch (group) {
-      case 1: fp4_decode_kernel<1><<<a.nwaves, 64, 0, stream>>>(a); break;
-      case 2: fp4_decode_kernel<2><<<a.nwaves, 64, 0, stream>>>(a); break;
-      case 4: fp4_decode_kernel<4><<<a.nwaves, 64, 0, stream>>>(a); break;
-      default: fp4_decode_kernel<8><<<a.nwaves, 64, 0, stream>>>(a); break;
+      case 1: fp4_decode_kernel<1><<<groups, kWaves * 64, 0, stream>>>(a); break;
+      case 2: fp4_decode_kernel<2><<<groups, kWaves * 64, 0, stream>>>(a); break;
+      case 4: fp4_decode_kernel<4><<<groups, kWaves * 64, 0, stream>>>(a); break;
+      default: fp4_decode_kernel<8><<<groups, kWaves * 64, 0, stream>>>(a); break;
     }
     XV_CHECK_LAUNCH();
     fp4_merge_kernel<<<(unsigned)(a.batch * num_q_heads), 64, 0, stream>>>(a);
