@@ -41,6 +41,7 @@ constexpr int kMaxBatch = 256;    // sequences per launch (larger batches are la
 constexpr int kWaves = 8;         // waves of a workgroup, one workgroup per CU
 constexpr int kMaxGroups = 256;   // workgroups at most
 constexpr int kMaxWaves = kWaves * kMaxGroups;
+constexpr int kMaxParts = 192;    // partials of a segment at most
 constexpr int kUnitOps = 10;      // LDS-DMA instructions a unit: 4 + 4 of codes, 1 + 1 of scales
 // LDS of one unit: K codes, V codes, K scales, V scales
 constexpr int kVOff = 4096, kKsOff = 8192, kVsOff = 8448, kUnitLds = 8704;
@@ -463,9 +464,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   for (int b = lane; b < a.batch; b += 64) longest = max(longest, sl[b]);
   const int max_nu = ((int)wave_max((float)((longest + kUnit - 1) / kUnit)));  // exact in fp32 (below 2^24)
   const int64_t total = (int64_t)a.hkv * __builtin_amdgcn_readfirstlane(pref[a.batch]);
-  // units per range: every wave the same, and no segment in more than kMergeMaxParts ranges
+  // units per range: every wave the same, and no segment in more than kMaxParts ranges
   const int nwaves = gridDim.x * kWaves;
-  const int L = (int)max((int64_t)max(1, (max_nu + kMergeMaxParts - 2) / (kMergeMaxParts - 1)), (total + nwaves - 1) / nwaves);
+  const int L = (int)max((int64_t)max(1, (max_nu + kMaxParts - 2) / (kMaxParts - 1)), (total + nwaves - 1) / nwaves);
   const int id = wave * gridDim.x + blockIdx.x;  // short launches spread over the CUs first
   const int64_t f0 = (int64_t)id * L;
   const int n = (int)max((int64_t)0, min(f0 + L, total) - f0);
@@ -573,10 +574,15 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   finish(pc);
 }
 
-// One wave per (sequence, query head): zeros for an empty sequence, else the
-// weighted sum of its partials where the segment was cut.
-__global__ __launch_bounds__(64) void fp4_merge_kernel(Fp4DecodeArgs a) {
-  const int b = blockIdx.x / a.hq, h = blockIdx.x - b * a.hq, lane = threadIdx.x;
+// One wave per (sequence, query head), four a workgroup: zeros for an empty
+// sequence, else the sum of its partials, each by its share of the segment's
+// mass, where the segment was cut.  16 lanes hold a row (8 values each), the
+// four lane rows take every fourth partial, four in flight each: up to sixteen
+// partials cost one memory round trip after the segment's record.
+__global__ __launch_bounds__(256) void fp4_merge_kernel(Fp4DecodeArgs a) {
+  const int task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  if (task >= a.batch * a.hq) return;
+  const int b = task / a.hq, h = task - b * a.hq;
   const int kvh = h / a.group, hg = h - kvh * a.group;
   const int ctx = a.seqlens[b];
   const int2 seg = a.ws_seg[b * a.hkv + kvh];  // stale when ctx <= 0: not used then
@@ -585,17 +591,53 @@ __global__ __launch_bounds__(64) void fp4_merge_kernel(Fp4DecodeArgs a) {
     *reinterpret_cast<uint32_t*>(orow + 2 * lane) = 0u;
     return;
   }
-  if (seg.y <= 1) return;
-  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.group + hg; };
-  merge_general<false>(
-      seg.y,
-      [&](int j, int i, float4& lo, float4& hi) {
-        float f[8];
-        unpack8(load_vec8(a.ws_o + slot(j) * kD + 8 * i), f);
-        lo = make_float4(f[0], f[1], f[2], f[3]);
-        hi = make_float4(f[4], f[5], f[6], f[7]);
-      },
-      [&](int j) { return a.ws_lse[slot(j)]; }, 0.f, orow, lane);
+  const int n = seg.y;
+  if (n <= 1) return;
+  auto slot = [&](int j) { return (j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.group + hg; };  // < 2^15
+  const int g = lane >> 4, i = lane & 15;
+  constexpr int kAhead = 4;  // partials in flight per lane row
+  Vec8 r[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (4 * k < n) r[k] = load_vec8(a.ws_o + slot(min(4 * k + g, n - 1)) * kD + 8 * i);
+  // lane j: the log2-sum-exps of partials j, 64 + j, 128 + j
+  const float la = lane < n ? a.ws_lse[slot(lane)] : -INFINITY;
+  float lb = -INFINITY, lc = -INFINITY;
+  if (n > 64) {
+    if (64 + lane < n) lb = a.ws_lse[slot(64 + lane)];
+    if (128 + lane < n) lc = a.ws_lse[slot(128 + lane)];
+  }
+  const float mx = wave_max(fmaxf(la, fmaxf(lb, lc)));
+  const float wa = __builtin_amdgcn_exp2f(la - mx), wb = __builtin_amdgcn_exp2f(lb - mx), wc = __builtin_amdgcn_exp2f(lc - mx);
+  const float den = wave_sum(wa + wb + wc);
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto fold = [&](const Vec8& row, int j) {  // partial j of this lane row (the four rows' lie in one block of 64)
+    const float w = __shfl(j < 64 ? wa : j < 128 ? wb : wc, j & 63);
+    float f[8];
+    unpack8(row, f);
+    if (j < n) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += w * f[e];
+    }
+  };
+  for (int j0 = 0; j0 < n; j0 += 4 * kAhead) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int j = j0 + 4 * k;
+      if (j >= n) break;
+      const Vec8 cur = r[k];
+      if (j + 4 * kAhead < n) r[k] = load_vec8(a.ws_o + slot(min(j + 4 * kAhead + g, n - 1)) * kD + 8 * i);
+      fold(cur, j + g);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = xor32_sum(xor16_sum(acc[e]));
+  if (g == 0) {
+    const float inv = 1.0f / den;
+    uint32_t* o = reinterpret_cast<uint32_t*>(orow + 8 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  }
 }
 
 int fp4_groups() {
@@ -680,7 +722,7 @@ extern "C" int xv_paged_decode_attention_fp4(
       default: fp4_decode_kernel<8><<<groups, kWaves * 64, 0, stream>>>(a); break;
     }
     XV_CHECK_LAUNCH();
-    fp4_merge_kernel<<<(unsigned)(a.batch * num_q_heads), 64, 0, stream>>>(a);
+    fp4_merge_kernel<<<(unsigned)((a.batch * num_q_heads + 3) / 4), 256, 0, stream>>>(a);
     XV_CHECK_LAUNCH();
   }
   return 0;

@@ -28,16 +28,16 @@ def aligned16(t: torch.Tensor) -> bool:
     return t.data_ptr() % 16 == 0
 
 
-def call(name: str, t: torch.Tensor, *args) -> None:
-    """Run the C ABI entry `name` on t's device (made current for the call) and
-    that device's current stream, the last argument of every entry."""
+def call(name: str, device: int, *args) -> None:
+    """Run the C ABI entry `name` on the GPU of index `device` (made current for
+    the call) and its current stream, the last argument of every entry."""
     from . import _C
 
     fn = getattr(_C.lib(), name)
-    if t.device.index == torch.cuda.current_device():
-        code = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if device == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(t.device):
-            code = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(device):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     if code:
         _C.check(code, name)

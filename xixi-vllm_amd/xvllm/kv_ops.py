@@ -23,24 +23,29 @@ def fp4_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, k_block_scale: torch
     if v_cache.dtype != FP4_PAGES or k_block_scale.dtype != FP4_SCALE or v_block_scale.dtype != FP4_SCALE:
         raise TypeError(f"a 4-bit cache holds {FP4_PAGES} codes and {FP4_SCALE} scales, got {v_cache.dtype}, "
                         f"{k_block_scale.dtype}, {v_block_scale.dtype}")
-    shape, sshape = k_cache.shape, k_block_scale.shape
-    if (v_cache.shape != shape or v_block_scale.shape != sshape or k_cache.stride() != v_cache.stride()
-            or k_block_scale.stride() != v_block_scale.stride()):
+    shape, sshape, st, ss = k_cache.shape, k_block_scale.shape, k_cache.stride(), k_block_scale.stride()
+    if v_cache.shape != shape or v_block_scale.shape != sshape or v_cache.stride() != st or v_block_scale.stride() != ss:
         raise ValueError("k_cache and v_cache, and their scales, must share one layout")
-    if (len(shape) not in (3, 4) or sshape[:-1] != shape[:-1] or shape[-1] * 2 != sshape[-1] * FP4_BLOCK
-            or k_cache.stride(-1) != 1 or k_block_scale.stride(-1) != 1):
+    dims = len(shape)
+    if (dims not in (3, 4) or sshape[:-1] != shape[:-1] or shape[-1] * 2 != sshape[-1] * FP4_BLOCK or st[-1] != 1
+            or ss[-1] != 1):
         raise ValueError(f"codes {tuple(shape)} and scales {tuple(sshape)} are not [..., Hkv, D/2] and [..., Hkv, D/32] "
                          "of unit last stride")
-    dev = k_cache.device
-    if not k_cache.is_cuda or v_cache.device != dev or k_block_scale.device != dev or v_block_scale.device != dev:
+    dev = k_cache.get_device()  # -1 on the CPU
+    if dev < 0 or v_cache.get_device() != dev or k_block_scale.get_device() != dev or v_block_scale.get_device() != dev:
         raise RuntimeError("xvllm ops run on the GPU only (HIP kernels), a cache and its scales on one device")
-    st, ss = k_cache.stride(), k_block_scale.stride()
-    if len(shape) == 4:
+    if dims == 4:
         strides, sstrides, bs = st[:3], ss[:3], shape[1]
     else:
         strides, sstrides, bs = (st[0], 0, st[1]), (ss[0], 0, ss[1]), 1
-    return ((ptr(k_cache), ptr(v_cache), *strides), (ptr(k_block_scale), ptr(v_block_scale), *sstrides),
+    return ((k_cache.data_ptr(), v_cache.data_ptr(), *strides),
+            (k_block_scale.data_ptr(), v_block_scale.data_ptr(), *sstrides),
             (shape[0], bs, shape[-2], shape[-1] * 2))
+
+
+def as_int32(t: torch.Tensor) -> torch.Tensor:
+    """t as contiguous-enough int32 indexes (t itself where it is that already)."""
+    return t if t.dtype == torch.int32 else t.to(torch.int32)
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
@@ -57,11 +62,12 @@ def _store_fp4(key, value, k_cache, v_cache, slot_mapping, k_block_scale, v_bloc
     if key.shape != (n, hkv, d) or value.shape != (n, hkv, d):
         raise ValueError(f"key {tuple(key.shape)}, value {tuple(value.shape)}: a cache of {hkv} heads of {d} takes "
                          f"[{n}, {hkv}, {d}] for {n} slots")
-    if key.device != k_cache.device or value.device != k_cache.device or slot_mapping.device != k_cache.device:
+    dev = k_cache.get_device()
+    if key.get_device() != dev or value.get_device() != dev or slot_mapping.get_device() != dev:
         raise RuntimeError("key, value, slot_mapping and the cache must be on one device")
     key, value = _readable(key), _readable(value)
-    slots = slot_mapping.to(torch.int32).contiguous()
-    call("xv_store_kvcache_fp4", key, ptr(key), key.stride(0), key.stride(1), ptr(value), value.stride(0),
+    slots = as_int32(slot_mapping).contiguous()
+    call("xv_store_kvcache_fp4", dev, ptr(key), key.stride(0), key.stride(1), ptr(value), value.stride(0),
          value.stride(1), *codes, *scales, bs, ptr(slots), n, hkv, d)
 
 
@@ -170,8 +176,8 @@ def gather_kvcache(
     codes, scales, (_, bs, hkv, d) = fp4_pages(k_cache, v_cache, k_block_scale, v_block_scale)
     if k_cache.dim() != 4:
         raise ValueError(f"gather_kvcache needs a paged cache [NB, BS, Hkv, D/2], got {tuple(k_cache.shape)}")
-    dev = k_cache.device
-    if block_tables.device != dev or cu_seqlens_k.device != dev:
+    dev = k_cache.get_device()
+    if block_tables.get_device() != dev or cu_seqlens_k.get_device() != dev:
         raise RuntimeError("the cache, block_tables and cu_seqlens_k must be on one device")
     bsz = cu_seqlens_k.shape[0] - 1
     if cu_seqlens_k.dim() != 1 or bsz < 0 or block_tables.dim() != 2 or block_tables.shape[0] < bsz:
@@ -180,22 +186,22 @@ def gather_kvcache(
     if total_tokens < 0:
         raise ValueError("total_tokens must not be negative")
     if out is None:
-        ko, vo = (torch.empty((total_tokens, hkv, d), dtype=torch.bfloat16, device=dev) for _ in range(2))
+        ko, vo = torch.empty((2, total_tokens, hkv, d), dtype=torch.bfloat16, device=k_cache.device).unbind(0)
         row = hkv * d
     else:
         ko, vo = out
         require_bf16(ko, vo)
         for t in (ko, vo):
-            if (t.shape != (total_tokens, hkv, d) or t.device != dev or t.stride() != ko.stride() or t.stride(2) != 1
+            if (t.shape != (total_tokens, hkv, d) or t.get_device() != dev or t.stride() != ko.stride() or t.stride(2) != 1
                     or t.stride(1) != d or t.stride(0) % 8 or t.stride(0) < hkv * d or not aligned16(t)):
                 raise ValueError(f"out: two bf16 [{total_tokens}, {hkv}, {d}] of contiguous, 16-byte aligned rows")
         row = ko.stride(0)
     if total_tokens == 0 or bsz == 0:
         return ko, vo
-    bt = block_tables.to(torch.int32)
+    bt = as_int32(block_tables)
     if bt.stride(-1) != 1:
         bt = bt.contiguous()
-    cu = cu_seqlens_k.to(torch.int32).contiguous()
-    call("xv_gather_kv_fp4", k_cache, *codes, *scales, bs, ptr(bt), bt.stride(0), bt.shape[1], ptr(cu), bsz,
+    cu = as_int32(cu_seqlens_k).contiguous()
+    call("xv_gather_kv_fp4", dev, *codes, *scales, bs, ptr(bt), bt.stride(0), bt.shape[1], ptr(cu), bsz,
          int(total_tokens), hkv, d, ptr(ko), ptr(vo), row)
     return ko, vo

@@ -16,7 +16,7 @@ import torch.nn as nn
 
 from .. import _C
 from .._torch_glue import aligned16, call, ptr, require_bf16, require_cuda, stream_of
-from ..kv_ops import FP4_PAGES, fp4_pages, store_kvcache
+from ..kv_ops import FP4_PAGES, as_int32, fp4_pages, store_kvcache
 
 
 @dataclass
@@ -129,25 +129,32 @@ def _paged_decode_fp4(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv,
     if q3.shape[1:] != (hq, d) or block_tables.dim() != 2 or block_tables.shape[0] < bsz or cache_seqlens.numel() < bsz:
         raise ValueError(f"q {tuple(q.shape)}, block_tables {tuple(block_tables.shape)}, cache_seqlens "
                          f"{tuple(cache_seqlens.shape)}: not {hq} heads of {d} with a table row and a length each")
-    dev = k_cache.device
-    if q.device != dev or block_tables.device != dev or cache_seqlens.device != dev:
+    dev = k_cache.get_device()
+    if q.get_device() != dev or block_tables.get_device() != dev or cache_seqlens.get_device() != dev:
         raise RuntimeError("q, the cache, block_tables and cache_seqlens must be on one device")
-    bt = block_tables.to(torch.int32)
-    if bt.stride(-1) != 1 or (bsz > 1 and bt.stride(0) < bt.shape[1]):
+    bt = as_int32(block_tables)
+    max_blocks = bt.shape[1]
+    bt_st, inner = bt.stride()
+    if inner != 1 or (bsz > 1 and bt_st < max_blocks):
         bt = bt.contiguous()
-    sl = cache_seqlens.to(torch.int32).contiguous()
+        bt_st = max_blocks
+    sl = as_int32(cache_seqlens).contiguous()
     if out is None:
-        out = torch.empty((bsz, hq * d), dtype=q.dtype, device=dev)
-    elif out.shape != (bsz, hq * d) or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1:
-        raise ValueError(f"out must be bf16 [{bsz}, {hq * d}] of unit last stride")
+        out = torch.empty((bsz, hq * d), dtype=q.dtype, device=q.device)
+        out_st = hq * d
+    elif out.shape != (bsz, hq * d) or out.dtype != q.dtype or out.get_device() != dev or out.stride(-1) != 1:
+        raise ValueError(f"out must be bf16 [{bsz}, {hq * d}] of unit last stride on the cache's device")
+    else:
+        out_st = out.stride(0)
     if bsz == 0:
         return out
-    max_blocks = bt.shape[1]
     # a workspace of the call's own, from the caching allocator: calls on several streams and captured graphs share none
-    ws = torch.empty(_C.lib().xv_paged_decode_fp4_workspace_size(bsz, hq, hkv), dtype=torch.uint8, device=dev)
-    scale = 1.0 / math.sqrt(d) if softmax_scale is None else softmax_scale
-    call("xv_paged_decode_attention_fp4", q3, ptr(q3), qs0, qs1, *codes, *scales, ptr(bt), max(bt.stride(0), max_blocks),
-         ptr(sl), ptr(out), out.stride(0), ptr(ws), ws.numel(), bsz, hq, hkv, d, bs, max_blocks, float(scale))
+    ws_bytes = _C.lib().xv_paged_decode_fp4_workspace_size(bsz, hq, hkv)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
+    call("xv_paged_decode_attention_fp4", dev, q3.data_ptr(), qs0, qs1, *codes, *scales, bt.data_ptr(),
+         max(bt_st, max_blocks), sl.data_ptr(), out.data_ptr(), out_st, ws.data_ptr(), ws_bytes, bsz, hq, hkv, d, bs,
+         max_blocks, scale)
     return out
 
 
@@ -177,10 +184,10 @@ def paged_decode_attention(
     scales k_block_scale / v_block_scale [NB, BS, Hkv, D/32].  The 4-bit form
     takes a workspace of its own per call; the others share one per device
     (decode_workspace)."""
-    require_cuda(q, k_cache, v_cache, block_tables, cache_seqlens)
     if k_cache.dtype == FP4_PAGES:
         return _paged_decode_fp4(q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim,
                                  softmax_scale, out, k_block_scale, v_block_scale)
+    require_cuda(q, k_cache, v_cache, block_tables, cache_seqlens)
     fp8 = k_cache.dtype == torch.float8_e4m3fn
     require_bf16(q, *(() if fp8 else (k_cache, v_cache)))
     if fp8 and v_cache.dtype != torch.float8_e4m3fn:

@@ -353,20 +353,28 @@ def streamed_into_norm(x: torch.Tensor, w) -> PartialSums:
     return PartialSums(torch.ops.xv.stream_gemm(x, w, GEMM_PARTS, p))
 
 
-@torch.library.custom_op("xv::mxfp4_linear", mutates_args=())
-def _mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
-    """mxfp4_linear on x [M, K] with codes and scales as bytes."""
-    from .._torch_glue import aligned16, call, ptr
+def _mxfp4_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
+    """mxfp4_linear on x [M, K], arguments checked."""
+    from .._torch_glue import call
 
     m, k = x.shape
     n = w.shape[0]
-    if x.stride(1) != 1 or x.stride(0) % 8 or (m > 1 and x.stride(0) < k) or not aligned16(x):
+    st, inner = x.stride()
+    if inner != 1 or st % 8 or (m > 1 and st < k) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((m, n // 2 if silu_mul else n), dtype=torch.bfloat16, device=x.device)
-    if out.numel():
-        call("xv_mxfp4_gemm", x, ptr(x), x.stride(0), ptr(w), w.stride(0), ptr(w_scale), w_scale.stride(0), ptr(out),
-             out.shape[1], m, n, k, int(silu_mul))
+        st = k
+    cols = n // 2 if silu_mul else n
+    out = torch.empty((m, cols), dtype=torch.bfloat16, device=x.device)
+    if m and cols:
+        call("xv_mxfp4_gemm", x.get_device(), x.data_ptr(), st, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
+             w_scale.stride(0), out.data_ptr(), cols, m, n, k, silu_mul)
     return out
+
+
+@torch.library.custom_op("xv::mxfp4_linear", mutates_args=())
+def _mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
+    """_mxfp4_product as an op that a compiler's trace holds."""
+    return _mxfp4_product(x, w, w_scale, silu_mul)
 
 
 @_mxfp4_linear.register_fake
@@ -384,25 +392,29 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, sil
     K is a multiple of 32, N any (even with silu_mul).  w's rows start 16-byte
     aligned and have unit stride, as w_scale's have; x of any layout.  For
     inference: it has no backward."""
-    from .._torch_glue import aligned16, require_bf16, require_cuda
-
-    require_cuda(x, w, w_scale)
-    require_bf16(x)
-    if w.dtype != torch.float4_e2m1fn_x2 or w_scale.dtype != torch.float8_e8m0fnu:
-        raise TypeError(f"mxfp4_linear takes float4_e2m1fn_x2 codes and float8_e8m0fnu scales, got {w.dtype} and "
-                        f"{w_scale.dtype}")
-    k = x.shape[-1]
-    if w.dim() != 2 or w_scale.dim() != 2 or k % 32 or k == 0 or w.shape[1] * 2 != k or w_scale.shape != (w.shape[0], k // 32):
-        raise ValueError(f"mxfp4_linear: x {tuple(x.shape)}, codes {tuple(w.shape)}, scales {tuple(w_scale.shape)} are not "
-                         "[..., K], [N, K/2] and [N, K/32], K a multiple of 32")
-    if silu_mul and w.shape[0] % 2:
-        raise ValueError(f"mxfp4_linear: a gate/up weight has an even number of rows, got {w.shape[0]}")
-    if x.device != w.device or x.device != w_scale.device:
-        raise RuntimeError("mxfp4_linear: x, w and w_scale must be on one device")
-    if (w.stride(1) != 1 or w_scale.stride(1) != 1 or w.stride(0) % 16 or w.stride(0) < k // 2 or w_scale.stride(0) < k // 32
-            or not aligned16(w)):
+    if x.dtype != torch.bfloat16 or w.dtype != torch.float4_e2m1fn_x2 or w_scale.dtype != torch.float8_e8m0fnu:
+        raise TypeError(f"mxfp4_linear takes bfloat16 x, float4_e2m1fn_x2 codes and float8_e8m0fnu scales, got {x.dtype}, "
+                        f"{w.dtype} and {w_scale.dtype}")
+    xs, ws, ss = x.shape, w.shape, w_scale.shape
+    k = xs[-1] if len(xs) else 0
+    if len(ws) != 2 or len(ss) != 2 or k % 32 or k == 0 or ws[1] * 2 != k or ss[0] != ws[0] or ss[1] * 32 != k:
+        raise ValueError(f"mxfp4_linear: x {tuple(xs)}, codes {tuple(ws)}, scales {tuple(ss)} are not [..., K], [N, K/2] "
+                         "and [N, K/32], K a multiple of 32")
+    if silu_mul and ws[0] % 2:
+        raise ValueError(f"mxfp4_linear: a gate/up weight has an even number of rows, got {ws[0]}")
+    wst, sst = w.stride(), w_scale.stride()
+    if wst[1] != 1 or sst[1] != 1 or wst[0] % 16 or wst[0] < ws[1] or sst[0] < ss[1]:
         raise ValueError("mxfp4_linear reads w in place: rows of unit stride, whole and 16-byte aligned")
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("mxfp4_linear has no backward: call it under torch.no_grad()")
-    y = torch.ops.xv.mxfp4_linear(x.reshape(-1, k), w.view(torch.uint8), w_scale.view(torch.uint8), silu_mul)
-    return y.view(*x.shape[:-1], y.shape[1])
+    x2 = x if len(xs) == 2 else x.reshape(-1, k)
+    if torch.compiler.is_compiling():
+        y = torch.ops.xv.mxfp4_linear(x2, w.view(torch.uint8), w_scale.view(torch.uint8), silu_mul)
+    else:
+        dev = x.get_device()
+        if dev < 0 or w.get_device() != dev or w_scale.get_device() != dev:
+            raise RuntimeError("xvllm ops run on the GPU only (HIP kernels); mxfp4_linear needs x, w and w_scale on one device")
+        if w.data_ptr() % 16:
+            raise ValueError("mxfp4_linear reads w in place: rows of unit stride, whole and 16-byte aligned")
+        y = _mxfp4_product(x2, w, w_scale, silu_mul)
+    return y if len(xs) == 2 else y.view(*xs[:-1], y.shape[1])
