@@ -65,7 +65,7 @@ def _store(lib, **kw):
 def test_store_rejects_bad_arguments(lib):
     for kw in (dict(k=A + 8), dict(v=A + 2), dict(kst=1020), dict(vsh=132), dict(kc=A + 2), dict(kc=None), dict(ks=None),
                dict(ts=510), dict(hs=66), dict(BS=0), dict(BS=-16), dict(D=100), dict(D=16), dict(D=0), dict(H=0),
-               dict(n=-1), dict(n=1 << 25)):
+               dict(n=-1), dict(n=1 << 36)):
         assert _store(lib, **kw) == INVALID, kw
     assert _store(lib, n=0) == 0
 
