@@ -11,11 +11,12 @@
 //
 // A workgroup owns T tiles of 16 weight rows, its eight waves take turns of KS
 // values along K (their fp32 sums meet in LDS at the end), and a wave runs its T tiles
-// over one slice before the next: x is read once per workgroup and waits in
-// registers, while the weight streams through a private LDS ring by LDS-DMA.
-// Direct loads into the operand registers, where neighbouring lanes are
-// neighbouring rows, were bound by the address unit instead (a gate / up
-// weight of 24576 x 4096 at one row: 22 us, 2.4 TB/s).
+// over one slice before the next: x is read once per workgroup and its slice
+// waits in registers, while the weight streams through a private LDS ring.
+// Both travel by LDS-DMA, whole row segments per instruction.  Direct loads into the
+// operand registers, where neighbouring lanes are neighbouring rows, were
+// bound by the address unit instead (weights so: a gate / up weight of 24576 x
+// 4096 at one row 22 us; x alone so: 8 rows through 4096 x 12288 12.7 us).
 #include "xv_decode.h"
 #include "xv_fp4.h"
 #include "xv_kernels.h"
@@ -106,16 +107,43 @@ XV_INLINE void read_stage(u32x4_t (&w)[N], uint32_t (&s)[N], const uint32_t (&wa
   }
 }
 
-template <int MT, int KS, int T, bool SILU, bool WIDE>
+// Eight operand reads of x (pairs of 4, `b` apart) in one asm block with one wait.
+XV_INLINE void read_x8(u32x4_t (&v)[8], const uint32_t (&at)[8]) {
+  __asm__ __volatile__(
+      "ds_read_b128 %0, %8\n\t"
+      "ds_read_b128 %1, %9\n\t"
+      "ds_read_b128 %2, %10\n\t"
+      "ds_read_b128 %3, %11\n\t"
+      "ds_read_b128 %4, %12\n\t"
+      "ds_read_b128 %5, %13\n\t"
+      "ds_read_b128 %6, %14\n\t"
+      "ds_read_b128 %7, %15\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7])
+      : "memory");
+}
+
+template <int N>
+XV_INLINE void wait_vm() {
+  __asm__ __volatile__("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// MT column tiles of 16 rows of x, XR of them fetched (8: the tile's upper
+// half repeats the lower, its outputs are not stored); XD slices of x in LDS.
+template <int MT, int XR, int KS, int XD, int T, bool SILU, bool WIDE>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_gemm_kernel(Fp4GemmArgs a) {
   using S = Stage<KS, WIDE>;
-  constexpr int kRing = kWaves * kDepth * S::kBytes;
-  constexpr int TR = SILU ? 2 : 1;                       // tiles summed over the waves at a time
+  constexpr int kXBytes = XR * KS * 2, kXLoads = kXBytes / 1024, kXPieces = KS / 8;
+  constexpr int kWave = kDepth * S::kBytes + XD * kXBytes;  // LDS of one wave
+  constexpr int TR = SILU ? 2 : 1;                          // tiles summed over the waves at a time
   constexpr int kRed = kWaves * TR * MT * 1024;
-  __shared__ __attribute__((aligned(16))) char lds[kRing > kRed ? kRing : kRed];
+  static_assert(kXLoads >= 1 && kWaves * kWave <= 163840 && kRed <= 163840, "LDS of a CU");
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * kWave > kRed ? kWaves * kWave : kRed];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * (SILU ? T / 2 : T) * 16, m0 = blockIdx.y * (MT * 16);
-  char* const ring = lds + wave * kDepth * S::kBytes;
+  char* const ring = lds + wave * kWave;
+  char* const xring = ring + kDepth * S::kBytes;
   const int blocks = a.k / kFp4Block;
   const int slices = (a.k + KS - 1) / KS;
   const int mine = slices > wave ? (slices - wave + kWaves - 1) / kWaves : 0;  // slices wave, wave + 8, ...
@@ -140,9 +168,16 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
     const int at = min(64 * q + lane, 16 * S::SW - 1);
     soff[q] = (at / S::SW) * (uint32_t)a.s_st + 4 * (at % S::SW);
   }
+  // LDS-DMA instructions issued so far, and the count when each stage's and slice's last one left: what
+  // was issued since may still be in flight when it is waited for
+  int ops = 0, wmark[kDepth], xmark[XD];
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) wmark[d] = 0;
+#pragma unroll
+  for (int d = 0; d < XD; ++d) xmark[d] = 0;
   int issued = 0, it = 0, is = wave;  // stages issued; the next one's tile and slice
-  auto issue = [&]() {
-    char* buf = ring + (issued % kDepth) * S::kBytes;
+  auto issue = [&](int slot) {
+    char* buf = ring + slot * S::kBytes;
     const int b0 = is * S::kPieces;  // the slice's first block
     const int o0 = n0 + (SILU ? it >> 1 : it) * 16;
     const bool whole = o0 + 16 <= a.n && b0 + S::kPieces <= blocks;
@@ -177,27 +212,52 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
       }
     }
     ++issued;
+    ops += S::kOps;
+    wmark[slot] = ops;
     if (++it == T) {
       it = 0;
       is += kWaves;
     }
   };
+  // Slice `slice` of x: row r's KS values (2 KS bytes, 16-byte piece j in slot j ^ (r % 16)) at r * 2 KS.
+  auto issue_x = [&](int slice, int slot) {
+#pragma unroll
+    for (int q = 0; q < kXLoads; ++q) {
+      const int at = 64 * q + lane, row = at / kXPieces, piece = (at % kXPieces) ^ (row & 15);
+      const int k = min(slice * KS + 8 * piece, a.k - 8);  // past the end: any valid piece (zeroed below)
+      const bf16_t* src = a.x + (int64_t)min(m0 + row, a.m - 1) * a.x_st + k;
+      __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(xring + slot * kXBytes + 1024 * q), 16, 0, 0);
+    }
+    ops += kXLoads;
+    xmark[slot] = ops;
+  };
 
-  // x of a slice as operand B: lane (g, i) of step h, substep j holds row i's values 128 h + 32 g + 8 j .. + 7
-  struct X { uint4 v[S::kSteps][MT][4]; };
-  const bf16_t* xrow[MT];
+  // operand B: lane (g, i) of step h, substep j holds row i's values 128 h + 32 g + 8 j .. + 7
+  u32x4_t x[S::kSteps * MT * 4];
+  auto take_x = [&](int slice, int slot) {
+    const uint32_t b = (uint32_t)reinterpret_cast<uintptr_t>(xring + slot * kXBytes);
 #pragma unroll
-  for (int u = 0; u < MT; ++u) xrow[u] = a.x + (int64_t)min(m0 + 16 * u + i, a.m - 1) * a.x_st + 32 * g;
-  auto load_x = [&](X& x, int slice) {
+    for (int p = 0; p < S::kSteps * MT; p += 2) {
+      uint32_t at[8];
+      u32x4_t v[8];
 #pragma unroll
-    for (int h = 0; h < S::kSteps; ++h) {
-      const int k0 = slice * KS + 128 * h;
-      const bool in = k0 + 32 * g < a.k;  // whole blocks
+      for (int e = 0; e < 8; ++e) {
+        const int pe = min(p + (e >> 2), S::kSteps * MT - 1), h = pe / MT, u = pe % MT;
+        const int row = (16 * u + i) % XR;
+        at[e] = b + row * (KS * 2) + (((16 * h + 4 * g + (e & 3)) ^ (row & 15)) << 4);
+      }
+      read_x8(v, at);
 #pragma unroll
-      for (int u = 0; u < MT; ++u)
+      for (int e = 0; e < 8; ++e)
+        if (p + (e >> 2) < S::kSteps * MT) x[(p + (e >> 2)) * 4 + (e & 3)] = v[e];
+    }
+    if (slice * KS + KS > a.k) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x.v[h][u][j] = in ? *reinterpret_cast<const uint4*>(xrow[u] + k0 + 8 * j) : make_uint4(0, 0, 0, 0);
+      for (int h = 0; h < S::kSteps; ++h)
+        if (slice * KS + 128 * h + 32 * g >= a.k) {  // whole blocks: a lane's 32 values lie inside or outside
+#pragma unroll
+          for (int e = 0; e < MT * 4; ++e) x[h * MT * 4 + e] = u32x4_t{0, 0, 0, 0};
+        }
     }
   };
 
@@ -207,58 +267,74 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
     for (int u = 0; u < MT; ++u) acc[t][u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
 
-  // this lane's pieces and scale bytes within a stage
+  // this lane's pieces within a stage
   uint32_t wat[S::kSteps];
 #pragma unroll
   for (int h = 0; h < S::kSteps; ++h)
     wat[h] = (uint32_t)(i * (KS / 2) + (((4 * h + g) ^ ((i * S::kPieces) >> 4)) << 4));
-  int done = 0;
-  auto slice_work = [&](const X& x, int slice) {
+  int wslot = 0, xslot = 0;  // ring slots of the next stage and slice to use
+  if (mine > 0) {
+#pragma unroll
+    for (int d = 0; d < XD; ++d)
+      if (d < mine) issue_x(wave + d * kWaves, d);
+#pragma unroll
+    for (int d = 0; d < kDepth - 1; ++d)
+      if (issued < total) issue(d);
+  }
+  for (int s = 0; s < mine; ++s) {
+    const int slice = wave + s * kWaves;
+    {
+      int since = ops;
+#pragma unroll
+      for (int d = 0; d < XD; ++d)
+        if (d == xslot) since = ops - xmark[d];
+      constexpr int kFull = XD > 1 ? XD * S::kOps + (XD - 1) * kXLoads : (T < kDepth ? T : kDepth - 1) * S::kOps;
+      constexpr int kFirst = (kDepth - 1) * S::kOps + (XD - 1) * kXLoads;  // the first slice: the first loads of all
+      if (since >= kFull) wait_vm<kFull>();
+      else if (kFirst < kFull && since >= kFirst) wait_vm<kFirst>();
+      else wait_vm<0>();
+      take_x(slice, xslot);
+      if (s + XD < mine) issue_x(slice + XD * kWaves, xslot);
+      if (++xslot == XD) xslot = 0;
+    }
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      const bool more = issued < total;
-      if (more) issue();
-      const uint32_t b = (uint32_t)reinterpret_cast<uintptr_t>(ring + (done % kDepth) * S::kBytes);
+      if (issued < total) issue(wslot == 0 ? kDepth - 1 : wslot - 1);
+      const uint32_t b = (uint32_t)reinterpret_cast<uintptr_t>(ring + wslot * S::kBytes);
       uint32_t wa[S::kSteps];
 #pragma unroll
       for (int h = 0; h < S::kSteps; ++h) wa[h] = b + wat[h];
-      uint32_t m4 = 0;
+      uint32_t m4 = 0;  // where in its first dword the row's scale bytes start
       if constexpr (WIDE) m4 = (uint32_t)((reinterpret_cast<uintptr_t>(a.s) + (uint64_t)(wrow(t, i) * a.s_st + slice * S::kPieces)) & 3);
       const uint32_t sa = b + S::kCodes + i * (4 * S::SW) + m4 + g;
+      int since = ops;
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d)
+        if (d == wslot) since = ops - wmark[d];
+      if (++wslot == kDepth) wslot = 0;
       u32x4_t w[S::kSteps];
-      uint32_t s[S::kSteps];
-      if (more) read_stage<S::kSteps, S::kOps * (kDepth - 1)>(w, s, wa, sa);
-      else read_stage<S::kSteps, 0>(w, s, wa, sa);
-      ++done;
+      uint32_t sc[S::kSteps];
+      constexpr int kTwo = (kDepth - 1) * S::kOps;
+      constexpr int kOne = kTwo + kXLoads, kBoth = kTwo + 2 * kXLoads;  // with the x slices issued since
+      if (T == 1 && since >= kBoth) read_stage<S::kSteps, kBoth>(w, sc, wa, sa);
+      else if (since >= kOne) read_stage<S::kSteps, kOne>(w, sc, wa, sa);
+      else if (since >= kTwo) read_stage<S::kSteps, kTwo>(w, sc, wa, sa);
+      else read_stage<S::kSteps, 0>(w, sc, wa, sa);
 #pragma unroll
       for (int h = 0; h < S::kSteps; ++h) {
-        // blocks past the end: scale 0 keeps their products at x = 0 finite
-        const float f = fp4_scale(slice * KS + 128 * h + 32 * g < a.k ? s[h] : 0u);
+        // blocks past the end: scale 0 keeps their products with x = 0 finite
+        const float f = fp4_scale(slice * KS + 128 * h + 32 * g < a.k ? sc[h] : 0u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const bf16x8_t av = widen8(w[h][j], f);
 #pragma unroll
           for (int u = 0; u < MT; ++u) {
             bf16x8_t bv;
-            __builtin_memcpy(&bv, &x.v[h][u][j], 16);
+            __builtin_memcpy(&bv, &x[(h * MT + u) * 4 + j], 16);
             acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, acc[t][u], 0, 0, 0);
           }
         }
       }
-    }
-  };
-  if (mine > 0) {
-    X x0, x1;
-    load_x(x0, wave);
-#pragma unroll
-    for (int d = 0; d < kDepth - 1; ++d)
-      if (issued < total) issue();
-    for (int s = 0; s < mine; s += 2) {
-      if (s + 1 < mine) load_x(x1, wave + (s + 1) * kWaves);
-      slice_work(x0, wave + s * kWaves);
-      if (s + 1 >= mine) break;
-      if (s + 2 < mine) load_x(x0, wave + (s + 2) * kWaves);
-      slice_work(x1, wave + (s + 1) * kWaves);
     }
   }
   // the waves' sums: lane (g, i) of tile (t, u) holds weight rows 4g + r of x row i
@@ -288,24 +364,24 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   }
 }
 
-template <int MT, int KS, int T, bool SILU>
+template <int MT, int XR, int KS, int XD, int T, bool SILU>
 void launch(const Fp4GemmArgs& a, hipStream_t stream) {
   constexpr int outs = (SILU ? T / 2 : T) * 16;
   const dim3 grid((unsigned)((a.n + outs - 1) / outs), (unsigned)((a.m + MT * 16 - 1) / (MT * 16)));
   // scale rows that start at multiples of 4 bytes have narrower windows
-  if (((uintptr_t)a.s | (uint64_t)a.s_st) & 3) fp4_gemm_kernel<MT, KS, T, SILU, true><<<grid, kWaves * 64, 0, stream>>>(a);
-  else fp4_gemm_kernel<MT, KS, T, SILU, false><<<grid, kWaves * 64, 0, stream>>>(a);
+  if (((uintptr_t)a.s | (uint64_t)a.s_st) & 3) fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, true><<<grid, kWaves * 64, 0, stream>>>(a);
+  else fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, false><<<grid, kWaves * 64, 0, stream>>>(a);
 }
 
 // Tiles per workgroup: the fewest turns of the chip (one workgroup per CU),
 // each as long as its tiles plus its start and end, about one and a half tiles.
 template <bool SILU>
-int tiles_per_group(int n, int most) {
+int tiles_per_group(int n) {
   const int tiles = (n + 15) / 16 * (SILU ? 2 : 1);
   int best = SILU ? 2 : 1;
   double cost = 1e30;
   for (int t : {1, 2, 4, 6}) {
-    if (t > most || (SILU && t % 2)) continue;
+    if (SILU && t % 2) continue;
     const int groups = (tiles + t - 1) / t;
     const double c = ((groups + 255) / 256) * (t + 1.5);
     if (c <= cost) { cost = c; best = t; }
@@ -313,21 +389,24 @@ int tiles_per_group(int n, int most) {
   return best;
 }
 
-template <int MT, int KS, bool SILU>
+// One tile a workgroup takes a new slice of x with every stage: as many in
+// flight (XD) as stages, in shorter slices where 16 rows of x would not fit.
+template <int MT, int XR, int KS1, int XD1, int KS, bool SILU>
 void launch_tiles(const Fp4GemmArgs& a, hipStream_t stream) {
-  switch (tiles_per_group<SILU>(a.n, MT == 4 ? 2 : MT == 2 ? 4 : 6)) {
-    case 1: if constexpr (!SILU) launch<MT, KS, 1, SILU>(a, stream); break;
-    case 2: launch<MT, KS, 2, SILU>(a, stream); break;
-    case 4: if constexpr (MT < 4) launch<MT, KS, 4, SILU>(a, stream); break;
-    default: if constexpr (MT == 1) launch<MT, KS, 6, SILU>(a, stream); break;
+  switch (tiles_per_group<SILU>(a.n)) {
+    case 1: if constexpr (!SILU) launch<MT, XR, KS1, XD1, 1, SILU>(a, stream); break;
+    case 2: launch<MT, XR, KS, 1, 2, SILU>(a, stream); break;
+    case 4: launch<MT, XR, KS, 1, 4, SILU>(a, stream); break;
+    default: launch<MT, XR, KS, 1, 6, SILU>(a, stream); break;
   }
 }
 
 template <bool SILU>
 void dispatch(const Fp4GemmArgs& a, hipStream_t stream) {
-  if (a.m <= 16) launch_tiles<1, 512, SILU>(a, stream);
-  else if (a.m <= 32) launch_tiles<2, 256, SILU>(a, stream);
-  else launch_tiles<4, 128, SILU>(a, stream);
+  if (a.m <= 8) launch_tiles<1, 8, 256, 3, 256, SILU>(a, stream);
+  else if (a.m <= 16) launch_tiles<1, 16, 128, 3, 256, SILU>(a, stream);
+  else if (a.m <= 32) launch_tiles<2, 32, 128, 1, 128, SILU>(a, stream);
+  else launch_tiles<4, 64, 128, 1, 128, SILU>(a, stream);
 }
 
 }  // namespace
