@@ -546,11 +546,14 @@ int xv_stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_str
  *   out       row i at i * out_stride, 2-byte aligned.
  *   silu_mul  nonzero: W is the gate / up weight [2I, k] (n = 2I, gate rows first)
  *             and out[m, I] = silu(g) * u of the two fp32 products.
- * k a multiple of 32; any m >= 0 and n > 0.
+ *   workspace xv_mxfp4_gemm_workspace_size(...) bytes (0 up to 64 rows, and
+ *             where K is not split), 16-byte aligned, no initial contents.
+ * k a multiple of 32; any m >= 0 (up to 4 million) and n > 0.
  */
+size_t xv_mxfp4_gemm_workspace_size(int m, int n, int k, int silu_mul);
 int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* w_scale,
                   int64_t scale_stride, void* out, int64_t out_stride, int m, int n, int k, int silu_mul,
-                  hipStream_t stream);
+                  void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /*
  * Streaming copy of `bytes` (a multiple of 16; both pointers 16-byte aligned)

@@ -142,7 +142,7 @@ def test_decode_workspace_never_shrinks(lib):
 
 
 def _gemm(lib, **kw):
-    a = dict(x=A, xst=4096, w=A, wst=2048, s=A, sst=128, out=A, ost=1024, m=4, n=1024, k=4096, silu=0)
+    a = dict(x=A, xst=4096, w=A, wst=2048, s=A, sst=128, out=A, ost=1024, m=4, n=1024, k=4096, silu=0, ws=None, wsb=0)
     a.update(kw)
     return lib.xv_mxfp4_gemm(*a.values(), None)
 
@@ -150,6 +150,6 @@ def _gemm(lib, **kw):
 def test_gemm_rejects_bad_arguments(lib):
     for kw in (dict(x=None), dict(x=A + 8), dict(xst=4092), dict(xst=4088), dict(w=A + 8), dict(w=None), dict(wst=2040),
                dict(wst=2032), dict(s=None), dict(sst=127), dict(out=None), dict(out=A + 1), dict(ost=1023), dict(m=-1),
-               dict(n=0), dict(k=0), dict(k=4080), dict(n=1023, silu=1), dict(m=1 << 21)):
+               dict(n=0), dict(k=0), dict(k=4080), dict(n=1023, silu=1), dict(m=1 << 23), dict(m=200), dict(ws=A + 8)):
         assert _gemm(lib, **kw) == INVALID, kw
     assert _gemm(lib, m=0) == 0

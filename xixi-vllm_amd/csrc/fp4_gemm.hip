@@ -20,6 +20,9 @@
 #include "xv_decode.h"
 #include "xv_fp4.h"
 #include "xv_kernels.h"
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -401,29 +404,354 @@ void launch_tiles(const Fp4GemmArgs& a, hipStream_t stream) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// More rows than that are bound by the matrix units (200 rows of a 51200 x 5120
+// weight: 105 GFLOP against 139 MB), and x is worth sharing: a workgroup takes
+// 64 NT weight rows and up to 224 rows of x, eight waves as 2 halves of x by 4
+// of the weight, steps of 128 values along K double-buffered in LDS (x, codes,
+// scales by LDS-DMA).  Where that gives too few workgroups, K is split and a
+// second kernel adds the fp32 parts.
+struct Fp4TileArgs {
+  Fp4GemmArgs g;
+  float* parts;       // null: out is written
+  int64_t part_size;  // floats of a part: m x (rows of the weight)
+  int per;            // steps of a part
+};
+
+constexpr int kMaxM = 7;  // column tiles per wave at most: 2 x 7 x 16 rows of x fit LDS twice beside the weight
+
+// Codes and scale bytes of N row tiles; the scales of even and odd tiles have
+// their own address (gate and up rows need not start alike within a dword).
+template <int N>
+XV_INLINE void read_w(u32x4_t (&w)[N], uint32_t (&s)[N], uint32_t wa, uint32_t sa, uint32_t sb) {
+  if constexpr (N == 4) {
+    __asm__ __volatile__(
+        "ds_read_b128 %0, %8\n\t"
+        "ds_read_b128 %1, %8 offset:1024\n\t"
+        "ds_read_b128 %2, %8 offset:2048\n\t"
+        "ds_read_b128 %3, %8 offset:3072\n\t"
+        "ds_read_u8 %4, %9\n\t"
+        "ds_read_u8 %5, %10 offset:128\n\t"
+        "ds_read_u8 %6, %9 offset:256\n\t"
+        "ds_read_u8 %7, %10 offset:384\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+        : "v"(wa), "v"(sa), "v"(sb)
+        : "memory");
+  } else if constexpr (N == 2) {
+    __asm__ __volatile__(
+        "ds_read_b128 %0, %4\n\t"
+        "ds_read_b128 %1, %4 offset:1024\n\t"
+        "ds_read_u8 %2, %5\n\t"
+        "ds_read_u8 %3, %6 offset:128\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(s[0]), "=&v"(s[1])
+        : "v"(wa), "v"(sa), "v"(sb)
+        : "memory");
+  } else {
+    __asm__ __volatile__(
+        "ds_read_b128 %0, %2\n\t"
+        "ds_read_u8 %1, %3\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(w[0]), "=&v"(s[0])
+        : "v"(wa), "v"(sa)
+        : "memory");
+  }
+}
+
+// The operands of N column tiles (16 rows of 256 bytes apart) in one asm block with one wait.
+template <int N>
+XV_INLINE void read_xt(u32x4_t (&v)[kMaxM], uint32_t a) {
+  static_assert(N >= 2 && N <= kMaxM, "column tiles of a wave");
+#define XV_R(i) "ds_read_b128 %" #i ", %[a] offset:4096*" #i "\n\t"
+#define XV_O3 "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2])
+#define XV_END "s_waitcnt lgkmcnt(0)"
+  if constexpr (N == 2) __asm__ __volatile__(XV_R(0) XV_R(1) XV_END : "=&v"(v[0]), "=&v"(v[1]) : [a] "v"(a) : "memory");
+  else if constexpr (N == 3) __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_END : XV_O3 : [a] "v"(a) : "memory");
+  else if constexpr (N == 4)
+    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_END : XV_O3, "=&v"(v[3]) : [a] "v"(a) : "memory");
+  else if constexpr (N == 5)
+    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_R(4) XV_END
+                         : XV_O3, "=&v"(v[3]), "=&v"(v[4]) : [a] "v"(a) : "memory");
+  else if constexpr (N == 6)
+    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_R(4) XV_R(5) XV_END
+                         : XV_O3, "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]) : [a] "v"(a) : "memory");
+  else
+    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_R(4) XV_R(5) XV_R(6) XV_END
+                         : XV_O3, "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]) : [a] "v"(a) : "memory");
+#undef XV_R
+#undef XV_O3
+#undef XV_END
+}
+
+template <int NT, int MTW, bool SILU>
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_tile_kernel(Fp4TileArgs ta) {
+  const Fp4GemmArgs& a = ta.g;
+  constexpr int BM = 32 * MTW, BN = 64 * NT;
+  constexpr int kXB = BM * 256, kWB = BN * 64 + BN * 8;  // bytes of a step; scale rows have windows of two dwords
+  constexpr int kLds = 163840;
+  constexpr int DX = 3 * (kXB + kWB) <= kLds ? 3 : 2;    // steps of x in LDS, and of the weight
+  constexpr int DW = (kLds - DX * kXB) / kWB < 6 ? (kLds - DX * kXB) / kWB : 6;
+  static_assert(DW >= 2, "two steps of the weight");
+  // Waves 0 .. 3 fetch the weight, 4 .. 7 x: loads return in order within a
+  // wave, so that one that fetched both would wait for weight steps it does not
+  // need yet with every step of x.
+  constexpr int kXQ = BM / 16, kWQ = NT, kSQ = (NT + 1) / 2;  // LDS-DMA instructions of a wave and step
+  __shared__ __attribute__((aligned(16))) char lds[DX * kXB + DW * kWB];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int nw = wave & 3, mw = wave >> 2;
+  const int n0 = blockIdx.x * (SILU ? BN / 2 : BN), m0 = blockIdx.y * BM;
+  const int blocks = a.k / kFp4Block, steps = (a.k + 127) / 128;
+  const int s0 = blockIdx.z * ta.per, s1 = min(steps, s0 + ta.per);
+  // weight row of the workgroup's row R (SILU: 16 gate and 16 up rows of the same outputs in turn), clamped
+  auto wrow = [&](int R) {
+    const int t = R >> 4, o = min(n0 + (SILU ? t >> 1 : t) * 16 + (R & 15), a.n - 1);
+    return (int64_t)o + (SILU && (t & 1) ? a.n : 0);
+  };
+  const uintptr_t s_base = reinterpret_cast<uintptr_t>(a.s);
+  const uintptr_t s_last = (s_base + (uint64_t)((SILU ? 2 * (int64_t)a.n : a.n) - 1) * a.s_st + blocks - 1) & ~(uintptr_t)3;
+  // this lane's sources of its wave's instructions, at step 0
+  const bf16_t* xsrc[kXQ];
+  const uint8_t* wsrc[kWQ];
+  uintptr_t ssrc[kSQ];
+  auto xrow = [&](int q) { return 4 * (4 * q + nw) + (lane >> 4); };
+  auto wrow_of = [&](int q) { return 16 * (4 * q + nw) + (lane >> 2); };
+  auto srow_of = [&](int q) { return (32 * (4 * q + nw) + (lane >> 1)) % BN; };  // (64 rows: two waves repeat the others)
+  if (mw == 1) {
+#pragma unroll
+    for (int q = 0; q < kXQ; ++q)
+      xsrc[q] = a.x + (int64_t)min(m0 + xrow(q), a.m - 1) * a.x_st + 8 * ((lane & 15) ^ (xrow(q) & 15));
+  } else {
+#pragma unroll
+    for (int q = 0; q < kWQ; ++q)
+      wsrc[q] = a.w + wrow(wrow_of(q)) * a.w_st + 16 * ((lane & 3) ^ ((wrow_of(q) >> 2) & 3));
+#pragma unroll
+    for (int q = 0; q < kSQ; ++q) ssrc[q] = s_base + (uint64_t)(wrow(srow_of(q)) * a.s_st);
+  }
+  // Steps past the end of the range repeat its last: every call issues the same loads.
+  auto issue_x = [&](int s_at, int slot) {
+    const int s = min(s_at, s1 - 1);
+    const bool whole = 4 * (s + 1) <= blocks;
+#pragma unroll
+    for (int q = 0; q < kXQ; ++q) {
+      const int piece = (lane & 15) ^ (xrow(q) & 15);
+      const int back = whole ? 0 : max(0, 128 * s + 8 * piece - (a.k - 8));  // past the end: any valid piece (zeroed below)
+      __builtin_amdgcn_global_load_lds((global_cptr)(xsrc[q] + 128 * s - back), (lds_void*)(lds + slot * kXB + 1024 * (4 * q + nw)),
+                                       16, 0, 0);
+    }
+  };
+  auto issue_w = [&](int s_at, int slot) {
+    const int s = min(s_at, s1 - 1);
+    char* buf = lds + DX * kXB + slot * kWB;
+    const bool whole = 4 * (s + 1) <= blocks;
+#pragma unroll
+    for (int q = 0; q < kWQ; ++q) {
+      const int piece = (lane & 3) ^ ((wrow_of(q) >> 2) & 3);
+      const int back = whole ? 0 : max(0, 4 * s + piece - (blocks - 1));
+      __builtin_amdgcn_global_load_lds((global_cptr)(wsrc[q] + 64 * (int64_t)s - 16 * back), (lds_void*)(buf + 1024 * (4 * q + nw)),
+                                       16, 0, 0);
+    }
+#pragma unroll
+    for (int q = 0; q < kSQ; ++q) {
+      const uintptr_t src = min(((ssrc[q] + 4 * s) & ~(uintptr_t)3) + 4 * (lane & 1), s_last);
+      __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(buf + BN * 64 + (256 * (4 * q + nw)) % (BN * 8)), 4, 0, 0);
+    }
+  };
+  floatx4_t acc[NT][MTW];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int u = 0; u < MTW; ++u) acc[t][u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+  // where in its window a row's scale bytes start: the same 16 rows on, but not for gate and up rows
+  uint32_t mis[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) mis[t] = (uint32_t)((s_base + (uint64_t)(wrow((nw * NT + t) * 16 + i) * a.s_st)) & 3);
+  const uint32_t base = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+
+  auto step = [&](auto count, int s, int xslot, int wslot) {
+    constexpr int MU = decltype(count)::value;  // column tiles of this wave that hold rows of x
+    const uint32_t xb = base + xslot * kXB, wb = base + DX * kXB + wslot * kWB;
+    u32x4_t w[NT];
+    uint32_t sc[NT];
+    const uint32_t sa = wb + BN * 64 + (nw * NT * 16 + i) * 8 + g;
+    read_w<NT>(w, sc, wb + (nw * NT * 16 + i) * 64 + ((g ^ (i >> 2)) << 4), sa + mis[0], sa + mis[1]);
+    const bool in = 128 * s + 32 * g < a.k;  // whole blocks: a lane's 32 values lie inside or outside
+    const bool whole = 4 * (s + 1) <= blocks;
+    float f[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) f[t] = fp4_scale(in ? sc[t] : 0u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u32x4_t x[kMaxM];
+      read_xt<MU>(x, xb + (mw * MTW * 16 + i) * 256 + (((4 * g + j) ^ i) << 4));
+      if (!whole && !in) {
+#pragma unroll
+        for (int u = 0; u < MU; ++u) x[u] = u32x4_t{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const bf16x8_t av = widen8(w[t][j], f[t]);
+#pragma unroll
+        for (int u = 0; u < MU; ++u) {
+          bf16x8_t bv;
+          __builtin_memcpy(&bv, &x[u], 16);
+          acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, acc[t][u], 0, 0, 0);
+        }
+      }
+    }
+  };
+  auto run = [&](auto count) {
+    if (mw == 1) {
+#pragma unroll
+      for (int d = 0; d < DX - 1; ++d) issue_x(s0 + d, d);
+    } else {
+#pragma unroll
+      for (int d = 0; d < DW - 1; ++d) issue_w(s0 + d, d);
+    }
+    int xslot = 0, wslot = 0;
+    for (int s = s0; s < s1; ++s) {
+      // all but the later steps of what this wave fetches has arrived; nobody reads step s - 1 any more
+      if (mw == 1) wait_vm<(DX - 2) * kXQ>();
+      else wait_vm<(DW - 2) * (kWQ + kSQ)>();
+      __builtin_amdgcn_s_barrier();
+      if (mw == 1) issue_x(s + DX - 1, xslot == 0 ? DX - 1 : xslot - 1);
+      else issue_w(s + DW - 1, wslot == 0 ? DW - 1 : wslot - 1);
+      step(count, s, xslot, wslot);
+      if (++xslot == DX) xslot = 0;
+      if (++wslot == DW) wslot = 0;
+    }
+    wait_vm<0>();  // nothing still writes LDS when the workgroup ends
+  };
+  // the second half of the waves may have one column tile fewer
+  if (s0 < s1) {
+    if (m0 + (mw * MTW + MTW - 1) * 16 < a.m) run(std::integral_constant<int, MTW>{});
+    else run(std::integral_constant<int, MTW - 1>{});
+  }
+  // lane (g, i) of tile (t, u): weight rows 4g .. 4g + 3 of x row i
+#pragma unroll
+  for (int u = 0; u < MTW; ++u) {
+    const int m = m0 + (mw * MTW + u) * 16 + i;
+    if (m >= a.m) continue;
+#pragma unroll
+    for (int t = 0; t < NT; t += SILU ? 2 : 1) {
+      const int n = n0 + (SILU ? (nw * NT + t) >> 1 : nw * NT + t) * 16 + 4 * g;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (n + r >= a.n) continue;
+        if (ta.parts != nullptr) {
+          float* p = ta.parts + blockIdx.z * ta.part_size + (int64_t)m * (SILU ? 2 * a.n : a.n) + n + r;
+          p[0] = acc[t][u][r];
+          if constexpr (SILU) p[a.n] = acc[t + 1][u][r];
+        } else {
+          float v = acc[t][u][r];
+          if constexpr (SILU) v = silu_mul(v, acc[t + 1][u][r]);
+          a.out[(int64_t)m * a.out_st + n + r] = (bf16_t)f32_to_bf16(v);
+        }
+      }
+    }
+  }
+}
+
+// The sum of the parts of a split product, one output per thread.
 template <bool SILU>
-void dispatch(const Fp4GemmArgs& a, hipStream_t stream) {
+__global__ __launch_bounds__(256) void fp4_sum_kernel(Fp4TileArgs ta, int parts) {
+  const Fp4GemmArgs& a = ta.g;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(idx / a.n), n = (int)(idx - (int64_t)m * a.n);
+  if (m >= a.m) return;
+  const float* p = ta.parts + (int64_t)m * (SILU ? 2 * a.n : a.n) + n;
+  float v = 0.f, up = 0.f;
+  for (int z = 0; z < parts; ++z) {
+    v += p[z * ta.part_size];
+    if constexpr (SILU) up += p[z * ta.part_size + a.n];
+  }
+  a.out[(int64_t)m * a.out_st + n] = (bf16_t)f32_to_bf16(SILU ? silu_mul(v, up) : v);
+}
+
+// How a product of more than kShort rows is cut: column tiles per wave,
+// weight tiles per wave, parts of K.  The cheapest by cycles: a step costs its
+// matrix instructions (16 cycles each, two waves a SIMD) or its x through
+// LDS-DMA (64 bytes a cycle), a workgroup about 6000 more at its ends, parts
+// their second kernel and the traffic between.
+constexpr int kShort = 64;
+struct TilePlan { int mtw, nt, parts; };
+TilePlan tile_plan(int m, int rows, int k, bool silu) {
+  const int my = (m + 32 * kMaxM - 1) / (32 * kMaxM);
+  const int mtw = std::max(3, ((m + my - 1) / my + 31) / 32);  // 65 rows and more: at least 3, the last tile may be empty
+  const int steps = (k + 127) / 128, gy = (m + 32 * mtw - 1) / (32 * mtw);
+  TilePlan best = {mtw, 4, 1};
+  double cost = 1e300;
+  for (int nt : {4, 2, 1}) {
+    if (silu && nt == 1) continue;
+    for (int parts : {1, 2, 4, 8}) {
+      if (parts > 1 && steps / parts < 4) break;
+      const double groups = (double)((rows + 64 * nt - 1) / (64 * nt)) * gy * parts;
+      const double step = std::max(128.0 * nt * mtw, 128.0 * mtw) + 300.0;
+      double c = std::ceil(groups / 256) * ((steps + parts - 1) / parts * step + 6000.0);
+      if (parts > 1) c += 7000.0 + (double)parts * m * rows * 8.0 / 2000.0;
+      if (c < cost) { cost = c; best = {mtw, nt, parts}; }
+    }
+  }
+  return best;
+}
+
+template <int NT, bool SILU>
+void launch_tile(const Fp4TileArgs& ta, int mtw, dim3 grid, hipStream_t stream) {
+  switch (mtw) {
+    case 3: fp4_tile_kernel<NT, 3, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
+    case 4: fp4_tile_kernel<NT, 4, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
+    case 5: fp4_tile_kernel<NT, 5, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
+    case 6: fp4_tile_kernel<NT, 6, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
+    default: fp4_tile_kernel<NT, 7, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
+  }
+}
+
+template <bool SILU>
+void dispatch_tile(const Fp4GemmArgs& a, float* ws, hipStream_t stream) {
+  const int rows = SILU ? 2 * a.n : a.n, steps = (a.k + 127) / 128;
+  const TilePlan p = tile_plan(a.m, rows, a.k, SILU);
+  const Fp4TileArgs ta = {a, p.parts > 1 ? ws : nullptr, (int64_t)a.m * rows, (steps + p.parts - 1) / p.parts};
+  const dim3 grid((unsigned)((rows + 64 * p.nt - 1) / (64 * p.nt)), (unsigned)((a.m + 32 * p.mtw - 1) / (32 * p.mtw)),
+                  (unsigned)p.parts);
+  if (p.nt == 4) launch_tile<4, SILU>(ta, p.mtw, grid, stream);
+  else if (p.nt == 2) launch_tile<2, SILU>(ta, p.mtw, grid, stream);
+  else if constexpr (!SILU) launch_tile<1, SILU>(ta, p.mtw, grid, stream);
+  if (p.parts > 1)
+    fp4_sum_kernel<SILU><<<(unsigned)(((int64_t)a.m * a.n + 255) / 256), 256, 0, stream>>>(ta, p.parts);
+}
+
+template <bool SILU>
+void dispatch(const Fp4GemmArgs& a, float* ws, hipStream_t stream) {
   if (a.m <= 8) launch_tiles<1, 8, 256, 3, 256, SILU>(a, stream);
   else if (a.m <= 16) launch_tiles<1, 16, 128, 3, 256, SILU>(a, stream);
   else if (a.m <= 32) launch_tiles<2, 32, 128, 1, 128, SILU>(a, stream);
-  else launch_tiles<4, 64, 128, 1, 128, SILU>(a, stream);
+  else if (a.m <= kShort) launch_tiles<4, 64, 128, 1, 128, SILU>(a, stream);
+  else dispatch_tile<SILU>(a, ws, stream);
 }
 
 }  // namespace
 
+extern "C" size_t xv_mxfp4_gemm_workspace_size(int m, int n, int k, int silu_mul) {
+  if (m <= kShort || n <= 0 || k <= 0) return 0;
+  const int parts = tile_plan(m, n, k, silu_mul != 0).parts;
+  return parts > 1 ? (size_t)parts * m * n * sizeof(float) : 0;
+}
+
 extern "C" int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_stride, const void* w_scale,
                              int64_t scale_stride, void* out, int64_t out_stride, int m, int n, int k, int silu_mul,
-                             hipStream_t stream) {
+                             void* workspace, size_t workspace_bytes, hipStream_t stream) {
   if (m < 0 || n <= 0 || k <= 0 || k % kFp4Block || (silu_mul && n % 2)) return (int)hipErrorInvalidValue;
   if (!x || !w || !w_scale || !out || !xv_al16(x) || !xv_al16(w) || !xv_st8(x_stride) || w_stride & 15 ||
       (m > 1 && x_stride < k) || w_stride < k / 2 || scale_stride < k / kFp4Block || (uintptr_t)out & 1 ||
       (m > 1 && out_stride < (silu_mul ? n / 2 : n)))
     return (int)hipErrorInvalidValue;
-  if (m > 65535 * 16 || w_stride > (1 << 27) || scale_stride > (1 << 27)) return (int)hipErrorInvalidValue;  // 32-bit offsets
+  if (m > 65535 * 64 || w_stride > (1 << 27) || scale_stride > (1 << 27)) return (int)hipErrorInvalidValue;  // 32-bit offsets
   if (m == 0) return 0;
+  if (workspace_bytes < xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) || (uintptr_t)workspace & 15)
+    return (int)hipErrorInvalidValue;
   const Fp4GemmArgs a = {(const bf16_t*)x, x_stride, (const uint8_t*)w, w_stride, (const uint8_t*)w_scale, scale_stride,
                          (bf16_t*)out, out_stride, m, silu_mul ? n / 2 : n, k};
-  silu_mul ? dispatch<true>(a, stream) : dispatch<false>(a, stream);
+  silu_mul ? dispatch<true>(a, (float*)workspace, stream) : dispatch<false>(a, (float*)workspace, stream);
   XV_CHECK_LAUNCH();
   return 0;
 }

@@ -86,7 +86,8 @@ SIGNATURES: dict[str, tuple] = {
         [vp, i64, i64, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, vp, i64, vp, sz,
          i32, i32, i32, i32, i32, i32, f32, vp],
     ),
-    "xv_mxfp4_gemm": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp]),
+    "xv_mxfp4_gemm_workspace_size": (sz, [i32, i32, i32, i32]),
+    "xv_mxfp4_gemm": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, sz, vp]),
     "xv_silu_and_mul": (i32, [vp, i64, vp, i64, i64, i32, vp]),
     "xv_dense_gemm": (i32, [vp, i64, vp, vp, i64, i64, i32, i32, i32, i32, i32, i32, i32, vp]),
     "xv_stream_gemm_parts": (i32, [i32, i32, i32, i32]),

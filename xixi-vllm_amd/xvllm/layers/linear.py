@@ -355,6 +355,7 @@ def streamed_into_norm(x: torch.Tensor, w) -> PartialSums:
 
 def _mxfp4_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
     """mxfp4_linear on x [M, K], arguments checked."""
+    from .. import _C
     from .._torch_glue import call
 
     m, k = x.shape
@@ -366,8 +367,10 @@ def _mxfp4_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu
     cols = n // 2 if silu_mul else n
     out = torch.empty((m, cols), dtype=torch.bfloat16, device=x.device)
     if m and cols:
+        nbytes = _C.lib().xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) if m > STREAM_MAX_ROWS else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         call("xv_mxfp4_gemm", x.get_device(), x.data_ptr(), st, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
-             w_scale.stride(0), out.data_ptr(), cols, m, n, k, silu_mul)
+             w_scale.stride(0), out.data_ptr(), cols, m, n, k, silu_mul, None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
