@@ -113,8 +113,7 @@ XV_INLINE void advance(Fp4Cursor& c, const int* pref, const int* sl, int hkv, in
 }
 
 // LDS offsets of a lane within a unit, and of its 16-byte piece within a page
-// of codes.  Piece j of a row sits in piece j ^ (row / 4) of the row's 64
-// bytes: the 16 rows of a K read (one piece) then cover all banks once.
+// of codes.  Piece j of a row sits in slot j ^ swz4(row) of the row's 64 bytes.
 struct Fp4Lane {
   uint32_t g;      // global byte offset of this lane's piece of a 16-token page
   uint32_t k;      // K operand, row block 0 (block p: + 1024 p)
@@ -126,12 +125,12 @@ XV_INLINE Fp4Lane lane_offsets(uint32_t tok_stride, int lane) {
   Fp4Lane o;
   const int i = lane & 15, g = lane >> 4;
   const int row = lane >> 2;
-  o.g = row * tok_stride + (((lane & 3) ^ (row >> 2)) << 4);
-  o.k = (uint32_t)(64 * i + ((g ^ (i >> 2)) << 4));
+  o.g = row * tok_stride + (((lane & 3) ^ swz4(row)) << 4);
+  o.k = (uint32_t)(64 * i + ((g ^ swz4(i)) << 4));
   // input lane L of group g addresses token 16 (L / 4) + 4g + L % 4: output nibble L
 #pragma unroll
   for (int m = 0; m < 4; ++m)
-    o.v[m] = (uint32_t)(kVOff + 1024 * (i >> 2) + 64 * (4 * g + (i & 3)) + ((m ^ g) << 4));
+    o.v[m] = (uint32_t)(kVOff + 1024 * (i >> 2) + 64 * (4 * g + (i & 3)) + ((m ^ swz4(4 * g)) << 4));
   o.ks = (uint32_t)(kKsOff + 4 * i);
   o.vs = (uint32_t)(kVsOff + 16 * g);
   return o;

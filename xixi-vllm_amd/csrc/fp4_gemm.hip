@@ -9,14 +9,17 @@
 // conversion (one instruction per pair, exact); operand B is x, column = row
 // of x, the same values.
 //
-// A workgroup owns T tiles of 16 weight rows, its eight waves take turns of KS
-// values along K (their fp32 sums meet in LDS at the end), and a wave runs its T tiles
-// over one slice before the next: x is read once per workgroup and its slice
-// waits in registers, while the weight streams through a private LDS ring.
-// Both travel by LDS-DMA, whole row segments per instruction.  Direct loads into the
-// operand registers, where neighbouring lanes are neighbouring rows, were
-// bound by the address unit instead (weights so: a gate / up weight of 24576 x
-// 4096 at one row 22 us; x alone so: 8 rows through 4096 x 12288 12.7 us).
+// Up to kShort rows: a workgroup owns T tiles of 16 weight rows, its eight
+// waves take turns of KS values along K (their fp32 sums meet in LDS at the
+// end), and a wave runs its T tiles over one slice before the next: x is read
+// once per workgroup and its slice waits in registers, while the weight streams
+// through a private LDS ring.  Both travel by LDS-DMA, whole row segments per
+// instruction.  One row through a gate / up weight of 24576 x 4096 takes 12.1 us
+// (4.4 TB/s), 8 rows through 4096 x 12288 9.6 us.  Direct loads into the operand
+// registers, where neighbouring lanes are neighbouring rows, were bound by the
+// address unit (weights so: 22 us for the first; x alone so: 12.7 us for the
+// second).  Every workgroup reads all of x, so that 64 rows of a weight of few
+// rows are bound by L2 (64 through 4096 x 12288: 400 MB in 23 us).
 #include "xv_decode.h"
 #include "xv_fp4.h"
 #include "xv_kernels.h"
@@ -50,44 +53,41 @@ constexpr int kWaves = 8;
 constexpr int kDepth = 3;  // stages in a wave's ring, kDepth - 1 of them in flight
 
 // One stage: 16 weight rows x KS values.  LDS image: the rows' codes (KS / 2
-// bytes each, 16-byte piece j in slot j ^ (row * pieces / 16): the 16 rows of
-// an operand read cover all banks once), then a window of SW dwords of each row's
-// scale bytes.  A scale row need not start at a multiple of 4 bytes
-// (WIDE): the window then starts at the dword that holds the first byte.
+// bytes each, swizzled), then a window of SW dwords of each row's scale bytes.
+// A scale row need not start at a multiple of 4 bytes (WIDE): the window then
+// starts at the dword that holds the first byte.
 template <int KS, bool WIDE>
 struct Stage {
   static constexpr int kPieces = KS / 32;               // 16-byte pieces (scale blocks) of a row
   static constexpr int kCodes = 16 * KS / 2;
   static constexpr int kLoads = kCodes / 1024;          // LDS-DMA instructions of the codes
   static constexpr int kRowsPer = 64 / kPieces;         // rows one of them covers
-  static constexpr int SW = !WIDE ? KS / 128 : KS == 512 ? 8 : KS / 64;
+  static constexpr int SW = !WIDE ? KS / 128 : KS / 64;
   static constexpr int kScaleLoads = (16 * SW + 63) / 64;
   static constexpr int kBytes = kCodes + kScaleLoads * 256;
   static constexpr int kOps = kLoads + kScaleLoads;
   static constexpr int kSteps = KS / 128;               // operand loads of 128 values
+  static XV_INLINE int swz(int row) {
+    static_assert(KS == 128 || KS == 256, "rows of 64 or 128 bytes");
+    return KS == 128 ? swz4(row) : swz8p(row);
+  }
 };
 
-// Pieces of 128 values each from the stage's image (address `a`, the lane's
-// pieces at a ^ (64 * step), see below) and their scale bytes, once at most VM
-// vector-memory operations are outstanding: one asm block with one wait.
+// Where piece j of x row r sits in LDS: slot j ^ swz_x(r).  Eight rows serve
+// all sixteen lanes of a group; bit 2, where neighbouring groups' pieces
+// differ, stays free.
+template <int XR>
+XV_INLINE int swz_x(int r) {
+  return XR == 8 ? (r & 3) | ((r & 4) << 1) : swz16(r);
+}
+
+// A stage's operands of the lane, one piece of codes (at wa) and one scale byte
+// (sa, 4 bytes on) for each 128 values, once at most VM vector-memory
+// operations are outstanding: one asm block with one wait.
 template <int N, int VM>
 XV_INLINE void read_stage(u32x4_t (&w)[N], uint32_t (&s)[N], const uint32_t (&wa)[N], uint32_t sa) {
-  if constexpr (N == 4) {
-    __asm__ __volatile__(
-        "s_waitcnt vmcnt(%13)\n\t"
-        "ds_read_b128 %0, %8\n\t"
-        "ds_read_b128 %1, %9\n\t"
-        "ds_read_b128 %2, %10\n\t"
-        "ds_read_b128 %3, %11\n\t"
-        "ds_read_u8 %4, %12\n\t"
-        "ds_read_u8 %5, %12 offset:4\n\t"
-        "ds_read_u8 %6, %12 offset:8\n\t"
-        "ds_read_u8 %7, %12 offset:12\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
-        : "v"(wa[0]), "v"(wa[1]), "v"(wa[2]), "v"(wa[3]), "v"(sa), "n"(VM)
-        : "memory");
-  } else if constexpr (N == 2) {
+  static_assert(N == 1 || N == 2, "slices of 128 or 256 values");
+  if constexpr (N == 2) {
     __asm__ __volatile__(
         "s_waitcnt vmcnt(%7)\n\t"
         "ds_read_b128 %0, %4\n\t"
@@ -110,7 +110,7 @@ XV_INLINE void read_stage(u32x4_t (&w)[N], uint32_t (&s)[N], const uint32_t (&wa
   }
 }
 
-// Eight operand reads of x (pairs of 4, `b` apart) in one asm block with one wait.
+// Eight operand reads of x in one asm block with one wait.
 XV_INLINE void read_x8(u32x4_t (&v)[8], const uint32_t (&at)[8]) {
   __asm__ __volatile__(
       "ds_read_b128 %0, %8\n\t"
@@ -132,19 +132,23 @@ XV_INLINE void wait_vm() {
   __asm__ __volatile__("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// MT column tiles of 16 rows of x, XR of them fetched (8: the tile's upper
-// half repeats the lower, its outputs are not stored); XD slices of x in LDS.
+// m <= XR rows of x as MT column tiles of 16 (XR = 8: the tile's upper half
+// repeats the lower, its outputs are not stored); XD slices of x in LDS.
 template <int MT, int XR, int KS, int XD, int T, bool SILU, bool WIDE>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_gemm_kernel(Fp4GemmArgs a) {
   using S = Stage<KS, WIDE>;
   constexpr int kXBytes = XR * KS * 2, kXLoads = kXBytes / 1024, kXPieces = KS / 8;
   constexpr int kWave = kDepth * S::kBytes + XD * kXBytes;  // LDS of one wave
+  // Weight loads are non-temporal where a wave runs through whole 128-byte lines of several tiles (one row of a 24576 x
+  // 4096 weight 12.1 us against 13.0), not where two waves share a line (64 rows through 4096 x 12288 22.9 against 29.2)
+  // or the workgroup has one tile (8 rows through it 9.5 against 11.1).
+  constexpr int kPolicy = KS == 256 && T > 2 ? kNontemporal : 0;
   constexpr int TR = SILU ? 2 : 1;                          // tiles summed over the waves at a time
   constexpr int kRed = kWaves * TR * MT * 1024;
   static_assert(kXLoads >= 1 && kWaves * kWave <= 163840 && kRed <= 163840, "LDS of a CU");
   __shared__ __attribute__((aligned(16))) char lds[kWaves * kWave > kRed ? kWaves * kWave : kRed];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * (SILU ? T / 2 : T) * 16, m0 = blockIdx.y * (MT * 16);
+  const int n0 = blockIdx.x * (SILU ? T / 2 : T) * 16;
   char* const ring = lds + wave * kWave;
   char* const xring = ring + kDepth * S::kBytes;
   const int blocks = a.k / kFp4Block;
@@ -164,7 +168,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
   for (int q = 0; q < S::kLoads; ++q) {
     const int row = S::kRowsPer * q + lane / S::kPieces;
-    coff[q] = row * (uint32_t)a.w_st + 16 * ((lane % S::kPieces) ^ ((row * S::kPieces) >> 4));
+    coff[q] = row * (uint32_t)a.w_st + 16 * ((lane % S::kPieces) ^ S::swz(row));
   }
 #pragma unroll
   for (int q = 0; q < S::kScaleLoads; ++q) {
@@ -189,15 +193,15 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
       const uint8_t* src = a.w + row0 * a.w_st + 16 * (int64_t)b0;
 #pragma unroll
       for (int q = 0; q < S::kLoads; ++q)
-        __builtin_amdgcn_global_load_lds((global_cptr)(src + coff[q]), (lds_void*)(buf + 1024 * q), 16, 0, kNontemporal);
+        __builtin_amdgcn_global_load_lds((global_cptr)(src + coff[q]), (lds_void*)(buf + 1024 * q), 16, 0, kPolicy);
     } else {
 #pragma unroll
       for (int q = 0; q < S::kLoads; ++q) {
         const int row = S::kRowsPer * q + lane / S::kPieces;
-        const int piece = (lane % S::kPieces) ^ ((row * S::kPieces) >> 4);
+        const int piece = (lane % S::kPieces) ^ S::swz(row);
         // rows and blocks past the end: valid ones (not stored, and their x is zero)
         const uint8_t* src = a.w + wrow(it, row) * a.w_st + 16 * (int64_t)min(b0 + piece, blocks - 1);
-        __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(buf + 1024 * q), 16, 0, kNontemporal);
+        __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(buf + 1024 * q), 16, 0, kPolicy);
       }
     }
     if (whole && !WIDE) {
@@ -222,13 +226,13 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
       is += kWaves;
     }
   };
-  // Slice `slice` of x: row r's KS values (2 KS bytes, 16-byte piece j in slot j ^ (r % 16)) at r * 2 KS.
+  // Slice `slice` of x: row r's KS values (2 KS bytes, swizzled) at r * 2 KS.
   auto issue_x = [&](int slice, int slot) {
 #pragma unroll
     for (int q = 0; q < kXLoads; ++q) {
-      const int at = 64 * q + lane, row = at / kXPieces, piece = (at % kXPieces) ^ (row & 15);
+      const int at = 64 * q + lane, row = at / kXPieces, piece = (at % kXPieces) ^ swz_x<XR>(row);
       const int k = min(slice * KS + 8 * piece, a.k - 8);  // past the end: any valid piece (zeroed below)
-      const bf16_t* src = a.x + (int64_t)min(m0 + row, a.m - 1) * a.x_st + k;
+      const bf16_t* src = a.x + (int64_t)min(row, a.m - 1) * a.x_st + k;
       __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(xring + slot * kXBytes + 1024 * q), 16, 0, 0);
     }
     ops += kXLoads;
@@ -247,7 +251,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
       for (int e = 0; e < 8; ++e) {
         const int pe = min(p + (e >> 2), S::kSteps * MT - 1), h = pe / MT, u = pe % MT;
         const int row = (16 * u + i) % XR;
-        at[e] = b + row * (KS * 2) + (((16 * h + 4 * g + (e & 3)) ^ (row & 15)) << 4);
+        at[e] = b + row * (KS * 2) + (((16 * h + 4 * g + (e & 3)) ^ swz_x<XR>(row)) << 4);
       }
       read_x8(v, at);
 #pragma unroll
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   uint32_t wat[S::kSteps];
 #pragma unroll
   for (int h = 0; h < S::kSteps; ++h)
-    wat[h] = (uint32_t)(i * (KS / 2) + (((4 * h + g) ^ ((i * S::kPieces) >> 4)) << 4));
+    wat[h] = (uint32_t)(i * (KS / 2) + (((4 * h + g) ^ S::swz(i)) << 4));
   int wslot = 0, xslot = 0;  // ring slots of the next stage and slice to use
   if (mine > 0) {
 #pragma unroll
@@ -355,14 +359,14 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
       const int o = e & 15, m = e >> 4;  // output within the tile, x row
       const int at = (m >> 4) * 256 + (o >> 2) * 64 + (m & 15) * 4 + (o & 3);
       const int n = n0 + (t0 / TR) * 16 + o;
-      if (n >= a.n || m0 + m >= a.m) continue;
+      if (n >= a.n || m >= a.m) continue;
       float v = 0.f, up = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         v += red[(w * TR * MT) * 256 + at];
         if constexpr (SILU) up += red[((w * TR + 1) * MT) * 256 + at];
       }
-      a.out[(int64_t)(m0 + m) * a.out_st + n] = (bf16_t)f32_to_bf16(SILU ? silu_mul(v, up) : v);
+      a.out[(int64_t)m * a.out_st + n] = (bf16_t)f32_to_bf16(SILU ? silu_mul(v, up) : v);
     }
   }
 }
@@ -370,7 +374,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 template <int MT, int XR, int KS, int XD, int T, bool SILU>
 void launch(const Fp4GemmArgs& a, hipStream_t stream) {
   constexpr int outs = (SILU ? T / 2 : T) * 16;
-  const dim3 grid((unsigned)((a.n + outs - 1) / outs), (unsigned)((a.m + MT * 16 - 1) / (MT * 16)));
+  const dim3 grid((unsigned)((a.n + outs - 1) / outs));
   // scale rows that start at multiples of 4 bytes have narrower windows
   if (((uintptr_t)a.s | (uint64_t)a.s_st) & 3) fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, true><<<grid, kWaves * 64, 0, stream>>>(a);
   else fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, false><<<grid, kWaves * 64, 0, stream>>>(a);
@@ -408,9 +412,17 @@ void launch_tiles(const Fp4GemmArgs& a, hipStream_t stream) {
 // More rows than that are bound by the matrix units (200 rows of a 51200 x 5120
 // weight: 105 GFLOP against 139 MB), and x is worth sharing: a workgroup takes
 // 64 NT weight rows and up to 224 rows of x, eight waves as 2 halves of x by 4
-// of the weight, steps of 128 values along K double-buffered in LDS (x, codes,
-// scales by LDS-DMA).  Where that gives too few workgroups, K is split and a
-// second kernel adds the fp32 parts.
+// of the weight.  Along K the weight comes in steps of 128 values (whole
+// 64-byte pieces of its rows), several of them ahead since they come from HBM;
+// x, from L2, in half steps, so that the LDS it leaves holds those.  The two
+// halves of the waves, one of each on every SIMD, take turns: between two
+// barriers one reads its operands and then runs its products, the other runs
+// the products of what it read before and then reads, so that the matrix units
+// and LDS work at once: 200 rows of a 51200 x 5120 weight in 119 us, 880
+// TFLOP/s.  (All waves in step, reading and multiplying together, 129 us.  The
+// products alone take 79, the loads and reads alone 84.  Weight loads are not
+// non-temporal: a step takes half a line, and 133 us then.)  Where the tiles give too few workgroups, K is split
+// and a second kernel adds the fp32 parts.
 struct Fp4TileArgs {
   Fp4GemmArgs g;
   float* parts;       // null: out is written
@@ -418,85 +430,65 @@ struct Fp4TileArgs {
   int per;            // steps of a part
 };
 
-constexpr int kMaxM = 7;  // column tiles per wave at most: 2 x 7 x 16 rows of x fit LDS twice beside the weight
+constexpr int kMaxM = 7;  // column tiles per wave at most (224 rows of x)
 
-// Codes and scale bytes of N row tiles; the scales of even and odd tiles have
-// their own address (gate and up rows need not start alike within a dword).
-template <int N>
-XV_INLINE void read_w(u32x4_t (&w)[N], uint32_t (&s)[N], uint32_t wa, uint32_t sa, uint32_t sb) {
-  if constexpr (N == 4) {
-    __asm__ __volatile__(
-        "ds_read_b128 %0, %8\n\t"
-        "ds_read_b128 %1, %8 offset:1024\n\t"
-        "ds_read_b128 %2, %8 offset:2048\n\t"
-        "ds_read_b128 %3, %8 offset:3072\n\t"
-        "ds_read_u8 %4, %9\n\t"
-        "ds_read_u8 %5, %10 offset:128\n\t"
-        "ds_read_u8 %6, %9 offset:256\n\t"
-        "ds_read_u8 %7, %10 offset:384\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
-        : "v"(wa), "v"(sa), "v"(sb)
-        : "memory");
-  } else if constexpr (N == 2) {
-    __asm__ __volatile__(
-        "ds_read_b128 %0, %4\n\t"
-        "ds_read_b128 %1, %4 offset:1024\n\t"
-        "ds_read_u8 %2, %5\n\t"
-        "ds_read_u8 %3, %6 offset:128\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(s[0]), "=&v"(s[1])
-        : "v"(wa), "v"(sa), "v"(sb)
-        : "memory");
-  } else {
-    __asm__ __volatile__(
-        "ds_read_b128 %0, %2\n\t"
-        "ds_read_u8 %1, %3\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(w[0]), "=&v"(s[0])
-        : "v"(wa), "v"(sa)
-        : "memory");
+// The operands of a half step in one asm block with one wait: of N column
+// tiles (16 rows of 128 bytes apart) both substeps, of NT row tiles (16 rows of
+// 64 bytes apart) two words of codes and the scale byte.  The scales of even and
+// odd tiles have their own address: gate and up rows need not start alike
+// within a dword.
+#define XV_XR(j, u) "ds_read_b128 %[x" #j #u "], %[a" #j "] offset:2048*" #u "\n\t"
+#define XV_XO(j, u) [x##j##u] "=&v"(x[j][u])
+#define XV_XR2 XV_XR(0, 0) XV_XR(0, 1) XV_XR(1, 0) XV_XR(1, 1)
+#define XV_XO2 XV_XO(0, 0), XV_XO(0, 1), XV_XO(1, 0), XV_XO(1, 1)
+#define XV_XR3 XV_XR2 XV_XR(0, 2) XV_XR(1, 2)
+#define XV_XO3 XV_XO2, XV_XO(0, 2), XV_XO(1, 2)
+#define XV_XR4 XV_XR3 XV_XR(0, 3) XV_XR(1, 3)
+#define XV_XO4 XV_XO3, XV_XO(0, 3), XV_XO(1, 3)
+#define XV_XR5 XV_XR4 XV_XR(0, 4) XV_XR(1, 4)
+#define XV_XO5 XV_XO4, XV_XO(0, 4), XV_XO(1, 4)
+#define XV_XR6 XV_XR5 XV_XR(0, 5) XV_XR(1, 5)
+#define XV_XO6 XV_XO5, XV_XO(0, 5), XV_XO(1, 5)
+#define XV_XR7 XV_XR6 XV_XR(0, 6) XV_XR(1, 6)
+#define XV_XO7 XV_XO6, XV_XO(0, 6), XV_XO(1, 6)
+#define XV_WR(t, e) "ds_read_b64 %[w" #t "], %[wa] offset:1024*" #t "\n\t" "ds_read_u8 %[s" #t "], %[s" #e "a] offset:128*" #t "\n\t"
+#define XV_WO(t) [w##t] "=&v"(w[t]), [s##t] "=&v"(s[t])
+#define XV_WR1 XV_WR(0, 0)
+#define XV_WO1 XV_WO(0)
+#define XV_WR2 XV_WR1 XV_WR(1, 1)
+#define XV_WO2 XV_WO1, XV_WO(1)
+#define XV_WR4 XV_WR2 XV_WR(2, 0) XV_WR(3, 1)
+#define XV_WO4 XV_WO2, XV_WO(2), XV_WO(3)
+#define XV_HALF(N, T)                                                                                               \
+  if constexpr (MU == N && NT == T) {                                                                               \
+    __asm__ __volatile__(XV_WR##T XV_XR##N "s_waitcnt lgkmcnt(0)"                                                   \
+                         : XV_WO##T, XV_XO##N                                                                       \
+                         : [wa] "v"(wa), [s0a] "v"(sa0), [s1a] "v"(sa1), [a0] "v"(xa[0]), [a1] "v"(xa[1])           \
+                         : "memory");                                                                               \
   }
-}
-
-// The operands of N column tiles (16 rows of 256 bytes apart) in one asm block with one wait.
-template <int N>
-XV_INLINE void read_xt(u32x4_t (&v)[kMaxM], uint32_t a) {
-  static_assert(N >= 2 && N <= kMaxM, "column tiles of a wave");
-#define XV_R(i) "ds_read_b128 %" #i ", %[a] offset:4096*" #i "\n\t"
-#define XV_O3 "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2])
-#define XV_END "s_waitcnt lgkmcnt(0)"
-  if constexpr (N == 2) __asm__ __volatile__(XV_R(0) XV_R(1) XV_END : "=&v"(v[0]), "=&v"(v[1]) : [a] "v"(a) : "memory");
-  else if constexpr (N == 3) __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_END : XV_O3 : [a] "v"(a) : "memory");
-  else if constexpr (N == 4)
-    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_END : XV_O3, "=&v"(v[3]) : [a] "v"(a) : "memory");
-  else if constexpr (N == 5)
-    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_R(4) XV_END
-                         : XV_O3, "=&v"(v[3]), "=&v"(v[4]) : [a] "v"(a) : "memory");
-  else if constexpr (N == 6)
-    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_R(4) XV_R(5) XV_END
-                         : XV_O3, "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]) : [a] "v"(a) : "memory");
-  else
-    __asm__ __volatile__(XV_R(0) XV_R(1) XV_R(2) XV_R(3) XV_R(4) XV_R(5) XV_R(6) XV_END
-                         : XV_O3, "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]) : [a] "v"(a) : "memory");
-#undef XV_R
-#undef XV_O3
-#undef XV_END
+#define XV_HALVES(N) XV_HALF(N, 1) XV_HALF(N, 2) XV_HALF(N, 4)
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <int MU, int NT>
+XV_INLINE void read_half(u32x4_t (&x)[2][MU], u32x2_t (&w)[NT], uint32_t (&s)[NT], const uint32_t (&xa)[2], uint32_t wa,
+                         uint32_t sa0, uint32_t sa1) {
+  static_assert(MU >= 2 && MU <= kMaxM && (NT == 1 || NT == 2 || NT == 4), "tiles of a wave");
+  XV_HALVES(2) XV_HALVES(3) XV_HALVES(4) XV_HALVES(5) XV_HALVES(6) XV_HALVES(7)
 }
 
 template <int NT, int MTW, bool SILU>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_tile_kernel(Fp4TileArgs ta) {
   const Fp4GemmArgs& a = ta.g;
   constexpr int BM = 32 * MTW, BN = 64 * NT;
-  constexpr int kXB = BM * 256, kWB = BN * 64 + BN * 8;  // bytes of a step; scale rows have windows of two dwords
+  constexpr int kXB = BM * 128;                // bytes of a half step of x
+  constexpr int kWB = BN * 64 + BN * 8;        // of a step of the weight; scale rows have windows of two dwords
   constexpr int kLds = 163840;
-  constexpr int DX = 3 * (kXB + kWB) <= kLds ? 3 : 2;    // steps of x in LDS, and of the weight
-  constexpr int DW = (kLds - DX * kXB) / kWB < 6 ? (kLds - DX * kXB) / kWB : 6;
-  static_assert(DW >= 2, "two steps of the weight");
+  constexpr int DX = MTW <= 5 ? 4 : 3;         // half steps of x in LDS, and steps of the weight
+  constexpr int DW = (kLds - DX * kXB) / kWB < 8 ? (kLds - DX * kXB) / kWB : 8;
+  static_assert(DW >= 3, "two steps of the weight in flight");
   // Waves 0 .. 3 fetch the weight, 4 .. 7 x: loads return in order within a
-  // wave, so that one that fetched both would wait for weight steps it does not
-  // need yet with every step of x.
-  constexpr int kXQ = BM / 16, kWQ = NT, kSQ = (NT + 1) / 2;  // LDS-DMA instructions of a wave and step
+  // wave, so that one that fetched both would wait with every half step of x for
+  // weight steps it does not need yet.
+  constexpr int kXQ = MTW, kWQ = NT, kSQ = (NT + 1) / 2;  // LDS-DMA instructions of a wave and half step, or step
   __shared__ __attribute__((aligned(16))) char lds[DX * kXB + DW * kWB];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int nw = wave & 3, mw = wave >> 2;
@@ -510,124 +502,166 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   };
   const uintptr_t s_base = reinterpret_cast<uintptr_t>(a.s);
   const uintptr_t s_last = (s_base + (uint64_t)((SILU ? 2 * (int64_t)a.n : a.n) - 1) * a.s_st + blocks - 1) & ~(uintptr_t)3;
-  // this lane's sources of its wave's instructions, at step 0
-  const bf16_t* xsrc[kXQ];
-  const uint8_t* wsrc[kWQ];
-  uintptr_t ssrc[kSQ];
-  auto xrow = [&](int q) { return 4 * (4 * q + nw) + (lane >> 4); };
-  auto wrow_of = [&](int q) { return 16 * (4 * q + nw) + (lane >> 2); };
-  auto srow_of = [&](int q) { return (32 * (4 * q + nw) + (lane >> 1)) % BN; };  // (64 rows: two waves repeat the others)
-  if (mw == 1) {
-#pragma unroll
-    for (int q = 0; q < kXQ; ++q)
-      xsrc[q] = a.x + (int64_t)min(m0 + xrow(q), a.m - 1) * a.x_st + 8 * ((lane & 15) ^ (xrow(q) & 15));
-  } else {
-#pragma unroll
-    for (int q = 0; q < kWQ; ++q)
-      wsrc[q] = a.w + wrow(wrow_of(q)) * a.w_st + 16 * ((lane & 3) ^ ((wrow_of(q) >> 2) & 3));
-#pragma unroll
-    for (int q = 0; q < kSQ; ++q) ssrc[q] = s_base + (uint64_t)(wrow(srow_of(q)) * a.s_st);
-  }
-  // Steps past the end of the range repeat its last: every call issues the same loads.
-  auto issue_x = [&](int s_at, int slot) {
-    const int s = min(s_at, s1 - 1);
-    const bool whole = 4 * (s + 1) <= blocks;
-#pragma unroll
-    for (int q = 0; q < kXQ; ++q) {
-      const int piece = (lane & 15) ^ (xrow(q) & 15);
-      const int back = whole ? 0 : max(0, 128 * s + 8 * piece - (a.k - 8));  // past the end: any valid piece (zeroed below)
-      __builtin_amdgcn_global_load_lds((global_cptr)(xsrc[q] + 128 * s - back), (lds_void*)(lds + slot * kXB + 1024 * (4 * q + nw)),
-                                       16, 0, 0);
-    }
-  };
-  auto issue_w = [&](int s_at, int slot) {
-    const int s = min(s_at, s1 - 1);
-    char* buf = lds + DX * kXB + slot * kWB;
-    const bool whole = 4 * (s + 1) <= blocks;
-#pragma unroll
-    for (int q = 0; q < kWQ; ++q) {
-      const int piece = (lane & 3) ^ ((wrow_of(q) >> 2) & 3);
-      const int back = whole ? 0 : max(0, 4 * s + piece - (blocks - 1));
-      __builtin_amdgcn_global_load_lds((global_cptr)(wsrc[q] + 64 * (int64_t)s - 16 * back), (lds_void*)(buf + 1024 * (4 * q + nw)),
-                                       16, 0, 0);
-    }
-#pragma unroll
-    for (int q = 0; q < kSQ; ++q) {
-      const uintptr_t src = min(((ssrc[q] + 4 * s) & ~(uintptr_t)3) + 4 * (lane & 1), s_last);
-      __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(buf + BN * 64 + (256 * (4 * q + nw)) % (BN * 8)), 4, 0, 0);
-    }
-  };
+  const uint32_t base = (uint32_t)reinterpret_cast<uintptr_t>(lds), wbase = base + DX * kXB;
   floatx4_t acc[NT][MTW];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int u = 0; u < MTW; ++u) acc[t][u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
-  // where in its window a row's scale bytes start: the same 16 rows on, but not for gate and up rows
-  uint32_t mis[2];
+  // this lane's operands within the buffers; a row's scale bytes start where in its window: the same 16 rows
+  // on, but not for gate and up rows
+  const uint32_t xoff[2] = {(uint32_t)((mw * MTW * 16 + i) * 128 + (((2 * g) ^ swz8p(i)) << 4)),
+                            (uint32_t)((mw * MTW * 16 + i) * 128 + (((2 * g + 1) ^ swz8p(i)) << 4))};
+  uint32_t soff[2], woff[2];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) mis[t] = (uint32_t)((s_base + (uint64_t)(wrow((nw * NT + t) * 16 + i) * a.s_st)) & 3);
-  const uint32_t base = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+  for (int t = 0; t < 2; ++t) {
+    soff[t] = (uint32_t)(BN * 64 + (nw * NT * 16 + i) * 8 + (g >> 1)) +
+              (uint32_t)((s_base + (uint64_t)(wrow((nw * NT + t) * 16 + i) * a.s_st)) & 3);
+    woff[t] = (uint32_t)((nw * NT * 16 + i) * 64 + (((2 * t + (g >> 1)) ^ swz4(i)) << 4) + 8 * (g & 1));  // half step t
+  }
 
-  auto step = [&](auto count, int s, int xslot, int wslot) {
-    constexpr int MU = decltype(count)::value;  // column tiles of this wave that hold rows of x
-    const uint32_t xb = base + xslot * kXB, wb = base + DX * kXB + wslot * kWB;
-    u32x4_t w[NT];
-    uint32_t sc[NT];
-    const uint32_t sa = wb + BN * 64 + (nw * NT * 16 + i) * 8 + g;
-    read_w<NT>(w, sc, wb + (nw * NT * 16 + i) * 64 + ((g ^ (i >> 2)) << 4), sa + mis[0], sa + mis[1]);
-    const bool in = 128 * s + 32 * g < a.k;  // whole blocks: a lane's 32 values lie inside or outside
-    const bool whole = 4 * (s + 1) <= blocks;
-    float f[NT];
+  // Half step 2s + H: lane (g, i) takes values 16g .. + 15 of its row, half of scale block 2 H + g / 2.
+  auto read = [&](auto count, auto parity, u32x4_t (&x)[2][decltype(count)::value], u32x2_t (&w)[NT], uint32_t (&sc)[NT], int s,
+                  int xslot, int wslot) {
+    constexpr int MU = decltype(count)::value, H = decltype(parity)::value;
+    const uint32_t xb = base + xslot * kXB, wb = wbase + wslot * kWB;
+    const uint32_t xa[2] = {xb + xoff[0], xb + xoff[1]};
+    read_half<MU, NT>(x, w, sc, xa, wb + woff[H], wb + soff[0] + 2 * H, wb + soff[1] + 2 * H);
+    if (128 * s + 64 * (H + 1) > a.k) {  // the last half steps: blocks past the end
+      if (128 * s + 64 * H + 16 * g >= a.k) {  // whole blocks: a lane's 16 values lie inside or outside
 #pragma unroll
-    for (int t = 0; t < NT; ++t) f[t] = fp4_scale(in ? sc[t] : 0u);
+        for (int u = 0; u < MU; ++u) { x[0][u] = u32x4_t{0, 0, 0, 0}; x[1][u] = u32x4_t{0, 0, 0, 0}; }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      u32x4_t x[kMaxM];
-      read_xt<MU>(x, xb + (mw * MTW * 16 + i) * 256 + (((4 * g + j) ^ i) << 4));
-      if (!whole && !in) {
-#pragma unroll
-        for (int u = 0; u < MU; ++u) x[u] = u32x4_t{0, 0, 0, 0};
+        for (int t = 0; t < NT; ++t) sc[t] = 0u;  // keeps the products with x = 0 finite
       }
+    }
+  };
+  auto multiply = [&](auto count, const u32x4_t (&x)[2][decltype(count)::value], const u32x2_t (&w)[NT], const uint32_t (&sc)[NT]) {
+    constexpr int MU = decltype(count)::value;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const bf16x8_t av = widen8(w[t][j], f[t]);
+        const bf16x8_t av = widen8(w[t][j], fp4_scale(sc[t]));
 #pragma unroll
         for (int u = 0; u < MU; ++u) {
           bf16x8_t bv;
-          __builtin_memcpy(&bv, &x[u], 16);
+          __builtin_memcpy(&bv, &x[j][u], 16);
           acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, acc[t][u], 0, 0, 0);
         }
       }
-    }
   };
-  auto run = [&](auto count) {
-    if (mw == 1) {
+  const std::integral_constant<int, 0> even{};
+  const std::integral_constant<int, 1> odd{};
+  // Every step has two barriers: past one, what its half step reads has arrived and nobody reads the half step
+  // before any more.  Loads of steps past the end of the range repeat its last: every step issues the same.
+
+  // Waves 0 .. 3: fetch the weight; read, then multiply.
+  auto run_w = [&](auto count) {
+    constexpr int MU = decltype(count)::value;
+    const int wr = lane >> 2, wpiece = (lane & 3) ^ swz4(wr);
+    const uint8_t* from[kWQ];  // instruction q: the 16-row tile 4q + nw
+    uint32_t row[kWQ];
 #pragma unroll
-      for (int d = 0; d < DX - 1; ++d) issue_x(s0 + d, d);
-    } else {
-#pragma unroll
-      for (int d = 0; d < DW - 1; ++d) issue_w(s0 + d, d);
+    for (int q = 0; q < kWQ; ++q) {
+      from[q] = a.w + wrow(16 * (4 * q + nw)) * a.w_st;
+      row[q] = (uint32_t)(wrow(16 * (4 * q + nw) + wr) - wrow(16 * (4 * q + nw))) * (uint32_t)a.w_st;
     }
+    uintptr_t ssrc[kSQ];
+#pragma unroll
+    for (int q = 0; q < kSQ; ++q)  // (64 rows: two waves repeat the others)
+      ssrc[q] = s_base + (uint64_t)(wrow((32 * (4 * q + nw) + (lane >> 1)) % BN) * a.s_st);
+    auto issue = [&](int s_at, int slot) {
+      const int s = min(s_at, s1 - 1);
+      char* buf = lds + DX * kXB + slot * kWB;
+      const uint32_t piece = 16 * (uint32_t)min(4 * s + wpiece, blocks - 1);  // past the end: any valid one
+#pragma unroll
+      for (int q = 0; q < kWQ; ++q)
+        __builtin_amdgcn_global_load_lds((global_cptr)(from[q] + (size_t)(row[q] + piece)), (lds_void*)(buf + 1024 * (4 * q + nw)),
+                                         16, 0, 0);
+#pragma unroll
+      for (int q = 0; q < kSQ; ++q) {
+        const uintptr_t src = min(((ssrc[q] + 4 * s) & ~(uintptr_t)3) + 4 * (lane & 1), s_last);
+        __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(buf + BN * 64 + (256 * (4 * q + nw)) % (BN * 8)), 4, 0, 0);
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < DW - 1; ++d) issue(s0 + d, d);
+    u32x4_t x[2][MU];
+    u32x2_t w[NT];
+    uint32_t sc[NT];
     int xslot = 0, wslot = 0;
     for (int s = s0; s < s1; ++s) {
-      // all but the later steps of what this wave fetches has arrived; nobody reads step s - 1 any more
-      if (mw == 1) wait_vm<(DX - 2) * kXQ>();
-      else wait_vm<(DW - 2) * (kWQ + kSQ)>();
+      wait_vm<(DW - 2) * (kWQ + kSQ)>();
       __builtin_amdgcn_s_barrier();
-      if (mw == 1) issue_x(s + DX - 1, xslot == 0 ? DX - 1 : xslot - 1);
-      else issue_w(s + DW - 1, wslot == 0 ? DW - 1 : wslot - 1);
-      step(count, s, xslot, wslot);
-      if (++xslot == DX) xslot = 0;
-      if (++wslot == DW) wslot = 0;
+      issue(s + DW - 1, wslot == 0 ? DW - 1 : wslot - 1);
+      read(count, even, x, w, sc, s, xslot, wslot);
+      multiply(count, x, w, sc);
+      xslot = xslot + 1 == DX ? 0 : xslot + 1;
+      __builtin_amdgcn_s_barrier();
+      read(count, odd, x, w, sc, s, xslot, wslot);
+      multiply(count, x, w, sc);
+      xslot = xslot + 1 == DX ? 0 : xslot + 1;
+      wslot = wslot + 1 == DW ? 0 : wslot + 1;
     }
-    wait_vm<0>();  // nothing still writes LDS when the workgroup ends
   };
-  // the second half of the waves may have one column tile fewer
+  // Waves 4 .. 7: fetch x; multiply what the last half step read, then read.
+  auto run_x = [&](auto count) {
+    constexpr int MU = decltype(count)::value;
+    // instruction q: 8 rows of 128 bytes
+    const char* const from = reinterpret_cast<const char*>(a.x + (int64_t)m0 * a.x_st);
+    uint32_t row[kXQ];
+    int piece[kXQ];
+#pragma unroll
+    for (int q = 0; q < kXQ; ++q) {
+      const int r = 8 * (4 * q + nw) + (lane >> 3);
+      row[q] = 2 * (uint32_t)min(r, a.m - 1 - m0) * (uint32_t)a.x_st;
+      piece[q] = 8 * ((lane & 7) ^ swz8p(r & 15));
+    }
+    auto issue = [&](int h_at, int slot) {
+      const int h = min(h_at, 2 * s1 - 1);
+#pragma unroll
+      for (int q = 0; q < kXQ; ++q) {
+        const uint32_t at = row[q] + 2 * (uint32_t)min(64 * h + piece[q], a.k - 8);  // past the end: any valid piece
+        __builtin_amdgcn_global_load_lds((global_cptr)(from + (size_t)at), (lds_void*)(lds + slot * kXB + 1024 * (4 * q + nw)), 16,
+                                         0, 0);
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < DX - 1; ++d) issue(2 * s0 + d, d);
+    u32x4_t x[2][MU];
+    u32x2_t w[NT];
+    uint32_t sc[NT];
+#pragma unroll
+    for (int u = 0; u < MU; ++u) { x[0][u] = u32x4_t{0, 0, 0, 0}; x[1][u] = u32x4_t{0, 0, 0, 0}; }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) { w[t] = u32x2_t{0, 0}; sc[t] = 0u; }
+    int xslot = 0, wslot = 0;
+    for (int s = s0; s < s1; ++s) {
+      wait_vm<(DX - 2) * kXQ>();
+      __builtin_amdgcn_s_barrier();
+      issue(2 * s + DX - 1, xslot == 0 ? DX - 1 : xslot - 1);
+      multiply(count, x, w, sc);
+      read(count, even, x, w, sc, s, xslot, wslot);
+      xslot = xslot + 1 == DX ? 0 : xslot + 1;
+      wait_vm<(DX - 2) * kXQ>();
+      __builtin_amdgcn_s_barrier();
+      issue(2 * s + DX, xslot == 0 ? DX - 1 : xslot - 1);
+      multiply(count, x, w, sc);
+      read(count, odd, x, w, sc, s, xslot, wslot);
+      xslot = xslot + 1 == DX ? 0 : xslot + 1;
+      wslot = wslot + 1 == DW ? 0 : wslot + 1;
+    }
+    multiply(count, x, w, sc);
+  };
   if (s0 < s1) {
-    if (m0 + (mw * MTW + MTW - 1) * 16 < a.m) run(std::integral_constant<int, MTW>{});
-    else run(std::integral_constant<int, MTW - 1>{});
+    if (mw == 0) run_w(std::integral_constant<int, MTW>{});
+    else if (m0 + (2 * MTW - 1) * 16 < a.m) run_x(std::integral_constant<int, MTW>{});
+    else run_x(std::integral_constant<int, MTW - 1>{});  // the second half may have one column tile fewer
+    wait_vm<0>();  // nothing still writes LDS when the workgroup ends
   }
   // lane (g, i) of tile (t, u): weight rows 4g .. 4g + 3 of x row i
+  const bool quads = (a.out_st & 3) == 0 && ((uintptr_t)a.out & 7) == 0 && (a.n & 3) == 0;
 #pragma unroll
   for (int u = 0; u < MTW; ++u) {
     const int m = m0 + (mw * MTW + u) * 16 + i;
@@ -635,59 +669,96 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
     for (int t = 0; t < NT; t += SILU ? 2 : 1) {
       const int n = n0 + (SILU ? (nw * NT + t) >> 1 : nw * NT + t) * 16 + 4 * g;
+      if (ta.parts != nullptr) {
+        float* p = ta.parts + blockIdx.z * ta.part_size + (int64_t)m * (SILU ? 2 * a.n : a.n) + n;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (n + r >= a.n) continue;
-        if (ta.parts != nullptr) {
-          float* p = ta.parts + blockIdx.z * ta.part_size + (int64_t)m * (SILU ? 2 * a.n : a.n) + n + r;
-          p[0] = acc[t][u][r];
-          if constexpr (SILU) p[a.n] = acc[t + 1][u][r];
+        for (int e = 0; e < (SILU ? 2 : 1); ++e) {
+          const floatx4_t v = acc[t + e][u];
+          if (quads) {
+            if (n < a.n) *reinterpret_cast<floatx4_t*>(p + (e ? a.n : 0)) = v;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n + r < a.n) p[(e ? a.n : 0) + r] = v[r];
+          }
+        }
+      } else {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          v[r] = acc[t][u][r];
+          if constexpr (SILU) v[r] = silu_mul(v[r], acc[t + 1][u][r]);
+        }
+        bf16_t* o = a.out + (int64_t)m * a.out_st + n;
+        if (quads) {
+          if (n < a.n) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
         } else {
-          float v = acc[t][u][r];
-          if constexpr (SILU) v = silu_mul(v, acc[t + 1][u][r]);
-          a.out[(int64_t)m * a.out_st + n + r] = (bf16_t)f32_to_bf16(v);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < a.n) o[r] = (bf16_t)f32_to_bf16(v[r]);
         }
       }
     }
   }
 }
 
-// The sum of the parts of a split product, one output per thread.
-template <bool SILU>
+// The sum of the parts of a split product, four outputs per thread where rows
+// are whole fours (QUAD), else one.
+template <bool SILU, bool QUAD>
 __global__ __launch_bounds__(256) void fp4_sum_kernel(Fp4TileArgs ta, int parts) {
   const Fp4GemmArgs& a = ta.g;
+  constexpr int V = QUAD ? 4 : 1;
+  const int per = a.n / V;
   const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int m = (int)(idx / a.n), n = (int)(idx - (int64_t)m * a.n);
+  const int m = (int)(idx / per), n = (int)(idx - (int64_t)m * per) * V;
   if (m >= a.m) return;
   const float* p = ta.parts + (int64_t)m * (SILU ? 2 * a.n : a.n) + n;
-  float v = 0.f, up = 0.f;
+  float v[V], up[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = up[e] = 0.f;
+  auto add = [&](float (&to)[V], const float* from) {
+    if constexpr (QUAD) {
+      const floatx4_t f = *reinterpret_cast<const floatx4_t*>(from);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) to[e] += f[e];
+    } else {
+      to[0] += *from;
+    }
+  };
+#pragma unroll 8
   for (int z = 0; z < parts; ++z) {
-    v += p[z * ta.part_size];
-    if constexpr (SILU) up += p[z * ta.part_size + a.n];
+    add(v, p + z * ta.part_size);
+    if constexpr (SILU) add(up, p + z * ta.part_size + a.n);
   }
-  a.out[(int64_t)m * a.out_st + n] = (bf16_t)f32_to_bf16(SILU ? silu_mul(v, up) : v);
+  if constexpr (SILU) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = silu_mul(v[e], up[e]);
+  }
+  bf16_t* o = a.out + (int64_t)m * a.out_st + n;
+  if constexpr (QUAD) *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  else *o = (bf16_t)f32_to_bf16(v[0]);
 }
 
-// How a product of more than kShort rows is cut: column tiles per wave,
-// weight tiles per wave, parts of K.  The cheapest by cycles: a step costs its
+// How a product of more than kShort rows is cut: column tiles per wave, row
+// tiles of the weight per wave, parts of K.  The cheapest by cycles: a step costs its
 // matrix instructions (16 cycles each, two waves a SIMD) or its x through
-// LDS-DMA (64 bytes a cycle), a workgroup about 6000 more at its ends, parts
+// LDS-DMA (about 40 bytes a cycle), a workgroup about 8000 more at its ends, parts
 // their second kernel and the traffic between.
 constexpr int kShort = 64;
 struct TilePlan { int mtw, nt, parts; };
 TilePlan tile_plan(int m, int rows, int k, bool silu) {
-  const int my = (m + 32 * kMaxM - 1) / (32 * kMaxM);
-  const int mtw = std::max(3, ((m + my - 1) / my + 31) / 32);  // 65 rows and more: at least 3, the last tile may be empty
-  const int steps = (k + 127) / 128, gy = (m + 32 * mtw - 1) / (32 * mtw);
+  const int gy = (m + 32 * kMaxM - 1) / (32 * kMaxM);
+  const int mtw = std::max(3, ((m + gy - 1) / gy + 31) / 32);
+  const int steps = (k + 127) / 128;
   TilePlan best = {mtw, 4, 1};
   double cost = 1e300;
   for (int nt : {4, 2, 1}) {
     if (silu && nt == 1) continue;
     for (int parts : {1, 2, 4, 8}) {
       if (parts > 1 && steps / parts < 4) break;
-      const double groups = (double)((rows + 64 * nt - 1) / (64 * nt)) * gy * parts;
-      const double step = std::max(128.0 * nt * mtw, 128.0 * mtw) + 300.0;
-      double c = std::ceil(groups / 256) * ((steps + parts - 1) / parts * step + 6000.0);
+      const double groups = (double)((rows + 64 * nt - 1) / (64 * nt)) * ((m + 32 * mtw - 1) / (32 * mtw)) * parts;
+      const double step = std::max(128.0 * nt * mtw, 200.0 * mtw) + 700.0;
+      double c = std::ceil(groups / 256) * ((steps + parts - 1) / parts * step + 8000.0);
       if (parts > 1) c += 7000.0 + (double)parts * m * rows * 8.0 / 2000.0;
       if (c < cost) { cost = c; best = {mtw, nt, parts}; }
     }
@@ -697,12 +768,13 @@ TilePlan tile_plan(int m, int rows, int k, bool silu) {
 
 template <int NT, bool SILU>
 void launch_tile(const Fp4TileArgs& ta, int mtw, dim3 grid, hipStream_t stream) {
+  constexpr int threads = kWaves * 64;
   switch (mtw) {
-    case 3: fp4_tile_kernel<NT, 3, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
-    case 4: fp4_tile_kernel<NT, 4, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
-    case 5: fp4_tile_kernel<NT, 5, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
-    case 6: fp4_tile_kernel<NT, 6, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
-    default: fp4_tile_kernel<NT, 7, SILU><<<grid, kWaves * 64, 0, stream>>>(ta); break;
+    case 3: fp4_tile_kernel<NT, 3, SILU><<<grid, threads, 0, stream>>>(ta); break;
+    case 4: fp4_tile_kernel<NT, 4, SILU><<<grid, threads, 0, stream>>>(ta); break;
+    case 5: fp4_tile_kernel<NT, 5, SILU><<<grid, threads, 0, stream>>>(ta); break;
+    case 6: fp4_tile_kernel<NT, 6, SILU><<<grid, threads, 0, stream>>>(ta); break;
+    default: fp4_tile_kernel<NT, 7, SILU><<<grid, threads, 0, stream>>>(ta); break;
   }
 }
 
@@ -716,8 +788,12 @@ void dispatch_tile(const Fp4GemmArgs& a, float* ws, hipStream_t stream) {
   if (p.nt == 4) launch_tile<4, SILU>(ta, p.mtw, grid, stream);
   else if (p.nt == 2) launch_tile<2, SILU>(ta, p.mtw, grid, stream);
   else if constexpr (!SILU) launch_tile<1, SILU>(ta, p.mtw, grid, stream);
-  if (p.parts > 1)
-    fp4_sum_kernel<SILU><<<(unsigned)(((int64_t)a.m * a.n + 255) / 256), 256, 0, stream>>>(ta, p.parts);
+  if (p.parts > 1) {
+    if ((a.out_st & 3) == 0 && ((uintptr_t)a.out & 7) == 0 && (a.n & 3) == 0)
+      fp4_sum_kernel<SILU, true><<<(unsigned)(((int64_t)a.m * a.n / 4 + 255) / 256), 256, 0, stream>>>(ta, p.parts);
+    else
+      fp4_sum_kernel<SILU, false><<<(unsigned)(((int64_t)a.m * a.n + 255) / 256), 256, 0, stream>>>(ta, p.parts);
+  }
 }
 
 template <bool SILU>
@@ -745,7 +821,8 @@ extern "C" int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int
       (m > 1 && x_stride < k) || w_stride < k / 2 || scale_stride < k / kFp4Block || (uintptr_t)out & 1 ||
       (m > 1 && out_stride < (silu_mul ? n / 2 : n)))
     return (int)hipErrorInvalidValue;
-  if (m > 65535 * 64 || w_stride > (1 << 27) || scale_stride > (1 << 27)) return (int)hipErrorInvalidValue;  // 32-bit offsets
+  // 32-bit offsets within a tile
+  if (m > 65535 * 64 || w_stride > (1 << 27) || scale_stride > (1 << 27) || x_stride > (1 << 22)) return (int)hipErrorInvalidValue;
   if (m == 0) return 0;
   if (workspace_bytes < xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) || (uintptr_t)workspace & 15)
     return (int)hipErrorInvalidValue;
