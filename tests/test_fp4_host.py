@@ -153,3 +153,51 @@ def test_gemm_rejects_bad_arguments(lib):
                dict(n=0), dict(k=0), dict(k=4080), dict(n=1023, silu=1), dict(m=1 << 23), dict(m=200), dict(ws=A + 8)):
         assert _gemm(lib, **kw) == INVALID, kw
     assert _gemm(lib, m=0) == 0
+
+
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_pool_of_4bit_pages(layout):
+    from xvllm.config import Qwen3Shape
+    from xvllm.kv_pool import KVPool
+
+    cfg = Qwen3Shape(256, 8, 2, 128, 512, 3)
+    kv = KVPool(cfg, num_blocks=5, block_size=16, device="cpu", dtype=torch.float4_e2m1fn_x2, layout=layout)
+    assert kv.kv_cache.shape == (2, 3, 5, 16, 2, 64) and kv.kv_cache.dtype == torch.float4_e2m1fn_x2
+    assert kv.block_scale.shape == (2, 3, 5, 16, 2, 4) and kv.block_scale.dtype == torch.float8_e8m0fnu
+    assert kv.block_bytes * 5 == kv.kv_cache.numel() + kv.block_scale.numel()
+    assert kv.kv_cache.stride()[3:5] == ((2 * 64, 64) if layout == "nhd" else (64, 16 * 64))
+    other = KVPool(cfg, num_blocks=2, block_size=16, device="cpu", dtype=torch.bfloat16)
+    assert other.block_scale is None and other.block_bytes == 2 * 3 * 16 * 2 * 128 * 2
+
+
+def test_pool_and_runner_refusals():
+    from xvllm.config import Qwen3Shape
+    from xvllm.kv_pool import KVPool
+    from xvllm.model_runner import ModelRunner
+
+    make = lambda d=128, **kw: KVPool(Qwen3Shape(256, 8, 2, d, 512, 1), num_blocks=2, block_size=16, device="cpu",
+                                      dtype=torch.float4_e2m1fn_x2, **kw)
+    with pytest.raises(ValueError, match="blocks of 32"):
+        make(80)
+    with pytest.raises(ValueError, match="k_scale"):
+        make(k_scale=0.5)
+    with pytest.raises(ValueError, match="cascade"):
+        ModelRunner(None, make(), cascade_groups=2)
+
+
+def test_attention_over_4bit_pages_refusals():
+    from xvllm.layers.attention import (Attention, AttnInputs, AttnMetadata, CascadePlan, attention_context,
+                                        cascade_decode_attention)
+
+    pool, scale = codes(np.zeros((2, 1, 3, 16, 2, 64), np.uint8)), scales(np.zeros((2, 1, 3, 16, 2, 4), np.uint8))
+    z = torch.zeros(1, dtype=torch.int32)
+    plan = CascadePlan(z, z.view(1, 1), z, 1, 1)
+    q, k = torch.zeros((1, 1024), dtype=torch.bfloat16), torch.zeros((1, 256), dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="cascade"):
+        cascade_decode_attention(q, pool[0, 0], pool[1, 0], z.view(1, 1), z, plan, 8, 2, 128)
+    attn = Attention(8, 128, 2)
+    decode = AttnInputs(z, False, block_tables=z.view(1, 1), cache_seqlens=z)
+    with attention_context(AttnMetadata(pool, block_scale=scale)), pytest.raises(TypeError, match="cascade"):
+        attn(q, k, k, decode._replace(cascade=plan))
+    with attention_context(AttnMetadata(pool)), pytest.raises(ValueError, match="block_scale"):
+        attn(q, k, k, decode)

@@ -16,7 +16,7 @@ import torch.nn as nn
 
 from .. import _C
 from .._torch_glue import aligned16, call, ptr, require_bf16, require_cuda, stream_of
-from ..kv_ops import FP4_PAGES, as_int32, fp4_pages, store_kvcache
+from ..kv_ops import FP4_PAGES, as_int32, fp4_pages, gather_kvcache, store_kvcache
 
 
 @dataclass
@@ -52,6 +52,8 @@ class AttnMetadata:
     # build's optional pool format; the reference's pool holds the model dtype)
     k_scale: float = 1.0
     v_scale: float = 1.0
+    # 4-bit pools only (kv_cache [..., D/2] of two codes to a byte): the block scales [2, L, NB, BS, Hkv, D/32]
+    block_scale: Optional[torch.Tensor] = None
 
 
 # Active metadata, innermost context last (the reference keeps one module
@@ -83,6 +85,22 @@ def _layer_caches(layer_id: int) -> tuple[torch.Tensor, torch.Tensor]:
         raise RuntimeError("vllm::attention needs an active attention_context(AttnMetadata(kv_cache=...))")
     pool = _META_STACK[-1].kv_cache
     return pool[0, layer_id], pool[1, layer_id]
+
+
+def _layer_scales(layer_id: int) -> dict:
+    """The scales of a layer's cache, as store_kvcache and paged_decode_attention take them."""
+    ks, vs = kv_scales()
+    meta = _META_STACK[-1]
+    if meta.kv_cache.dtype != FP4_PAGES:
+        return {"k_scale": ks, "v_scale": vs}
+    if meta.block_scale is None:
+        raise ValueError("a 4-bit pool needs its block scales: AttnMetadata(block_scale=...)")
+    return {"k_block_scale": meta.block_scale[0, layer_id], "v_block_scale": meta.block_scale[1, layer_id]}
+
+
+def _refuse_cascade(k_cache: torch.Tensor) -> None:
+    if k_cache.dtype == FP4_PAGES:
+        raise TypeError("no cascade decode over 4-bit pages: paged_decode_attention reads them")
 
 
 _WORKSPACE: dict[tuple[str, int | None], torch.Tensor] = {}
@@ -252,7 +270,8 @@ def cascade_decode_attention(
     """paged_decode_attention with the shared prefixes of `plan` read once per
     group (xv_cascade_decode_attention, or _fp8 on an fp8 cache with the
     scales of paged_decode_attention).  Same output as the plain decode up
-    to fp32 summation order."""
+    to fp32 summation order.  Not over 4-bit pages."""
+    _refuse_cascade(k_cache)
     require_cuda(q, k_cache, v_cache, block_tables, cache_seqlens, plan.prefix_tokens)
     fp8 = k_cache.dtype == torch.float8_e4m3fn
     require_bf16(q, *(() if fp8 else (k_cache, v_cache)))
@@ -310,12 +329,14 @@ def prefill_attention(
     softmax_scale: float | None = None,
     max_seqlen_k: int = 0,
     kv_scale: tuple[float, float] | None = None,
+    k_block_scale: torch.Tensor | None = None,
+    v_block_scale: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Varlen causal attention, bottom-right aligned.  With block_tables the
     keys come from the paged cache (cached prefix + this chunk), otherwise
     from k/v rows cu_seqlens_k[b] .. cu_seqlens_k[b+1].  An fp8 paged cache
     needs max_seqlen_k and its (k_scale, v_scale) (default: the active
-    attention_context's)."""
+    attention_context's), a 4-bit one max_seqlen_k and its block scales."""
     q3, qs0, qs1 = _q_view(q, num_qo_heads, head_dim)
     require_cuda(q3, cu_seqlens_q, cu_seqlens_k)
     require_bf16(q3)
@@ -324,6 +345,14 @@ def prefill_attention(
     cuk = cu_seqlens_k.to(torch.int32).contiguous()
     out = torch.empty((q3.shape[0], num_qo_heads * head_dim), dtype=q.dtype, device=q.device)
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else softmax_scale
+    if block_tables is not None and k_cache is not None and k_cache.dtype == FP4_PAGES:
+        # 4-bit pages: the sequences' keys and values as varlen bf16 rows (exact), then the dense path
+        if max_seqlen_k <= 0:
+            raise ValueError("prefill over a 4-bit paged cache needs max_seqlen_k (the longest key run)")
+        kd, vd = gather_kvcache(k_cache, v_cache, block_tables, cuk, bsz * int(max_seqlen_k),
+                                k_block_scale=k_block_scale, v_block_scale=v_block_scale)
+        return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
+                                 head_dim, softmax_scale=softmax_scale)
     if block_tables is not None and k_cache is not None and k_cache.dtype == torch.float8_e4m3fn:
         # fp8 pages: the sequences' keys dequantized into varlen bf16 rows, then the dense path
         k_scale, v_scale = kv_scales() if kv_scale is None else kv_scale
@@ -402,22 +431,21 @@ def attention(
     k_cache, v_cache = _layer_caches(layer_id)
     k3 = k.view(-1, num_kv_heads, head_dim)
     v3 = v.view(-1, num_kv_heads, head_dim)
-    ks, vs = kv_scales()
+    scales = _layer_scales(layer_id)
     if slot_mapping is not None:  # None: this step's K/V are already in the cache (fused store)
-        store_kvcache(k3, v3, k_cache, v_cache, slot_mapping, k_scale=ks, v_scale=vs)  # paged view, in place
+        store_kvcache(k3, v3, k_cache, v_cache, slot_mapping, **scales)  # paged view, in place
     if is_prefill:
         if block_tables is not None:
             return prefill_attention(
                 q, None, None, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
                 head_dim, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, max_seqlen_k=max_seqlen_k,
-                kv_scale=(ks, vs),
+                **(scales if k_cache.dtype == FP4_PAGES else {"kv_scale": kv_scales()}),
             )
         return prefill_attention(
             q, k3, v3, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads, head_dim
         )
     return paged_decode_attention(
-        q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim,
-        k_scale=ks, v_scale=vs,
+        q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim, **scales,
     )
 
 
@@ -445,6 +473,7 @@ class Attention(nn.Module):
         if attn.cascade is not None and not attn.is_prefill:
             # shared-prefix decode: the plan does not fit the vllm::attention schema
             k_cache, v_cache = _layer_caches(self.layer_id)
+            _refuse_cascade(k_cache)
             ks, vs = kv_scales()
             if attn.slot_mapping is not None:
                 store_kvcache(k.view(-1, self.num_kv_heads, self.head_dim), v.view(-1, self.num_kv_heads, self.head_dim),

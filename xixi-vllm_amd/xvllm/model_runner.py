@@ -19,6 +19,7 @@ from . import _C
 from .batch import Batch, SeqSchedule
 from .config import head_dim as _head_dim
 from .cuda_graph import HipGraphRunner
+from .kv_ops import FP4_PAGES
 from .kv_pool import KVPool
 from .layers.attention import AttnInputs, AttnMetadata, attention_context
 from .sampler import Sampler, reserve_workspace, sample
@@ -75,6 +76,8 @@ class ModelRunner:
         this runner does not see: size it with that figure as reserve_bytes.
         Packed copies an earlier runner made are kept either way (its graphs
         read them), and every runner of the model then uses them."""
+        if cascade_groups > 0 and kv.dtype == FP4_PAGES:
+            raise ValueError("no cascade decode over a 4-bit KV pool: cascade_groups must be 0")
         self.model = model
         if stream_decode_gemms and hasattr(model, "pack_decode_weights"):
             model.pack_decode_weights()
@@ -86,7 +89,7 @@ class ModelRunner:
         cfg = model.config
         self.hidden_size = cfg.hidden_size
         self._meta = AttnMetadata(kv_cache=kv.kv_cache, k_scale=getattr(kv, "k_scale", 1.0),
-                                  v_scale=getattr(kv, "v_scale", 1.0))
+                                  v_scale=getattr(kv, "v_scale", 1.0), block_scale=getattr(kv, "block_scale", None))
         n_model_layers = len(model.model.layers)
         if kv.num_layers < n_model_layers:  # layer aliasing: layer i reads pool layer i % pool layers
             for i, layer in enumerate(model.model.layers):
@@ -101,7 +104,7 @@ class ModelRunner:
                            cascade_token_bytes=cfg.num_key_value_heads * _head_dim(cfg) * 2 * kv.dtype.itemsize,
                            cascade_min_shared_bytes=cascade_min_shared_bytes)
         self.vocab_size = cfg.vocab_size
-        act_dtype = torch.bfloat16 if kv.dtype == torch.float8_e4m3fn else kv.dtype  # activations stay bf16
+        act_dtype = torch.bfloat16 if kv.dtype in (torch.float8_e4m3fn, FP4_PAGES) else kv.dtype  # activations stay bf16
         self._decode_out = torch.zeros(self.max_bs, self.hidden_size, dtype=act_dtype, device=self.device)
         self._decode_ids = torch.zeros(self.max_bs, dtype=torch.int64, device=self.device)
         self._uniforms = torch.zeros(self.max_bs, dtype=torch.float32, device=self.device)

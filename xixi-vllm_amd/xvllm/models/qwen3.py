@@ -21,6 +21,7 @@ from torch import nn
 
 from ..config import head_dim as _head_dim
 from ..config import rope_theta as _rope_theta
+from ..kv_ops import FP4_PAGES
 from ..layers import Attention, AttnInputs, RMSNorm, RotaryEmbedding
 from ..layers.attention import kv_cache_of, kv_scales
 from ..layers.linear import (GEMM_PARTS, GEMM_SILU_MUL, STREAM_MAX_ROWS, in_place_parts, linear_into_norm, pack_weight,
@@ -129,8 +130,10 @@ class Qwen3Attention(nn.Module):
     def forward(self, positions, hidden, attn: AttnInputs):
         """qkv -> q/k norm + RoPE -> attention -> o GEMM (PartialSums when
         split along K, for post_attention_layernorm)."""
-        w = None if attn.is_prefill or not self.split_k else stream_operand(hidden, self.qkv_proj, None, GEMM_PARTS,
-                                                                            internal=True)
+        # the fused norm + RoPE + store kernels write bf16 and fp8 caches; into 4-bit pages Attention stores
+        fused = not attn.is_prefill and kv_cache_of(self.attn.layer_id)[0].dtype != FP4_PAGES
+        w = None if not fused or not self.split_k else stream_operand(hidden, self.qkv_proj, None, GEMM_PARTS,
+                                                                      internal=True)
         if w is not None:
             # decode: the qkv partial sums go into norm + RoPE + KV store
             qkv = streamed_into_norm(hidden, w)
@@ -140,7 +143,7 @@ class Qwen3Attention(nn.Module):
                 _, k, v = self._views(qkv.materialize())
             # Attention itself takes k and v from the cache (no slots to store at) and reads neither argument
             o = self.attn(q, k, v, attn._replace(slot_mapping=None))
-        elif not attn.is_prefill:
+        elif fused:
             # decode: norm + RoPE + KV store in one kernel, attention reads the cache
             q, k, v = self._split_norm_rope_store(positions, F.linear(hidden, self.qkv_proj), attn.slot_mapping)
             o = self.attn(q.view(q.shape[0], self.q_size), k, v, attn._replace(slot_mapping=None))
