@@ -546,7 +546,7 @@ int xv_stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_str
  *   out       row i at i * out_stride, 2-byte aligned.
  *   silu_mul  nonzero: W is the gate / up weight [2I, k] (n = 2I, gate rows first)
  *             and out[m, I] = silu(g) * u of the two fp32 products.
- *   workspace xv_mxfp4_gemm_workspace_size(...) bytes (0 up to 64 rows, and
+ *   workspace xv_mxfp4_gemm_workspace_size(...) bytes (0 up to 16 rows, and
  *             where K is not split), 16-byte aligned, no initial contents.
  * k a multiple of 32; any m >= 0 (up to 4 million) and n > 0.
  */

@@ -47,6 +47,7 @@ def _check(got, x, w, s, silu):
 @pytest.mark.parametrize("m,n,k", [
     (1, 16, 32), (1, 4096, 4096), (3, 34, 64), (16, 130, 96), (17, 1000, 416), (33, 258, 2080), (64, 512, 1024),
     (65, 20, 160), (200, 96, 512), (256, 514, 288), (100, 320, 2080), (160, 1026, 1024), (190, 200, 4000), (225, 66, 3200), (8, 2, 12288), (300, 18, 32), (15, 6000, 224), (130, 1538, 1056),
+    (64, 514, 8224), (40, 512, 4128), (33, 66, 12288), (20, 48, 9024), (17, 4096, 4096), (48, 1000, 5152),
 ])
 def test_product_matches_oracle(dev, m, n, k, silu):
     rng = np.random.default_rng(m * 7 + n + k)

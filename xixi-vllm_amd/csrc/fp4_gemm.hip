@@ -18,8 +18,8 @@
 // (4.4 TB/s), 8 rows through 4096 x 12288 9.6 us.  Direct loads into the operand
 // registers, where neighbouring lanes are neighbouring rows, were bound by the
 // address unit (weights so: 22 us for the first; x alone so: 12.7 us for the
-// second).  Every workgroup reads all of x, so that 64 rows of a weight of few
-// rows are bound by L2 (64 through 4096 x 12288: 400 MB in 23 us).
+// second).  Every workgroup reads all of its part of x through its LDS-DMA, which
+// is what bounds more than 16 rows (37 rows of an odd 5003 x 4704 weight 12.0 us).
 #include "xv_decode.h"
 #include "xv_fp4.h"
 #include "xv_kernels.h"
@@ -37,6 +37,23 @@ struct Fp4GemmArgs {
   int m, n, k;                      // n: outputs (of SILU: half the weight's rows)
 };
 
+// A product whose K may be cut into parts, which a second kernel adds.
+struct Fp4PartArgs {
+  Fp4GemmArgs g;
+  float* parts;       // null: out is written
+  int64_t part_size;  // floats of a part: m x (rows of the weight)
+  int per;            // slices or steps of a part
+};
+
+// 16 bytes a lane, `off` behind `base` (both of these wave uniform), into LDS in lane order, with the bytes from base to
+// end as the buffer's size: past it nothing is read.
+template <int POLICY>
+XV_INLINE void load_lds(const void* base, const void* end, char* to, uint32_t off) {
+  const uint64_t n = reinterpret_cast<uint64_t>(end) - reinterpret_cast<uint64_t>(base);
+  const __amdgpu_buffer_rsrc_t r = page_rsrc(static_cast<const bf16_t*>(base), n < 0xffffffffu ? (uint32_t)n : 0xffffffffu);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)to, 16, off, 0, 0, POLICY);
+}
+
 XV_INLINE float silu_mul(float g, float u) { return g / (1.0f + __expf(-g)) * u; }
 
 XV_INLINE bf16x8_t widen8(uint32_t w, float scale) {
@@ -50,22 +67,20 @@ XV_INLINE bf16x8_t widen8(uint32_t w, float scale) {
 typedef const __attribute__((address_space(1))) void* global_cptr;
 
 constexpr int kWaves = 8;
-constexpr int kDepth = 3;  // stages in a wave's ring, kDepth - 1 of them in flight
 
-// One stage: 16 weight rows x KS values.  LDS image: the rows' codes (KS / 2
-// bytes each, swizzled), then a window of SW dwords of each row's scale bytes.
+// One stage: the codes of 16 weight rows x KS values, rows of KS / 2 bytes,
+// swizzled.  Scales come with a slice of x, a window of SW dwords of each of the
+// workgroup's rows: a load of few lanes costs what a full one does (with every
+// stage its own scales: 32 rows through a 24576 x 4096 gate / up weight 21.6 us).
 // A scale row need not start at a multiple of 4 bytes (WIDE): the window then
 // starts at the dword that holds the first byte.
 template <int KS, bool WIDE>
 struct Stage {
   static constexpr int kPieces = KS / 32;               // 16-byte pieces (scale blocks) of a row
-  static constexpr int kCodes = 16 * KS / 2;
-  static constexpr int kLoads = kCodes / 1024;          // LDS-DMA instructions of the codes
+  static constexpr int kBytes = 16 * KS / 2;
+  static constexpr int kLoads = kBytes / 1024;          // LDS-DMA instructions
   static constexpr int kRowsPer = 64 / kPieces;         // rows one of them covers
   static constexpr int SW = !WIDE ? KS / 128 : KS / 64;
-  static constexpr int kScaleLoads = (16 * SW + 63) / 64;
-  static constexpr int kBytes = kCodes + kScaleLoads * 256;
-  static constexpr int kOps = kLoads + kScaleLoads;
   static constexpr int kSteps = KS / 128;               // operand loads of 128 values
   static XV_INLINE int swz(int row) {
     static_assert(KS == 128 || KS == 256, "rows of 64 or 128 bytes");
@@ -81,31 +96,28 @@ XV_INLINE int swz_x(int r) {
   return XR == 8 ? (r & 3) | ((r & 4) << 1) : swz16(r);
 }
 
-// A stage's operands of the lane, one piece of codes (at wa) and one scale byte
-// (sa, 4 bytes on) for each 128 values, once at most VM vector-memory
-// operations are outstanding: one asm block with one wait.
-template <int N, int VM>
+// A stage's operands of the lane in one asm block with one wait: one piece of
+// codes (at wa) and one scale byte (sa, 4 bytes on) for each 128 values.
+template <int N>
 XV_INLINE void read_stage(u32x4_t (&w)[N], uint32_t (&s)[N], const uint32_t (&wa)[N], uint32_t sa) {
   static_assert(N == 1 || N == 2, "slices of 128 or 256 values");
   if constexpr (N == 2) {
     __asm__ __volatile__(
-        "s_waitcnt vmcnt(%7)\n\t"
         "ds_read_b128 %0, %4\n\t"
         "ds_read_b128 %1, %5\n\t"
         "ds_read_u8 %2, %6\n\t"
         "ds_read_u8 %3, %6 offset:4\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(w[0]), "=&v"(w[1]), "=&v"(s[0]), "=&v"(s[1])
-        : "v"(wa[0]), "v"(wa[1]), "v"(sa), "n"(VM)
+        : "v"(wa[0]), "v"(wa[1]), "v"(sa)
         : "memory");
   } else {
     __asm__ __volatile__(
-        "s_waitcnt vmcnt(%4)\n\t"
         "ds_read_b128 %0, %2\n\t"
         "ds_read_u8 %1, %3\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(w[0]), "=&v"(s[0])
-        : "v"(wa[0]), "v"(sa), "n"(VM)
+        : "v"(wa[0]), "v"(sa)
         : "memory");
   }
 }
@@ -129,21 +141,37 @@ XV_INLINE void read_x8(u32x4_t (&v)[8], const uint32_t (&at)[8]) {
 
 template <int N>
 XV_INLINE void wait_vm() {
+  static_assert(N >= 0 && N <= 63, "the counter's range");
   __asm__ __volatile__("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Wait until at most A + min(n, MAX) * B are outstanding; n known where it is unrolled.
+template <int A, int B, int MAX>
+XV_INLINE void wait_vm_of(int n) {
+  if constexpr (MAX > 0) {
+    if (n < MAX) return wait_vm_of<A, B, MAX - 1>(n);
+  }
+  wait_vm<A + B * MAX>();
 }
 
 // m <= XR rows of x as MT column tiles of 16 (XR = 8: the tile's upper half
 // repeats the lower, its outputs are not stored); XD slices of x in LDS.
 template <int MT, int XR, int KS, int XD, int T, bool SILU, bool WIDE>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_gemm_kernel(Fp4GemmArgs a) {
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_gemm_kernel(Fp4PartArgs pa) {
+  const Fp4GemmArgs& a = pa.g;
   using S = Stage<KS, WIDE>;
   constexpr int kXBytes = XR * KS * 2, kXLoads = kXBytes / 1024, kXPieces = KS / 8;
-  constexpr int kWave = kDepth * S::kBytes + XD * kXBytes;  // LDS of one wave
+  constexpr int kSLoads = (T * 16 * S::SW + 63) / 64, kSBytes = kSLoads * 256;  // the scales of a slice
+  constexpr int kSlice = kXLoads + kSLoads;                                      // instructions that come with a slice
+  // Stages in a wave's ring, one less of them in flight.  (Four to eight: no faster.)
+  constexpr int kRest = XD * kXBytes + (XD + 1) * kSBytes, kDepth = kRest + 3 * S::kBytes <= 163840 / kWaves ? 3 : 2;
+  constexpr int kWave = kDepth * S::kBytes + kRest;         // LDS of one wave
   // Weight loads are non-temporal where a wave runs through whole 128-byte lines of several tiles (one row of a 24576 x
   // 4096 weight 12.1 us against 13.0), not where two waves share a line (64 rows through 4096 x 12288 22.9 against 29.2)
   // or the workgroup has one tile (8 rows through it 9.5 against 11.1).
   constexpr int kPolicy = KS == 256 && T > 2 ? kNontemporal : 0;
-  constexpr int TR = SILU ? 2 : 1;                          // tiles summed over the waves at a time
+  constexpr int P = SILU ? 2 : 1;
+  // tiles summed over the waves at a time: all that LDS holds
+  constexpr int kTR = 163840 / (kWaves * MT * 1024) / P * P, TR = T < kTR ? T : kTR;
   constexpr int kRed = kWaves * TR * MT * 1024;
   static_assert(kXLoads >= 1 && kWaves * kWave <= 163840 && kRed <= 163840, "LDS of a CU");
   __shared__ __attribute__((aligned(16))) char lds[kWaves * kWave > kRed ? kWaves * kWave : kRed];
@@ -151,91 +179,73 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   const int n0 = blockIdx.x * (SILU ? T / 2 : T) * 16;
   char* const ring = lds + wave * kWave;
   char* const xring = ring + kDepth * S::kBytes;
+  char* const sring = xring + XD * kXBytes;
   const int blocks = a.k / kFp4Block;
-  const int slices = (a.k + KS - 1) / KS;
-  const int mine = slices > wave ? (slices - wave + kWaves - 1) / kWaves : 0;  // slices wave, wave + 8, ...
-  const int total = mine * T;                                                   // stages of this wave
+  const int first = blockIdx.y * pa.per + wave, last = min((a.k + KS - 1) / KS, (int)(blockIdx.y + 1) * pa.per);
+  const int mine = last > first ? (last - first + kWaves - 1) / kWaves : 0;  // slices first, first + 8, ... below last
+  const int total = mine * T;                                                // stages of this wave
 
   // weight row of operand row r of tile t: SILU has the gate and the up rows of the same outputs in tiles 2p, 2p + 1
   auto wrow = [&](int t, int r) {
     const int o = min(n0 + (SILU ? t >> 1 : t) * 16 + r, a.n - 1);
     return (int64_t)o + (SILU && (t & 1) ? a.n : 0);
   };
-  const uint8_t* const s_last = reinterpret_cast<const uint8_t*>(
-      (reinterpret_cast<uintptr_t>(a.s) + (uint64_t)((SILU ? 2 * (int64_t)a.n : a.n) - 1) * a.s_st + blocks - 1) & ~(uintptr_t)3);
-  // this lane's offsets within a stage of whole rows and blocks
-  uint32_t coff[S::kLoads], soff[S::kScaleLoads];
+  const uintptr_t s_last =  // the dword that holds the last scale
+      (reinterpret_cast<uintptr_t>(a.s) + (uint64_t)((SILU ? 2 * (int64_t)a.n : a.n) - 1) * a.s_st + blocks - 1) & ~(uintptr_t)3;
+  // This lane's offsets within a stage and within a slice of x.  The code of a stage is short on purpose: a wave
+  // runs it few times, mostly for the first time.  Rows and blocks past the end are left to the buffers' bounds (their
+  // outputs are not stored, or x is zero there).  (With clamped rows by address, twice the instructions: 64 rows
+  // of the 24576 x 4096 gate / up weight 26.7 us against 25.9.)
+  uint32_t coff[S::kLoads], xoff[kXLoads];
 #pragma unroll
   for (int q = 0; q < S::kLoads; ++q) {
     const int row = S::kRowsPer * q + lane / S::kPieces;
     coff[q] = row * (uint32_t)a.w_st + 16 * ((lane % S::kPieces) ^ S::swz(row));
   }
 #pragma unroll
-  for (int q = 0; q < S::kScaleLoads; ++q) {
-    const int at = min(64 * q + lane, 16 * S::SW - 1);
-    soff[q] = (at / S::SW) * (uint32_t)a.s_st + 4 * (at % S::SW);
+  for (int q = 0; q < kXLoads; ++q) {
+    const int row = (64 * q + lane) / kXPieces;
+    xoff[q] = row * 2 * (uint32_t)a.x_st + 16 * ((lane % kXPieces) ^ swz_x<XR>(row));
   }
-  // LDS-DMA instructions issued so far, and the count when each stage's and slice's last one left: what
-  // was issued since may still be in flight when it is waited for
-  int ops = 0, wmark[kDepth], xmark[XD];
+  const uint8_t* const w_end = a.w + ((SILU ? 2 * (int64_t)a.n : a.n) - 1) * a.w_st + 16 * (int64_t)blocks;
+  const uint8_t* const wg = a.w + n0 * a.w_st;
+  const uint8_t* const wu = wg + (SILU ? (int64_t)a.n * a.w_st : 0);
+  const bf16_t* const x_end = a.x + (a.m - 1) * a.x_st + a.k;
+  // the scale rows this lane fetches from, and the dword of the window
+  uintptr_t srow[kSLoads];
+  uint32_t sdw[kSLoads];
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) wmark[d] = 0;
+  for (int q = 0; q < kSLoads; ++q) {
+    const int at = min(64 * q + lane, T * 16 * S::SW - 1);
+    srow[q] = reinterpret_cast<uintptr_t>(a.s) + (uint64_t)(wrow(at / (16 * S::SW), at / S::SW % 16) * a.s_st);
+    sdw[q] = 4 * (at % S::SW);
+  }
+  // LDS-DMA instructions issued so far, and the count when each slice of x's last one left: what was issued
+  // since may still be in flight when it is waited for
+  int ops = 0, xmark[XD];
 #pragma unroll
   for (int d = 0; d < XD; ++d) xmark[d] = 0;
-  int issued = 0, it = 0, is = wave;  // stages issued; the next one's tile and slice
-  auto issue = [&](int slot) {
+  int issued = 0, is = first;  // stages issued, the next one's slice
+  auto issue = [&](int slot, int it) {  // it: the next one's tile
     char* buf = ring + slot * S::kBytes;
-    const int b0 = is * S::kPieces;  // the slice's first block
-    const int o0 = n0 + (SILU ? it >> 1 : it) * 16;
-    const bool whole = o0 + 16 <= a.n && b0 + S::kPieces <= blocks;
-    const int64_t row0 = (int64_t)o0 + (SILU && (it & 1) ? a.n : 0);
-    if (whole) {
-      const uint8_t* src = a.w + row0 * a.w_st + 16 * (int64_t)b0;
+    const uint32_t at = (uint32_t)(SILU ? it >> 1 : it) * 16 * (uint32_t)a.w_st + 16 * S::kPieces * (uint32_t)is;
 #pragma unroll
-      for (int q = 0; q < S::kLoads; ++q)
-        __builtin_amdgcn_global_load_lds((global_cptr)(src + coff[q]), (lds_void*)(buf + 1024 * q), 16, 0, kPolicy);
-    } else {
-#pragma unroll
-      for (int q = 0; q < S::kLoads; ++q) {
-        const int row = S::kRowsPer * q + lane / S::kPieces;
-        const int piece = (lane % S::kPieces) ^ S::swz(row);
-        // rows and blocks past the end: valid ones (not stored, and their x is zero)
-        const uint8_t* src = a.w + wrow(it, row) * a.w_st + 16 * (int64_t)min(b0 + piece, blocks - 1);
-        __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(buf + 1024 * q), 16, 0, kPolicy);
-      }
-    }
-    if (whole && !WIDE) {
-      const uint8_t* src = a.s + row0 * a.s_st + b0;
-#pragma unroll
-      for (int q = 0; q < S::kScaleLoads; ++q)
-        __builtin_amdgcn_global_load_lds((global_cptr)(src + soff[q]), (lds_void*)(buf + S::kCodes + 256 * q), 4, 0, 0);
-    } else {
-#pragma unroll
-      for (int q = 0; q < S::kScaleLoads; ++q) {
-        const int at = min(64 * q + lane, 16 * S::SW - 1);
-        uintptr_t src = (reinterpret_cast<uintptr_t>(a.s) + (uint64_t)(wrow(it, at / S::SW) * a.s_st + b0)) & ~(uintptr_t)3;
-        src = min(src + 4 * (at % S::SW), reinterpret_cast<uintptr_t>(s_last));  // dwords that hold a byte of the tensor
-        __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(buf + S::kCodes + 256 * q), 4, 0, 0);
-      }
-    }
+    for (int q = 0; q < S::kLoads; ++q) load_lds<kPolicy>(SILU && (it & 1) ? wu : wg, w_end, buf + 1024 * q, coff[q] + at);
     ++issued;
-    ops += S::kOps;
-    wmark[slot] = ops;
-    if (++it == T) {
-      it = 0;
-      is += kWaves;
-    }
+    ops += S::kLoads;
+    if (it == T - 1) is += kWaves;
   };
-  // Slice `slice` of x: row r's KS values (2 KS bytes, swizzled) at r * 2 KS.
-  auto issue_x = [&](int slice, int slot) {
+  // Slice `slice` of x: row r's KS values (2 KS bytes, swizzled) at r * 2 KS; and its scales.
+  auto issue_x = [&](int slice, int slot, int sslot) {
 #pragma unroll
-    for (int q = 0; q < kXLoads; ++q) {
-      const int at = 64 * q + lane, row = at / kXPieces, piece = (at % kXPieces) ^ swz_x<XR>(row);
-      const int k = min(slice * KS + 8 * piece, a.k - 8);  // past the end: any valid piece (zeroed below)
-      const bf16_t* src = a.x + (int64_t)min(row, a.m - 1) * a.x_st + k;
-      __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(xring + slot * kXBytes + 1024 * q), 16, 0, 0);
+    for (int q = 0; q < kXLoads; ++q)
+      load_lds<0>(a.x, x_end, xring + slot * kXBytes + 1024 * q, xoff[q] + 2 * KS * (uint32_t)slice);
+#pragma unroll
+    for (int q = 0; q < kSLoads; ++q) {
+      const uintptr_t src = min(((srow[q] + (uint32_t)(slice * S::kPieces)) & ~(uintptr_t)3) + sdw[q], s_last);
+      __builtin_amdgcn_global_load_lds((global_cptr)src, (lds_void*)(sring + sslot * kSBytes + 256 * q), 4, 0, 0);
     }
-    ops += kXLoads;
+    ops += kSlice;
     xmark[slot] = ops;
   };
 
@@ -279,54 +289,58 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
   for (int h = 0; h < S::kSteps; ++h)
     wat[h] = (uint32_t)(i * (KS / 2) + (((4 * h + g) ^ S::swz(i)) << 4));
-  int wslot = 0, xslot = 0;  // ring slots of the next stage and slice to use
+  int wslot = 0, xslot = 0, sslot = 0;  // ring slots of the next stage, slice and its scales to use
   if (mine > 0) {
 #pragma unroll
     for (int d = 0; d < XD; ++d)
-      if (d < mine) issue_x(wave + d * kWaves, d);
+      if (d < mine) issue_x(first + d * kWaves, d, d);
 #pragma unroll
     for (int d = 0; d < kDepth - 1; ++d)
-      if (issued < total) issue(d);
+      if (issued < total) issue(d, d % T);
   }
   for (int s = 0; s < mine; ++s) {
-    const int slice = wave + s * kWaves;
+    const int slice = first + s * kWaves;
     {
       int since = ops;
 #pragma unroll
       for (int d = 0; d < XD; ++d)
         if (d == xslot) since = ops - xmark[d];
-      constexpr int kFull = XD > 1 ? XD * S::kOps + (XD - 1) * kXLoads : (T < kDepth ? T : kDepth - 1) * S::kOps;
-      constexpr int kFirst = (kDepth - 1) * S::kOps + (XD - 1) * kXLoads;  // the first slice: the first loads of all
+      constexpr int kFull = XD > 1 ? XD * S::kLoads + (XD - 1) * kSlice : (T < kDepth ? T : kDepth - 1) * S::kLoads;
+      constexpr int kFirst = (kDepth - 1) * S::kLoads + (XD - 1) * kSlice;  // the first slice: the first loads of all
       if (since >= kFull) wait_vm<kFull>();
       else if (kFirst < kFull && since >= kFirst) wait_vm<kFirst>();
       else wait_vm<0>();
       take_x(slice, xslot);
-      if (s + XD < mine) issue_x(slice + XD * kWaves, xslot);
+      if (s + XD < mine) issue_x(slice + XD * kWaves, xslot, sslot == 0 ? XD : sslot - 1);  // past the last slice's scales
       if (++xslot == XD) xslot = 0;
     }
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-      if (issued < total) issue(wslot == 0 ? kDepth - 1 : wslot - 1);
+      // This stage left kDepth - 1 stages ago.  Slices that began since, each with a slice of x (of which at most XD
+      // are still in flight):
+      constexpr int kSince = kDepth - 1;
+      const int kSlices = t < kSince ? (kSince - t + T - 1) / T : 0;
+      const bool steady = issued < total;
+      if (steady) issue(wslot == 0 ? kDepth - 1 : wslot - 1, (t + kSince) % T);
       const uint32_t b = (uint32_t)reinterpret_cast<uintptr_t>(ring + wslot * S::kBytes);
       uint32_t wa[S::kSteps];
 #pragma unroll
       for (int h = 0; h < S::kSteps; ++h) wa[h] = b + wat[h];
       uint32_t m4 = 0;  // where in its first dword the row's scale bytes start
       if constexpr (WIDE) m4 = (uint32_t)((reinterpret_cast<uintptr_t>(a.s) + (uint64_t)(wrow(t, i) * a.s_st + slice * S::kPieces)) & 3);
-      const uint32_t sa = b + S::kCodes + i * (4 * S::SW) + m4 + g;
-      int since = ops;
-#pragma unroll
-      for (int d = 0; d < kDepth; ++d)
-        if (d == wslot) since = ops - wmark[d];
+      const uint32_t sa = (uint32_t)reinterpret_cast<uintptr_t>(sring + sslot * kSBytes) + (t * 16 + i) * (4 * S::SW) + m4 + g;
       if (++wslot == kDepth) wslot = 0;
+      if (steady) {
+        if (s + XD < mine && s * T + t >= kSince - 1) wait_vm_of<kSince * S::kLoads, kSlice, XD>(kSlices);
+        else wait_vm<kSince * S::kLoads>();
+      } else {
+        // the stages behind it were all issued: of the last slice, those of its further tiles
+        if (s + 1 == mine) wait_vm_of<0, S::kLoads, kSince - 1>(T - 1 - t);
+        else wait_vm<0>();
+      }
       u32x4_t w[S::kSteps];
       uint32_t sc[S::kSteps];
-      constexpr int kTwo = (kDepth - 1) * S::kOps;
-      constexpr int kOne = kTwo + kXLoads, kBoth = kTwo + 2 * kXLoads;  // with the x slices issued since
-      if (T == 1 && since >= kBoth) read_stage<S::kSteps, kBoth>(w, sc, wa, sa);
-      else if (since >= kOne) read_stage<S::kSteps, kOne>(w, sc, wa, sa);
-      else if (since >= kTwo) read_stage<S::kSteps, kTwo>(w, sc, wa, sa);
-      else read_stage<S::kSteps, 0>(w, sc, wa, sa);
+      read_stage<S::kSteps>(w, sc, wa, sa);
 #pragma unroll
       for (int h = 0; h < S::kSteps; ++h) {
         // blocks past the end: scale 0 keeps their products with x = 0 finite
@@ -343,68 +357,62 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
         }
       }
     }
+    if (++sslot == XD + 1) sslot = 0;
   }
-  // the waves' sums: lane (g, i) of tile (t, u) holds weight rows 4g + r of x row i
-  float* red = reinterpret_cast<float*>(lds);
+  // The waves' sums: lane (g, i) of tile (t, u) holds weight rows 4g .. 4g + 3 of x row i.  A thread adds whole
+  // lanes of eight waves and writes four outputs.  (Two tiles at a time by single floats: 64 rows of the 24576 x 4096
+  // gate / up weight 5 us in this end, 27.5 in all.)
+  floatx4_t* const red = reinterpret_cast<floatx4_t*>(lds);
+  const bool quads = (a.out_st & 3) == 0 && ((uintptr_t)a.out & 7) == 0 && (a.n & 3) == 0;
 #pragma unroll
   for (int t0 = 0; t0 < T; t0 += TR) {
+    const int tiles = T - t0 < TR ? T - t0 : TR;
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < TR; ++t)
+      if (t < tiles) {
 #pragma unroll
-      for (int u = 0; u < MT; ++u)
-        *reinterpret_cast<floatx4_t*>(&red[((wave * TR + t) * MT + u) * 256 + lane * 4]) = acc[t0 + t][u];
+        for (int u = 0; u < MT; ++u) red[((wave * TR + t) * MT + u) * 64 + lane] = acc[t0 + t < T ? t0 + t : 0][u];
+      }
     __syncthreads();
-    for (int e = threadIdx.x; e < MT * 256; e += kWaves * 64) {
-      const int o = e & 15, m = e >> 4;  // output within the tile, x row
-      const int at = (m >> 4) * 256 + (o >> 2) * 64 + (m & 15) * 4 + (o & 3);
-      const int n = n0 + (t0 / TR) * 16 + o;
+    for (int e = threadIdx.x; e < tiles / P * MT * 64; e += kWaves * 64) {
+      const int at = e & 63, u = (e >> 6) % MT, p = (e >> 6) / MT;
+      const int n = n0 + (t0 / P + p) * 16 + 4 * (at >> 4), m = u * 16 + (at & 15);
       if (n >= a.n || m >= a.m) continue;
-      float v = 0.f, up = 0.f;
+      floatx4_t v = {0.f, 0.f, 0.f, 0.f}, up = v;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        v += red[(w * TR * MT) * 256 + at];
-        if constexpr (SILU) up += red[((w * TR + 1) * MT) * 256 + at];
+        v += red[((w * TR + p * P) * MT + u) * 64 + at];
+        if constexpr (SILU) up += red[((w * TR + p * P + 1) * MT + u) * 64 + at];
       }
-      a.out[(int64_t)m * a.out_st + n] = (bf16_t)f32_to_bf16(SILU ? silu_mul(v, up) : v);
+      if (pa.parts != nullptr) {
+        float* to = pa.parts + blockIdx.y * pa.part_size + (int64_t)m * (P * a.n) + n;
+        if (quads) {
+          *reinterpret_cast<floatx4_t*>(to) = v;
+          if constexpr (SILU) *reinterpret_cast<floatx4_t*>(to + a.n) = up;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < a.n) {
+              to[r] = v[r];
+              if constexpr (SILU) to[a.n + r] = up[r];
+            }
+        }
+        continue;
+      }
+      if constexpr (SILU) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = silu_mul(v[r], up[r]);
+      }
+      bf16_t* o = a.out + (int64_t)m * a.out_st + n;
+      if (quads) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < a.n) o[r] = (bf16_t)f32_to_bf16(v[r]);
+      }
     }
-  }
-}
-
-template <int MT, int XR, int KS, int XD, int T, bool SILU>
-void launch(const Fp4GemmArgs& a, hipStream_t stream) {
-  constexpr int outs = (SILU ? T / 2 : T) * 16;
-  const dim3 grid((unsigned)((a.n + outs - 1) / outs));
-  // scale rows that start at multiples of 4 bytes have narrower windows
-  if (((uintptr_t)a.s | (uint64_t)a.s_st) & 3) fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, true><<<grid, kWaves * 64, 0, stream>>>(a);
-  else fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, false><<<grid, kWaves * 64, 0, stream>>>(a);
-}
-
-// Tiles per workgroup: the fewest turns of the chip (one workgroup per CU),
-// each as long as its tiles plus its start and end, about one and a half tiles.
-template <bool SILU>
-int tiles_per_group(int n) {
-  const int tiles = (n + 15) / 16 * (SILU ? 2 : 1);
-  int best = SILU ? 2 : 1;
-  double cost = 1e30;
-  for (int t : {1, 2, 4, 6}) {
-    if (SILU && t % 2) continue;
-    const int groups = (tiles + t - 1) / t;
-    const double c = ((groups + 255) / 256) * (t + 1.5);
-    if (c <= cost) { cost = c; best = t; }
-  }
-  return best;
-}
-
-// One tile a workgroup takes a new slice of x with every stage: as many in
-// flight (XD) as stages, in shorter slices where 16 rows of x would not fit.
-template <int MT, int XR, int KS1, int XD1, int KS, bool SILU>
-void launch_tiles(const Fp4GemmArgs& a, hipStream_t stream) {
-  switch (tiles_per_group<SILU>(a.n)) {
-    case 1: if constexpr (!SILU) launch<MT, XR, KS1, XD1, 1, SILU>(a, stream); break;
-    case 2: launch<MT, XR, KS, 1, 2, SILU>(a, stream); break;
-    case 4: launch<MT, XR, KS, 1, 4, SILU>(a, stream); break;
-    default: launch<MT, XR, KS, 1, 6, SILU>(a, stream); break;
   }
 }
 
@@ -423,13 +431,6 @@ void launch_tiles(const Fp4GemmArgs& a, hipStream_t stream) {
 // products alone take 79, the loads and reads alone 84.  Weight loads are not
 // non-temporal: a step takes half a line, and 133 us then.)  Where the tiles give too few workgroups, K is split
 // and a second kernel adds the fp32 parts.
-struct Fp4TileArgs {
-  Fp4GemmArgs g;
-  float* parts;       // null: out is written
-  int64_t part_size;  // floats of a part: m x (rows of the weight)
-  int per;            // steps of a part
-};
-
 constexpr int kMaxM = 7;  // column tiles per wave at most (224 rows of x)
 
 // The operands of a half step in one asm block with one wait: of N column
@@ -476,7 +477,7 @@ XV_INLINE void read_half(u32x4_t (&x)[2][MU], u32x2_t (&w)[NT], uint32_t (&s)[NT
 }
 
 template <int NT, int MTW, bool SILU>
-__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_tile_kernel(Fp4TileArgs ta) {
+__global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp4_tile_kernel(Fp4PartArgs ta) {
   const Fp4GemmArgs& a = ta.g;
   constexpr int BM = 32 * MTW, BN = 64 * NT;
   constexpr int kXB = BM * 128;                // bytes of a half step of x
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 // The sum of the parts of a split product, four outputs per thread where rows
 // are whole fours (QUAD), else one.
 template <bool SILU, bool QUAD>
-__global__ __launch_bounds__(256) void fp4_sum_kernel(Fp4TileArgs ta, int parts) {
+__global__ __launch_bounds__(256) void fp4_sum_kernel(Fp4PartArgs ta, int parts) {
   const Fp4GemmArgs& a = ta.g;
   constexpr int V = QUAD ? 4 : 1;
   const int per = a.n / V;
@@ -739,6 +740,73 @@ __global__ __launch_bounds__(256) void fp4_sum_kernel(Fp4TileArgs ta, int parts)
   else *o = (bf16_t)f32_to_bf16(v[0]);
 }
 
+template <bool SILU>
+void launch_sum(const Fp4PartArgs& pa, int parts, hipStream_t stream) {
+  const Fp4GemmArgs& a = pa.g;
+  if ((a.out_st & 3) == 0 && ((uintptr_t)a.out & 7) == 0 && (a.n & 3) == 0)
+    fp4_sum_kernel<SILU, true><<<(unsigned)(((int64_t)a.m * a.n / 4 + 255) / 256), 256, 0, stream>>>(pa, parts);
+  else
+    fp4_sum_kernel<SILU, false><<<(unsigned)(((int64_t)a.m * a.n + 255) / 256), 256, 0, stream>>>(pa, parts);
+}
+
+template <int MT, int XR, int KS, int XD, int T, bool SILU>
+void launch(const Fp4PartArgs& pa, dim3 grid, hipStream_t stream) {
+  // scale rows that start at multiples of 4 bytes have narrower windows
+  if (((uintptr_t)pa.g.s | (uint64_t)pa.g.s_st) & 3)
+    fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, true><<<grid, kWaves * 64, 0, stream>>>(pa);
+  else fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, false><<<grid, kWaves * 64, 0, stream>>>(pa);
+}
+
+// How a product of up to kShort rows is cut: tiles per workgroup, parts of K.
+// The cheapest by cycles, a workgroup per CU at a time.  Up to 16 rows a
+// workgroup costs its tiles and its start and end, about one and a half tiles.
+// Of more, it costs what goes through its LDS-DMA, about 40 bytes a cycle, most
+// of it x: more tiles on parts of K read less of that, where it pays for the second
+// kernel (64 rows through 4096 x 12288 17.6 us against 23.2 with K whole, 32 rows
+// 13.6 against 14.8; through 4096 x 4096 K stays whole, 11.5).
+struct ShortPlan { int tiles, parts; };
+ShortPlan short_plan(int m, int rows, int k, bool silu) {
+  const int tiles = (rows / (silu ? 2 : 1) + 15) / 16 * (silu ? 2 : 1);
+  const int xr = m <= 16 ? 16 : (m + 15) / 16 * 16;
+  ShortPlan best = {silu ? 2 : 1, 1};
+  double cost = 1e300;
+  for (int t : {1, 2, 4, 6}) {
+    if (silu && t % 2) continue;
+    const int groups = (tiles + t - 1) / t;
+    if (m <= 16) {
+      const double c = ((groups + 255) / 256) * (t + 1.5);
+      if (c <= cost) { cost = c; best = {t, 1}; }
+      continue;
+    }
+    for (int parts : {1, 2, 4}) {
+      if (parts > 1 && k / parts < 128 * kWaves) break;
+      const double bytes = (double)k / parts * (2 * xr + t * 8.5);
+      double c = std::ceil((double)groups * parts / 256) * (bytes / 40 + 6000);
+      if (parts > 1) c += 8000 + (double)parts * m * rows * 8 / 2000;
+      if (c <= cost) { cost = c; best = {t, parts}; }
+    }
+  }
+  return best;
+}
+
+// One tile a workgroup takes a new slice of x with every stage: as many in
+// flight (XD) as stages, in shorter slices where 16 rows of x would not fit.
+template <int MT, int XR, int KS1, int XD1, int KS, bool SILU>
+void launch_tiles(const Fp4GemmArgs& a, float* ws, hipStream_t stream) {
+  const int rows = SILU ? 2 * a.n : a.n;
+  const ShortPlan p = short_plan(a.m, rows, a.k, SILU);
+  const int slices = p.tiles == 1 ? (a.k + KS1 - 1) / KS1 : (a.k + KS - 1) / KS, outs = p.tiles / (SILU ? 2 : 1) * 16;
+  const Fp4PartArgs pa = {a, p.parts > 1 ? ws : nullptr, (int64_t)a.m * rows, (slices + p.parts - 1) / p.parts};
+  const dim3 grid((unsigned)((a.n + outs - 1) / outs), (unsigned)p.parts);
+  switch (p.tiles) {
+    case 1: if constexpr (!SILU) launch<MT, XR, KS1, XD1, 1, SILU>(pa, grid, stream); break;
+    case 2: launch<MT, XR, KS, 1, 2, SILU>(pa, grid, stream); break;
+    case 4: launch<MT, XR, KS, 1, 4, SILU>(pa, grid, stream); break;
+    default: launch<MT, XR, KS, 1, 6, SILU>(pa, grid, stream); break;
+  }
+  if (p.parts > 1) launch_sum<SILU>(pa, p.parts, stream);
+}
+
 // How a product of more than kShort rows is cut: column tiles per wave, row
 // tiles of the weight per wave, parts of K.  The cheapest by cycles: a step costs its
 // matrix instructions (16 cycles each, two waves a SIMD) or its x through
@@ -767,7 +835,7 @@ TilePlan tile_plan(int m, int rows, int k, bool silu) {
 }
 
 template <int NT, bool SILU>
-void launch_tile(const Fp4TileArgs& ta, int mtw, dim3 grid, hipStream_t stream) {
+void launch_tile(const Fp4PartArgs& ta, int mtw, dim3 grid, hipStream_t stream) {
   constexpr int threads = kWaves * 64;
   switch (mtw) {
     case 3: fp4_tile_kernel<NT, 3, SILU><<<grid, threads, 0, stream>>>(ta); break;
@@ -782,34 +850,30 @@ template <bool SILU>
 void dispatch_tile(const Fp4GemmArgs& a, float* ws, hipStream_t stream) {
   const int rows = SILU ? 2 * a.n : a.n, steps = (a.k + 127) / 128;
   const TilePlan p = tile_plan(a.m, rows, a.k, SILU);
-  const Fp4TileArgs ta = {a, p.parts > 1 ? ws : nullptr, (int64_t)a.m * rows, (steps + p.parts - 1) / p.parts};
+  const Fp4PartArgs ta = {a, p.parts > 1 ? ws : nullptr, (int64_t)a.m * rows, (steps + p.parts - 1) / p.parts};
   const dim3 grid((unsigned)((rows + 64 * p.nt - 1) / (64 * p.nt)), (unsigned)((a.m + 32 * p.mtw - 1) / (32 * p.mtw)),
                   (unsigned)p.parts);
   if (p.nt == 4) launch_tile<4, SILU>(ta, p.mtw, grid, stream);
   else if (p.nt == 2) launch_tile<2, SILU>(ta, p.mtw, grid, stream);
   else if constexpr (!SILU) launch_tile<1, SILU>(ta, p.mtw, grid, stream);
-  if (p.parts > 1) {
-    if ((a.out_st & 3) == 0 && ((uintptr_t)a.out & 7) == 0 && (a.n & 3) == 0)
-      fp4_sum_kernel<SILU, true><<<(unsigned)(((int64_t)a.m * a.n / 4 + 255) / 256), 256, 0, stream>>>(ta, p.parts);
-    else
-      fp4_sum_kernel<SILU, false><<<(unsigned)(((int64_t)a.m * a.n + 255) / 256), 256, 0, stream>>>(ta, p.parts);
-  }
+  if (p.parts > 1) launch_sum<SILU>(ta, p.parts, stream);
 }
 
 template <bool SILU>
 void dispatch(const Fp4GemmArgs& a, float* ws, hipStream_t stream) {
-  if (a.m <= 8) launch_tiles<1, 8, 256, 3, 256, SILU>(a, stream);
-  else if (a.m <= 16) launch_tiles<1, 16, 128, 3, 256, SILU>(a, stream);
-  else if (a.m <= 32) launch_tiles<2, 32, 128, 1, 128, SILU>(a, stream);
-  else if (a.m <= kShort) launch_tiles<4, 64, 128, 1, 128, SILU>(a, stream);
+  if (a.m <= 8) launch_tiles<1, 8, 256, 3, 256, SILU>(a, ws, stream);
+  else if (a.m <= 16) launch_tiles<1, 16, 128, 3, 256, SILU>(a, ws, stream);
+  else if (a.m <= 32) launch_tiles<2, 32, 128, 1, 128, SILU>(a, ws, stream);
+  else if (a.m <= 48) launch_tiles<3, 48, 128, 1, 128, SILU>(a, ws, stream);
+  else if (a.m <= kShort) launch_tiles<4, 64, 128, 1, 128, SILU>(a, ws, stream);
   else dispatch_tile<SILU>(a, ws, stream);
 }
 
 }  // namespace
 
 extern "C" size_t xv_mxfp4_gemm_workspace_size(int m, int n, int k, int silu_mul) {
-  if (m <= kShort || n <= 0 || k <= 0) return 0;
-  const int parts = tile_plan(m, n, k, silu_mul != 0).parts;
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const int parts = m <= kShort ? short_plan(m, n, k, silu_mul != 0).parts : tile_plan(m, n, k, silu_mul != 0).parts;
   return parts > 1 ? (size_t)parts * m * n * sizeof(float) : 0;
 }
 
@@ -822,11 +886,11 @@ extern "C" int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int
       (m > 1 && out_stride < (silu_mul ? n / 2 : n)))
     return (int)hipErrorInvalidValue;
   // 32-bit offsets within a tile
-  if (m > 65535 * 64 || w_stride > (1 << 27) || scale_stride > (1 << 27) || x_stride > (1 << 22)) return (int)hipErrorInvalidValue;
+  if (m > 65535 * 64 || w_stride > (1 << 25) || scale_stride > (1 << 27) || x_stride > (1 << 22)) return (int)hipErrorInvalidValue;
   if (m == 0) return 0;
   if (workspace_bytes < xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) || (uintptr_t)workspace & 15)
     return (int)hipErrorInvalidValue;
-  const Fp4GemmArgs a = {(const bf16_t*)x, x_stride, (const uint8_t*)w, w_stride, (const uint8_t*)w_scale, scale_stride,
+  const Fp4GemmArgs a = {(const bf16_t*)x, m > 1 ? x_stride : k, (const uint8_t*)w, w_stride, (const uint8_t*)w_scale, scale_stride,
                          (bf16_t*)out, out_stride, m, silu_mul ? n / 2 : n, k};
   silu_mul ? dispatch<true>(a, (float*)workspace, stream) : dispatch<false>(a, (float*)workspace, stream);
   XV_CHECK_LAUNCH();

@@ -353,6 +353,9 @@ def streamed_into_norm(x: torch.Tensor, w) -> PartialSums:
     return PartialSums(torch.ops.xv.stream_gemm(x, w, GEMM_PARTS, p))
 
 
+MXFP4_WHOLE_ROWS = 16  # up to so many rows xv_mxfp4_gemm never splits K and needs no workspace
+
+
 def _mxfp4_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
     """mxfp4_linear on x [M, K], arguments checked."""
     from .. import _C
@@ -361,13 +364,13 @@ def _mxfp4_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu
     m, k = x.shape
     n = w.shape[0]
     st, inner = x.stride()
-    if inner != 1 or st % 8 or (m > 1 and st < k) or x.data_ptr() % 16:
+    if inner != 1 or st % 8 or (m > 1 and not k <= st <= 1 << 22) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
         st = k
     cols = n // 2 if silu_mul else n
     out = torch.empty((m, cols), dtype=torch.bfloat16, device=x.device)
     if m and cols:
-        nbytes = _C.lib().xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) if m > STREAM_MAX_ROWS else 0
+        nbytes = _C.lib().xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) if m > MXFP4_WHOLE_ROWS else 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         call("xv_mxfp4_gemm", x.get_device(), x.data_ptr(), st, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
              w_scale.stride(0), out.data_ptr(), cols, m, n, k, silu_mul, None if ws is None else ws.data_ptr(), nbytes)
