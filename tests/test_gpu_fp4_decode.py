@@ -3,13 +3,12 @@ attention over the same codes and scales.
 
 Tolerance.  K, V and q are exact in the kernel's bf16 operands, products and
 sums are fp32.  A rounding to bf16 is off by at most 2^-8 of the value (8
-significant bits).  Three count: each weight p * scale (so at most 2^-8 of sum
-p |v| / l, the weighted mean magnitude A of the column), the normalised partial
-of a cut segment (values of at most A, weights summing to 1), the output.  fp32
-sums, exp2 and the score's 2^-24 roundings add less than 2^-12 of A for the
-score sizes here (|s| < 64: an absolute 2^-16 in the exponent).  Together at
-most 3 * 2^-8 A + 2^-12 A < 3.1 * 2^-8 A.  A single rounding is rarely at its
-bound; the kernel is held to 4 * 2^-9 A."""
+significant bits).  Two count: each weight p * scale (so at most 2^-8 of sum
+p |v| / l, the weighted mean magnitude A of the column) and the output; partials
+of a cut segment stay in fp32.  fp32 sums, exp2 and the score's 2^-24 roundings
+add less than 2^-12 of A for the score sizes here (|s| < 64: an absolute 2^-16
+in the exponent).  Together at most 2 * 2^-8 A + 2^-12 A < 2.1 * 2^-8 A.  A
+single rounding is rarely at its bound; the kernel is held to 4 * 2^-9 A."""
 import numpy as np
 import pytest
 import torch

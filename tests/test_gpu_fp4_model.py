@@ -4,8 +4,8 @@ back, chunked prefill and decode, and the model and runner on a 4-bit pool.
 Each stage is held to the oracle's for the very inputs that it had, so that a
 code that falls the other way (one unit in the last place of a key before it)
 is no difference: the store and read back are exact; decode is held to 4 * 2^-9
-of the weighted mean magnitude (roundings of the weights, of a cut segment's
-partial and of the output, 2^-8 each at most); products to 2^-8 of the value
+of the weighted mean magnitude (roundings of the weights and of the output,
+2^-8 each at most); products to 2^-8 of the value
 and (K + 8) 2^-24 of the sum of magnitudes; the dense prefill and the layer's
 other kernels to the bf16 tolerance that their own tests have."""
 import numpy as np

@@ -6,7 +6,7 @@
 //
 // Work split: the (sequence, kv head, 64-token unit) space is flattened in
 // that order and cut into equal contiguous ranges, one per wave, eight waves a
-// CU; segments cut by a range boundary leave partials (normalised bf16 rows and
+// CU; segments cut by a range boundary leave partials (normalised fp32 rows and
 // their log2-sum-exp) for a merge kernel.  A range holds at most two cut
 // segments (its first and its last), so a wave has two partial slots and the
 // workspace does not grow with the table's width.
@@ -59,7 +59,7 @@ struct Fp4DecodeArgs {
   bf16_t* out; int64_t out_st;
   int2* ws_seg;     // (first wave, partials) per (sequence, kv head)
   float* ws_lse;    // log2-sum-exp of partial slot s, head h at s * G + h
-  bf16_t* ws_o;     // its rows, kD values each
+  float* ws_o;      // its rows, kD values each
   int batch, hq, hkv, group;
   int nsub;         // 16-token pages per cache block
   int max_ctx;      // tokens the block table has room for
@@ -315,7 +315,8 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const QSplit& q, int n
       for (int r = 0; r < 4; ++r)
         if (16 * p + 4 * g + r >= ntok) pr[p][r] = 0.f;
   }
-  // p in fp32 for the sum; times the V scale and rounded to bf16 as the operand
+  // p in fp32 for the sum; times the V scale and rounded to bf16 as the operand, as the bf16 pages' kernel rounds it
+  // (a second operand for what that cuts off: 64 rows 43.7 us against 41.0, 48 with 8 heads a group 47.0 against 42.7)
   constexpr int NV = G == 8 ? 2 : 1;
   bf16x8_t pa[NV][2];
   const int shift = 8 * (G == 8 ? c >> 3 : G == 4 ? c >> 2 : (c / G) & 3);
@@ -372,9 +373,26 @@ XV_INLINE void read_q(u32x4_t (&raw)[4], const char* slot, int lane) {
       : "memory");
 }
 
+// 1 KB or less from the stage to row pieces of ROW bytes, BYTES apart in memory.
+template <int SIZE, int ROW, typename Dst>
+XV_INLINE void unstage(uint32_t s0, char* dst, int64_t stride, int lane) {
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes precede its reads
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int k = 0; k < (SIZE + 1023) / 1024; ++k) {
+    const int off = 1024 * k + 16 * lane;
+    if (off < SIZE) {
+      u32x4_t v;
+      __asm__ __volatile__("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(s0 + off) : "memory");
+      *reinterpret_cast<Dst*>(dst + off / ROW * stride + off % ROW) = v;
+    }
+  }
+}
+
 // The finished segment's G rows: the bf16 output if the wave covered the whole
-// segment (part < 0), else partial slot `part`.  They go through `stage` (the
-// q slot, its q in registers) and leave in 16-byte pieces; LDS access in asm.
+// segment (part < 0), else partial slot `part`, in fp32.  They go through
+// `stage` (the q slot, its q in registers), a partial by halves of its rows, and
+// leave in 16-byte pieces; LDS access in asm.
 template <int G>
 XV_INLINE void finish_segment(const Fp4DecodeArgs& a, const Fp4State& st, int b, int kvh, int part, int lane, char* stage) {
   const int c = lane & 15, g = lane >> 4;
@@ -383,34 +401,36 @@ XV_INLINE void finish_segment(const Fp4DecodeArgs& a, const Fp4State& st, int b,
   const float inv[4] = {head_of_row<G, 0>(inv_mine, g), head_of_row<G, 1>(inv_mine, g), head_of_row<G, 2>(inv_mine, g),
                         head_of_row<G, 3>(inv_mine, g)};
   const uint32_t s0 = (uint32_t)reinterpret_cast<uintptr_t>(stage);
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
+  constexpr int kStage = G * kD * 2;
+  auto put = [&](int n, auto store) {  // column tile n: store(head, column within the tile, value)
     const int rep = G == 8 ? (n >> 1) & 1 : n >> 1;  // which operand rows hold the scale block of tile n
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int row = 4 * g + r;
-      if (row / G == rep) {
-        const uint32_t at = s0 + (row % G) * (kD * 2) + 2 * (16 * n + c);
-        __asm__ __volatile__("ds_write_b16 %0, %1" ::"v"(at), "v"(f32_to_bf16(st.o[n][r] * inv[r])) : "memory");
-      }
+      if (row / G == rep) store(row % G, c, st.o[n][r] * inv[r]);
     }
-  }
-  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes precede its reads
-  __builtin_amdgcn_wave_barrier();
-  char* dst = part < 0 ? reinterpret_cast<char*>(a.out + (int64_t)b * a.out_st + (int64_t)kvh * G * kD)
-                       : reinterpret_cast<char*>(a.ws_o + (int64_t)part * G * kD);
-  constexpr int kBytes = G * kD * 2;
+  };
+  if (part < 0) {
 #pragma unroll
-  for (int k = 0; k < (kBytes + 1023) / 1024; ++k) {
-    const int off = 1024 * k + 16 * lane;
-    if (off < kBytes) {
-      u32x4_t v;
-      __asm__ __volatile__("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(s0 + off) : "memory");
-      typedef u32x4_t __attribute__((aligned(4))) u32x4_a4;  // the caller's rows need not be 16-byte aligned
-      *reinterpret_cast<u32x4_a4*>(dst + off) = v;
-    }
+    for (int n = 0; n < 8; ++n)
+      put(n, [&](int h, int col, float v) {
+        __asm__ __volatile__("ds_write_b16 %0, %1" ::"v"(s0 + h * (kD * 2) + 2 * (16 * n + col)), "v"(f32_to_bf16(v)) : "memory");
+      });
+    typedef u32x4_t __attribute__((aligned(4))) u32x4_a4;  // the caller's rows need not be 16-byte aligned
+    unstage<kStage, kStage, u32x4_a4>(s0, reinterpret_cast<char*>(a.out + (int64_t)b * a.out_st + (int64_t)kvh * G * kD), 0, lane);
+    return;
   }
-  if (part >= 0 && lane < G) a.ws_lse[(int64_t)part * G + lane] = st.m + __log2f(lsum);
+  char* const dst = reinterpret_cast<char*>(a.ws_o + (int64_t)part * G * kD);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+#pragma unroll
+    for (int n = 4 * half; n < 4 * half + 4; ++n)
+      put(n, [&](int h, int col, float v) {
+        __asm__ __volatile__("ds_write_b32 %0, %1" ::"v"(s0 + h * (kD * 2) + 4 * (16 * (n & 3) + col)), "v"(v) : "memory");
+      });
+    unstage<kStage, kD * 2, u32x4_t>(s0, dst + half * (kD * 2), kD * 4, lane);
+  }
+  if (lane < G) a.ws_lse[(int64_t)part * G + lane] = st.m + __log2f(lsum);
 }
 
 // Block ids of the wave's stream, 4 pages a unit, in a double-buffered LDS
@@ -595,10 +615,15 @@ __global__ __launch_bounds__(256) void fp4_merge_kernel(Fp4DecodeArgs a) {
   auto slot = [&](int j) { return (j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.group + hg; };  // < 2^15
   const int g = lane >> 4, i = lane & 15;
   constexpr int kAhead = 4;  // partials in flight per lane row
-  Vec8 r[kAhead];
+  floatx4_t r[kAhead][2];
+  auto load = [&](int k, int j) {
+    const floatx4_t* from = reinterpret_cast<const floatx4_t*>(a.ws_o + slot(min(j, n - 1)) * kD + 8 * i);
+    r[k][0] = from[0];
+    r[k][1] = from[1];
+  };
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
-    if (4 * k < n) r[k] = load_vec8(a.ws_o + slot(min(4 * k + g, n - 1)) * kD + 8 * i);
+    if (4 * k < n) load(k, 4 * k + g);
   // lane j: the log2-sum-exps of partials j, 64 + j, 128 + j
   const float la = lane < n ? a.ws_lse[slot(lane)] : -INFINITY;
   float lb = -INFINITY, lc = -INFINITY;
@@ -610,13 +635,14 @@ __global__ __launch_bounds__(256) void fp4_merge_kernel(Fp4DecodeArgs a) {
   const float wa = __builtin_amdgcn_exp2f(la - mx), wb = __builtin_amdgcn_exp2f(lb - mx), wc = __builtin_amdgcn_exp2f(lc - mx);
   const float den = wave_sum(wa + wb + wc);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto fold = [&](const Vec8& row, int j) {  // partial j of this lane row (the four rows' lie in one block of 64)
+  auto fold = [&](floatx4_t lo, floatx4_t hi, int j) {  // partial j of this lane row (the four rows' lie in one block of 64)
     const float w = __shfl(j < 64 ? wa : j < 128 ? wb : wc, j & 63);
-    float f[8];
-    unpack8(row, f);
     if (j < n) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += w * f[e];
+      for (int e = 0; e < 4; ++e) {
+        acc[e] += w * lo[e];
+        acc[4 + e] += w * hi[e];
+      }
     }
   };
   for (int j0 = 0; j0 < n; j0 += 4 * kAhead) {
@@ -624,9 +650,9 @@ __global__ __launch_bounds__(256) void fp4_merge_kernel(Fp4DecodeArgs a) {
     for (int k = 0; k < kAhead; ++k) {
       const int j = j0 + 4 * k;
       if (j >= n) break;
-      const Vec8 cur = r[k];
-      if (j + 4 * kAhead < n) r[k] = load_vec8(a.ws_o + slot(min(j + 4 * kAhead + g, n - 1)) * kD + 8 * i);
-      fold(cur, j + g);
+      const floatx4_t lo = r[k][0], hi = r[k][1];
+      if (j + 4 * kAhead < n) load(k, j + 4 * kAhead + g);
+      fold(lo, hi, j + g);
     }
   }
 #pragma unroll
@@ -660,7 +686,7 @@ size_t lse_bytes(int group) { return al256((size_t)kMaxWaves * 2 * group * sizeo
 extern "C" size_t xv_paged_decode_fp4_workspace_size(int batch, int num_q_heads, int num_kv_heads) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads) return 256;
   const int group = num_q_heads / num_kv_heads;
-  return seg_bytes(batch, num_kv_heads) + lse_bytes(group) + (size_t)kMaxWaves * 2 * group * kD * sizeof(bf16_t);
+  return seg_bytes(batch, num_kv_heads) + lse_bytes(group) + (size_t)kMaxWaves * 2 * group * kD * sizeof(float);
 }
 
 extern "C" int xv_paged_decode_attention_fp4(
@@ -701,7 +727,7 @@ extern "C" int xv_paged_decode_attention_fp4(
   a.bt_stride = bt_stride; a.out_st = out_stride_tok;
   a.ws_seg = (int2*)workspace;
   a.ws_lse = (float*)((char*)workspace + seg_bytes(batch, num_kv_heads));
-  a.ws_o = (bf16_t*)((char*)a.ws_lse + lse_bytes(group));
+  a.ws_o = (float*)((char*)a.ws_lse + lse_bytes(group));
   a.hq = num_q_heads; a.hkv = num_kv_heads; a.group = group;
   a.nsub = block_size / 16; a.max_ctx = (int)max_ctx;
   a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
