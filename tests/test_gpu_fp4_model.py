@@ -185,6 +185,8 @@ def test_prefill_over_pages_refuses_what_it_cannot_size(dev):
         prefill_attention(*args, **scales)
     with pytest.raises(ValueError, match="block_scale"):
         prefill_attention(*args, max_seqlen_k=3)
+    with pytest.raises(ValueError, match="not 4-bit pages"):
+        prefill_attention(*args[:7], 4, *args[8:], max_seqlen_k=3, **scales)
 
 
 def test_layer_decode_on_a_4bit_pool(dev):

@@ -349,6 +349,8 @@ def prefill_attention(
         # 4-bit pages: the sequences' keys and values as varlen bf16 rows (exact), then the dense path
         if max_seqlen_k <= 0:
             raise ValueError("prefill over a 4-bit paged cache needs max_seqlen_k (the longest key run)")
+        if k_cache.dim() != 4 or k_cache.shape[2] != num_kv_heads or k_cache.shape[3] * 2 != head_dim:
+            raise ValueError(f"cache {tuple(k_cache.shape)} is not 4-bit pages [NB, BS, {num_kv_heads}, {head_dim} / 2]")
         kd, vd = gather_kvcache(k_cache, v_cache, block_tables, cuk, bsz * int(max_seqlen_k),
                                 k_block_scale=k_block_scale, v_block_scale=v_block_scale)
         return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
