@@ -25,7 +25,8 @@ bool cache_ok(const Fp4Cache& c) {
 // of a 32-value block agree on its scale over DPP.  A workgroup takes 16 tokens
 // and kHeads heads, a lane the same place of each, so that its token's slot is
 // looked up once and the heads' loads travel together.  (One flat index per 8
-// values, with its three divisions, took 10.0 us for 8192 tokens of 8 heads.)
+// values, with its three divisions, took 10.0 us for 8192 tokens of 8 heads; this
+// 9.6 us, 4.4 TB/s.)
 constexpr int kTokens = 16, kHeads = 4;
 __global__ __launch_bounds__(256) void store_kvcache_fp4_kernel(
     const bf16_t* __restrict__ key, int64_t ks_tok, int64_t ks_head, const bf16_t* __restrict__ value, int64_t vs_tok,
@@ -94,7 +95,12 @@ extern "C" int xv_store_kvcache_fp4(const void* key, int64_t key_stride_tok, int
 // values, 8 of K and of V each (4 bytes in, 16 out), the heads' loads in
 // flight together.  Rows past the last sequence (or of blocks past the table's
 // width) are left as they are.
-constexpr int kGatherHeads = 8;
+// Bound by the rows it writes: 16 sequences of 1229 tokens on average, 8 heads
+// (81 MB out), with the store of their last 512 before it 28.9 us, of which this
+// about 19.  The codes are loaded as usual, a chunk's store has just written some
+// of them (non-temporal: 31.2); eight heads in place of four: no faster, and 77
+// tokens 7.1 us against 6.4.
+constexpr int kGatherHeads = 4;
 __global__ __launch_bounds__(256) void gather_kv_fp4_kernel(
     Fp4Cache cd, const int32_t* __restrict__ bt, int64_t bt_stride, int max_blocks, const int32_t* __restrict__ cu,
     int batch, int total_rows, int heads, int chunks_per_head, bf16_t* __restrict__ ko, bf16_t* __restrict__ vo,
@@ -132,8 +138,8 @@ __global__ __launch_bounds__(256) void gather_kv_fp4_kernel(
     for (int j = 0; j < kGatherHeads; ++j) {
       if (h0 + j >= heads) break;
       const int64_t at = at0 + (h0 + j) * cd.hs + d8 * 4, sat = sat0 + (h0 + j) * cd.shs + (d8 >> 2);
-      kw[j] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(cd.kc + at));
-      vw[j] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(cd.vc + at));
+      kw[j] = *reinterpret_cast<const uint32_t*>(cd.kc + at);
+      vw[j] = *reinterpret_cast<const uint32_t*>(cd.vc + at);
       kb[j] = cd.ks[sat];
       vb[j] = cd.vs[sat];
     }
