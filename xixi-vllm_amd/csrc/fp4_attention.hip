@@ -27,6 +27,11 @@
 //   of the 16 operand rows, so row rep * G + h takes head h scaled for block
 //   rep (G = 8: two operands of two blocks): all blocks in one product, and
 //   the outputs of the other blocks' rows are not used.
+//
+// 64 sequences of 512 .. 4096 tokens (32 heads over 8) take 41.0 us: 12 of
+// launches, start (lengths, then block ids, then pages) and merge, the rest at
+// a copy's rate; four of 40000 .. 130000 (16 over 8) 76 us, 5.1 TB/s over the
+// whole call.
 #include "xv_decode.h"
 #include "xv_fp4.h"
 #include "xv_kernels.h"

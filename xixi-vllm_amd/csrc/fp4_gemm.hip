@@ -14,8 +14,8 @@
 // end), and a wave runs its T tiles over one slice before the next: x is read
 // once per workgroup and its slice waits in registers, while the weight streams
 // through a private LDS ring.  Both travel by LDS-DMA, whole row segments per
-// instruction.  One row through a gate / up weight of 24576 x 4096 takes 12.1 us
-// (4.4 TB/s), 8 rows through 4096 x 12288 9.6 us.  Direct loads into the operand
+// instruction.  One row through a gate / up weight of 24576 x 4096 takes 12.5 us
+// (4.3 TB/s), 8 rows through 4096 x 12288 9.5 us.  Direct loads into the operand
 // registers, where neighbouring lanes are neighbouring rows, were bound by the
 // address unit (weights so: 22 us for the first; x alone so: 12.7 us for the
 // second).  Every workgroup reads all of its part of x through its LDS-DMA, which
