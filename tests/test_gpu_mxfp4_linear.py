@@ -148,3 +148,28 @@ def test_refusals(dev):
         mxfp4_linear(x, w.view(torch.uint8).t().contiguous().t().view(w.dtype), s)
     with pytest.raises(RuntimeError):
         mxfp4_linear(x.requires_grad_(), w, s)
+
+
+@pytest.mark.parametrize("silu", [False, True])
+def test_product_in_a_compiled_function(dev, silu):
+    """A compiler's trace holds the product as one op, with the eager result."""
+    from xvllm.layers.linear import mxfp4_linear
+
+    rng = np.random.default_rng(31)
+    w, s = _weight(rng, 64, 96)
+    w, s = as_codes(torch.from_numpy(w).to(dev)), as_scales(torch.from_numpy(s).to(dev))
+    x = torch.from_numpy(rng.standard_normal((2, 5, 96)).astype(np.float32)).to(torch.bfloat16).to(dev)
+    f = torch.compile(lambda t: mxfp4_linear(t * 2, w, s, silu_mul=silu) + 1, backend="eager", fullgraph=True)
+    with torch.no_grad():
+        got, want = f(x), mxfp4_linear(x * 2, w, s, silu_mul=silu) + 1
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_product_op_registration(dev):
+    import xvllm.layers.linear  # noqa: F401  (registers the op)
+
+    rng = np.random.default_rng(32)
+    w, s = (torch.from_numpy(a).to(dev) for a in _weight(rng, 32, 64))
+    x = torch.zeros((3, 64), dtype=torch.bfloat16, device=dev)
+    torch.library.opcheck(torch.ops.xv.mxfp4_linear, (x, w, s, False), test_utils=("test_schema", "test_faketensor"))

@@ -158,7 +158,7 @@ XV_INLINE void read_unit(UnitRegs& u, const char* buf, const Fp4Lane& lo, const 
       "ds_read_b128 %0, %21\n\t"
       "ds_read_b128 %1, %21 offset:1024\n\t"
       "ds_read_b128 %2, %21 offset:2048\n\t"
-      "ds_read_b128 %3, %21 offset:3072\n\t"
+      "ds_read_b128 %3, %21 offset:0xc00\n\t"
       "ds_read_b32 %4, %26\n\t"
       "ds_read_b32 %5, %26 offset:64\n\t"
       "ds_read_b32 %6, %26 offset:128\n\t"

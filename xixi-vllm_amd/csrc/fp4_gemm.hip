@@ -886,7 +886,7 @@ extern "C" int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int
       (m > 1 && out_stride < (silu_mul ? n / 2 : n)))
     return (int)hipErrorInvalidValue;
   // 32-bit offsets within a tile
-  if (m > 65535 * 64 || w_stride > (1 << 25) || scale_stride > (1 << 27) || x_stride > (1 << 22)) return (int)hipErrorInvalidValue;
+  if (m > 65535 * 64 || w_stride > (1 << 25) || scale_stride > (1 << 27) || (m > 1 && x_stride > (1 << 22))) return (int)hipErrorInvalidValue;
   if (m == 0) return 0;
   if (workspace_bytes < xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) || (uintptr_t)workspace & 15)
     return (int)hipErrorInvalidValue;
