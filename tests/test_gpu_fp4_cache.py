@@ -123,6 +123,31 @@ def test_gather_is_exact(dev, ctx, hkv, d, page, layout):
         assert (got[total:] == 7).all()
 
 
+def test_gather_of_more_than_the_last_level_cache(dev):
+    """Outputs of more than 256 MB are written another way: every row of four
+    long sequences over the same few blocks, the rows behind them untouched."""
+    from xvllm.kv_ops import gather_kvcache
+
+    rng = np.random.default_rng(6)
+    ctx, page, nb = [16500, 16401, 17000, 16001], 16, 40
+    kc, ks = random_pages(rng, nb, page, 8, 128)
+    vc, vs = random_pages(rng, nb, page, 8, 128)
+    bt = rng.integers(0, nb, (4, -(-max(ctx) // page))).astype(np.int32)
+    cu = np.concatenate([[0], np.cumsum(ctx)])
+    total = int(cu[-1]) + 5
+    assert total * 8 * 128 * 4 > 256 << 20
+    out = tuple(torch.full((total, 8, 128), 77.0, dtype=torch.bfloat16, device=dev) for _ in "kv")
+    dkc, dvc, dks, dvs = (on_device(a, dev, "hnd") for a in (kc, vc, ks, vs))
+    gather_kvcache(as_codes(dkc), as_codes(dvc), torch.from_numpy(bt).to(dev), torch.from_numpy(cu.astype(np.int32)).to(dev), total,
+                   k_block_scale=as_scales(dks), v_block_scale=as_scales(dvs), out=out)
+    torch.cuda.synchronize()
+    rows = torch.from_numpy(np.concatenate([bt[b, np.arange(n) // page] * page + np.arange(n) % page for b, n in enumerate(ctx)]))
+    for got, c, s in ((out[0], kc, ks), (out[1], vc, vs)):
+        pool = torch.from_numpy(O.dequantize_fp4(c, s).reshape(nb * page, 8, 128)).to(torch.bfloat16).to(dev)
+        assert torch.equal(got[:-5], pool[rows.to(dev)])
+        assert (got[-5:] == 77).all()
+
+
 def test_written_rows_read_back_in_a_graph(dev):
     """Store and read back recorded into one graph and replayed over new
     inputs: every replay equals the eager pair."""

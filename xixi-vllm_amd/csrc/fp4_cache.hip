@@ -96,11 +96,18 @@ extern "C" int xv_store_kvcache_fp4(const void* key, int64_t key_stride_tok, int
 // flight together.  Rows past the last sequence (or of blocks past the table's
 // width) are left as they are.
 // Bound by the rows it writes: 16 sequences of 1229 tokens on average, 8 heads
-// (81 MB out), with the store of their last 512 before it 28.9 us, of which this
-// about 19.  The codes are loaded as usual, a chunk's store has just written some
-// of them (non-temporal: 31.2); eight heads in place of four: no faster, and 77
-// tokens 7.1 us against 6.4.
-constexpr int kGatherHeads = 4;
+// (81 MB out), with the store of their last 512 before it 28.8 us, of which this
+// about 19; three of 20000 to 35000 (306 MB out) 78 us, 6.2 TB/s.  The codes are
+// loaded as usual, a chunk's store has just written some of them (non-temporal:
+// 31.2 us for the first); four heads in place of two: two sequences of 64000 124 us
+// against 120, eight: 77 tokens 7.1 us against 6.5.
+// Outputs that the last-level cache (256 MB) can hold are written as usual, for
+// the prefill that reads them next (189 MB of them and that prefill 721 us against
+// 737 non-temporal); larger ones non-temporally (NT: the second case 78 us against
+// 104, though with its prefill 2594 against 2575).
+constexpr int kGatherHeads = 2;
+constexpr int64_t kCached = 256ll << 20;
+template <bool NT>
 __global__ __launch_bounds__(256) void gather_kv_fp4_kernel(
     Fp4Cache cd, const int32_t* __restrict__ bt, int64_t bt_stride, int max_blocks, const int32_t* __restrict__ cu,
     int batch, int total_rows, int heads, int chunks_per_head, bf16_t* __restrict__ ko, bf16_t* __restrict__ vo,
@@ -150,8 +157,13 @@ __global__ __launch_bounds__(256) void gather_kv_fp4_kernel(
       fp4x8_to_bf16(kw[j], fp4_scale(kb[j]), k.w);
       fp4x8_to_bf16(vw[j], fp4_scale(vb[j]), v.w);
       const int64_t dst = (int64_t)(row0 + r) * o_st + ((h0 + j) * chunks_per_head + d8) * 8;
-      store_vec8(ko + dst, k);
-      store_vec8(vo + dst, v);
+      if constexpr (NT) {
+        store_vec8_nt(ko + dst, k);
+        store_vec8_nt(vo + dst, v);
+      } else {
+        store_vec8(ko + dst, k);
+        store_vec8(vo + dst, v);
+      }
     }
   }
 }
@@ -175,9 +187,10 @@ extern "C" int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_
   if (batch == 0 || total_tokens == 0) return 0;
   if (num_kv_heads > 65535 * kGatherHeads || (int64_t)num_kv_heads * head_dim > INT32_MAX) return (int)hipErrorInvalidValue;
   const dim3 grid((unsigned)((total_tokens + kTokens - 1) / kTokens), (unsigned)((num_kv_heads + kGatherHeads - 1) / kGatherHeads));
-  gather_kv_fp4_kernel<<<grid, 256, 0, stream>>>(cd, block_tables, bt_stride, max_blocks_per_seq, cu_seqlens_k, batch,
-                                                 (int)total_tokens, num_kv_heads, head_dim / 8, (bf16_t*)k_out,
-                                                 (bf16_t*)v_out, out_stride_tok);
+  const bool large = total_tokens * num_kv_heads * head_dim * 4 > kCached;
+  (large ? gather_kv_fp4_kernel<true> : gather_kv_fp4_kernel<false>)<<<grid, 256, 0, stream>>>(
+      cd, block_tables, bt_stride, max_blocks_per_seq, cu_seqlens_k, batch, (int)total_tokens, num_kv_heads, head_dim / 8,
+      (bf16_t*)k_out, (bf16_t*)v_out, out_stride_tok);
   XV_CHECK_LAUNCH();
   return 0;
 }
