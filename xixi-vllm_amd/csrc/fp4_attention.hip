@@ -518,7 +518,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
 
   // Unit y, whose cursor is ic and whose block ids are idv, into its ring
-  // slot.  A page's rows past the sequence's end are read as they are (they are
+  // slot, non-temporally (64 rows 41.2 us, 44.6 through the caches).  A page's rows past the sequence's end are read as they are (they are
   // masked, and every code is finite); their scales are those of the last token.
   auto issue = [&](int y, const u32x4_t& idv) {
     char* buf = mine + (y & 1) * kUnitLds;

@@ -778,7 +778,7 @@ ShortPlan short_plan(int m, int rows, int k, bool silu) {
       if (c <= cost) { cost = c; best = {t, 1}; }
       continue;
     }
-    for (int parts : {1, 2, 4}) {
+    for (int parts : {1, 2, 4, 8}) {
       if (parts > 1 && k / parts < 128 * kWaves) break;
       const double bytes = (double)k / parts * (2 * xr + t * 8.5);
       double c = std::ceil((double)groups * parts / 256) * (bytes / 40 + 6000);
@@ -822,7 +822,7 @@ TilePlan tile_plan(int m, int rows, int k, bool silu) {
   double cost = 1e300;
   for (int nt : {4, 2, 1}) {
     if (silu && nt == 1) continue;
-    for (int parts : {1, 2, 4, 8}) {
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (parts > 1 && steps / parts < 4) break;
       const double groups = (double)((rows + 64 * nt - 1) / (64 * nt)) * ((m + 32 * mtw - 1) / (32 * mtw)) * parts;
       const double step = std::max(128.0 * nt * mtw, 200.0 * mtw) + 700.0;
