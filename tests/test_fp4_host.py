@@ -150,7 +150,7 @@ def _gemm(lib, **kw):
 def test_gemm_rejects_bad_arguments(lib):
     for kw in (dict(x=None), dict(x=A + 8), dict(xst=4092), dict(xst=4088), dict(w=A + 8), dict(w=None), dict(wst=2040),
                dict(wst=2032), dict(s=None), dict(sst=127), dict(out=None), dict(out=A + 1), dict(ost=1023), dict(m=-1),
-               dict(n=0), dict(k=0), dict(k=4080), dict(n=1023, silu=1), dict(m=1 << 23), dict(m=200), dict(ws=A + 8)):
+               dict(n=0), dict(k=0), dict(k=4080), dict(n=1023, silu=1), dict(m=1 << 23), dict(n=(1 << 30) + 2), dict(m=200), dict(ws=A + 8)):
         assert _gemm(lib, **kw) == INVALID, kw
     assert _gemm(lib, m=0) == 0
 

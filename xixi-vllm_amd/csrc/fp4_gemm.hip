@@ -767,7 +767,7 @@ void launch(const Fp4PartArgs& pa, dim3 grid, hipStream_t stream) {
 struct ShortPlan { int tiles, parts; };
 ShortPlan short_plan(int m, int rows, int k, bool silu) {
   const int tiles = (rows / (silu ? 2 : 1) + 15) / 16 * (silu ? 2 : 1);
-  const int xr = m <= 16 ? 16 : (m + 15) / 16 * 16;
+  const int xr = (m + 15) / 16 * 16;  // rows of x that are fetched
   ShortPlan best = {silu ? 2 : 1, 1};
   double cost = 1e300;
   for (int t : {1, 2, 4, 6}) {
@@ -885,8 +885,8 @@ extern "C" int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int
       (m > 1 && x_stride < k) || w_stride < k / 2 || scale_stride < k / kFp4Block || (uintptr_t)out & 1 ||
       (m > 1 && out_stride < (silu_mul ? n / 2 : n)))
     return (int)hipErrorInvalidValue;
-  // 32-bit offsets within a tile
-  if (m > 65535 * 64 || w_stride > (1 << 25) || scale_stride > (1 << 27) || (m > 1 && x_stride > (1 << 22))) return (int)hipErrorInvalidValue;
+  // 32-bit offsets within a tile, rows that round up
+  if (m > 65535 * 64 || n > (1 << 30) || w_stride > (1 << 25) || scale_stride > (1 << 27) || (m > 1 && x_stride > (1 << 22))) return (int)hipErrorInvalidValue;
   if (m == 0) return 0;
   if (workspace_bytes < xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) || (uintptr_t)workspace & 15)
     return (int)hipErrorInvalidValue;
