@@ -320,14 +320,16 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const QSplit& q, int n
       for (int r = 0; r < 4; ++r)
         if (16 * p + 4 * g + r >= ntok) pr[p][r] = 0.f;
   }
-  // p in fp32 for the sum; times the V scale and rounded to bf16 as the operand, as the bf16 pages' kernel rounds it
-  // (a second operand for what that cuts off: 64 rows 43.7 us against 41.0, 48 with 8 heads a group 47.0 against 42.7)
+  // p in fp32 for the sum; times the V scale as the sum of two bf16 operands, its nearest bf16 and the nearest one
+  // of the rest, together within 2^-16 of it.  (The first alone, within 2^-8: 64 rows 40.8 us against 43.5, 48 with 8
+  // heads a group 43.0 against 46.2, but where few tokens share the weight its error is as large as the output's own
+  // rounding.)
   constexpr int NV = G == 8 ? 2 : 1;
-  bf16x8_t pa[NV][2];
+  bf16x8_t pa[NV][2], pb[NV][2];
   const int shift = 8 * (G == 8 ? c >> 3 : G == 4 ? c >> 2 : (c / G) & 3);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    uint32_t w[NV][4];
+    uint32_t w[NV][4], rest[NV][4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       const int p = 2 * j + e / 4, r = e % 4;
@@ -337,17 +339,26 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const QSplit& q, int n
         // the low mantissa bit turns scale 255 into a NaN and moves the others by 2^-23 of themselves
         const float f0 = __uint_as_float((__builtin_amdgcn_ubfe(u.vs[p][r], shift + 16 * v, 8) << 23) | 1u);
         const float f1 = __uint_as_float((__builtin_amdgcn_ubfe(u.vs[p][r + 1], shift + 16 * v, 8) << 23) | 1u);
-        w[v][e / 2] = pack_bf16x2(pr[p][r] * f0, pr[p][r + 1] * f1);
+        const float p0 = pr[p][r] * f0, p1 = pr[p][r + 1] * f1;
+        w[v][e / 2] = pack_bf16x2(p0, p1);
+        rest[v][e / 2] = pack_bf16x2(p0 - bf16lo(w[v][e / 2]), p1 - bf16hi(w[v][e / 2]));
       }
     }
 #pragma unroll
-    for (int v = 0; v < NV; ++v) __builtin_memcpy(&pa[v][j], w[v], 16);
+    for (int v = 0; v < NV; ++v) {
+      __builtin_memcpy(&pa[v][j], w[v], 16);
+      __builtin_memcpy(&pb[v][j], rest[v], 16);
+    }
   }
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
     const int v = NV == 2 ? n / 4 : 0;
-    st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[v][0], widen8(u.v[n][0]), st.o[n], 0, 0, 0);
-    st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[v][1], widen8(u.v[n][1]), st.o[n], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bf16x8_t t = widen8(u.v[n][j]);
+      st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pb[v][j], t, st.o[n], 0, 0, 0);
+      st.o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa[v][j], t, st.o[n], 0, 0, 0);
+    }
   }
 }
 
