@@ -187,8 +187,10 @@ int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_pag
 /*
  * xv_paged_decode_attention over a 4-bit (MXFP4) cache written by
  * xv_store_kvcache_fp4.  No counterpart in the reference (its pool holds the
- * model dtype).  K and V are the codes times their block scales, exactly;
- * strides of the codes and of the scales in bytes as there, the codes' base and
+ * model dtype).  K and V are the codes times their block scales, exactly, at
+ * every scale byte (255: NaN; a softmax weight times V's scale is held to 2^-16
+ * of itself, and to 2^-134 where it is below 2^-118, or to 2^-94 below 2^-78 in
+ * 64 tokens that also hold a V scale of 2^65 or more); strides of the codes and of the scales in bytes as there, the codes' base and
  * strides multiples of 16, the scales' of 4, head_dim 128.  A sequence is read
  * up to max_blocks_per_seq * block_size tokens at most (256M at most).
  * workspace: xv_paged_decode_fp4_workspace_size(...) bytes, 16-byte aligned, no

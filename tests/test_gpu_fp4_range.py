@@ -1,6 +1,6 @@
-"""Decode attention over 4-bit pages to more than the output's own rounding:
-weights that few tokens share, queries whose 32-value blocks differ widely in
-size.
+"""Decode attention over 4-bit pages to more than the output's own rounding, and
+at the ends of its number formats: V scale
+bytes from 0 to 252, weights that few tokens share, queries whose 32-value blocks differ widely in size.
 
 Tolerance, by element: one rounding of the output to bf16, at most 2^-8 of the
 value (2^-134 where the result is subnormal); the weights, held in two bf16
@@ -8,7 +8,10 @@ terms (the second rounds what the first left, 2^-8 of the weight at most, by
 at most 2^-8 of itself), off by at most 2^-16 of A, the weighted mean magnitude
 of the column; the exponent of a weight off by the score's own error E (absolute,
 in units of the exponent), which moves weights and their sum by E each: 2 E A.
-fp32 sums and exp2 add less than 2^-13 A.  E is 2^-24 (128 + 8) sum |q k| scale
+fp32 sums and exp2 add less than 2^-13 A.  Weights times a V scale are off by
+2^-134 where they are subnormal, times 6 at most, n tokens of them over a sum of
+weights of at least 1, or 2^-40 with V scales of 2^65 and more (whose weights are
+kept that much lower): 6 n 2^-134, or 2^-94.  E is 2^-24 (128 + 8) sum |q k| scale
 for the 128-term sums, plus what q's two e4m3 terms leave: nothing of a value
 within 2^-10 of its block's largest, at most 2^-21 of the largest otherwise."""
 import numpy as np
@@ -40,7 +43,8 @@ def _reference(q, kc, ks, vc, vs, bt, ctx):
             w /= w.sum()
             a = w @ np.abs(vh)
             out[b, h] = w @ vh
-            tol[b, h] = 2.0 ** -8 * np.abs(out[b, h]) + (2.0 ** -16 + 2.0 ** -13 + 2 * e) * a + 2.0 ** -134
+            small = 6 * n * 2.0 ** (-94 if (vs[ids][..., h // (hq // hkv), :] >= 192).any() else -134)
+            tol[b, h] = 2.0 ** -8 * np.abs(out[b, h]) + (2.0 ** -16 + 2.0 ** -13 + 2 * e) * a + 2.0 ** -134 + small
     return out, tol
 
 
@@ -81,6 +85,31 @@ def test_few_tokens_share_the_weight(dev, hq, hkv):
     case = _inputs(rng, ctx, hq, hkv)
     q, *rest = case
     _check(_call(dev, *case, ctx, hkv), *_reference(q.double().numpy(), *rest, ctx))
+
+
+@pytest.mark.parametrize("hq,hkv", GROUPS)
+@pytest.mark.parametrize("low,high", [(0, 0), (0, 3), (1, 40), (0, 130), (100, 252), (192, 215), (245, 252), (0, 252)])
+def test_v_scale_bytes_of_any_size(dev, hq, hkv, low, high):
+    """Short, cut and ragged sequences whose V scales span a part of the format."""
+    rng = np.random.default_rng(low * 256 + high + hq)
+    ctx = [1, 5, 64, 65, 700, 130, 33, 2100]
+    case = _inputs(rng, ctx, hq, hkv, v=(low, high))
+    q, *rest = case
+    _check(_call(dev, *case, ctx, hkv), *_reference(q.double().numpy(), *rest, ctx))
+
+
+@pytest.mark.parametrize("hq,hkv", GROUPS)
+def test_v_scales_that_change_along_the_sequence(dev, hq, hkv):
+    """Units of 64 tokens of tiny, ordinary and huge V in turn, with scores that climb, fall or stay."""
+    rng = np.random.default_rng(hq + 50)
+    ctx, page = [900, 901, 902], 16
+    q, kc, ks, vc, vs, bt = _inputs(rng, ctx, hq, hkv)
+    for b in range(3):
+        for j, p in enumerate(bt[b, : -(-ctx[b] // page)]):
+            vs[p] = rng.integers(*[(0, 30), (118, 130), (230, 253)][(j // 4 + b) % 3], vs[p].shape)
+            ks[p] = [110 + j // 4, 124 - j // 4, 122][b]
+    case = q, kc, ks, vc, vs, bt
+    _check(_call(dev, *case, ctx, hkv), *_reference(q.double().numpy(), *case[1:], ctx))
 
 
 @pytest.mark.parametrize("hq,hkv", GROUPS)

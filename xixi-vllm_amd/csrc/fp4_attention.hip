@@ -124,6 +124,7 @@ struct Fp4Lane {
   uint32_t k;      // K operand, row block 0 (block p: + 1024 p)
   uint32_t v[4];   // transposed V reads of tiles 2m (tile 2m + 1: 8 bytes on)
   uint32_t ks, vs; // scales
+  uint32_t own;    // V scales of token `lane`
 };
 
 XV_INLINE Fp4Lane lane_offsets(uint32_t tok_stride, int lane) {
@@ -138,6 +139,7 @@ XV_INLINE Fp4Lane lane_offsets(uint32_t tok_stride, int lane) {
     o.v[m] = (uint32_t)(kVOff + 1024 * (i >> 2) + 64 * (4 * g + (i & 3)) + ((m ^ swz4(4 * g)) << 4));
   o.ks = (uint32_t)(kKsOff + 4 * i);
   o.vs = (uint32_t)(kVsOff + 16 * g);
+  o.own = (uint32_t)(kVsOff + 4 * lane);
   return o;
 }
 
@@ -146,6 +148,7 @@ struct UnitRegs {
   uint32_t ks[4];    // the scale bytes of those tokens
   uint32_t v[8][2];  // V codes of column tiles 0..7, 16 tokens each
   u32x4_t vs[4];     // scale bytes of tokens 16p + 4g .. + 3
+  uint32_t own;      // those of token `lane`
   u32x4_t ids;       // block ids of a later unit
 };
 
@@ -155,33 +158,35 @@ XV_INLINE void read_unit(UnitRegs& u, const char* buf, const Fp4Lane& lo, const 
   const uint32_t b = (uint32_t)reinterpret_cast<uintptr_t>(buf);
   u32x2_t v[8];
   __asm__ __volatile__(
-      "ds_read_b128 %0, %21\n\t"
-      "ds_read_b128 %1, %21 offset:1024\n\t"
-      "ds_read_b128 %2, %21 offset:2048\n\t"
-      "ds_read_b128 %3, %21 offset:0xc00\n\t"
-      "ds_read_b32 %4, %26\n\t"
-      "ds_read_b32 %5, %26 offset:64\n\t"
-      "ds_read_b32 %6, %26 offset:128\n\t"
-      "ds_read_b32 %7, %26 offset:192\n\t"
-      "ds_read_b64_tr_b4 %8, %22\n\t"
-      "ds_read_b64_tr_b4 %9, %22 offset:8\n\t"
-      "ds_read_b64_tr_b4 %10, %23\n\t"
-      "ds_read_b64_tr_b4 %11, %23 offset:8\n\t"
-      "ds_read_b64_tr_b4 %12, %24\n\t"
-      "ds_read_b64_tr_b4 %13, %24 offset:8\n\t"
-      "ds_read_b64_tr_b4 %14, %25\n\t"
-      "ds_read_b64_tr_b4 %15, %25 offset:8\n\t"
-      "ds_read_b128 %16, %27\n\t"
-      "ds_read_b128 %17, %27 offset:64\n\t"
-      "ds_read_b128 %18, %27 offset:128\n\t"
-      "ds_read_b128 %19, %27 offset:192\n\t"
-      "ds_read_b128 %20, %28\n\t"
+      "ds_read_b128 %0, %22\n\t"
+      "ds_read_b128 %1, %22 offset:1024\n\t"
+      "ds_read_b128 %2, %22 offset:2048\n\t"
+      "ds_read_b128 %3, %22 offset:0xc00\n\t"
+      "ds_read_b32 %4, %27\n\t"
+      "ds_read_b32 %5, %27 offset:64\n\t"
+      "ds_read_b32 %6, %27 offset:128\n\t"
+      "ds_read_b32 %7, %27 offset:192\n\t"
+      "ds_read_b64_tr_b4 %8, %23\n\t"
+      "ds_read_b64_tr_b4 %9, %23 offset:8\n\t"
+      "ds_read_b64_tr_b4 %10, %24\n\t"
+      "ds_read_b64_tr_b4 %11, %24 offset:8\n\t"
+      "ds_read_b64_tr_b4 %12, %25\n\t"
+      "ds_read_b64_tr_b4 %13, %25 offset:8\n\t"
+      "ds_read_b64_tr_b4 %14, %26\n\t"
+      "ds_read_b64_tr_b4 %15, %26 offset:8\n\t"
+      "ds_read_b128 %16, %28\n\t"
+      "ds_read_b128 %17, %28 offset:64\n\t"
+      "ds_read_b128 %18, %28 offset:128\n\t"
+      "ds_read_b128 %19, %28 offset:192\n\t"
+      "ds_read_b128 %20, %29\n\t"
+      "ds_read_b32 %21, %30\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(u.k[0]), "=&v"(u.k[1]), "=&v"(u.k[2]), "=&v"(u.k[3]), "=&v"(u.ks[0]), "=&v"(u.ks[1]), "=&v"(u.ks[2]),
         "=&v"(u.ks[3]), "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]),
-        "=&v"(v[7]), "=&v"(u.vs[0]), "=&v"(u.vs[1]), "=&v"(u.vs[2]), "=&v"(u.vs[3]), "=&v"(u.ids)
+        "=&v"(v[7]), "=&v"(u.vs[0]), "=&v"(u.vs[1]), "=&v"(u.vs[2]), "=&v"(u.vs[3]), "=&v"(u.ids),
+        "=&v"(u.own)
       : "v"(b + lo.k), "v"(b + lo.v[0]), "v"(b + lo.v[1]), "v"(b + lo.v[2]), "v"(b + lo.v[3]), "v"(b + lo.ks),
-        "v"(b + lo.vs), "v"((uint32_t)reinterpret_cast<uintptr_t>(ids))
+        "v"(b + lo.vs), "v"((uint32_t)reinterpret_cast<uintptr_t>(ids)), "v"(b + lo.own)
       : "memory");
 #pragma unroll
   for (int n = 0; n < 8; ++n) { u.v[n][0] = v[n][0]; u.v[n][1] = v[n][1]; }
@@ -265,6 +270,20 @@ XV_INLINE bf16x8_t widen8(uint32_t w) {
   return r;
 }
 
+// The scales 2^(byte - 127) of one byte each of t0 and t1 (sel: a v_perm_b32 selector that brings them to bytes 0 and
+// 2), as the two bf16 of a dword.  Byte 0 is the subnormal 2^-127; 255 is an infinity here, which the second
+// operand of P turns into a NaN (infinity less infinity).
+XV_INLINE uint32_t v_scales(uint32_t t0, uint32_t t1, uint32_t sel) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t w = __builtin_amdgcn_perm(t1, t0, sel);
+  u16x2 b;
+  __builtin_memcpy(&b, &w, 4);
+  b = __builtin_elementwise_max((u16x2)(b << (uint16_t)7), (u16x2){0x0040, 0x0040});
+  uint32_t r;
+  __builtin_memcpy(&r, &b, 4);
+  return r;
+}
+
 template <int G, int RR>
 XV_INLINE void rescale_row(Fp4State& st, float alpha, int g) {
   const float ar = head_of_row<G, RR>(alpha, g);
@@ -296,7 +315,12 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const QSplit& q, int n
   float mx = -INFINITY;
 #pragma unroll
   for (int p = 0; p < 4; ++p) mx = fmaxf(mx, fmaxf(fmaxf(acc[p][0], acc[p][1]), fmaxf(acc[p][2], acc[p][3])));
-  mx = xor32_max(xor16_max(mx)) * scale_log2;
+  // Weights reach 2^kLazy, times V's scale they are bf16 operands, times up to 6 and summed over up to 2^28 tokens
+  // fp32 outputs: where a scale of the unit is 2^65 or more (two top bits set; 2^125 is the largest that the store
+  // writes) its weights stay 2^40 lower, and where all are below 2^-63 they go 2^64 higher, out of the subnormals.
+  // The maximum in use moves by as much, and the sum of the weights with it.
+  const bool huge = __any(u.own & (u.own << 1) & 0x80808080u), tiny = !__any(u.own & 0xc0c0c0c0u);
+  mx = xor32_max(xor16_max(mx)) * scale_log2 + (huge ? 40.f : tiny ? -64.f : 0.f);
   // the maximum in use moves only when some head's grew by more than kLazy
   const float m_new = fmaxf(st.m, mx);
   if (__any(m_new > st.m + kLazy)) {
@@ -326,7 +350,7 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const QSplit& q, int n
   // rounding.)
   constexpr int NV = G == 8 ? 2 : 1;
   bf16x8_t pa[NV][2], pb[NV][2];
-  const int shift = 8 * (G == 8 ? c >> 3 : G == 4 ? c >> 2 : (c / G) & 3);
+  const uint32_t sel = 0x0c040c00u + 0x10001u * (uint32_t)(G == 8 ? c >> 3 : G == 4 ? c >> 2 : (c / G) & 3);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     uint32_t w[NV][4], rest[NV][4];
@@ -336,10 +360,8 @@ XV_INLINE void unit_math(Fp4State& st, const UnitRegs& u, const QSplit& q, int n
       st.l += pr[p][r] + pr[p][r + 1];
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        // the low mantissa bit turns scale 255 into a NaN and moves the others by 2^-23 of themselves
-        const float f0 = __uint_as_float((__builtin_amdgcn_ubfe(u.vs[p][r], shift + 16 * v, 8) << 23) | 1u);
-        const float f1 = __uint_as_float((__builtin_amdgcn_ubfe(u.vs[p][r + 1], shift + 16 * v, 8) << 23) | 1u);
-        const float p0 = pr[p][r] * f0, p1 = pr[p][r + 1] * f1;
+        const uint32_t f = v_scales(u.vs[p][r], u.vs[p][r + 1], sel + 0x20002u * v);
+        const float p0 = pr[p][r] * bf16lo(f), p1 = pr[p][r + 1] * bf16hi(f);
         w[v][e / 2] = pack_bf16x2(p0, p1);
         rest[v][e / 2] = pack_bf16x2(p0 - bf16lo(w[v][e / 2]), p1 - bf16hi(w[v][e / 2]));
       }
