@@ -1,6 +1,7 @@
 """Decode attention over 4-bit pages to more than the output's own rounding, and
-at the ends of its number formats: V scale
-bytes from 0 to 252, weights that few tokens share, queries whose 32-value blocks differ widely in size.
+at the ends of its number formats: V scale bytes from 0 to 252, whole caches of
+the largest and smallest values, weights that few tokens share, queries whose
+32-value blocks differ widely in size.
 
 Tolerance, by element: one rounding of the output to bf16, at most 2^-8 of the
 value (2^-134 where the result is subnormal); the weights, held in two bf16
@@ -110,6 +111,21 @@ def test_v_scales_that_change_along_the_sequence(dev, hq, hkv):
             ks[p] = [110 + j // 4, 124 - j // 4, 122][b]
     case = q, kc, ks, vc, vs, bt
     _check(_call(dev, *case, ctx, hkv), *_reference(q.double().numpy(), *case[1:], ctx))
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 1), (1, 1)])
+@pytest.mark.parametrize("byte,code", [(252, 0x77), (252, 0xff), (0, 0x11), (1, 0x77)])
+def test_the_largest_and_smallest_values_alone(dev, hq, hkv, byte, code):
+    """One value everywhere in V: the weighted mean is that value, exactly, also where many waves' partials are joined."""
+    rng = np.random.default_rng(3)
+    ctx = [9000, 1, 64]
+    q, kc, ks, vc, vs, bt = _inputs(rng, ctx, hq, hkv)
+    vc[:], vs[:] = code, byte
+    got = _call(dev, q, kc, ks, vc, vs, bt, ctx, hkv)
+    want = O.dequantize_fp4(vc[0, 0, 0, :16], vs[0, 0, 0, :1])[0]
+    # the sum of the weights times one value over the sum of the weights: exact to about 2^-14, far below half a bf16
+    # step, and the value is a bf16
+    assert got.min() == got.max() == want
 
 
 @pytest.mark.parametrize("hq,hkv", GROUPS)

@@ -670,8 +670,9 @@ __global__ __launch_bounds__(256) void fp4_merge_kernel(Fp4DecodeArgs a) {
     if (128 + lane < n) lc = a.ws_lse[slot(128 + lane)];
   }
   const float mx = wave_max(fmaxf(la, fmaxf(lb, lc)));
-  const float wa = __builtin_amdgcn_exp2f(la - mx), wb = __builtin_amdgcn_exp2f(lb - mx), wc = __builtin_amdgcn_exp2f(lc - mx);
-  const float den = wave_sum(wa + wb + wc);
+  float wa = __builtin_amdgcn_exp2f(la - mx), wb = __builtin_amdgcn_exp2f(lb - mx), wc = __builtin_amdgcn_exp2f(lc - mx);
+  const float inv = 1.0f / wave_sum(wa + wb + wc);  // before the rows: their sum stays within their own range
+  wa *= inv; wb *= inv; wc *= inv;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   auto fold = [&](floatx4_t lo, floatx4_t hi, int j) {  // partial j of this lane row (the four rows' lie in one block of 64)
     const float w = __shfl(j < 64 ? wa : j < 128 ? wb : wc, j & 63);
@@ -696,10 +697,9 @@ __global__ __launch_bounds__(256) void fp4_merge_kernel(Fp4DecodeArgs a) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = xor32_sum(xor16_sum(acc[e]));
   if (g == 0) {
-    const float inv = 1.0f / den;
     uint32_t* o = reinterpret_cast<uint32_t*>(orow + 8 * i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(acc[2 * e], acc[2 * e + 1]);
   }
 }
 
