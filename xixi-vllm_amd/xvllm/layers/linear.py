@@ -356,11 +356,34 @@ def streamed_into_norm(x: torch.Tensor, w) -> PartialSums:
 MXFP4_WHOLE_ROWS = 16  # up to so many rows xv_mxfp4_gemm never splits K and needs no workspace
 
 
+def _check_mxfp4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool, codes: torch.dtype,
+                 scales: torch.dtype) -> None:
+    """Types, shapes and strides of mxfp4_linear's operands, w of dtype `codes` and w_scale of `scales`."""
+    if x.dtype != torch.bfloat16 or w.dtype != codes or w_scale.dtype != scales:
+        raise TypeError(f"mxfp4_linear takes bfloat16 x, {codes} codes and {scales} scales, got {x.dtype}, {w.dtype} and "
+                        f"{w_scale.dtype}")
+    xs, ws, ss = x.shape, w.shape, w_scale.shape
+    k = xs[-1] if len(xs) else 0
+    if len(ws) != 2 or len(ss) != 2 or k % 32 or k == 0 or ws[1] * 2 != k or ss[0] != ws[0] or ss[1] * 32 != k:
+        raise ValueError(f"mxfp4_linear: x {tuple(xs)}, codes {tuple(ws)}, scales {tuple(ss)} are not [..., K], [N, K/2] "
+                         "and [N, K/32], K a multiple of 32")
+    if silu_mul and ws[0] % 2:
+        raise ValueError(f"mxfp4_linear: a gate/up weight has an even number of rows, got {ws[0]}")
+    wst, sst = w.stride(), w_scale.stride()
+    if wst[1] != 1 or sst[1] != 1 or wst[0] % 16 or wst[0] < ws[1] or sst[0] < ss[1]:
+        raise ValueError("mxfp4_linear reads w in place: rows of unit stride, whole and 16-byte aligned")
+
+
 def _mxfp4_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
-    """mxfp4_linear on x [M, K], arguments checked."""
+    """mxfp4_linear on x [M, K], types, shapes and strides checked."""
     from .. import _C
     from .._torch_glue import call
 
+    dev = x.get_device()  # -1 on the CPU
+    if dev < 0 or w.get_device() != dev or w_scale.get_device() != dev:
+        raise RuntimeError("xvllm ops run on the GPU only (HIP kernels); mxfp4_linear needs x, w and w_scale on one device")
+    if w.data_ptr() % 16:
+        raise ValueError("mxfp4_linear reads w in place: rows of unit stride, whole and 16-byte aligned")
     m, k = x.shape
     n = w.shape[0]
     st, inner = x.stride()
@@ -372,14 +395,17 @@ def _mxfp4_product(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu
     if m and cols:
         nbytes = _C.lib().xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) if m > MXFP4_WHOLE_ROWS else 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        call("xv_mxfp4_gemm", x.get_device(), x.data_ptr(), st, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
+        call("xv_mxfp4_gemm", dev, x.data_ptr(), st, w.data_ptr(), w.stride(0), w_scale.data_ptr(),
              w_scale.stride(0), out.data_ptr(), cols, m, n, k, silu_mul, None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
 @torch.library.custom_op("xv::mxfp4_linear", mutates_args=())
 def _mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, silu_mul: bool) -> torch.Tensor:
-    """_mxfp4_product as an op that a compiler's trace holds."""
+    """mxfp4_linear on x [M, K] and the bytes of w and w_scale, as an op that a compiler's trace holds."""
+    _check_mxfp4(x, w, w_scale, silu_mul, torch.uint8, torch.uint8)
+    if x.dim() != 2:
+        raise ValueError(f"xv::mxfp4_linear takes x [M, K], got {tuple(x.shape)}")
     return _mxfp4_product(x, w, w_scale, silu_mul)
 
 
@@ -398,29 +424,12 @@ def mxfp4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, sil
     K is a multiple of 32, N any (even with silu_mul).  w's rows start 16-byte
     aligned and have unit stride, as w_scale's have; x of any layout.  For
     inference: it has no backward."""
-    if x.dtype != torch.bfloat16 or w.dtype != torch.float4_e2m1fn_x2 or w_scale.dtype != torch.float8_e8m0fnu:
-        raise TypeError(f"mxfp4_linear takes bfloat16 x, float4_e2m1fn_x2 codes and float8_e8m0fnu scales, got {x.dtype}, "
-                        f"{w.dtype} and {w_scale.dtype}")
-    xs, ws, ss = x.shape, w.shape, w_scale.shape
-    k = xs[-1] if len(xs) else 0
-    if len(ws) != 2 or len(ss) != 2 or k % 32 or k == 0 or ws[1] * 2 != k or ss[0] != ws[0] or ss[1] * 32 != k:
-        raise ValueError(f"mxfp4_linear: x {tuple(xs)}, codes {tuple(ws)}, scales {tuple(ss)} are not [..., K], [N, K/2] "
-                         "and [N, K/32], K a multiple of 32")
-    if silu_mul and ws[0] % 2:
-        raise ValueError(f"mxfp4_linear: a gate/up weight has an even number of rows, got {ws[0]}")
-    wst, sst = w.stride(), w_scale.stride()
-    if wst[1] != 1 or sst[1] != 1 or wst[0] % 16 or wst[0] < ws[1] or sst[0] < ss[1]:
-        raise ValueError("mxfp4_linear reads w in place: rows of unit stride, whole and 16-byte aligned")
+    _check_mxfp4(x, w, w_scale, silu_mul, torch.float4_e2m1fn_x2, torch.float8_e8m0fnu)
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("mxfp4_linear has no backward: call it under torch.no_grad()")
-    x2 = x if len(xs) == 2 else x.reshape(-1, k)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if torch.compiler.is_compiling():
         y = torch.ops.xv.mxfp4_linear(x2, w.view(torch.uint8), w_scale.view(torch.uint8), silu_mul)
     else:
-        dev = x.get_device()
-        if dev < 0 or w.get_device() != dev or w_scale.get_device() != dev:
-            raise RuntimeError("xvllm ops run on the GPU only (HIP kernels); mxfp4_linear needs x, w and w_scale on one device")
-        if w.data_ptr() % 16:
-            raise ValueError("mxfp4_linear reads w in place: rows of unit stride, whole and 16-byte aligned")
         y = _mxfp4_product(x2, w, w_scale, silu_mul)
-    return y if len(xs) == 2 else y.view(*xs[:-1], y.shape[1])
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
