@@ -201,3 +201,33 @@ def test_attention_over_4bit_pages_refusals():
         attn(q, k, k, decode._replace(cascade=plan))
     with attention_context(AttnMetadata(pool)), pytest.raises(ValueError, match="block_scale"):
         attn(q, k, k, decode)
+
+
+def _prefill_rows(monkeypatch, **kw):
+    """The rows that a prefill over 4-bit pages (three sequences of 130, 1 and 20 keys) reads back, nothing launched."""
+    from xvllm.layers import attention as A
+
+    class Asked(Exception):
+        pass
+
+    def gather(k_cache, v_cache, block_tables, cu_seqlens_k, total_tokens, **scales):
+        raise Asked(total_tokens)
+
+    monkeypatch.setattr(A, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(A, "gather_kvcache", gather)
+    pool, scale = codes(np.zeros((2, 1, 12, 16, 2, 64), np.uint8)), scales(np.zeros((2, 1, 12, 16, 2, 4), np.uint8))
+    q, k = torch.zeros((6, 1024), dtype=torch.bfloat16), torch.zeros((6, 256), dtype=torch.bfloat16)
+    cu_q, cu_k = torch.tensor([0, 3, 4, 6], dtype=torch.int32), torch.tensor([0, 130, 131, 151], dtype=torch.int32)
+    attn = A.AttnInputs(None, True, cu_q, cu_k, 3, block_tables=torch.zeros((3, 9), dtype=torch.int32), **kw)
+    with A.attention_context(A.AttnMetadata(pool, block_scale=scale)), pytest.raises(Asked) as asked:
+        A.Attention(8, 128, 2)(q, k, k, attn)
+    return asked.value.args[0]
+
+
+def test_prefill_reads_back_the_keys_there_are(monkeypatch):
+    assert _prefill_rows(monkeypatch, max_seqlen_k=130, total_seqlen_k=151) == 151
+    assert _prefill_rows(monkeypatch, total_seqlen_k=151) == 151
+    assert _prefill_rows(monkeypatch, max_seqlen_k=130) == 390  # only the longest is known: room for three of it
+    for total in (129, 391, -1):
+        with pytest.raises(ValueError, match="total_seqlen_k"):
+            _prefill_rows(monkeypatch, max_seqlen_k=130, total_seqlen_k=total)

@@ -1,7 +1,7 @@
 """``vllm::attention`` custom op (reference ``src/compute/layers/attention.py:13-143``):
 stores this step's K/V at ``slot_mapping`` (kv_ops.store_kvcache), then runs
 paged GQA decode attention or varlen causal prefill attention, both as gfx950
-HIP kernels.  Same signature, same module-global ``attention_context`` pool
+HIP kernels.  Same signature (and one optional argument more), same module-global ``attention_context`` pool
 handle, same ``AttnInputs`` record.
 """
 from __future__ import annotations
@@ -43,6 +43,7 @@ class AttnInputs(NamedTuple):
     block_tables: Optional[torch.Tensor] = None
     cache_seqlens: Optional[torch.Tensor] = None
     cascade: Optional[CascadePlan] = None  # decode only: shared-prefix groups (no reference counterpart)
+    total_seqlen_k: int = 0  # prefill: the keys of all sequences, cu_seqlens_k's last, where the host knows it
 
 
 @dataclass
@@ -331,12 +332,15 @@ def prefill_attention(
     kv_scale: tuple[float, float] | None = None,
     k_block_scale: torch.Tensor | None = None,
     v_block_scale: torch.Tensor | None = None,
+    total_seqlen_k: int = 0,
 ) -> torch.Tensor:
     """Varlen causal attention, bottom-right aligned.  With block_tables the
     keys come from the paged cache (cached prefix + this chunk), otherwise
     from k/v rows cu_seqlens_k[b] .. cu_seqlens_k[b+1].  An fp8 paged cache
     needs max_seqlen_k and its (k_scale, v_scale) (default: the active
-    attention_context's), a 4-bit one max_seqlen_k and its block scales."""
+    attention_context's), a 4-bit one its block scales and total_seqlen_k, the
+    keys of all sequences (cu_seqlens_k's last): they are read back as so many
+    bf16 rows.  With max_seqlen_k alone room is made for B of the longest run."""
     q3, qs0, qs1 = _q_view(q, num_qo_heads, head_dim)
     require_cuda(q3, cu_seqlens_q, cu_seqlens_k)
     require_bf16(q3)
@@ -347,11 +351,14 @@ def prefill_attention(
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else softmax_scale
     if block_tables is not None and k_cache is not None and k_cache.dtype == FP4_PAGES:
         # 4-bit pages: the sequences' keys and values as varlen bf16 rows (exact), then the dense path
-        if max_seqlen_k <= 0:
-            raise ValueError("prefill over a 4-bit paged cache needs max_seqlen_k (the longest key run)")
+        if max_seqlen_k <= 0 and total_seqlen_k <= 0:
+            raise ValueError("prefill over a 4-bit paged cache needs total_seqlen_k (the keys of all sequences) or "
+                             "max_seqlen_k (the longest key run)")
+        if total_seqlen_k < 0 or (total_seqlen_k and max_seqlen_k > 0 and not max_seqlen_k <= total_seqlen_k <= bsz * max_seqlen_k):
+            raise ValueError(f"total_seqlen_k {total_seqlen_k} is not the keys of {bsz} sequences of up to {max_seqlen_k}")
         if k_cache.dim() != 4 or k_cache.shape[2] != num_kv_heads or k_cache.shape[3] * 2 != head_dim:
             raise ValueError(f"cache {tuple(k_cache.shape)} is not 4-bit pages [NB, BS, {num_kv_heads}, {head_dim} / 2]")
-        kd, vd = gather_kvcache(k_cache, v_cache, block_tables, cuk, bsz * int(max_seqlen_k),
+        kd, vd = gather_kvcache(k_cache, v_cache, block_tables, cuk, int(total_seqlen_k) or bsz * int(max_seqlen_k),
                                 k_block_scale=k_block_scale, v_block_scale=v_block_scale)
         return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
                                  head_dim, softmax_scale=softmax_scale)
@@ -429,7 +436,9 @@ def attention(
     num_qo_heads: int,
     num_kv_heads: int,
     head_dim: int,
+    total_seqlen_k: int = 0,
 ) -> torch.Tensor:
+    """The reference's arguments and, at their end, AttnInputs' total_seqlen_k."""
     k_cache, v_cache = _layer_caches(layer_id)
     k3 = k.view(-1, num_kv_heads, head_dim)
     v3 = v.view(-1, num_kv_heads, head_dim)
@@ -441,7 +450,7 @@ def attention(
             return prefill_attention(
                 q, None, None, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
                 head_dim, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, max_seqlen_k=max_seqlen_k,
-                **(scales if k_cache.dtype == FP4_PAGES else {"kv_scale": kv_scales()}),
+                total_seqlen_k=total_seqlen_k, **(scales if k_cache.dtype == FP4_PAGES else {"kv_scale": kv_scales()}),
             )
         return prefill_attention(
             q, k3, v3, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads, head_dim
@@ -455,7 +464,7 @@ def attention(
 def _attention_fake(
     q, k, v, slot_mapping, is_prefill, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
     max_seqlen_k, block_tables, cache_seqlens, layer_id, num_qo_heads,
-    num_kv_heads, head_dim,
+    num_kv_heads, head_dim, total_seqlen_k=0,
 ):
     return torch.empty((q.shape[0], num_qo_heads * head_dim), dtype=q.dtype, device=q.device)
 
@@ -485,5 +494,5 @@ class Attention(nn.Module):
         return torch.ops.vllm.attention(
             q, k, v, attn.slot_mapping, attn.is_prefill, attn.cu_seqlens_q, attn.cu_seqlens_k,
             attn.max_seqlen_q, attn.max_seqlen_k, attn.block_tables, attn.cache_seqlens,
-            self.layer_id, self.num_heads, self.num_kv_heads, self.head_dim,
+            self.layer_id, self.num_heads, self.num_kv_heads, self.head_dim, attn.total_seqlen_k,
         )

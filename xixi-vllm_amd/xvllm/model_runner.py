@@ -221,6 +221,7 @@ class ModelRunner:
         attn = AttnInputs(slot_mapping=self.batch.slot_mapping[:nt], is_prefill=True,
                           cu_seqlens_q=self.batch.cu_seqlens_q[: bs + 1], cu_seqlens_k=self.batch.cu_seqlens_k[: bs + 1],
                           max_seqlen_q=max_q, max_seqlen_k=max_k,
+                          total_seqlen_k=sum(s.num_cached_tokens + len(s.token_ids) for s in seqs),
                           block_tables=self.batch.block_tables[:bs] if has_cache else None)
         with attention_context(self._meta):
             hidden = self.model(self.batch.input_ids[:nt], self.batch.positions[:nt], attn)
