@@ -550,7 +550,7 @@ int xv_stream_gemm(const void* x, int64_t x_stride, const void* w, int64_t w_str
  *             and out[m, I] = silu(g) * u of the two fp32 products.
  *   workspace xv_mxfp4_gemm_workspace_size(...) bytes (0 up to 16 rows, and
  *             where K is not split), 16-byte aligned, no initial contents.
- * k a multiple of 32; any m >= 0 (up to 4 million) and n > 0 (up to 2^30).  Strides of at most
+ * k a multiple of 32; any m >= 0 (up to 4 million) and n > 0 (up to 2^29).  Strides of at most
  * 2^22 values (x; one row: any), 2^25 bytes (w) and 2^27 bytes (w_scale).
  */
 size_t xv_mxfp4_gemm_workspace_size(int m, int n, int k, int silu_mul);

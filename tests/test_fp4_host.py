@@ -155,6 +155,15 @@ def test_gemm_rejects_bad_arguments(lib):
     assert _gemm(lib, m=0) == 0
 
 
+def test_gemm_refuses_more_rows_than_a_launch_holds(lib):
+    """A grid has fewer than 2^32 threads: at 96 weight rows to 512 threads no more than 805 million rows."""
+    for m in (1, 16, 64, 100):
+        for n in (1 << 30, 805306368, (1 << 29) + 2):
+            for silu in (0, 1):
+                ws = lib.xv_mxfp4_gemm_workspace_size(m, n, 32, silu)
+                assert _gemm(lib, m=m, n=n, k=32, xst=32, wst=16, sst=1, ost=n, silu=silu, ws=A, wsb=ws) == INVALID, (m, n, silu)
+
+
 @pytest.mark.parametrize("layout", ["hnd", "nhd"])
 def test_pool_of_4bit_pages(layout):
     from xvllm.config import Qwen3Shape

@@ -885,8 +885,10 @@ extern "C" int xv_mxfp4_gemm(const void* x, int64_t x_stride, const void* w, int
       (m > 1 && x_stride < k) || w_stride < k / 2 || scale_stride < k / kFp4Block || (uintptr_t)out & 1 ||
       (m > 1 && out_stride < (silu_mul ? n / 2 : n)))
     return (int)hipErrorInvalidValue;
-  // 32-bit offsets within a tile, rows that round up
-  if (m > 65535 * 64 || n > (1 << 30) || w_stride > (1 << 25) || scale_stride > (1 << 27) || (m > 1 && x_stride > (1 << 22))) return (int)hipErrorInvalidValue;
+  // 32-bit offsets within a tile, rows that round up; a grid of fewer than 2^32 threads (such weights have 96 or 256
+  // rows to a workgroup of 512)
+  if (m > 65535 * 64 || n > (1 << 29) || w_stride > (1 << 25) || scale_stride > (1 << 27) || (m > 1 && x_stride > (1 << 22)))
+    return (int)hipErrorInvalidValue;
   if (m == 0) return 0;
   if (workspace_bytes < xv_mxfp4_gemm_workspace_size(m, n, k, silu_mul) || (uintptr_t)workspace & 15)
     return (int)hipErrorInvalidValue;
