@@ -192,7 +192,8 @@ int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_pag
  * of itself, and to 2^-134 where it is below 2^-118, or to 2^-94 below 2^-78 in
  * 64 tokens that also hold a V scale of 2^65 or more); strides of the codes and of the scales in bytes as there, the codes' base and
  * strides multiples of 16, the scales' of 4, head_dim 128.  A sequence is read
- * up to max_blocks_per_seq * block_size tokens at most (256M at most).
+ * up to max_blocks_per_seq * block_size tokens at most (256M at most); the table
+ * rows of 256 sequences (of all, where there are fewer) take 2 GB at most.
  * workspace: xv_paged_decode_fp4_workspace_size(...) bytes, 16-byte aligned, no
  * initial contents; it grows neither with the table nor, past 256 sequences,
  * with the batch, and never decreases with either.  Calls sharing one must be ordered on one stream.

@@ -200,6 +200,19 @@ def test_decode_streams_and_graphs_share_nothing(dev):
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[0])
 
 
+@pytest.mark.parametrize("batch", [1, 3])
+def test_decode_through_a_wide_table(dev, batch):
+    """A table of 2.2 million columns (35 million tokens): its rows, not those of 256 sequences, have to be within 2 GB."""
+    rng = np.random.default_rng(batch)
+    ctx = [90, 5, 33][:batch]
+    q, kc, ks, vc, vs, bt = _inputs(rng, ctx, 8, 2, 16)
+    wide = np.full((batch, 2_200_000), -1, np.int32)
+    wide[:, : bt.shape[1]] = bt
+    out = _call(dev, q, kc, ks, vc, vs, wide, ctx, 2)
+    torch.cuda.synchronize()
+    _close(out, *_reference(q.double().numpy(), kc, ks, vc, vs, bt, ctx))
+
+
 def test_decode_refusals(dev):
     rng = np.random.default_rng(1)
     q, kc, ks, vc, vs, bt = _inputs(rng, [20, 20], 4, 2, 16)

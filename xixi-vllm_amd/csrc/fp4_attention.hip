@@ -748,8 +748,9 @@ extern "C" int xv_paged_decode_attention_fp4(
     return (int)hipErrorInvalidValue;
   if (tok_stride < kRow || tok_stride > (1 << 26) || scale_tok_stride < 4 || scale_tok_stride > (1 << 26) ||
       page_stride < 0 || page_stride > INT32_MAX || head_stride < 0 || head_stride > INT32_MAX || scale_page_stride < 0 ||
-      scale_page_stride > INT32_MAX || scale_head_stride < 0 || scale_head_stride > INT32_MAX || q_stride_head < 0 || q_stride_head > (1 << 26) || bt_stride < max_blocks_per_seq ||
-      (int64_t)kMaxBatch * bt_stride * 4 > INT32_MAX)
+      scale_page_stride > INT32_MAX || scale_head_stride < 0 || scale_head_stride > INT32_MAX || q_stride_head < 0 ||
+      q_stride_head > (1 << 26) || bt_stride < max_blocks_per_seq || bt_stride > INT32_MAX ||
+      min(batch, kMaxBatch) * bt_stride * 4 > INT32_MAX)  // the rows of a launch's table: one buffer
     return (int)hipErrorInvalidValue;
   if ((uintptr_t)out & 3 || out_stride_tok & 1) return (int)hipErrorInvalidValue;
   if (batch == 0) return 0;
