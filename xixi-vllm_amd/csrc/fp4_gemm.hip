@@ -22,9 +22,8 @@
 // is what bounds more than 16 rows (37 rows of an odd 5003 x 4704 weight 12.0 us).
 #include "xv_decode.h"
 #include "xv_fp4.h"
+#include "xv_fp4_plan.h"
 #include "xv_kernels.h"
-#include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -66,7 +65,7 @@ XV_INLINE bf16x8_t widen8(uint32_t w, float scale) {
 
 typedef const __attribute__((address_space(1))) void* global_cptr;
 
-constexpr int kWaves = 8;
+constexpr int kWaves = kFp4Waves;
 
 // One stage: the codes of 16 weight rows x KS values, rows of KS / 2 bytes,
 // swizzled.  Scales come with a slice of x, a window of SW dwords of each of the
@@ -431,7 +430,6 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
 // products alone take 79, the loads and reads alone 84.  Weight loads are not
 // non-temporal: a step takes half a line, and 133 us then.)  Where the tiles give too few workgroups, K is split
 // and a second kernel adds the fp32 parts.
-constexpr int kMaxM = 7;  // column tiles per wave at most (224 rows of x)
 
 // The operands of a half step in one asm block with one wait: of N column
 // tiles (16 rows of 128 bytes apart) both substeps, of NT row tiles (16 rows of
@@ -757,38 +755,6 @@ void launch(const Fp4PartArgs& pa, dim3 grid, hipStream_t stream) {
   else fp4_gemm_kernel<MT, XR, KS, XD, T, SILU, false><<<grid, kWaves * 64, 0, stream>>>(pa);
 }
 
-// How a product of up to kShort rows is cut: tiles per workgroup, parts of K.
-// The cheapest by cycles, a workgroup per CU at a time.  Up to 16 rows a
-// workgroup costs its tiles and its start and end, about one and a half tiles.
-// Of more, it costs what goes through its LDS-DMA, about 40 bytes a cycle, most
-// of it x: more tiles on parts of K read less of that, where it pays for the second
-// kernel (64 rows through 4096 x 12288 17.6 us against 23.2 with K whole, 32 rows
-// 13.6 against 14.8; through 4096 x 4096 K stays whole, 11.5).
-struct ShortPlan { int tiles, parts; };
-ShortPlan short_plan(int m, int rows, int k, bool silu) {
-  const int tiles = (rows / (silu ? 2 : 1) + 15) / 16 * (silu ? 2 : 1);
-  const int xr = (m + 15) / 16 * 16;  // rows of x that are fetched
-  ShortPlan best = {silu ? 2 : 1, 1};
-  double cost = 1e300;
-  for (int t : {1, 2, 4, 6}) {
-    if (silu && t % 2) continue;
-    const int groups = (tiles + t - 1) / t;
-    if (m <= 16) {
-      const double c = ((groups + 255) / 256) * (t + 1.5);
-      if (c <= cost) { cost = c; best = {t, 1}; }
-      continue;
-    }
-    for (int parts : {1, 2, 4, 8}) {
-      if (parts > 1 && k / parts < 128 * kWaves) break;
-      const double bytes = (double)k / parts * (2 * xr + t * 8.5);
-      double c = std::ceil((double)groups * parts / 256) * (bytes / 40 + 6000);
-      if (parts > 1) c += 8000 + (double)parts * m * rows * 8 / 2000;
-      if (c <= cost) { cost = c; best = {t, parts}; }
-    }
-  }
-  return best;
-}
-
 // One tile a workgroup takes a new slice of x with every stage: as many in
 // flight (XD) as stages, in shorter slices where 16 rows of x would not fit.
 template <int MT, int XR, int KS1, int XD1, int KS, bool SILU>
@@ -805,33 +771,6 @@ void launch_tiles(const Fp4GemmArgs& a, float* ws, hipStream_t stream) {
     default: launch<MT, XR, KS, 1, 6, SILU>(pa, grid, stream); break;
   }
   if (p.parts > 1) launch_sum<SILU>(pa, p.parts, stream);
-}
-
-// How a product of more than kShort rows is cut: column tiles per wave, row
-// tiles of the weight per wave, parts of K.  The cheapest by cycles: a step costs its
-// matrix instructions (16 cycles each, two waves a SIMD) or its x through
-// LDS-DMA (about 40 bytes a cycle), a workgroup about 8000 more at its ends, parts
-// their second kernel and the traffic between.
-constexpr int kShort = 64;
-struct TilePlan { int mtw, nt, parts; };
-TilePlan tile_plan(int m, int rows, int k, bool silu) {
-  const int gy = (m + 32 * kMaxM - 1) / (32 * kMaxM);
-  const int mtw = std::max(3, ((m + gy - 1) / gy + 31) / 32);
-  const int steps = (k + 127) / 128;
-  TilePlan best = {mtw, 4, 1};
-  double cost = 1e300;
-  for (int nt : {4, 2, 1}) {
-    if (silu && nt == 1) continue;
-    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
-      if (parts > 1 && steps / parts < 4) break;
-      const double groups = (double)((rows + 64 * nt - 1) / (64 * nt)) * ((m + 32 * mtw - 1) / (32 * mtw)) * parts;
-      const double step = std::max(128.0 * nt * mtw, 200.0 * mtw) + 700.0;
-      double c = std::ceil(groups / 256) * ((steps + parts - 1) / parts * step + 8000.0);
-      if (parts > 1) c += 7000.0 + (double)parts * m * rows * 8.0 / 2000.0;
-      if (c < cost) { cost = c; best = {mtw, nt, parts}; }
-    }
-  }
-  return best;
 }
 
 template <int NT, bool SILU>
