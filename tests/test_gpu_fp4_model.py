@@ -282,3 +282,32 @@ def test_serving_on_a_4bit_pool(dev):
     assert st.steps > 12 and st.prefill_tokens == sum(len(p) for p in prompts)
     sampled, _ = _serve(dev, model, kv, prompts, 12, dict(temperature=0.7, top_p=0.9, top_k=50), 7, check=True)
     assert all(0 <= t < V for o in sampled + greedy1 for t in o)
+
+
+@pytest.mark.parametrize("rows", [3, 64])
+def test_decode_layer_takes_buffers_of_a_larger_batch(dev, rows):
+    """Positions and slots longer than the batch: its own rows are read, as on the other pools."""
+    from xvllm.config import Qwen3Shape
+    from xvllm.layers.attention import AttnInputs, AttnMetadata, attention_context
+    from xvllm.models.qwen3 import Qwen3Attention
+
+    g = torch.Generator(device=dev).manual_seed(rows)
+    with torch.device(dev):
+        layer = Qwen3Attention(Qwen3Shape(1024, 16, 8, D, 2048, 1, max_position_embeddings=1024), 0).to(torch.bfloat16)
+    with torch.no_grad():
+        layer.qkv_proj.normal_(0.0, 0.02, generator=g)
+        layer.o_proj.normal_(0.0, 0.02, generator=g)
+        hidden = torch.randn((rows, 1024), generator=g, device=dev).to(torch.bfloat16)
+    lens = torch.randint(1, 64, (rows,), generator=g, device=dev, dtype=torch.int32)
+    bt = torch.arange(4 * rows, dtype=torch.int32, device=dev).view(rows, 4)
+    last = (lens - 1).long()
+    slots = bt.gather(1, (last // 16)[:, None])[:, 0] * 16 + (last % 16).to(torch.int32)
+    outs = []
+    for slack in (0, 9):
+        kv = _pool(dev, 16, 8, 4 * rows, 16, "hnd")
+        kv.block_scale.view(torch.uint8).fill_(124)
+        attn = AttnInputs(torch.cat([slots, slots.new_full((slack,), -1)]), False, block_tables=bt, cache_seqlens=lens)
+        with torch.no_grad(), attention_context(AttnMetadata(kv.kv_cache, block_scale=kv.block_scale)):
+            out = layer(torch.cat([last, last.new_zeros(slack)]), hidden, attn)
+        outs.append((getattr(out, "parts", out), kv.kv_cache.view(torch.uint8), kv.block_scale.view(torch.uint8)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))

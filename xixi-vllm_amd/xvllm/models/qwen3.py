@@ -149,6 +149,8 @@ class Qwen3Attention(nn.Module):
             o = self.attn(q.view(q.shape[0], self.q_size), k, v, attn._replace(slot_mapping=None))
         else:
             q, k, v = self._split_norm_rope(positions, F.linear(hidden, self.qkv_proj))
+            if not attn.is_prefill and attn.slot_mapping is not None:  # slots may come from a buffer of a larger batch
+                attn = attn._replace(slot_mapping=attn.slot_mapping.reshape(-1)[: q.shape[0]])
             o = self.attn(q.view(q.shape[0], self.q_size), k, v, attn)
         if not self.split_k:
             return F.linear(o, self.o_proj)
