@@ -213,6 +213,19 @@ def test_decode_through_a_wide_table(dev, batch):
     _close(out, *_reference(q.double().numpy(), kc, ks, vc, vs, bt, ctx))
 
 
+def test_decode_of_unaligned_rows(dev):
+    """q as whole rows that start 6 bytes into a buffer."""
+    rng = np.random.default_rng(12)
+    ctx, hq, hkv = [70, 1, 33], 8, 2
+    q, kc, ks, vc, vs, bt = _inputs(rng, ctx, hq, hkv, 16)
+    room = torch.zeros(q.numel() + 3, dtype=torch.bfloat16, device=dev)
+    room[3:] = q.to(dev).flatten()
+    out = _call(dev, room[3:].view(q.shape), kc, ks, vc, vs, bt, ctx, hkv)
+    torch.cuda.synchronize()
+    assert room[3:].view(q.shape).is_contiguous()
+    _close(out, *_reference(q.double().numpy(), kc, ks, vc, vs, bt, ctx))
+
+
 def test_decode_refusals(dev):
     rng = np.random.default_rng(1)
     q, kc, ks, vc, vs, bt = _inputs(rng, [20, 20], 4, 2, 16)

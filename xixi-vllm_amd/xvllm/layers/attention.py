@@ -133,7 +133,7 @@ def decode_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 def _q_view(q: torch.Tensor, num_heads: int, head_dim: int) -> tuple[torch.Tensor, int, int]:
     q3 = q.view(q.shape[0], num_heads, head_dim) if q.dim() == 2 else q
     if q3.stride(-1) != 1 or q3.stride(0) % 8 or q3.stride(1) % 8 or not aligned16(q3):
-        q3 = q3.contiguous()
+        q3 = q3.clone(memory_format=torch.contiguous_format)  # whole rows may be unaligned too: a fresh allocation
     return q3, q3.stride(0), q3.stride(1)
 
 
