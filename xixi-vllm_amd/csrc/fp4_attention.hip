@@ -26,12 +26,15 @@
 //   one operand for the columns of one scale block only.  The G heads fill G
 //   of the 16 operand rows, so row rep * G + h takes head h scaled for block
 //   rep (G = 8: two operands of two blocks): all blocks in one product, and
-//   the outputs of the other blocks' rows are not used.
+//   the outputs of the other blocks' rows are not used.  P times the scale goes
+//   in as two bf16 terms, two products each.
 //
-// 64 sequences of 512 .. 4096 tokens (32 heads over 8) take 41.0 us: 12 of
-// launches, start (lengths, then block ids, then pages) and merge, the rest at
-// a copy's rate; four of 40000 .. 130000 (16 over 8) 76 us, 5.1 TB/s over the
-// whole call.
+// 64 sequences of 512 .. 4096 tokens (32 heads over 8) take 44 us: 12 of
+// launches, start (lengths, then block ids, then pages) and merge, the rest the
+// page stream at 5 TB/s (its tail with the units' arithmetic); four of 40000 ..
+// 130000 (16 over 8) 80 us, 4.9 TB/s over the whole call.  A segment is cut into
+// kMaxParts at most, so one sequence of 130000 with one kv head has 185 of the
+// 2048 waves at work: 36 us.
 #include "xv_decode.h"
 #include "xv_fp4.h"
 #include "xv_kernels.h"
@@ -551,8 +554,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
 
   // Unit y, whose cursor is ic and whose block ids are idv, into its ring
-  // slot, non-temporally (64 rows 41.2 us, 44.6 through the caches).  A page's rows past the sequence's end are read as they are (they are
-  // masked, and every code is finite); their scales are those of the last token.
+  // slot, non-temporally (64 rows 44.3 us, 45.8 through the caches; four long ones 81 and 89).  A page's rows past the
+  // sequence's end are read as they are (they are masked, and every code is finite); their scales are those of the last
+  // token.
   auto issue = [&](int y, const u32x4_t& idv) {
     char* buf = mine + (y & 1) * kUnitLds;
     if (y % kIdWindow == 0 && y > 0)  // entering window k (in place since window k - 1 began): request window k + 1

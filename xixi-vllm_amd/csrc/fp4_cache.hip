@@ -97,7 +97,8 @@ extern "C" int xv_store_kvcache_fp4(const void* key, int64_t key_stride_tok, int
 // width) are left as they are.
 // Bound by the rows it writes: 16 sequences of 1229 tokens on average, 8 heads
 // (81 MB out), with the store of their last 512 before it 28.8 us, of which this
-// about 19; three of 20000 to 35000 (306 MB out) 78 us, 6.2 TB/s.  The codes are
+// about 19; three of 20000 to 35000 (306 MB out) 79 us, 6.1 TB/s, in a replayed
+// graph of such calls, 88 us between other work.  The codes are
 // loaded as usual, a chunk's store has just written some of them (non-temporal:
 // 31.2 us for the first); four heads in place of two: two sequences of 64000 124 us
 // against 120, eight: 77 tokens 7.1 us against 6.5.

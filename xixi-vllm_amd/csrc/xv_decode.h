@@ -1,6 +1,6 @@
 // Device helpers shared by the decode attention kernels: buffer resources of a
 // page, the lazily moved softmax maximum, the flat (sequence, kv head, page)
-// space, the merge of partial outputs.
+// space.
 #pragma once
 #include "xv_common.h"
 
