@@ -48,6 +48,34 @@ int xv_store_kvcache(const void* key, int64_t key_stride_tok, int64_t key_stride
                      int num_kv_heads, int head_dim, hipStream_t stream);
 
 /*
+ * A step's maps from its requests' lengths, in one launch.  The reference
+ * builds them on the host, request by request (src/compute/batch.py:119-215).
+ * Request b has seq_lens[b] tokens in the cache and adds new_lens[b] (negative
+ * lengths count as 0; rows <= 8192):
+ *   cu_seqlens_q, cu_seqlens_k [rows + 1]  running sums of new_lens and of
+ *       seq_lens + new_lens (below 2^31);  cache_seqlens [rows] = their sum
+ *   block_tables  int32 [rows, bt_stride] in place: row b's entries from
+ *       ceil(seq_lens / block_size) to ceil((seq_lens + new_lens) / block_size)
+ *       are taken, row after row, from free_pages[*free_head + 0, 1, ...]; the
+ *       others stay as they are
+ *   next_free_head  *free_head + the pages taken (free_head NULL: 0), not the
+ *       same word; past num_free where the list ran out: such entries get -1
+ *   positions int64 [total_tokens], slot_mapping int32 [total_tokens], both
+ *       16-byte aligned: token i of request b, at cu_seqlens_q[b] + i, has slot
+ *       page * block_size + row of token seq_lens[b] + i, and that position
+ *       (depths: seq_lens[b] + depths[t] instead, the nodes of drafted trees).
+ *       Slot -1, which the KV stores skip, where there is no page (entry -1,
+ *       past max_blocks_per_seq, past the free list) and, with position 0, from
+ *       cu_seqlens_q[rows] on; tokens from total_tokens on are not written.
+ * A pool has fewer than 2^31 slots.
+ */
+int xv_step_maps(const int32_t* seq_lens, const int32_t* new_lens, int rows, int32_t* block_tables,
+                 int64_t bt_stride, int max_blocks_per_seq, int block_size, const int32_t* free_pages,
+                 int num_free, const int32_t* free_head, const int32_t* depths, int total_tokens,
+                 int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, int32_t* cache_seqlens, int64_t* positions,
+                 int32_t* slot_mapping, int32_t* next_free_head, hipStream_t stream);
+
+/*
  * KV store into an fp8 (OCP e4m3fn) cache.  No counterpart in the reference,
  * whose pool holds the model dtype (src/compute/kv_pool.py:49-51): an optional
  * on-HBM format that halves the KV bytes the decode streams.  As
@@ -210,6 +238,51 @@ int xv_paged_decode_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q
                                   int block_size, int max_blocks_per_seq, float scale, hipStream_t stream);
 
 /*
+ * xv_paged_decode_attention with a sliding window and sinks.  No counterpart in
+ * the reference (its attention sees every cached token).  The query of a
+ * sequence of n tokens is its token n - 1 and sees the last `window` tokens (>=
+ * 1), itself among them, and the first `sink_tokens` (>= 0).  Block-table
+ * entries that hold no visible token are not read; values that no query sees
+ * may be anything.  bf16 pages.  A sequence is read up to max_blocks_per_seq *
+ * block_size tokens at most (256M at most); the table rows of 256 sequences
+ * (of all, where there are fewer) take 2 GB at most.  Layouts and supported
+ * shapes as xv_paged_decode_attention, any scale.
+ * workspace: xv_tree_attention_workspace_size(batch, 1, ...) bytes, 16-byte
+ * aligned, no initial contents.  Calls sharing one must be ordered on one stream.
+ */
+int xv_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                               const void* v_cache, int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                               const int32_t* block_tables, int64_t bt_stride, const int32_t* cache_seqlens,
+                               void* out, int64_t out_stride_tok, void* workspace, size_t workspace_bytes, int batch,
+                               int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                               int max_blocks_per_seq, int window, int sink_tokens, float scale,
+                               hipStream_t stream);
+
+/*
+ * Attention of trees of drafted tokens over the paged cache (the check of
+ * drafted tokens in one pass).  No counterpart in the reference.  Sequence b
+ * has cache_seqlens[b] tokens in the cache, the last n = cu_seqlens_q[b + 1] -
+ * cu_seqlens_q[b] of them its nodes; its node i is row cu_seqlens_q[b] + i of
+ * q and out, and sees every token before the nodes and node j where bit j % 64
+ * of word j / 64 of its mask is set (its own bit included: nothing is implied).
+ * A row that sees nothing is zeros; rows from cu_seqlens_q[batch] on are left
+ * as they are.  Values of nodes that no row sees may be anything.
+ *   tree_mask  int64 [rows][mask_words], rows mask_stride apart
+ *   max_nodes  nodes of the largest tree at most, <= 64 * mask_words and <= 1024
+ *   workspace  xv_tree_attention_workspace_size(...) bytes, 16-byte aligned, no
+ *              initial contents.  Calls sharing one must be ordered on one stream.
+ * Layouts, supported shapes and limits as xv_window_decode_attention.
+ */
+size_t xv_tree_attention_workspace_size(int batch, int max_nodes, int num_q_heads, int num_kv_heads);
+int xv_tree_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
+                      const void* v_cache, int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                      const int32_t* block_tables, int64_t bt_stride, const int32_t* cache_seqlens,
+                      const int32_t* cu_seqlens_q, const int64_t* tree_mask, int64_t mask_stride, int mask_words,
+                      void* out, int64_t out_stride_tok, void* workspace, size_t workspace_bytes, int batch,
+                      int max_nodes, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                      int max_blocks_per_seq, float scale, hipStream_t stream);
+
+/*
  * Shared-prefix (cascade) decode attention: xv_paged_decode_attention for a
  * batch whose rows may share their first tokens' cache blocks, as a radix
  * prefix cache maps them (the reference's prefix index,
@@ -322,6 +395,24 @@ int xv_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
                          void* out, int64_t out_stride_tok,
                          int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
                          int head_dim, int block_size, float scale, hipStream_t stream);
+
+/*
+ * xv_prefill_attention with a sliding window and sinks: the query at position p
+ * of its sequence sees keys j <= p with j > p - window (>= 1) or j < sink_tokens
+ * (>= 0).  No counterpart in the reference.  Block-table entries that hold no
+ * key that a query of the call sees are not read.  scale > 0; the rest as
+ * xv_prefill_attention.
+ */
+int xv_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                const void* k, const void* v, int64_t kv_stride_tok, int64_t kv_stride_head,
+                                const void* k_cache, const void* v_cache,
+                                int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                                const int32_t* block_tables, int64_t bt_stride,
+                                const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                void* out, int64_t out_stride_tok,
+                                int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+                                int head_dim, int block_size, int window, int sink_tokens, float scale,
+                                hipStream_t stream);
 
 /*
  * RMSNorm into a new buffer.

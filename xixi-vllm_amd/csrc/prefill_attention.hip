@@ -52,6 +52,7 @@ struct PrefillArgs {
   bf16_t* out; int64_t out_st;
   int hq, hkv, qblocks, batch;
   float scale_log2;
+  int window, sinks;  // windowed calls only: tokens a query sees up to itself, first tokens that stay visible
 };
 
 XV_INLINE int swz_k(int r) { return r & 15; }
@@ -69,11 +70,14 @@ XV_INLINE __amdgpu_buffer_rsrc_t rsrc(const bf16_t* base, uint32_t bytes) {
 
 // Wave w moves keys key0+16w .. +15 of the tile (one cache page when paged):
 // 4 LDS-DMA instructions for K and/or 4 for V, each 4 whole rows.
-template <bool PAGED, bool DO_K, bool DO_V>
+// WIN: keys sinks .. lo - 1 are seen by no query of the workgroup: their V
+// reads as zeros (whatever the cache holds there), and 16 keys that are all
+// such are not read at all (their block-table entry may be gone).
+template <bool PAGED, bool DO_K, bool DO_V, bool WIN>
 XV_INLINE void load_rows(char* buf, const PrefillArgs& a, int b, int kvh, int key0, int k0, int k_len,
-                         int64_t page_off, int wave, int lane) {
+                         int64_t page_off, int lo, int wave, int lane) {
   const int j0 = key0 + 16 * wave;
-  const int valid = min(16, k_len - j0);
+  const int valid = WIN && j0 >= a.sinks && j0 + 16 <= lo ? 0 : min(16, k_len - j0);
   const bf16_t *kb, *vb;
   int64_t rs;  // row stride (elements)
   if (PAGED) {
@@ -91,7 +95,8 @@ XV_INLINE void load_rows(char* buf, const PrefillArgs& a, int b, int kvh, int ke
     const int r = 4 * s + (lane >> 4);  // row within the wave's 16
     const int R = 16 * wave + r;        // row within the tile
     const int vo_k = (int)(r * rs * 2) + ((slot ^ swz_k(R)) << 4);
-    const int vo_v = (int)(r * rs * 2) + ((slot ^ swz_v(R)) << 4);
+    int vo_v = (int)(r * rs * 2) + ((slot ^ swz_v(R)) << 4);
+    if (WIN && j0 + r >= a.sinks && j0 + r < lo) vo_v = INT32_MIN;  // past every resource: zeros
     if (DO_K)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(buf + (16 * wave + 4 * s) * 256), 16, vo_k, 0, 0, 0);
     if (DO_V)
@@ -237,7 +242,7 @@ XV_INLINE int seq_by_work(const int* cu_q, const int* cu_k, int batch, int j) {
   return __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
 }
 
-template <int G, bool PAGED>
+template <int G, bool PAGED, bool WIN>
 __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   constexpr int GW = G < 4 ? G : 4;   // query heads per workgroup
   constexpr int QS = 4 / GW;          // 32-query sub-blocks per workgroup
@@ -265,11 +270,23 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   const int qw0 = qb0 + (wave / GW) * 32;  // the wave's first query
   const int my_q = qw0 + l32;
   const int kv_end = min(k_len, shift + min(qb0 + kBlockQ, q_len));  // keys the block needs
-  const int ntiles = (kv_end + kKeys - 1) / kKeys;
+  // WIN: the tiles of the block are those of the sinks, then those from its first query's window on
+  const int blk_lo = WIN ? max(0, shift + qb0 + 1 - a.window) : 0;
+  const int sink_tiles = WIN ? (min(a.sinks, blk_lo) + kKeys - 1) / kKeys : 0;
+  const int skip = WIN ? max(0, blk_lo / kKeys - sink_tiles) : 0;
+  const int ntiles = max(0, (kv_end + kKeys - 1) / kKeys - skip);
+  auto key_of = [&](int t) { return (WIN && t >= sink_tiles ? t + skip : t) * kKeys; };  // first key of tile t
   const bool active = qw0 < q_len;
   const int wave_kend = active ? min(k_len, shift + min(qw0 + 32, q_len)) : 0;  // keys any query of the wave sees
   const int wave_kfull = shift + qw0 + 1;  // keys every query of the wave sees
   const int my_kend = shift + my_q + 1;
+  const int my_lo = WIN ? my_kend - a.window : 0;            // first key of this lane's window
+  const int wave_lo = WIN ? wave_kfull - a.window : 0;       // of the wave's first query's, and of its last one's
+  const int wave_lo_last = WIN ? wave_lo + 31 : 0;
+  auto needed = [&](int t) {  // whether any query of the wave sees a key of tile t
+    const int key0 = key_of(t);
+    return key0 < wave_kend && (!WIN || key0 + kKeys > wave_lo || key0 < a.sinks);
+  };
 
   // Q^T B-operands: lane holds query my_q, d = 16s + 8(l/32) .. +7
   bf16x8_t qb[8];
@@ -293,8 +310,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   // cache block of block_size tokens): block bt[j / BS], token j % BS
   auto page_of = [&](int t) -> int64_t {
     if (!PAGED) return 0;
-    const int j = t * kKeys + 16 * wave;
-    if (j >= k_len) return 0;
+    const int j = key_of(t) + 16 * wave;
+    if (j >= k_len || (WIN && j >= a.sinks && j + 16 <= blk_lo)) return 0;
     const int blk = j / a.block_size;
     const int64_t page = __builtin_amdgcn_readfirstlane(a.bt[(int64_t)b * a.bt_stride + blk]);
     return page * a.page_stride + (int64_t)(j - blk * a.block_size) * a.tok_stride;
@@ -316,15 +333,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   };
   // online softmax of tile t's scores s -> P (bf16), O and l rescaled as needed
   auto softmax = [&](int t, floatx16_t (&s)[2], bf16x8_t (&pb)[2][2]) {
-    const int key0 = t * kKeys;
+    const int key0 = key_of(t);
     // (on raw scores: scale > 0 keeps the order; p = exp2(s*scale - m*scale))
-    if (key0 + kKeys > wave_kfull) {  // the tile crosses some query's diagonal
+    // the tile crosses some query's diagonal, or the first key of some query's window
+    if (key0 + kKeys > wave_kfull || (WIN && key0 < wave_lo_last && key0 + kKeys > a.sinks)) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int key = key0 + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
-          s[mt][r] = key < my_kend ? s[mt][r] : -INFINITY;
+          s[mt][r] = key < my_kend && (!WIN || key >= my_lo || key < a.sinks) ? s[mt][r] : -INFINITY;
         }
     }
     float mx = -INFINITY;
@@ -388,23 +406,26 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   // buffer S(t) used and V(t+1) into the V buffer P(t-1) V(t-1) used, both
   // freed by the barrier at its top.
   int64_t pv_page = ntiles > 1 ? page_of(1) : 0, pk_page = ntiles > 2 ? page_of(2) : 0;
-  if (ntiles > 0) load_rows<PAGED, true, true>(lds, a, b, kvh, 0, k0, k_len, page_of(0), wave, lane);
-  if (ntiles > 1) load_rows<PAGED, true, false>(lds + kBuf, a, b, kvh, kKeys, k0, k_len, pv_page, wave, lane);
+  if (ntiles > 0) load_rows<PAGED, true, true, WIN>(lds, a, b, kvh, key_of(0), k0, k_len, page_of(0), blk_lo, wave, lane);
+  if (ntiles > 1)
+    load_rows<PAGED, true, false, WIN>(lds + kBuf, a, b, kvh, key_of(1), k0, k_len, pv_page, blk_lo, wave, lane);
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   // scores of even tiles in s_even, of odd tiles in s_odd (no copies)
   floatx16_t s_even[2], s_odd[2];
-  if (ntiles > 0 && 0 < wave_kend) s_tile(std::integral_constant<int, 0>{}, s_even);
+  if (ntiles > 0 && needed(0)) s_tile(std::integral_constant<int, 0>{}, s_even);
   auto iter = [&](auto par_tag, int t, floatx16_t (&sc)[2], floatx16_t (&sn)[2]) {
     constexpr int PAR = decltype(par_tag)::value;  // t & 1
     __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // K(t+1) and V(t) are in LDS; every wave is done with iteration t-1
-    if (t + 2 < ntiles) load_rows<PAGED, true, false>(lds + PAR * kBuf, a, b, kvh, (t + 2) * kKeys, k0, k_len, pk_page, wave, lane);
-    if (t + 1 < ntiles) load_rows<PAGED, false, true>(lds + (1 - PAR) * kBuf, a, b, kvh, (t + 1) * kKeys, k0, k_len, pv_page, wave, lane);
+    if (t + 2 < ntiles)
+      load_rows<PAGED, true, false, WIN>(lds + PAR * kBuf, a, b, kvh, key_of(t + 2), k0, k_len, pk_page, blk_lo, wave, lane);
+    if (t + 1 < ntiles)
+      load_rows<PAGED, false, true, WIN>(lds + (1 - PAR) * kBuf, a, b, kvh, key_of(t + 1), k0, k_len, pv_page, blk_lo, wave, lane);
     pv_page = pk_page;
     if (t + 3 < ntiles) pk_page = page_of(t + 3);
-    if (t + 1 < ntiles && (t + 1) * kKeys < wave_kend) s_tile(std::integral_constant<int, 1 - PAR>{}, sn);
-    if (t * kKeys < wave_kend) {
+    if (t + 1 < ntiles && needed(t + 1)) s_tile(std::integral_constant<int, 1 - PAR>{}, sn);
+    if (needed(t)) {
       bf16x8_t pb[2][2];
       // the softmax is the serial link between MFMA phases: at raised issue
       // priority it runs ahead of the other wave on this SIMD, whose MFMAs
@@ -436,21 +457,26 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
 
 template <int G>
 void launch(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
-  if (a.bt) prefill_kernel<G, true><<<grid, kThreads, 0, stream>>>(a);
-  else prefill_kernel<G, false><<<grid, kThreads, 0, stream>>>(a);
+  if (a.window > 0) {
+    if (a.bt) prefill_kernel<G, true, true><<<grid, kThreads, 0, stream>>>(a);
+    else prefill_kernel<G, false, true><<<grid, kThreads, 0, stream>>>(a);
+  } else {
+    if (a.bt) prefill_kernel<G, true, false><<<grid, kThreads, 0, stream>>>(a);
+    else prefill_kernel<G, false, false><<<grid, kThreads, 0, stream>>>(a);
+  }
 }
 
-}  // namespace
-
-extern "C" int xv_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
-                                    const void* k, const void* v, int64_t kv_stride_tok, int64_t kv_stride_head,
-                                    const void* k_cache, const void* v_cache,
-                                    int64_t page_stride, int64_t tok_stride, int64_t head_stride,
-                                    const int32_t* block_tables, int64_t bt_stride,
-                                    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                                    void* out, int64_t out_stride_tok,
-                                    int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
-                                    int head_dim, int block_size, float scale, hipStream_t stream) {
+// window 0: every query sees all keys up to itself
+int prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+            const void* k, const void* v, int64_t kv_stride_tok, int64_t kv_stride_head,
+            const void* k_cache, const void* v_cache,
+            int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+            const int32_t* block_tables, int64_t bt_stride,
+            const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+            void* out, int64_t out_stride_tok,
+            int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+            int head_dim, int block_size, int window, int sink_tokens, float scale,
+            hipStream_t stream) {
   if (head_dim != kD || batch < 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
     return (int)hipErrorInvalidValue;
   const int group = num_q_heads / num_kv_heads;
@@ -478,6 +504,7 @@ extern "C" int xv_prefill_attention(const void* q, int64_t q_stride_tok, int64_t
   a.out = (bf16_t*)out; a.out_st = out_stride_tok;
   a.hq = num_q_heads; a.hkv = num_kv_heads; a.batch = batch;
   a.scale_log2 = scale * 1.4426950408889634f;
+  a.window = min(window, 1 << 30); a.sinks = sink_tokens;  // positions are below 2^30
   const int gw = group < 4 ? group : 4;
   const int block_q = 32 * (4 / gw);
   a.qblocks = (max_seqlen_q + block_q - 1) / block_q;
@@ -491,4 +518,36 @@ extern "C" int xv_prefill_attention(const void* q, int64_t q_stride_tok, int64_t
   }
   XV_CHECK_LAUNCH();
   return 0;
+}
+
+}  // namespace
+
+extern "C" int xv_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                    const void* k, const void* v, int64_t kv_stride_tok, int64_t kv_stride_head,
+                                    const void* k_cache, const void* v_cache,
+                                    int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                                    const int32_t* block_tables, int64_t bt_stride,
+                                    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                    void* out, int64_t out_stride_tok,
+                                    int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+                                    int head_dim, int block_size, float scale, hipStream_t stream) {
+  return prefill(q, q_stride_tok, q_stride_head, k, v, kv_stride_tok, kv_stride_head, k_cache, v_cache, page_stride,
+                 tok_stride, head_stride, block_tables, bt_stride, cu_seqlens_q, cu_seqlens_k, out, out_stride_tok, batch,
+                 max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, 0, 0, scale, stream);
+}
+
+extern "C" int xv_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                           const void* k, const void* v, int64_t kv_stride_tok, int64_t kv_stride_head,
+                                           const void* k_cache, const void* v_cache,
+                                           int64_t page_stride, int64_t tok_stride, int64_t head_stride,
+                                           const int32_t* block_tables, int64_t bt_stride,
+                                           const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                           void* out, int64_t out_stride_tok,
+                                           int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+                                           int head_dim, int block_size, int window, int sink_tokens, float scale,
+                                           hipStream_t stream) {
+  if (window < 1 || sink_tokens < 0 || !(scale > 0.f)) return (int)hipErrorInvalidValue;
+  return prefill(q, q_stride_tok, q_stride_head, k, v, kv_stride_tok, kv_stride_head, k_cache, v_cache, page_stride,
+                 tok_stride, head_stride, block_tables, bt_stride, cu_seqlens_q, cu_seqlens_k, out, out_stride_tok, batch,
+                 max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, window, sink_tokens, scale, stream);
 }

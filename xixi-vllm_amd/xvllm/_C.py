@@ -86,6 +86,25 @@ SIGNATURES: dict[str, tuple] = {
         [vp, i64, i64, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, vp, i64, vp, sz,
          i32, i32, i32, i32, i32, i32, f32, vp],
     ),
+    "xv_window_decode_attention": (
+        i32,
+        [vp, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, vp, i64, vp, sz,
+         i32, i32, i32, i32, i32, i32, i32, i32, f32, vp],
+    ),
+    "xv_tree_attention_workspace_size": (sz, [i32, i32, i32, i32]),
+    "xv_tree_attention": (
+        i32,
+        [vp, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, vp, vp, i64, i32, vp, i64, vp, sz,
+         i32, i32, i32, i32, i32, i32, i32, f32, vp],
+    ),
+    "xv_window_prefill_attention": (
+        i32,
+        [vp, i64, i64, vp, vp, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, vp, vp, i64,
+         i32, i32, i32, i32, i32, i32, i32, i32, f32, vp],
+    ),
+    "xv_step_maps": (
+        i32, [vp, vp, i32, vp, i64, i32, i32, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+    ),
     "xv_mxfp4_gemm_workspace_size": (sz, [i32, i32, i32, i32]),
     "xv_mxfp4_gemm": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, sz, vp]),
     "xv_silu_and_mul": (i32, [vp, i64, vp, i64, i64, i32, vp]),

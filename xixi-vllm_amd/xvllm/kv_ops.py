@@ -1,6 +1,9 @@
-"""KV store by slot mapping (reference ``src/compute/kv_ops.py:35-62``), and the
-read back of 4-bit pages as bf16 rows."""
+"""KV store by slot mapping (reference ``src/compute/kv_ops.py:35-62``), the
+read back of 4-bit pages as bf16 rows, and a step's block tables, slots and
+positions from its requests' lengths."""
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -205,3 +208,90 @@ def gather_kvcache(
     call("xv_gather_kv_fp4", dev, *codes, *scales, bs, ptr(bt), bt.stride(0), bt.shape[1], ptr(cu), bsz,
          int(total_tokens), hkv, d, ptr(ko), ptr(vo), row)
     return ko, vo
+
+
+class StepMaps(NamedTuple):
+    cu_seqlens_q: torch.Tensor   # int32 [B + 1]: new tokens before each request
+    cu_seqlens_k: torch.Tensor   # int32 [B + 1]: tokens in the cache after the step, before each request
+    cache_seqlens: torch.Tensor  # int32 [B]: tokens of each request in the cache after the step
+    positions: torch.Tensor      # int64 [total_tokens]
+    slot_mapping: torch.Tensor   # int32 [total_tokens], -1: none
+    free_head: torch.Tensor      # int32 [1]: the free list's first page after the step
+
+
+MAX_STEP_ROWS = 8192
+
+
+def _index_args(dev: int, **named: torch.Tensor) -> None:
+    """Check index operands: int32 vectors of unit stride on GPU `dev`."""
+    for name, t in named.items():
+        if t.dtype != torch.int32 or t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1):
+            raise TypeError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
+        if t.get_device() != dev:
+            raise RuntimeError(f"{name} must be on the block tables' device")
+
+
+def step_maps(
+    seq_lens: torch.Tensor,
+    new_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    free_pages: torch.Tensor,
+    block_size: int,
+    total_tokens: int,
+    *,
+    free_head: torch.Tensor | None = None,
+    depths: torch.Tensor | None = None,
+) -> StepMaps:
+    """The maps of a step whose request b has seq_lens[b] tokens in the cache and
+    adds new_lens[b] (int32 [B], on the GPU), in one launch and without a look at
+    the lengths on the host (which builds the same in Batch.build_decode and
+    build_prefill):
+
+    - block_tables int32 [B, max_blocks], in place: each row's blocks from
+      ceil(seq_lens / block_size) to ceil((seq_lens + new_lens) / block_size)
+      are taken from free_pages[free_head:] (int32; free_head int32 [1], 0 where
+      None), row after row; its other entries stay as they are.
+    - StepMaps.free_head: free_head and the pages taken; larger than
+      len(free_pages) where the list ran out (such blocks get -1).
+    - positions and slot_mapping of the new tokens, request after request
+      (StepMaps.cu_seqlens_q), total_tokens rows in all, which the host knows:
+      rows past the last new token get slot -1 and position 0, tokens past
+      total_tokens none.  A token without a page (no block in its row, free list
+      run out) gets slot -1, which store_kvcache skips.
+    - depths int32 [total_tokens]: the new tokens are nodes of drafted trees, at
+      position seq_lens + depth instead of their index (tree_attention).
+
+    The running sums stay below 2^31, and so do the pool's slots."""
+    require_cuda(block_tables)
+    dev = block_tables.get_device()
+    _index_args(dev, seq_lens=seq_lens, new_lens=new_lens, free_pages=free_pages)
+    rows = seq_lens.shape[0]
+    if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < rows
+            or block_tables.shape[1] < 1 or block_tables.stride(1) != 1):
+        raise ValueError(f"block_tables {block_tables.dtype} {tuple(block_tables.shape)}: not int32 [{rows}, max_blocks] of "
+                         "unit last stride")
+    if new_lens.shape[0] != rows or rows > MAX_STEP_ROWS:
+        raise ValueError(f"{rows} seq_lens and {new_lens.shape[0]} new_lens: as many of each, at most {MAX_STEP_ROWS}")
+    if block_size < 1 or not 0 <= total_tokens <= 1 << 30:
+        raise ValueError(f"block_size {block_size}, total_tokens {total_tokens}")
+    bt_st = block_tables.stride(0)
+    if rows > 1 and bt_st < block_tables.shape[1]:
+        raise ValueError("block_tables' rows overlap")
+    if free_head is not None:
+        _index_args(dev, free_head=free_head)
+        if free_head.shape[0] != 1:
+            raise ValueError(f"free_head must hold one index, got {tuple(free_head.shape)}")
+    if depths is not None:
+        _index_args(dev, depths=depths)
+        if depths.shape[0] != total_tokens:
+            raise ValueError(f"{depths.shape[0]} depths for {total_tokens} tokens")
+    pos = torch.empty(total_tokens, dtype=torch.int64, device=block_tables.device)
+    buf = torch.empty(total_tokens + 3 * rows + 3, dtype=torch.int32, device=block_tables.device)
+    slots, cu_q, cu_k, ends, head = buf.split_with_sizes((total_tokens, rows + 1, rows + 1, rows, 1))
+    base = buf.data_ptr()
+    at = base + 4 * total_tokens
+    call("xv_step_maps", dev, seq_lens.data_ptr(), new_lens.data_ptr(), rows, block_tables.data_ptr(),
+         max(bt_st, block_tables.shape[1]), block_tables.shape[1], block_size, free_pages.data_ptr(), free_pages.shape[0],
+         ptr(free_head), ptr(depths), total_tokens, at, at + 4 * (rows + 1), at + 8 * (rows + 1), pos.data_ptr(), base,
+         at + 8 * (rows + 1) + 4 * rows)
+    return StepMaps(cu_q, cu_k, ends, pos, slots, head)

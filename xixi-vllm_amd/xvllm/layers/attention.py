@@ -177,6 +177,128 @@ def _paged_decode_fp4(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv,
     return out
 
 
+def _windowed(window: int, sink_tokens: int) -> bool:
+    """Whether a call has a sliding window (0: none), after checking its sizes."""
+    if not window and not sink_tokens:
+        return False
+    if window < 1 or sink_tokens < 0:
+        raise ValueError(f"window {window}, sink_tokens {sink_tokens}: a window is at least 1, sinks go with one and are not "
+                         "negative")
+    return True
+
+
+def _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, bsz, out, what):
+    """Operands of the attention kernels that take bf16 pages and a workspace
+    per call: the C ABI's q, cache, table and length arguments, the output and
+    its row stride."""
+    require_bf16(q)
+    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
+        raise TypeError(f"{what} reads bf16 pages, got {k_cache.dtype} and {v_cache.dtype}")
+    st = k_cache.stride()
+    if k_cache.dim() != 4 or k_cache.shape[2:] != (hkv, d) or v_cache.shape != k_cache.shape or v_cache.stride() != st or st[3] != 1:
+        raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} are not pages [NB, BS, {hkv}, {d}] of one "
+                         "layout")
+    q3, qs0, qs1 = _q_view(q, hq, d)
+    if q3.dim() != 3 or q3.shape[1:] != (hq, d):
+        raise ValueError(f"q {tuple(q.shape)} is not rows of {hq} heads of {d}")
+    if block_tables.dim() != 2 or block_tables.shape[0] < bsz or cache_seqlens.dim() != 1 or cache_seqlens.shape[0] < bsz:
+        raise ValueError(f"block_tables {tuple(block_tables.shape)}, cache_seqlens {tuple(cache_seqlens.shape)}: not a row and a "
+                         f"length for each of {bsz} sequences")
+    dev = k_cache.get_device()
+    if (dev < 0 or v_cache.get_device() != dev or q.get_device() != dev or block_tables.get_device() != dev
+            or cache_seqlens.get_device() != dev):
+        raise RuntimeError("xvllm ops run on the GPU only (HIP kernels), q, the cache, block_tables and cache_seqlens on one device")
+    bt = as_int32(block_tables)
+    max_blocks = bt.shape[1]
+    bt_st, inner = bt.stride()
+    if inner != 1 or (bsz > 1 and bt_st < max_blocks):
+        bt = bt.contiguous()
+        bt_st = max_blocks
+    sl = as_int32(cache_seqlens).contiguous()
+    rows = q3.shape[0]
+    if out is None:
+        out = torch.empty((rows, hq * d), dtype=q.dtype, device=q.device)
+        out_st = hq * d
+    elif out.shape != (rows, hq * d) or out.dtype != q.dtype or out.get_device() != dev or out.stride(-1) != 1:
+        raise ValueError(f"out must be bf16 [{rows}, {hq * d}] of unit last stride on the cache's device")
+    else:
+        out_st = out.stride(0)
+    head = (q3.data_ptr(), qs0, qs1, k_cache.data_ptr(), v_cache.data_ptr(), *st[:3], bt.data_ptr(), max(bt_st, max_blocks),
+            sl.data_ptr())
+    return dev, head, (q3, bt, sl), out, out_st, k_cache.shape[1], max_blocks
+
+
+def _window_decode(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, softmax_scale, out, window,
+                   sink_tokens) -> torch.Tensor:
+    bsz = q.shape[0]
+    dev, head, keep, out, out_st, bs, max_blocks = _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, bsz,
+                                                               out, "a windowed decode")
+    if bsz == 0:
+        return out
+    ws_bytes = _C.lib().xv_tree_attention_workspace_size(bsz, 1, hq, hkv)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
+    call("xv_window_decode_attention", dev, *head, out.data_ptr(), out_st, ws.data_ptr(), ws_bytes, bsz, hq, hkv, d, bs,
+         max_blocks, window, sink_tokens, scale)
+    return out
+
+
+MAX_TREE_NODES = 1024
+
+
+def tree_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    tree_mask: torch.Tensor,
+    max_seqlen_q: int,
+    num_qo_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    softmax_scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of trees of drafted tokens over the paged cache: q [T, Hq*D] (or
+    [T, Hq, D]) -> [T, Hq*D].
+
+    Sequence b holds cache_seqlens[b] tokens (int32 [B]), the last n =
+    cu_seqlens_q[b+1] - cu_seqlens_q[b] of them its drafted nodes, whose K and V
+    are in the cache already (bf16 pages [NB, BS, Hkv, D]).  Its node i is row
+    cu_seqlens_q[b] + i and sees every token before the nodes and node j where
+    bit j % 64 of tree_mask[row, j // 64] is set (int64 [T, words] or, up to 64
+    nodes, [T]; a node's own bit is set by the caller too: tree_masks).
+    max_seqlen_q: nodes of the largest tree, at most 64 * words and 1024.  Rows
+    that see nothing are zeros; rows from cu_seqlens_q[B] on are left as they
+    are in `out`.  Takes a workspace of its own per call."""
+    if cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] < 1:
+        raise ValueError(f"cu_seqlens_q {tuple(cu_seqlens_q.shape)} is not [B + 1]")
+    bsz = cu_seqlens_q.shape[0] - 1
+    dev, head, keep, out, out_st, bs, max_blocks = _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads,
+                                                               num_kv_heads, head_dim, bsz, out, "tree attention")
+    mask = tree_mask if tree_mask.dim() == 2 else tree_mask.unsqueeze(-1)
+    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != q.shape[0] or mask.shape[1] < 1:
+        raise ValueError(f"tree_mask {tree_mask.dtype} {tuple(tree_mask.shape)} is not int64 [{q.shape[0]}, words]")
+    if mask.get_device() != dev or cu_seqlens_q.get_device() != dev:
+        raise RuntimeError("tree_mask and cu_seqlens_q must be on the cache's device")
+    words = mask.shape[1]
+    if not 0 <= max_seqlen_q <= min(64 * words, MAX_TREE_NODES):
+        raise ValueError(f"max_seqlen_q {max_seqlen_q}: {words} mask words hold {64 * words} nodes, a tree at most {MAX_TREE_NODES}")
+    if bsz == 0 or max_seqlen_q == 0 or q.shape[0] == 0:
+        return out
+    if (words > 1 and mask.stride(1) != 1) or mask.stride(0) < words:
+        mask = mask.contiguous()
+    cu = as_int32(cu_seqlens_q).contiguous()
+    ws_bytes = _C.lib().xv_tree_attention_workspace_size(bsz, max_seqlen_q, num_qo_heads, num_kv_heads)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
+    call("xv_tree_attention", dev, *head, cu.data_ptr(), mask.data_ptr(), max(mask.stride(0), words), words, out.data_ptr(), out_st,
+         ws.data_ptr(), ws_bytes, bsz, max_seqlen_q, num_qo_heads, num_kv_heads, head_dim, bs, max_blocks, scale)
+    return out
+
+
 def paged_decode_attention(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -193,6 +315,8 @@ def paged_decode_attention(
     v_scale: float = 1.0,
     k_block_scale: torch.Tensor | None = None,
     v_block_scale: torch.Tensor | None = None,
+    window: int = 0,
+    sink_tokens: int = 0,
 ) -> torch.Tensor:
     """Causal decode over the paged cache: q [B, Hq*D] (or [B, Hq, D]),
     k_cache/v_cache [NB, BS, Hkv, D], block_tables int32 [B, max_blocks],
@@ -200,9 +324,17 @@ def paged_decode_attention(
     (torch.float8_e4m3fn, written by store_kvcache with the same scales)
     attends to k_cache * k_scale and v_cache * v_scale; a 4-bit cache
     (torch.float4_e2m1fn_x2 [NB, BS, Hkv, D/2]) to its codes times the block
-    scales k_block_scale / v_block_scale [NB, BS, Hkv, D/32].  The 4-bit form
-    takes a workspace of its own per call; the others share one per device
-    (decode_workspace)."""
+    scales k_block_scale / v_block_scale [NB, BS, Hkv, D/32].
+
+    window > 0 (bf16 caches): the query sees the last `window` tokens of its
+    sequence, itself among them, and the first sink_tokens; block-table entries
+    that hold none of these are not read.
+
+    The 4-bit and the windowed form take a workspace of their own per call; the
+    others share one per device (decode_workspace)."""
+    if _windowed(window, sink_tokens):
+        return _window_decode(q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim,
+                              softmax_scale, out, window, sink_tokens)
     if k_cache.dtype == FP4_PAGES:
         return _paged_decode_fp4(q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim,
                                  softmax_scale, out, k_block_scale, v_block_scale)
@@ -333,6 +465,9 @@ def prefill_attention(
     k_block_scale: torch.Tensor | None = None,
     v_block_scale: torch.Tensor | None = None,
     total_seqlen_k: int = 0,
+    *,
+    window: int = 0,
+    sink_tokens: int = 0,
 ) -> torch.Tensor:
     """Varlen causal attention, bottom-right aligned.  With block_tables the
     keys come from the paged cache (cached prefix + this chunk), otherwise
@@ -340,7 +475,14 @@ def prefill_attention(
     needs max_seqlen_k and its (k_scale, v_scale) (default: the active
     attention_context's), a 4-bit one its block scales and total_seqlen_k, the
     keys of all sequences (cu_seqlens_k's last): they are read back as so many
-    bf16 rows.  With max_seqlen_k alone room is made for B of the longest run."""
+    bf16 rows.  With max_seqlen_k alone room is made for B of the longest run.
+
+    window > 0: a query sees the last `window` keys up to itself and the
+    sequence's first sink_tokens (softmax_scale > 0); block-table entries that
+    hold no key some query sees are not read from bf16 pages."""
+    windowed = _windowed(window, sink_tokens)
+    if windowed and softmax_scale is not None and not softmax_scale > 0:
+        raise ValueError(f"a windowed prefill needs softmax_scale > 0, got {softmax_scale}")
     q3, qs0, qs1 = _q_view(q, num_qo_heads, head_dim)
     require_cuda(q3, cu_seqlens_q, cu_seqlens_k)
     require_bf16(q3)
@@ -361,7 +503,7 @@ def prefill_attention(
         kd, vd = gather_kvcache(k_cache, v_cache, block_tables, cuk, int(total_seqlen_k) or bsz * int(max_seqlen_k),
                                 k_block_scale=k_block_scale, v_block_scale=v_block_scale)
         return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
-                                 head_dim, softmax_scale=softmax_scale)
+                                 head_dim, softmax_scale=softmax_scale, window=window, sink_tokens=sink_tokens)
     if block_tables is not None and k_cache is not None and k_cache.dtype == torch.float8_e4m3fn:
         # fp8 pages: the sequences' keys dequantized into varlen bf16 rows, then the dense path
         k_scale, v_scale = kv_scales() if kv_scale is None else kv_scale
@@ -383,7 +525,7 @@ def prefill_attention(
             "xv_gather_kv_fp8",
         )
         return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
-                                 head_dim, softmax_scale=softmax_scale)
+                                 head_dim, softmax_scale=softmax_scale, window=window, sink_tokens=sink_tokens)
     if block_tables is not None:
         assert k_cache is not None and v_cache is not None
         require_bf16(k_cache, v_cache)
@@ -408,6 +550,11 @@ def prefill_attention(
         kc = vc = bt = None
         ps = ts = hs = bts = 0
         page = 16
+    if windowed:
+        call("xv_window_prefill_attention", q3.get_device(), ptr(q3), qs0, qs1, ptr(kd), ptr(vd), kvs0, kvs1, ptr(kc), ptr(vc), ps,
+             ts, hs, ptr(bt), bts, ptr(cuq), ptr(cuk), ptr(out), out.stride(0), bsz, int(max_seqlen_q), num_qo_heads,
+             num_kv_heads, head_dim, page, int(window), int(sink_tokens), float(scale))
+        return out
     _C.check(
         _C.lib().xv_prefill_attention(
             ptr(q3), qs0, qs1, ptr(kd), ptr(vd), kvs0, kvs1, ptr(kc), ptr(vc), ps, ts, hs, ptr(bt), bts,
