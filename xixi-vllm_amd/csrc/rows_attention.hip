@@ -11,9 +11,8 @@
 // unit) space is flattened in that order and cut into equal contiguous ranges;
 // a range cut inside a segment leaves partials (normalised fp32 rows and their
 // log2-sum-exp) for a merge kernel, two partial slots per range at most.
-// Rows are taken 16 NT at a time by a wave (NT 1 or 2 tiles of 16): one wave
-// reads a range for up to 32 rows, RT waves of a workgroup the same range for
-// up to 32 RT rows.
+// A wave takes NT tiles of 16 rows, 1 or 2; sequences of more rows (large
+// trees) are the matter of tree_tiles.hip.
 //
 // A unit (32 tokens), all on v_mfma_f32_16x16x32_bf16:
 //   K and V rows go HBM -> LDS by LDS-DMA, two units in flight per wave.
@@ -24,19 +23,18 @@
 //   the lanes where the scores landed.  O^T has row c in lane c too, so the
 //   softmax maximum, sum and rescale stay in the lane.
 #include "xv_common.h"
-#include "xv_decode.h"
 #include "xv_kernels.h"
+#include "xv_rows.h"
 #include <math.h>
+
+using namespace xv_rows;
 
 namespace {
 
 constexpr int kD = 128;
-constexpr int kPage = 16;
 constexpr int kUnit = 32;          // tokens of a unit: two pages
-constexpr int kMaxBatch = 256;     // sequences per launch (larger batches are launched in chunks)
 constexpr int kWaves = 4;          // waves of a workgroup, one workgroup per CU
 constexpr int kMaxGroups = 256;    // workgroups at most
-constexpr int kMaxParts = 192;     // partials of a segment at most
 constexpr int kHalf = 4096;        // a page's K (or V) rows in LDS
 constexpr int kUnitLds = 4 * kHalf;  // page A: K, V; page B: K, V
 constexpr int kUnitOps = 16;       // LDS-DMA instructions a unit
@@ -47,35 +45,6 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
-struct RowsArgs {
-  const bf16_t* q; int64_t q_st, q_sh;
-  const bf16_t* kc; const bf16_t* vc; int64_t ps, ts, hs;
-  const int32_t* bt; int64_t bt_stride;
-  const int32_t* seqlens;
-  const int32_t* cu_q;                          // tree: first node of each sequence
-  const uint64_t* mask; int64_t mask_st; int words;  // tree: visible nodes of each node
-  bf16_t* out; int64_t out_st;
-  int2* ws_seg;     // (first range, partials) per (sequence, kv head)
-  float* ws_lse;    // log2-sum-exp of partial slot s, row r at s * rows + r
-  float* ws_o;      // its rows, kD values each
-  int batch, hq, hkv, glog;  // query heads per kv head: 1 << glog
-  int nsub;         // 16-token pages per cache block
-  int max_ctx;      // tokens the block table has room for
-  int window, sinks;
-  int rt;           // waves of a workgroup that share a range
-  int rows;         // rows of a partial slot
-  float scale_log2; // not negative: q_flip carries the sign of the scale
-  uint32_t q_flip;
-};
-
-XV_INLINE int lds_int(const int* p) {
-  int v;
-  __asm__ __volatile__("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)"
-                       : "=&v"(v)
-                       : "v"((uint32_t)reinterpret_cast<uintptr_t>(p))
-                       : "memory");
-  return __builtin_amdgcn_readfirstlane(v);
-}
 XV_INLINE u32x2_t lds_ids(const char* p) {
   u32x2_t v;
   __asm__ __volatile__("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)"
@@ -106,25 +75,6 @@ XV_INLINE int page_at(const Pages& p, int i) { return i < p.sink ? i : i + p.ski
 template <bool TREE>
 XV_INLINE int units_of(int ctx, int window, int sinks) {
   return (pages_of<TREE>(ctx, window, sinks).list + 1) / 2;
-}
-
-struct RowsCursor {
-  int b, kvh, u;   // sequence, kv head, unit within the sequence
-  int nu, ctx;     // units and tokens of sequence b
-};
-
-// The next unit of the flat space (LDS reads in asm: a plain one would wait
-// for every unit in flight).  Sequences without units are stepped over.
-XV_INLINE void advance(RowsCursor& c, const int* pref, const int* sl, int hkv, int batch) {
-  if (++c.u < c.nu) return;
-  c.u = 0;
-  if (++c.kvh < hkv) return;
-  c.kvh = 0;
-  do {
-    ++c.b;
-    c.nu = lds_int(pref + c.b + 1) - lds_int(pref + c.b);
-  } while (c.nu == 0 && c.b < batch - 1);
-  c.ctx = lds_int(sl + c.b);
 }
 
 // LDS image of a page's K or V rows of one kv head: token t's 256-byte row at
@@ -203,9 +153,6 @@ struct RowsState {
   floatx4_t o[NT][8];   // O^T of d-tile n: d = 16n + 4g + r, row c
 };
 
-// bits t of a unit: 0 .. 15 tokens of the first page, 16 .. 31 of the second
-XV_INLINE uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
-
 // Scores, softmax update and O^T += V^T P^T of one unit.  EDGE: seen[t] has the tokens that row c of tile t sees.
 template <int NT, bool EDGE>
 XV_INLINE void unit_math(RowsState<NT>& st, const UnitRegs& u, const bf16x8_t (&qb)[NT][4], const uint32_t (&seen)[NT],
@@ -249,12 +196,8 @@ XV_INLINE void unit_math(RowsState<NT>& st, const UnitRegs& u, const bf16x8_t (&
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int p = e >> 1, r = 2 * (e & 1);
-      float p0 = __builtin_amdgcn_exp2f(fmaf(a[t][p][r], scale_log2, nm));
-      float p1 = __builtin_amdgcn_exp2f(fmaf(a[t][p][r + 1], scale_log2, nm));
-      if (EDGE) {  // also where a scale of 0 makes -inf * scale a NaN
-        p0 = (bits >> (16 * p + r)) & 1 ? p0 : 0.f;
-        p1 = (bits >> (16 * p + r + 1)) & 1 ? p1 : 0.f;
-      }
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(a[t][p][r], scale_log2, nm));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(a[t][p][r + 1], scale_log2, nm));
       w[e] = pack_bf16x2(p0, p1);
       // the row sum takes the bf16 weights that the product multiplies: their rounding (2^-9 of a weight) moves
       // the output by that share of the values' spread only, and a row of one heavy token is exact
@@ -304,13 +247,12 @@ XV_INLINE void reset(RowsState<NT>& st) {
 // The finished segment's rows: bf16 output if the range covered the whole
 // segment (slot < 0), else fp32 rows of partial slot `slot`.
 template <int NT>
-XV_INLINE void finish_rows(const RowsArgs& a, const RowsState<NT>& st, int tok0, int kvh, int row0, int nrows, int slot,
-                           int lane) {
+XV_INLINE void finish_rows(const RowsArgs& a, const RowsState<NT>& st, int tok0, int kvh, int nrows, int slot, int lane) {
   typedef u32x2_t __attribute__((aligned(4))) u32x2_a4;  // the caller's rows need not be 8-byte aligned
   const int c = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int row = row0 + 16 * t + c;
+    const int row = 16 * t + c;
     const float lsum = xor32_sum(xor16_sum(st.l[t]));
     const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;  // a row that sees nothing: zeros; NaN stays NaN
     if (row >= nrows) continue;
@@ -336,17 +278,17 @@ XV_INLINE void finish_rows(const RowsArgs& a, const RowsState<NT>& st, int tok0,
 // table filled by LDS-DMA from the block table.  Units past the range, and
 // pages past a sequence's list, fetch an entry that exists.
 template <bool TREE>
-XV_INLINE void load_window(char* half, const RowsArgs& a, __amdgpu_buffer_rsrc_t rbt, const int* pref, const int* sl,
+XV_INLINE void load_window(char* half, const RowsArgs& a, __amdgpu_buffer_rsrc_t rbt, const Sequences& s,
                            int64_t f0, int base, int n, int lane) {
   static_assert(kIdWindow * 2 == 64, "one id per lane");
   const int y = base + (lane >> 1);
   int off = 0;
   if (y < n) {
     const int64_t f = f0 + y;
-    const int b = seq_of(pref, a.batch, a.hkv, f);
-    const int nu = pref[b + 1] - pref[b];
-    const int u = (int)(f - (int64_t)a.hkv * pref[b]) % nu;
-    const Pages p = pages_of<TREE>(sl[b], a.window, a.sinks);
+    const int b = seq_of(s.pref, a.batch, a.hkv, f);
+    const int nu = s.pref[b + 1] - s.pref[b];
+    const int u = (int)(f - (int64_t)a.hkv * s.pref[b]) % nu;
+    const Pages p = pages_of<TREE>(s.ctx[b], a.window, a.sinks);
     const int page = page_at(p, min(2 * u + (lane & 1), p.list - 1));
     off = (int)(((int64_t)b * a.bt_stride + page / a.nsub) * 4);
   }
@@ -365,71 +307,26 @@ XV_INLINE uint32_t node_bits(const uint64_t* words, int n, int at) {
 template <int NT, bool TREE>
 __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 1))) void rows_kernel(RowsArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[kWaves * kWaveLds];
-  __shared__ int pref[kMaxBatch + 1];  // units of sequences 0 .. b - 1
-  __shared__ int sl[kMaxBatch];        // their tokens
-  __shared__ int cq[kMaxBatch + 1];    // their first rows of q
+  __shared__ Sequences seqs;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (wave == 0) {
-    int carry = 0;
-    for (int c = 0; c < a.batch; c += 64) {
-      const int b = c + lane;
-      int ctx = 0, q0 = b, q1 = b + 1;
-      if (b < a.batch) {
-        ctx = min(max(a.seqlens[b], 0), a.max_ctx);
-        if (TREE) {
-          q0 = a.cu_q[b];
-          q1 = a.cu_q[b + 1];
-          if (q1 <= q0) ctx = 0;  // no rows: no units
-        }
-      }
-      int inc = ctx > 0 ? units_of<TREE>(ctx, a.window, a.sinks) : 0;
-      inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xf, 0xf, true);  // inclusive scan: row_shr 1, 2, 4, 8,
-      inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xf, 0xf, true);  // then the row sums across rows
-      inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xf, 0xf, true);
-      inc += __builtin_amdgcn_update_dpp(0, inc, 0x118, 0xf, 0xf, true);
-      inc += __builtin_amdgcn_update_dpp(0, inc, 0x142, 0xa, 0xf, true);
-      inc += __builtin_amdgcn_update_dpp(0, inc, 0x143, 0xc, 0xf, true);
-      if (b < a.batch) {
-        pref[b + 1] = carry + inc;
-        sl[b] = ctx;
-        cq[b] = q0;
-        cq[b + 1] = q1;  // the next lane writes the same value
-      }
-      carry += __builtin_amdgcn_readlane(inc, 63);
-    }
-    if (lane == 0) pref[0] = 0;
-  }
+  if (wave == 0)
+    load_sequences<TREE>(seqs, a, lane, [&](int ctx) { return units_of<TREE>(ctx, a.window, a.sinks); });
   __syncthreads();
-  int longest = 0;
-  for (int b = lane; b < a.batch; b += 64) longest = max(longest, pref[b + 1] - pref[b]);
-  const int max_nu = (int)wave_max((float)longest);  // exact in fp32 (below 2^24)
-  const int64_t total = (int64_t)a.hkv * __builtin_amdgcn_readfirstlane(pref[a.batch]);
-  // units per range: every range the same, and no segment in more than kMaxParts ranges
-  const int nranges = gridDim.x * (kWaves / a.rt);
-  const int L = (int)max((int64_t)max(1, (max_nu + kMaxParts - 2) / (kMaxParts - 1)), (total + nranges - 1) / nranges);
-  const int id = (wave / a.rt) * gridDim.x + blockIdx.x;  // short launches spread over the CUs first
-  const int row0 = (blockIdx.y * a.rt + wave % a.rt) * (16 * NT);
+  const Ranges rg = ranges_of(seqs, a, gridDim.x * kWaves, lane);
+  const int L = rg.len;
+  const int id = wave * gridDim.x + blockIdx.x;  // short launches spread over the CUs first
   const int64_t f0 = (int64_t)id * L;
-  const int n = (int)max((int64_t)0, min(f0 + L, total) - f0);
+  const int n = (int)max((int64_t)0, min(f0 + L, rg.total) - f0);
   if (n == 0) return;
   char* const mine = lds + wave * kWaveLds;
   char* const idtab = mine + 2 * kUnitLds;
   const RowsLane offs = lane_offsets(a.ts, lane);
 
-  RowsCursor c0;
-  c0.b = __builtin_amdgcn_readfirstlane(seq_of(pref, a.batch, a.hkv, f0));
-  c0.nu = __builtin_amdgcn_readfirstlane(pref[c0.b + 1] - pref[c0.b]);
-  c0.ctx = __builtin_amdgcn_readfirstlane(sl[c0.b]);
-  {
-    const int r = (int)(f0 - (int64_t)a.hkv * pref[c0.b]);
-    c0.kvh = __builtin_amdgcn_readfirstlane(r / c0.nu);
-    c0.u = __builtin_amdgcn_readfirstlane(r - c0.kvh * c0.nu);
-  }
-  RowsCursor ic = c0, pc = c0;  // issue and process cursors
+  Cursor ic = cursor_at(seqs, a, f0), pc = ic;  // issue and process cursors
   const __amdgpu_buffer_rsrc_t rbt =
       page_rsrc(reinterpret_cast<const bf16_t*>(a.bt), (uint32_t)((int64_t)a.batch * a.bt_stride * 4));
-  load_window<TREE>(idtab, a, rbt, pref, sl, f0, 0, n, lane);
-  if (n > kIdWindow) load_window<TREE>(idtab + kIdWindow * 8, a, rbt, pref, sl, f0, kIdWindow, n, lane);
+  load_window<TREE>(idtab, a, rbt, seqs, f0, 0, n, lane);
+  if (n > kIdWindow) load_window<TREE>(idtab + kIdWindow * 8, a, rbt, seqs, f0, kIdWindow, n, lane);
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
 
   const uint32_t page_bytes = (uint32_t)((15 * a.ts + kD) * 2);
@@ -437,7 +334,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
   auto issue = [&](int y) {
     char* buf = mine + (y & 1) * kUnitLds;
     if (y % kIdWindow == 0 && y > 0)  // entering window k (in place since window k - 1 began): request window k + 1
-      load_window<TREE>(idtab + ((y / kIdWindow + 1) & 1) * (kIdWindow * 8), a, rbt, pref, sl, f0, y + kIdWindow, n, lane);
+      load_window<TREE>(idtab + ((y / kIdWindow + 1) & 1) * (kIdWindow * 8), a, rbt, seqs, f0, y + kIdWindow, n, lane);
     const u32x2_t ids = lds_ids(idtab + ((y / kIdWindow) & 1) * (kIdWindow * 8) + (y % kIdWindow) * 8);
     const Pages p = pages_of<TREE>(ic.ctx, a.window, a.sinks);
 #pragma unroll
@@ -459,22 +356,14 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
   RowsState<NT> st;
   bf16x8_t qb[NT][4];
   int tok0 = 0, nrows = 0;  // the segment's first row of q, and its rows
-  auto finish = [&](const RowsCursor& c) {
-    const int64_t seg0 = (int64_t)a.hkv * lds_int(pref + c.b) + (int64_t)c.kvh * c.nu;
-    const bool first = seg0 >= f0, last = seg0 + c.nu <= f0 + n;
-    // a segment that starts in this range and ends after it: slot 1 of the range, one that started before: slot 0
-    finish_rows<NT>(a, st, tok0, c.kvh, row0, nrows, first && last ? -1 : 2 * id + (first ? 1 : 0), lane);
-    if (lane == 0 && last && row0 == 0) {
-      const int w0 = (int)(seg0 / L);
-      a.ws_seg[c.b * a.hkv + c.kvh] = make_int2(w0, id - w0 + 1);
-    }
+  auto finish = [&](const Cursor& c) {
+    finish_rows<NT>(a, st, tok0, c.kvh, nrows, finish_slot(seqs, a, c, f0, n, id, L, lane == 0), lane);
   };
-  auto row_of = [&](int t) { return min(row0 + 16 * t + (lane & 15), nrows - 1); };  // rows past the last: the last again
+  auto row_of = [&](int t) { return min(16 * t + (lane & 15), nrows - 1); };  // rows past the last: the last again
   auto begin = [&] {
-    tok0 = lds_int(cq + pc.b);
-    nrows = (TREE ? lds_int(cq + pc.b + 1) - tok0 : 1) << a.glog;
+    tok0 = lds_int(seqs.cq + pc.b);
+    nrows = (TREE ? lds_int(seqs.cq + pc.b + 1) - tok0 : 1) << a.glog;
     reset(st);
-    if (row0 >= nrows) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int row = row_of(t);
@@ -484,20 +373,20 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
       for (int s = 0; s < 4; ++s) {
         Vec8 v = load_vec8(src + 32 * s);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v.w[e] ^= a.q_flip;
+        for (int e = 0; e < 4; ++e) v.w[e] = (v.w[e] & a.q_keep) ^ a.q_flip;
         __builtin_memcpy(&qb[t][s], &v, 16);
       }
     }
   };
   issue(0);
   if (n > 1) {
-    advance(ic, pref, sl, a.hkv, a.batch);
+    advance(ic, seqs, a.hkv, a.batch);
     issue(1);
   }
   UnitRegs u;
   for (int x = 0; x < n; ++x) {
-    const RowsCursor prev = pc;
-    if (x > 0) advance(pc, pref, sl, a.hkv, a.batch);
+    const Cursor prev = pc;
+    if (x > 0) advance(pc, seqs, a.hkv, a.batch);
     if (x == 0 || pc.u == 0) {
       if (x > 0) finish(prev);
       begin();
@@ -507,10 +396,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
     else __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
     read_unit(u, mine + (x & 1) * kUnitLds, offs);
     if (x + 2 < n) {
-      advance(ic, pref, sl, a.hkv, a.batch);
+      advance(ic, seqs, a.hkv, a.batch);
       issue(x + 2);
     }
-    if (row0 >= nrows) continue;
     const Pages p = pages_of<TREE>(pc.ctx, a.window, a.sinks);
     uint32_t seen[NT];
     bool edge;
@@ -630,23 +518,16 @@ int rows_groups() {
   return cached;
 }
 
-// How a call's rows (query heads per kv head times the nodes of its largest tree) are taken.
-struct RowSplit {
-  int nt, rt, passes;
-};
-RowSplit row_split(int max_rows) {
-  RowSplit s;
-  s.nt = max_rows <= 16 ? 1 : 2;
-  s.rt = max_rows <= 32 ? 1 : max_rows <= 64 ? 2 : 4;
-  s.passes = (max_rows + 16 * s.nt * s.rt - 1) / (16 * s.nt * s.rt);
-  return s;
-}
-int slot_rows(const RowSplit& s) { return 16 * s.nt * s.rt * s.passes; }
+// Calls of up to 32 rows per sequence and kv head (query heads per kv head times
+// the nodes of the largest tree) run here, a wave on its own; larger trees share
+// their tiles among the waves of a workgroup (tree_tiles.hip).
+constexpr int kWaveRows = 32;
+int slot_rows(int max_rows) { return max_rows <= 16 ? 16 : max_rows <= kWaveRows ? 32 : tile_rows(max_rows); }
+size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : kTileGroups); }
 
 size_t al256(size_t x) { return (x + 255) / 256 * 256; }
 size_t seg_bytes(int batch, int hkv) { return al256((size_t)min(batch, kMaxBatch) * hkv * sizeof(int2)); }
-size_t slots(const RowSplit& s) { return (size_t)kMaxGroups * (kWaves / s.rt) * 2; }
-size_t lse_bytes(const RowSplit& s) { return al256(slots(s) * slot_rows(s) * sizeof(float)); }
+size_t lse_bytes(int max_rows) { return al256(slots(max_rows) * slot_rows(max_rows) * sizeof(float)); }
 
 bool valid_group(int hq, int hkv) {
   if (hkv <= 0 || hq <= 0 || hq % hkv) return false;
@@ -657,12 +538,11 @@ bool valid_group(int hq, int hkv) {
 template <bool TREE>
 int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* seqlens, const int32_t* cu_q, bf16_t* out,
                 int batch, int max_nodes, void* workspace, hipStream_t stream) {
-  const RowSplit s = row_split(max_nodes << a.glog);
-  a.rt = s.rt;
-  a.rows = slot_rows(s);
+  const int max_rows = max_nodes << a.glog;
+  a.rows = slot_rows(max_rows);
   a.ws_seg = (int2*)workspace;
   a.ws_lse = (float*)((char*)workspace + seg_bytes(batch, a.hkv));
-  a.ws_o = (float*)((char*)a.ws_lse + lse_bytes(s));
+  a.ws_o = (float*)((char*)a.ws_lse + lse_bytes(max_rows));
   // units that the widest visible list may hold
   const int64_t pages = TREE ? (a.max_ctx + kPage - 1) / kPage
                              : min((int64_t)(a.max_ctx + kPage - 1) / kPage,
@@ -675,12 +555,16 @@ int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* s
     a.bt = bt + (int64_t)b0 * a.bt_stride;
     a.seqlens = seqlens + b0;
     const int64_t units = (int64_t)a.batch * a.hkv * ((pages + 1) / 2);
-    const dim3 grid((unsigned)max((int64_t)1, min((int64_t)rows_groups(), units)), (unsigned)s.passes);
-    switch (s.nt) {
-      case 1: rows_kernel<1, TREE><<<grid, kWaves * 64, 0, stream>>>(a); break;
-      default:
-        if constexpr (TREE) rows_kernel<2, TREE><<<grid, kWaves * 64, 0, stream>>>(a);
-        break;
+    const unsigned groups = (unsigned)min((int64_t)rows_groups(), units);
+    if (max_rows <= 16) {
+      rows_kernel<1, TREE><<<groups, kWaves * 64, 0, stream>>>(a);
+    } else if constexpr (TREE) {
+      if (max_rows <= kWaveRows) {
+        rows_kernel<2, TREE><<<groups, kWaves * 64, 0, stream>>>(a);
+      } else {
+        const int e = launch_tiles(a, max_rows, stream);
+        if (e) return e;
+      }
     }
     XV_CHECK_LAUNCH();
     rows_merge_kernel<TREE><<<dim3((unsigned)((max_nodes * a.hq + 3) / 4), (unsigned)a.batch), 256, 0, stream>>>(a);
@@ -708,7 +592,8 @@ bool rows_args(RowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const voi
   a.glog = __builtin_ctz(hq / hkv);
   a.nsub = block_size / kPage;
   a.max_ctx = (int)max_ctx;
-  a.scale_log2 = fabsf(scale) * 1.4426950408889634f;
+  a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;
+  a.q_keep = scale == 0.f ? 0u : ~0u;
   a.q_flip = scale < 0.f ? 0x80008000u : 0u;
   return true;
 }
@@ -717,8 +602,8 @@ bool rows_args(RowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const voi
 
 extern "C" size_t xv_tree_attention_workspace_size(int batch, int max_nodes, int num_q_heads, int num_kv_heads) {
   if (batch <= 0 || max_nodes <= 0 || !valid_group(num_q_heads, num_kv_heads)) return 256;
-  const RowSplit s = row_split(max_nodes * (num_q_heads / num_kv_heads));
-  return seg_bytes(batch, num_kv_heads) + lse_bytes(s) + slots(s) * slot_rows(s) * kD * sizeof(float);
+  const int max_rows = max_nodes * (num_q_heads / num_kv_heads);
+  return seg_bytes(batch, num_kv_heads) + lse_bytes(max_rows) + slots(max_rows) * slot_rows(max_rows) * kD * sizeof(float);
 }
 
 extern "C" int xv_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
