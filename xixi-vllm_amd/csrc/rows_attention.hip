@@ -506,6 +506,60 @@ __global__ __launch_bounds__(256) void rows_merge_kernel(RowsArgs a) {
   }
 }
 
+// The same for many rows of few partials: four rows a wave, 16 lanes each (8 values a lane), one partial after the
+// other, four in flight.
+__global__ __launch_bounds__(256) void rows_merge4_kernel(RowsArgs a) {
+  const int lane = threadIdx.x & 63, i = lane & 15;
+  const int task = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4), b = blockIdx.y;
+  const int node = task / a.hq, h = task - node * a.hq;
+  const int tok0 = a.cu_q[b];
+  if (node >= a.cu_q[b + 1] - tok0) return;
+  const int kvh = h >> a.glog, r0 = (node << a.glog) + (h & ((1 << a.glog) - 1));
+  const int ctx = a.seqlens[b];
+  const int2 seg = a.ws_seg[b * a.hkv + kvh];  // stale when ctx <= 0: not used then
+  uint32_t* orow = reinterpret_cast<uint32_t*>(a.out + (int64_t)(tok0 + node) * a.out_st + (int64_t)h * kD + 8 * i);
+  if (ctx <= 0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) orow[e] = 0u;
+    return;
+  }
+  const int n = seg.y;
+  if (n <= 1) return;
+  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.rows + r0; };
+  float mx = -INFINITY;
+  for (int j = i; j < n; j += 16) mx = fmaxf(mx, a.ws_lse[slot(j)]);
+  mx = row16_max(mx);
+  if (mx == -INFINITY) mx = 0.f;  // the row sees nothing: weights of 0
+  float mass = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < n; j0 += 4) {
+    float lse[4];
+    floatx4_t lo[4], hi[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = slot(min(j0 + k, n - 1));
+      const floatx4_t* from = reinterpret_cast<const floatx4_t*>(a.ws_o + at * kD + 8 * i);
+      lse[k] = a.ws_lse[at];
+      lo[k] = from[0];
+      hi[k] = from[1];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = j0 + k < n ? __builtin_amdgcn_exp2f(lse[k] - mx) : 0.f;
+      mass += w;
+      if (j0 + k < n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[e] += w * lo[k][e];
+          acc[4 + e] += w * hi[k][e];
+        }
+      }
+    }
+  }
+  const float inv = mass == 0.f ? 0.f : 1.0f / mass;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) orow[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+}
+
 int rows_groups() {
   static int cached = 0;  // one GPU model per process
   if (!cached) {
@@ -522,6 +576,8 @@ int rows_groups() {
 // the nodes of the largest tree) run here, a wave on its own; larger trees share
 // their tiles among the waves of a workgroup (tree_tiles.hip).
 constexpr int kWaveRows = 32;
+// Rows of a tree call from which on the merge takes four rows a wave: enough waves then without spreading a row's partials.
+constexpr int kManyRows = 8192;
 int slot_rows(int max_rows) { return max_rows <= 16 ? 16 : max_rows <= kWaveRows ? 32 : tile_rows(max_rows); }
 size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : kTileGroups); }
 
@@ -567,7 +623,11 @@ int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* s
       }
     }
     XV_CHECK_LAUNCH();
-    rows_merge_kernel<TREE><<<dim3((unsigned)((max_nodes * a.hq + 3) / 4), (unsigned)a.batch), 256, 0, stream>>>(a);
+    const int64_t per_seq = (int64_t)max_nodes * a.hq;
+    if (TREE && per_seq * a.batch >= kManyRows)
+      rows_merge4_kernel<<<dim3((unsigned)((per_seq + 15) / 16), (unsigned)a.batch), 256, 0, stream>>>(a);
+    else
+      rows_merge_kernel<TREE><<<dim3((unsigned)((per_seq + 3) / 4), (unsigned)a.batch), 256, 0, stream>>>(a);
     XV_CHECK_LAUNCH();
   }
   return 0;
@@ -582,7 +642,7 @@ bool rows_args(RowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const voi
   if (max_ctx > (1 << 28)) return false;  // 256M tokens per sequence
   // rows move by 16-byte LDS-DMA at 32-bit offsets within a page
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15 || (q_st | q_sh | ps | ts | hs) & 7) return false;
-  if (ts < kD || ts > (1 << 26) || ps < 0 || hs < 0 || bt_stride < max_blocks || min(batch, kMaxBatch) * bt_stride * 4 > INT32_MAX)
+  if (ts < kD || ts > (1 << 26) || ps < 0 || ps > UINT32_MAX || hs < 0 || bt_stride < max_blocks || min(batch, kMaxBatch) * bt_stride * 4 > INT32_MAX)
     return false;
   if ((uintptr_t)out & 3 || out_st & 1) return false;
   a.q_st = q_st; a.q_sh = q_sh;

@@ -191,7 +191,7 @@ XV_INLINE void finish_row(const RowsArgs& a, const TileState& st, int tok0, int 
 }
 
 // Scalar load of a table entry at a wave-uniform index: it does not wait for the tiles in flight.
-XV_INLINE int table_entry(const int32_t* p) {
+XV_INLINE int load_index(const int32_t* p) {
   return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
 }
 
@@ -221,80 +221,126 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
   const int row0 = (blockIdx.y * WAVES + wave) * 32, row = row0 + l32;  // this lane's row of every segment
   const LdsAddr ad = lds_addr(lds, lane);
 
-  // This wave loads rows r0 .. r0 + kRows - 1 of a tile, all in one cache block.
+  // ---- The tiles' feed.  This wave loads rows r0 .. r0 + kRows - 1 of a tile, all in one cache block: row `r` on of block
+  // `blk`, of which `valid` (and more behind them) are in the sequence; rows past its end read as zeros, and so does every
+  // row past the range, so that an iteration issues the same number of loads wherever it is.
   const int r0 = kRows * wave;
   const int block = a.nsub * kPage;
-  auto block_of = [&](const Cursor& c) {  // 0 past the sequence's end: not read then
-    const int j = c.u * kKeys + r0;
-    return j < c.ctx ? table_entry(a.bt + (int64_t)c.b * a.bt_stride + j / block) : 0;
+  const int step_blocks = kKeys / block, step_rows = kKeys % block;
+  Cursor ic = cursor_at(seqs, a, f0);
+  int issued = 0, idx = 0, r = 0, valid = 0, blk = 0;
+  const int32_t* table = a.bt;
+  auto fetch = [&] { blk = valid > 0 ? load_index(table + idx) : 0; };
+  auto enter = [&] {  // at ic, wherever that is in its segment
+    const int j = ic.u * kKeys + r0;
+    idx = j / block;
+    r = j - idx * block;
+    valid = ic.ctx - j;
+    table = a.bt + (int64_t)ic.b * a.bt_stride;
   };
-  // The tile at c, its rows of this wave in cache block blk, into slot `slot`; rows past the sequence's end read as zeros.
-  auto load = [&](const Cursor& c, int blk, int slot) {
-    const int j = c.u * kKeys + r0;
-    const int valid = min(kRows, c.ctx - j);
-    const int64_t off = (int64_t)blk * a.ps + (int64_t)(j % block) * a.ts + (int64_t)c.kvh * a.hs;
-    const uint32_t bytes = valid > 0 ? (uint32_t)(((valid - 1) * a.ts + kD) * 2) : 0u;
+  auto issue = [&] {
+    const int64_t off = (int64_t)((uint64_t)(uint32_t)blk * (uint32_t)a.ps) + (int64_t)((uint64_t)(uint32_t)r * (uint32_t)a.ts) +
+                        (int64_t)ic.kvh * a.hs;
+    const uint32_t bytes = valid > 0 ? (uint32_t)(((min(valid, kRows) - 1) * (int)a.ts + kD) * 2) : 0u;
     const __amdgpu_buffer_rsrc_t rk = page_rsrc(a.kc + off, bytes), rv = page_rsrc(a.vc + off, bytes);
-    char* const buf = lds + slot * kBuf + r0 * 256;
+    char* const buf = lds + (issued % NB) * kBuf + r0 * 256;
 #pragma unroll
     for (int s = 0; s < kRows / 4; ++s) {
-      const int r = 4 * s + (lane >> 4), R = r0 + r;
-      const int vo = (int)(r * a.ts * 2);
+      const int rr = 4 * s + (lane >> 4), R = r0 + rr;
+      const int vo = (int)(rr * a.ts * 2);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void*)(buf + 1024 * s), 16, vo + (((lane & 15) ^ swz_k(R)) << 4), 0, 0, 0);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void*)(buf + kTile + 1024 * s), 16,
                                                vo + (((lane & 15) ^ swz_v(R)) << 4), 0, 0, 0);
     }
-  };
-
-  Cursor pc = cursor_at(seqs, a, f0), ic = pc;  // tile x, and the next one to load
-  int issued = 0, blk = block_of(ic);
-  auto issue = [&] {
-    load(ic, blk, issued % NB);
-    if (++issued < n) {
+    if (++issued >= n) {
+      valid = 0;
+    } else if (++ic.u < ic.nu) {
+      idx += step_blocks;
+      r += step_rows;
+      if (r >= block) {
+        r -= block;
+        ++idx;
+      }
+      valid -= kKeys;
+    } else {
+      --ic.u;
       advance(ic, seqs, a.hkv, a.batch);
-      blk = block_of(ic);
+      enter();
     }
+    fetch();
   };
-#pragma unroll
-  for (int k = 0; k < NB - 1; ++k)
-    if (issued < n) issue();
+  enter();
+  fetch();
 
-  TileState st;
+  // ---- Segments: the first row of q, the rows, and this lane's q
+  Cursor pc = ic;  // tile x
+  auto rows_in = [&](int b, int& tok, int& rows) {
+    tok = lds_int(seqs.cq + b);
+    rows = (lds_int(seqs.cq + b + 1) - tok) << a.glog;
+  };
+  Vec8 raw[8];
+  auto load_q = [&](int kvh, int tok, int rows) {
+    const int q = min(row, rows - 1);
+    const bf16_t* src = a.q + (int64_t)(tok + (q >> a.glog)) * a.q_st +
+                        (int64_t)((kvh << a.glog) + (q & ((1 << a.glog) - 1))) * a.q_sh + 8 * h;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) raw[s] = load_vec8(src + 16 * s);
+  };
   bf16x8_t qb[8];
-  int tok0 = 0, nrows = 0;  // the segment's first row of q, and its rows
-  auto begin = [&] {
-    tok0 = lds_int(seqs.cq + pc.b);
-    nrows = (lds_int(seqs.cq + pc.b + 1) - tok0) << a.glog;
-    reset(st);
-    if (row0 >= nrows) return;
-    const int r = min(row, nrows - 1);
-    const bf16_t* src = a.q + (int64_t)(tok0 + (r >> a.glog)) * a.q_st +
-                        (int64_t)((pc.kvh << a.glog) + (r & ((1 << a.glog) - 1))) * a.q_sh + 8 * h;
+  auto take_q = [&] {
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      Vec8 v = load_vec8(src + 16 * s);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v.w[e] = (v.w[e] & a.q_keep) ^ a.q_flip;
-      __builtin_memcpy(&qb[s], &v, 16);
+      for (int e = 0; e < 4; ++e) raw[s].w[e] = (raw[s].w[e] & a.q_keep) ^ a.q_flip;
+      __builtin_memcpy(&qb[s], &raw[s], 16);
     }
   };
-  begin();
+  // ---- Masks: a tile's first key as a node of its tree; where that is above -kKeys some row may not see every key.
+  // This lane's words are loaded an iteration ahead.
+  auto node_of = [&](const Cursor& c, int rows) { return c.u * kKeys - (c.ctx - (rows >> a.glog)); };
+  uint64_t w0 = 0, w1 = 0;
+  auto load_words = [&](int tok, int rows, int at) {
+    const uint64_t* m = a.mask + (int64_t)(tok + (min(row, rows - 1) >> a.glog)) * a.mask_st;
+    const int w = max(at, 0) >> 6;
+    w0 = w < a.words ? m[w] : 0;
+    w1 = at > 0 && (at & 63) && w + 1 < a.words ? m[w + 1] : 0;
+  };
+  int tok, nrows;
+  rows_in(pc.b, tok, nrows);
+  int at = node_of(pc, nrows);
+  if (row0 < nrows) {
+    load_q(pc.kvh, tok, nrows);
+    if (at > -kKeys) load_words(tok, nrows, at);
+  }
+#pragma unroll
+  for (int k = 0; k < NB - 1; ++k) issue();
+  if (row0 < nrows) take_q();
+  TileState st;
+  reset(st);
   for (int x = 0; x < n; ++x) {
-    if (x + NB - 2 < n) __asm__ __volatile__("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * kOps) : "memory");
-    else __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
+    __asm__ __volatile__("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * kOps) : "memory");
     barrier();  // tile x is in LDS; every wave is done with tile x - 1
-    if (issued < n) issue();
+    const uint64_t c0 = w0, c1 = w1;
+    Cursor nc = pc;
+    int tok1 = tok, nrows1 = nrows;
+    const bool last = x + 1 == n, turn = pc.u + 1 == pc.nu || last;  // tile x ends its segment, or the range
+    if (!last) {
+      advance(nc, seqs, a.hkv, a.batch);
+      if (turn) rows_in(nc.b, tok1, nrows1);
+    }
+    const int at1 = node_of(nc, nrows1);
+    if (row0 < nrows1) {  // ahead of the tiles: waiting for these does not wait for those
+      if (turn) load_q(nc.kvh, tok1, nrows1);
+      if (at1 > -kKeys) load_words(tok1, nrows1, at1);
+    }
+    issue();
     const uint32_t slot = (uint32_t)(x % NB) * kBuf;
-    const int first = pc.u * kKeys, at = first - (pc.ctx - (nrows >> a.glog));  // the tile's first key, as a node
-    const bool edge = at + kKeys > 0;
     uint64_t seen = 0;  // keys of the tile that this lane's row sees
+    const bool edge = at > -kKeys;
     if (edge) {
-      if (row0 < nrows) {
-        const uint64_t* m = a.mask + (int64_t)(tok0 + (min(row, nrows - 1) >> a.glog)) * a.mask_st;
-        const int w = max(at, 0) >> 6, sh = at & 63;
-        const uint64_t w0 = w < a.words ? m[w] : 0, w1 = at > 0 && sh && w + 1 < a.words ? m[w + 1] : 0;
-        seen = low_bits64(pc.ctx - first) & (at < 0 ? w0 << -at | low_bits64(-at) : sh ? w0 >> sh | w1 << (64 - sh) : w0);
-      }
+      const int sh = at & 63;
+      if (row0 < nrows)
+        seen = low_bits64(pc.ctx - pc.u * kKeys) & (at < 0 ? c0 << -at | low_bits64(-at) : sh ? c0 >> sh | c1 << (64 - sh) : c0);
       // V of keys that no row sees may be anything, NaN included: zeros in its place
       const uint64_t mine = wave_or(seen);
       if (lane == 0) any[wave] = mine;
@@ -322,13 +368,17 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
       softmax_tile(st, s, pb, a.scale_log2);
       pv_tile(st, pb, cur);
     }
-    const Cursor prev = pc;
-    if (x + 1 < n) advance(pc, seqs, a.hkv, a.batch);
-    if (x + 1 == n || pc.u == 0) {
-      finish_row(a, st, tok0, prev.kvh, row, nrows, finish_slot(seqs, a, prev, f0, n, id, rg.len, row == 0 && h == 0), h);
-      if (x + 1 < n) begin();
+    if (turn) {
+      finish_row(a, st, tok, pc.kvh, row, nrows, finish_slot(seqs, a, pc, f0, n, id, rg.len, row == 0 && h == 0), h);
+      reset(st);
+      tok = tok1;
+      nrows = nrows1;
+      if (row0 < nrows) take_q();
     }
+    pc = nc;
+    at = at1;
   }
+  __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way to LDS behind the wave's end
 }
 
 int tile_waves(int max_rows) { return max_rows <= 128 ? 4 : 8; }
