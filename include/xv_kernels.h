@@ -51,13 +51,16 @@ int xv_store_kvcache(const void* key, int64_t key_stride_tok, int64_t key_stride
  * A step's maps from its requests' lengths, in one launch.  The reference
  * builds them on the host, request by request (src/compute/batch.py:119-215).
  * Request b has seq_lens[b] tokens in the cache and adds new_lens[b] (negative
- * lengths count as 0; rows <= 8192):
+ * lengths count as 0; rows <= 4096):
  *   cu_seqlens_q, cu_seqlens_k [rows + 1]  running sums of new_lens and of
  *       seq_lens + new_lens (below 2^31);  cache_seqlens [rows] = their sum
- *   block_tables  int32 [rows, bt_stride] in place: row b's entries from
- *       ceil(seq_lens / block_size) to ceil((seq_lens + new_lens) / block_size)
- *       are taken, row after row, from free_pages[*free_head + 0, 1, ...]; the
- *       others stay as they are
+ *   block_tables  int32 [rows, bt_stride] in place: row b's entries from the
+ *       blocks it has, the larger of ceil(seq_lens / block_size) and row_blocks
+ *       (NULL: 0), to ceil((seq_lens + new_lens) / block_size) are taken, row
+ *       after row, from free_pages[*free_head + 0, 1, ...]; the others stay as
+ *       they are.  A row keeps blocks past its tokens (drafted ones that were
+ *       rejected) by its row_blocks; next_row_blocks [rows], another array, are
+ *       those after the step
  *   next_free_head  *free_head + the pages taken (free_head NULL: 0), not the
  *       same word; past num_free where the list ran out: such entries get -1
  *   positions int64 [total_tokens], slot_mapping int32 [total_tokens], both
@@ -69,11 +72,12 @@ int xv_store_kvcache(const void* key, int64_t key_stride_tok, int64_t key_stride
  *       cu_seqlens_q[rows] on; tokens from total_tokens on are not written.
  * A pool has fewer than 2^31 slots.
  */
-int xv_step_maps(const int32_t* seq_lens, const int32_t* new_lens, int rows, int32_t* block_tables,
-                 int64_t bt_stride, int max_blocks_per_seq, int block_size, const int32_t* free_pages,
-                 int num_free, const int32_t* free_head, const int32_t* depths, int total_tokens,
-                 int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, int32_t* cache_seqlens, int64_t* positions,
-                 int32_t* slot_mapping, int32_t* next_free_head, hipStream_t stream);
+int xv_step_maps(const int32_t* seq_lens, const int32_t* new_lens, const int32_t* row_blocks, int rows,
+                 int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq, int block_size,
+                 const int32_t* free_pages, int num_free, const int32_t* free_head, const int32_t* depths,
+                 int total_tokens, int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, int32_t* cache_seqlens,
+                 int32_t* next_row_blocks, int64_t* positions, int32_t* slot_mapping, int32_t* next_free_head,
+                 hipStream_t stream);
 
 /*
  * KV store into an fp8 (OCP e4m3fn) cache.  No counterpart in the reference,

@@ -7,12 +7,14 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
-def _host(old, new, bt, free, head, block, total, depths=None):
+def _host(old, new, bt, free, head, block, total, depths=None, owned=None):
     bt = [list(r) for r in bt]
     width = len(bt[0]) if bt else 0
-    pos, slots, cu_q, cu_k = [], [], [0], [0]
+    pos, slots, cu_q, cu_k, own = [], [], [0], [0], []
     for b, (o, n) in enumerate(zip(old, new)):
-        for blk in range(-(-o // block), -(-(o + n) // block)):
+        have = max(-(-o // block), owned[b] if owned else 0)
+        own.append(max(have, -(-(o + n) // block)))
+        for blk in range(have, -(-(o + n) // block)):
             if blk < width:
                 bt[b][blk] = free[head] if head < len(free) else -1
             head += 1
@@ -23,17 +25,19 @@ def _host(old, new, bt, free, head, block, total, depths=None):
         cu_q.append(cu_q[-1] + n)
         cu_k.append(cu_k[-1] + o + n)
     pos, slots = (pos + [0] * total)[:total], (slots + [-1] * total)[:total]
-    return cu_q, cu_k, [o + n for o, n in zip(old, new)], pos, slots, [head], bt
+    return cu_q, cu_k, [o + n for o, n in zip(old, new)], pos, slots, [head], own, bt
 
 
-def _run(dev, old, new, block, total=None, head=None, short=0, width=None, depths=None, seed=0):
+def _run(dev, old, new, block, total=None, head=None, short=0, width=None, depths=None, seed=0,
+         owned=None):
     from xvllm.kv_ops import step_maps
 
     r = np.random.RandomState(seed)
     need = [-(-(o + n) // block) for o, n in zip(old, new)]
     width = max(1, width or max(need, default=1) + 1)
-    have = [-(-o // block) for o in old]
-    pages = r.permutation(sum(need) + 5 + (head or 0)).tolist()
+    have = [max(-(-o // block), owned[b] if owned else 0) for b, o in enumerate(old)]
+    width = max([width] + have)
+    pages = r.permutation(sum(need) + sum(have) + 5 + (head or 0)).tolist()
     bt = [[-7] * width for _ in old]
     for b, k in enumerate(have):
         bt[b][: min(k, width)] = [pages.pop() for _ in range(k)][:width]
@@ -42,9 +46,9 @@ def _run(dev, old, new, block, total=None, head=None, short=0, width=None, depth
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
     tables = i32(bt).view(len(old), width)
     m = step_maps(i32(old), i32(new), tables, i32(free), block, total, free_head=None if head is None else i32([head]),
-                  depths=None if depths is None else i32(depths))
-    want = _host(old, new, bt, free, head or 0, block, total, depths)
-    for name, got, w in zip(("cu_q", "cu_k", "ends", "positions", "slots", "free_head", "tables"), (*m, tables), want):
+                  depths=None if depths is None else i32(depths), row_blocks=None if owned is None else i32(owned))
+    want = _host(old, new, bt, free, head or 0, block, total, depths, owned)
+    for name, got, w in zip(("cu_q", "cu_k", "ends", "positions", "slots", "free_head", "row_blocks", "tables"), (*m, tables), want):
         assert got.cpu().reshape(-1).tolist() == np.asarray(w, dtype=np.int64).reshape(-1).tolist(), name
     assert m.positions.dtype == torch.int64 and m.slot_mapping.dtype == torch.int32
 
@@ -56,7 +60,7 @@ def test_maps(dev, block, old, new):
     _run(dev, old, new, block)
 
 
-@pytest.mark.parametrize("rows", [63, 64, 65, 256, 257, 1000, 8192])
+@pytest.mark.parametrize("rows", [63, 64, 65, 256, 257, 1000, 4096])
 def test_rows(dev, rows):
     r = np.random.RandomState(rows)
     _run(dev, r.randint(0, 200, rows).tolist(), (r.randint(0, 9, rows) * r.randint(0, 2, rows)).tolist(), 16, seed=rows)
@@ -82,7 +86,21 @@ def test_free_list_runs_out(dev, short):
 
 
 def test_table_is_full(dev):
-    _run(dev, [3, 50, 20], [100, 1, 4], 16, width=3)
+    from xvllm.kv_ops import step_maps
+
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    bt = i32([[5, -1, -1], [6, 7, 8], [9, -1, -1]])
+    m = step_maps(i32([3, 40, 16]), i32([100, 1, 4]), bt, i32(list(range(20, 40))), 16, 105)
+    assert bt.tolist() == [[5, 20, 21], [6, 7, 8], [9, 26, -1]] and m.free_head.tolist() == [7]
+    slots = m.slot_mapping.tolist()
+    assert slots[:45] == [5 * 16 + i for i in range(3, 16)] + [20 * 16 + i for i in range(16)] + [21 * 16 + i for i in range(16)]
+    assert slots[45:100] == [-1] * 55 and slots[100:] == [8 * 16 + 8] + [26 * 16 + i for i in range(4)]
+
+
+def test_rows_keep_blocks_past_their_tokens(dev):
+    """Blocks of rejected tokens are used before the list is."""
+    _run(dev, [3, 50, 0, 16, 40], [30, 1, 30, 1, 0], 16, owned=[2, 3, 5, 0, 9])
+    _run(dev, [100, 7, 0], [3, 90, 20], 48, owned=[4, 1, 0], head=2)
 
 
 def test_depths(dev):
@@ -148,7 +166,7 @@ def test_steps_in_a_graph(dev):
     for _ in range(40):
         graph.replay()
         torch.cuda.synchronize()
-        cu_q, cu_k, ends, pos, slots, h, host_bt = _host(old, [1, 1, 0, 1], host_bt, list(range(50, 90)), at, 16, 4)
+        cu_q, cu_k, ends, pos, slots, h, own, host_bt = _host(old, [1, 1, 0, 1], host_bt, list(range(50, 90)), at, 16, 4)
         assert m.slot_mapping.tolist() == slots and m.positions.tolist() == pos and bt.tolist() == host_bt
         assert lens.tolist() == ends and head.tolist() == h
         old, at = ends, h[0]

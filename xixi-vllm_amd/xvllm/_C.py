@@ -103,7 +103,7 @@ SIGNATURES: dict[str, tuple] = {
          i32, i32, i32, i32, i32, i32, i32, i32, f32, vp],
     ),
     "xv_step_maps": (
-        i32, [vp, vp, i32, vp, i64, i32, i32, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp]
+        i32, [vp, vp, vp, i32, vp, i64, i32, i32, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp]
     ),
     "xv_mxfp4_gemm_workspace_size": (sz, [i32, i32, i32, i32]),
     "xv_mxfp4_gemm": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, sz, vp]),

@@ -20,6 +20,10 @@ class Qwen3Shape:
     rope_theta: float = 1e6
     max_position_embeddings: int = 40960
     attention_bias: bool = False
+    # layers from max_window_layers on see the last sliding_window tokens and the first attention_sinks (None: all)
+    sliding_window: int | None = None
+    max_window_layers: int = 0
+    attention_sinks: int = 0
 
 
 QWEN3_0_6B = Qwen3Shape(1024, 16, 8, 128, 3072, 28)
@@ -37,3 +41,16 @@ def rope_theta(cfg) -> float:
 
 def head_dim(cfg) -> int:
     return getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+
+
+def layer_window(cfg, layer_id: int) -> tuple[int, int]:
+    """(window, sink tokens) of a layer's attention, (0, 0) where it sees every
+    token: the layers that a transformers config names in layer_types, without
+    that list those from max_window_layers on (unless use_sliding_window is off)."""
+    window = getattr(cfg, "sliding_window", None)
+    if not window or getattr(cfg, "use_sliding_window", True) is False:
+        return 0, 0
+    types = getattr(cfg, "layer_types", None)
+    if types[layer_id] != "sliding_attention" if types else layer_id < (getattr(cfg, "max_window_layers", 0) or 0):
+        return 0, 0
+    return int(window), int(getattr(cfg, "attention_sinks", 0) or 0)

@@ -217,18 +217,10 @@ class StepMaps(NamedTuple):
     positions: torch.Tensor      # int64 [total_tokens]
     slot_mapping: torch.Tensor   # int32 [total_tokens], -1: none
     free_head: torch.Tensor      # int32 [1]: the free list's first page after the step
+    row_blocks: torch.Tensor     # int32 [B]: blocks of each request's row after the step
 
 
-MAX_STEP_ROWS = 8192
-
-
-def _index_args(dev: int, **named: torch.Tensor) -> None:
-    """Check index operands: int32 vectors of unit stride on GPU `dev`."""
-    for name, t in named.items():
-        if t.dtype != torch.int32 or t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1):
-            raise TypeError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
-        if t.get_device() != dev:
-            raise RuntimeError(f"{name} must be on the block tables' device")
+MAX_STEP_ROWS = 4096
 
 
 def step_maps(
@@ -241,16 +233,20 @@ def step_maps(
     *,
     free_head: torch.Tensor | None = None,
     depths: torch.Tensor | None = None,
+    row_blocks: torch.Tensor | None = None,
 ) -> StepMaps:
     """The maps of a step whose request b has seq_lens[b] tokens in the cache and
     adds new_lens[b] (int32 [B], on the GPU), in one launch and without a look at
     the lengths on the host (which builds the same in Batch.build_decode and
     build_prefill):
 
-    - block_tables int32 [B, max_blocks], in place: each row's blocks from
-      ceil(seq_lens / block_size) to ceil((seq_lens + new_lens) / block_size)
-      are taken from free_pages[free_head:] (int32; free_head int32 [1], 0 where
-      None), row after row; its other entries stay as they are.
+    - block_tables int32 [B, max_blocks], in place: each row's blocks from those
+      it has to ceil((seq_lens + new_lens) / block_size) are taken from
+      free_pages[free_head:] (int32; free_head int32 [1], 0 where None), row after
+      row; its other entries stay as they are.  A row has ceil(seq_lens /
+      block_size) blocks, or row_blocks (int32 [B]) where that is more: blocks of
+      drafted tokens that were rejected stay the row's.  StepMaps.row_blocks are
+      the next step's.
     - StepMaps.free_head: free_head and the pages taken; larger than
       len(free_pages) where the list ran out (such blocks get -1).
     - positions and slot_mapping of the new tokens, request after request
@@ -262,36 +258,41 @@ def step_maps(
       position seq_lens + depth instead of their index (tree_attention).
 
     The running sums stay below 2^31, and so do the pool's slots."""
-    require_cuda(block_tables)
     dev = block_tables.get_device()
-    _index_args(dev, seq_lens=seq_lens, new_lens=new_lens, free_pages=free_pages)
-    rows = seq_lens.shape[0]
-    if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] < rows
-            or block_tables.shape[1] < 1 or block_tables.stride(1) != 1):
-        raise ValueError(f"block_tables {block_tables.dtype} {tuple(block_tables.shape)}: not int32 [{rows}, max_blocks] of "
+    rows, i32 = seq_lens.shape[0], torch.int32
+    if dev < 0 or seq_lens.get_device() != dev or new_lens.get_device() != dev or free_pages.get_device() != dev:
+        raise RuntimeError("xvllm ops run on the GPU only (HIP kernels), all operands on one device")
+    if seq_lens.dtype != i32 or new_lens.dtype != i32 or free_pages.dtype != i32 or block_tables.dtype != i32:
+        raise TypeError(f"lengths, pages and block tables are int32, got {seq_lens.dtype}, {new_lens.dtype}, {free_pages.dtype}, "
+                        f"{block_tables.dtype}")
+    if (seq_lens.dim() != 1 or new_lens.shape != seq_lens.shape or free_pages.dim() != 1 or rows > MAX_STEP_ROWS
+            or not (seq_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous())):
+        raise ValueError(f"seq_lens {tuple(seq_lens.shape)}, new_lens {tuple(new_lens.shape)}, free_pages "
+                         f"{tuple(free_pages.shape)}: contiguous vectors, as many lengths of each, at most {MAX_STEP_ROWS}")
+    if block_tables.dim() != 2:
+        raise ValueError(f"block_tables {tuple(block_tables.shape)} is not [{rows}, max_blocks]")
+    max_blocks = block_tables.shape[1]
+    bt_st, inner = block_tables.stride()
+    if block_tables.shape[0] < rows or max_blocks < 1 or (inner != 1 and max_blocks > 1) or (bt_st < max_blocks and rows > 1):
+        raise ValueError(f"block_tables {tuple(block_tables.shape)} of strides {block_tables.stride()} is not [{rows}, max_blocks] of "
                          "unit last stride")
-    if new_lens.shape[0] != rows or rows > MAX_STEP_ROWS:
-        raise ValueError(f"{rows} seq_lens and {new_lens.shape[0]} new_lens: as many of each, at most {MAX_STEP_ROWS}")
     if block_size < 1 or not 0 <= total_tokens <= 1 << 30:
         raise ValueError(f"block_size {block_size}, total_tokens {total_tokens}")
-    bt_st = block_tables.stride(0)
-    if rows > 1 and bt_st < block_tables.shape[1]:
-        raise ValueError("block_tables' rows overlap")
-    if free_head is not None:
-        _index_args(dev, free_head=free_head)
-        if free_head.shape[0] != 1:
-            raise ValueError(f"free_head must hold one index, got {tuple(free_head.shape)}")
-    if depths is not None:
-        _index_args(dev, depths=depths)
-        if depths.shape[0] != total_tokens:
-            raise ValueError(f"{depths.shape[0]} depths for {total_tokens} tokens")
-    pos = torch.empty(total_tokens, dtype=torch.int64, device=block_tables.device)
-    buf = torch.empty(total_tokens + 3 * rows + 3, dtype=torch.int32, device=block_tables.device)
-    slots, cu_q, cu_k, ends, head = buf.split_with_sizes((total_tokens, rows + 1, rows + 1, rows, 1))
+    for name, t, n in (("free_head", free_head, 1), ("depths", depths, total_tokens), ("row_blocks", row_blocks, rows)):
+        if t is not None:
+            if t.dtype != i32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous int32 vector of {n}, got {t.dtype} {tuple(t.shape)}")
+            if t.get_device() != dev:
+                raise RuntimeError(f"{name} must be on the block tables' device")
+    # one allocation: positions (int64), slots, both running sums, the lengths, the rows' blocks, the list's head
+    total_tokens = int(total_tokens)
+    buf = torch.empty(3 * total_tokens + total_tokens % 2 * 2 + 4 * rows + 3, dtype=i32, device=block_tables.device)
+    wide = 2 * total_tokens + total_tokens % 2 * 2  # the slots start 16-byte aligned
+    pos, slots, cu_q, cu_k, ends, own, head = buf.split_with_sizes((wide, total_tokens, rows + 1, rows + 1, rows, rows, 1))
     base = buf.data_ptr()
-    at = base + 4 * total_tokens
-    call("xv_step_maps", dev, seq_lens.data_ptr(), new_lens.data_ptr(), rows, block_tables.data_ptr(),
-         max(bt_st, block_tables.shape[1]), block_tables.shape[1], block_size, free_pages.data_ptr(), free_pages.shape[0],
-         ptr(free_head), ptr(depths), total_tokens, at, at + 4 * (rows + 1), at + 8 * (rows + 1), pos.data_ptr(), base,
-         at + 8 * (rows + 1) + 4 * rows)
-    return StepMaps(cu_q, cu_k, ends, pos, slots, head)
+    at = base + 4 * (wide + total_tokens)
+    call("xv_step_maps", dev, seq_lens.data_ptr(), new_lens.data_ptr(), ptr(row_blocks), rows, block_tables.data_ptr(),
+         max(bt_st, max_blocks), max_blocks, block_size, free_pages.data_ptr(), free_pages.shape[0], ptr(free_head), ptr(depths),
+         total_tokens, at, at + 4 * (rows + 1), at + 8 * (rows + 1), at + 12 * rows + 8, base, base + 4 * wide, at + 16 * rows + 8)
+    pos = pos.view(torch.int64)
+    return StepMaps(cu_q, cu_k, ends, pos[:total_tokens] if total_tokens % 2 else pos, slots, head, own)

@@ -9,7 +9,7 @@ from __future__ import annotations
 import math
 from contextlib import contextmanager
 from dataclasses import dataclass
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 import torch.nn as nn
@@ -33,6 +33,17 @@ class CascadePlan:
     max_prefix_blocks: int
 
 
+@dataclass
+class TreePlan:
+    """Trees of drafted tokens of a step (device tensors): rows cu_seqlens_q[b]
+    .. cu_seqlens_q[b+1] - 1 are sequence b's nodes, the last of its
+    cache_seqlens tokens, and row t sees the nodes of mask[t] (tree_attention).
+    max_nodes: those of the largest tree at most."""
+    cu_seqlens_q: torch.Tensor
+    mask: torch.Tensor
+    max_nodes: int
+
+
 class AttnInputs(NamedTuple):
     slot_mapping: torch.Tensor
     is_prefill: bool
@@ -44,6 +55,7 @@ class AttnInputs(NamedTuple):
     cache_seqlens: Optional[torch.Tensor] = None
     cascade: Optional[CascadePlan] = None  # decode only: shared-prefix groups (no reference counterpart)
     total_seqlen_k: int = 0  # prefill: the keys of all sequences, cu_seqlens_k's last, where the host knows it
+    tree: Optional[TreePlan] = None  # not prefill: the rows are trees of drafted tokens (no reference counterpart)
 
 
 @dataclass
@@ -244,6 +256,24 @@ def _window_decode(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d,
 
 
 MAX_TREE_NODES = 1024
+
+
+def tree_masks(parents: Sequence[int]) -> tuple[torch.Tensor, torch.Tensor]:
+    """(mask int64 [n, words], depths int32 [n]) of a tree of drafted tokens by
+    its nodes' parents (a node before its children; -1: a child of the last
+    token before the tree): a node sees its ancestors and itself (tree_attention),
+    and its position is the context's length plus its depth (step_maps)."""
+    n = len(parents)
+    rows, depths = [], []
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"node {i}: parent {p} is not -1 or a node before it")
+        rows.append((rows[p] if p >= 0 else 0) | 1 << i)
+        depths.append(depths[p] + 1 if p >= 0 else 0)
+    words = max(1, -(-n // 64))
+    signed = lambda w: w - (1 << 64) if w >> 63 else w
+    mask = [[signed(r >> 64 * w & (1 << 64) - 1) for w in range(words)] for r in rows]
+    return torch.tensor(mask, dtype=torch.int64).view(n, words), torch.tensor(depths, dtype=torch.int32)
 
 
 def tree_attention(
@@ -584,8 +614,11 @@ def attention(
     num_kv_heads: int,
     head_dim: int,
     total_seqlen_k: int = 0,
+    window: int = 0,
+    sink_tokens: int = 0,
 ) -> torch.Tensor:
-    """The reference's arguments and, at their end, AttnInputs' total_seqlen_k."""
+    """The reference's arguments and, at their end, AttnInputs' total_seqlen_k
+    and the layer's sliding window and sinks (0: none)."""
     k_cache, v_cache = _layer_caches(layer_id)
     k3 = k.view(-1, num_kv_heads, head_dim)
     v3 = v.view(-1, num_kv_heads, head_dim)
@@ -597,13 +630,16 @@ def attention(
             return prefill_attention(
                 q, None, None, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
                 head_dim, k_cache=k_cache, v_cache=v_cache, block_tables=block_tables, max_seqlen_k=max_seqlen_k,
-                total_seqlen_k=total_seqlen_k, **(scales if k_cache.dtype == FP4_PAGES else {"kv_scale": kv_scales()}),
+                total_seqlen_k=total_seqlen_k, window=window, sink_tokens=sink_tokens,
+                **(scales if k_cache.dtype == FP4_PAGES else {"kv_scale": kv_scales()}),
             )
         return prefill_attention(
-            q, k3, v3, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads, head_dim
+            q, k3, v3, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads, head_dim, window=window,
+            sink_tokens=sink_tokens,
         )
     return paged_decode_attention(
-        q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim, **scales,
+        q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim, window=window,
+        sink_tokens=sink_tokens, **scales,
     )
 
 
@@ -611,7 +647,7 @@ def attention(
 def _attention_fake(
     q, k, v, slot_mapping, is_prefill, cu_seqlens_q, cu_seqlens_k, max_seqlen_q,
     max_seqlen_k, block_tables, cache_seqlens, layer_id, num_qo_heads,
-    num_kv_heads, head_dim, total_seqlen_k=0,
+    num_kv_heads, head_dim, total_seqlen_k=0, window=0, sink_tokens=0,
 ):
     return torch.empty((q.shape[0], num_qo_heads * head_dim), dtype=q.dtype, device=q.device)
 
@@ -622,24 +658,39 @@ def kv_cache_of(layer_id: int) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 class Attention(nn.Module):
-    def __init__(self, num_heads: int, head_dim: int, num_kv_heads: int, layer_id: int = 0) -> None:
+    """window > 0: a query sees the last `window` tokens of its sequence, itself
+    among them, and the first sink_tokens; else every one before it."""
+
+    def __init__(self, num_heads: int, head_dim: int, num_kv_heads: int, layer_id: int = 0, window: int = 0,
+                 sink_tokens: int = 0) -> None:
         super().__init__()
+        _windowed(window, sink_tokens)
         self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
         self.layer_id = layer_id
+        self.window, self.sink_tokens = window, sink_tokens
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, attn: AttnInputs) -> torch.Tensor:
-        if attn.cascade is not None and not attn.is_prefill:
-            # shared-prefix decode: the plan does not fit the vllm::attention schema
+        if attn.tree is not None and attn.is_prefill:
+            raise ValueError("a prefill step takes no tree plan")
+        if not attn.is_prefill and (attn.cascade is not None or attn.tree is not None):
+            # shared-prefix decode, or trees of drafted tokens: the plan does not fit the vllm::attention schema
+            if self.window or (attn.cascade is not None and attn.tree is not None):
+                raise ValueError("a sliding window, a shared-prefix plan and a tree plan exclude each other")
             k_cache, v_cache = _layer_caches(self.layer_id)
-            _refuse_cascade(k_cache)
-            ks, vs = kv_scales()
+            if attn.tree is None:
+                _refuse_cascade(k_cache)
+            scales = _layer_scales(self.layer_id)
             if attn.slot_mapping is not None:
                 store_kvcache(k.view(-1, self.num_kv_heads, self.head_dim), v.view(-1, self.num_kv_heads, self.head_dim),
-                              k_cache, v_cache, attn.slot_mapping, k_scale=ks, v_scale=vs)
+                              k_cache, v_cache, attn.slot_mapping, **scales)
+            if attn.tree is not None:
+                return tree_attention(q, k_cache, v_cache, attn.block_tables, attn.cache_seqlens, attn.tree.cu_seqlens_q,
+                                      attn.tree.mask, attn.tree.max_nodes, self.num_heads, self.num_kv_heads, self.head_dim)
             return cascade_decode_attention(q, k_cache, v_cache, attn.block_tables, attn.cache_seqlens, attn.cascade,
-                                            self.num_heads, self.num_kv_heads, self.head_dim, k_scale=ks, v_scale=vs)
+                                            self.num_heads, self.num_kv_heads, self.head_dim, **scales)
         return torch.ops.vllm.attention(
             q, k, v, attn.slot_mapping, attn.is_prefill, attn.cu_seqlens_q, attn.cu_seqlens_k,
             attn.max_seqlen_q, attn.max_seqlen_k, attn.block_tables, attn.cache_seqlens,
-            self.layer_id, self.num_heads, self.num_kv_heads, self.head_dim, attn.total_seqlen_k,
+            self.layer_id, self.num_heads, self.num_kv_heads, self.head_dim, attn.total_seqlen_k, self.window,
+            self.sink_tokens,
         )

@@ -21,7 +21,7 @@ from .config import head_dim as _head_dim
 from .cuda_graph import HipGraphRunner
 from .kv_ops import FP4_PAGES
 from .kv_pool import KVPool
-from .layers.attention import AttnInputs, AttnMetadata, attention_context
+from .layers.attention import Attention, AttnInputs, AttnMetadata, attention_context
 from .sampler import Sampler, reserve_workspace, sample
 
 
@@ -78,6 +78,12 @@ class ModelRunner:
         read them), and every runner of the model then uses them."""
         if cascade_groups > 0 and kv.dtype == FP4_PAGES:
             raise ValueError("no cascade decode over a 4-bit KV pool: cascade_groups must be 0")
+        windowed = [m for m in model.modules() if isinstance(m, Attention) and m.window] if hasattr(model, "modules") else []
+        if windowed:
+            if cascade_groups > 0:
+                raise ValueError("no cascade decode with a sliding window: cascade_groups must be 0")
+            if kv.dtype in (torch.float8_e4m3fn, FP4_PAGES):
+                raise ValueError(f"layers with a sliding window decode over bf16 pages, the pool holds {kv.dtype}")
         self.model = model
         if stream_decode_gemms and hasattr(model, "pack_decode_weights"):
             model.pack_decode_weights()

@@ -12,6 +12,9 @@ size, others where the library's product would split too.  Larger batches and
 the products and shapes outside this run on PyTorch (hipBLASLt).  Weights are plain
 tensors (random init for the benchmarks; the reference's checkpoint loader is
 out of scope).
+
+A config's sliding window (layer_window) goes to the layers' Attention;
+AttnInputs.tree makes a step's rows trees of drafted tokens.
 """
 from __future__ import annotations
 
@@ -20,6 +23,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from ..config import head_dim as _head_dim
+from ..config import layer_window
 from ..config import rope_theta as _rope_theta
 from ..kv_ops import FP4_PAGES
 from ..layers import Attention, AttnInputs, RMSNorm, RotaryEmbedding
@@ -122,7 +126,9 @@ class Qwen3Attention(nn.Module):
         self.q_norm = RMSNorm(self.head_dim, cfg.rms_norm_eps)
         self.k_norm = RMSNorm(self.head_dim, cfg.rms_norm_eps)
         self.rotary_emb = RotaryEmbedding(self.head_dim, self.head_dim, cfg.max_position_embeddings, _rope_theta(cfg))
-        self.attn = Attention(self.num_heads, self.head_dim, self.num_kv_heads, layer_id=layer_id)
+        window, sinks = layer_window(cfg, layer_id)
+        self.attn = Attention(self.num_heads, self.head_dim, self.num_kv_heads, layer_id=layer_id, window=window,
+                              sink_tokens=sinks)
         self.eps = cfg.rms_norm_eps
         self.split_k = True
         self._copies = None  # pack(): the packed copy of (o_proj,), None if read in place
