@@ -59,6 +59,12 @@ XV_INLINE __amdgpu_buffer_rsrc_t rsrc(const bf16_t* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(q, (short)0, (int)__builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
+// A wave's 16 keys of a tile in the cache: block id, first row in it.
+struct Page {
+  int block;
+  int row;
+};
+
 // Wave w moves keys key0+16w .. +15 of the tile (one cache page when paged):
 // 4 LDS-DMA instructions for K and/or 4 for V, each 4 whole rows.
 // WIN: keys sinks .. lo - 1 are seen by no query of the workgroup: their V
@@ -66,13 +72,13 @@ XV_INLINE __amdgpu_buffer_rsrc_t rsrc(const bf16_t* base, uint32_t bytes) {
 // such are not read at all (their block-table entry may be gone).
 template <bool PAGED, bool DO_K, bool DO_V, bool WIN>
 XV_INLINE void load_rows(char* buf, const PrefillArgs& a, int b, int kvh, int key0, int k0, int k_len,
-                         int64_t page_off, int lo, int wave, int lane) {
+                         Page page, int lo, int wave, int lane) {
   const int j0 = key0 + 16 * wave;
   const int valid = WIN && j0 >= a.sinks && j0 + 16 <= lo ? 0 : min(16, k_len - j0);
   const bf16_t *kb, *vb;
   int64_t rs;  // row stride (elements)
   if (PAGED) {
-    const int64_t off = page_off + (int64_t)kvh * a.head_stride;
+    const int64_t off = (int64_t)page.block * a.page_stride + (int64_t)page.row * a.tok_stride + (int64_t)kvh * a.head_stride;
     kb = a.kc + off; vb = a.vc + off; rs = a.tok_stride;
   } else {
     const int64_t off = (int64_t)(k0 + j0) * a.kv_st + (int64_t)kvh * a.kv_sh;
@@ -102,12 +108,19 @@ XV_INLINE void load_rows(char* buf, const PrefillArgs& a, int b, int kvh, int ke
 // cheapest ones finish the grid.  Each sequence's blocks stay together in the
 // dispatch order (they share K/V tiles in L2).  Batches above 64 keep their
 // own order.
-XV_INLINE int seq_by_work(const int* cu_q, const int* cu_k, int batch, int j) {
-  if (batch > 64) return j;
+struct Sequence {
+  int b, q0, q_len, k0, k_len;
+};
+XV_INLINE Sequence seq_by_work(const int* cu_q, const int* cu_k, int batch, int j) {
+  if (batch > 64) return Sequence{j, cu_q[j], cu_q[j + 1] - cu_q[j], cu_k[j], cu_k[j + 1] - cu_k[j]};
   const int lane = threadIdx.x & 63;
   int64_t w = -1;
+  int q0 = 0, ql = 0, k0 = 0, kl = 0;
   if (lane < batch) {
-    const int ql = cu_q[lane + 1] - cu_q[lane], kl = cu_k[lane + 1] - cu_k[lane];
+    q0 = cu_q[lane];
+    k0 = cu_k[lane];
+    ql = cu_q[lane + 1] - q0;
+    kl = cu_k[lane + 1] - k0;
     w = (int64_t)ql * (kl - ql) + (int64_t)ql * (ql + 1) / 2;
   }
   int pos = 0;
@@ -118,7 +131,10 @@ XV_INLINE int seq_by_work(const int* cu_q, const int* cu_k, int batch, int j) {
     pos += (wt > w || (wt == w && t < lane)) ? 1 : 0;
   }
   const uint64_t m = __ballot(lane < batch && pos == j);
-  return __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
+  const int b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
+  // its lengths from the lane that has them: a second trip to memory costs every workgroup a microsecond
+  return Sequence{b, __builtin_amdgcn_readlane(q0, b), __builtin_amdgcn_readlane(ql, b), __builtin_amdgcn_readlane(k0, b),
+                  __builtin_amdgcn_readlane(kl, b)};
 }
 
 template <int G, bool PAGED, bool WIN>
@@ -134,13 +150,13 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   // slot fastest every XCD serves the same kv head(s) and keeps their K/V tiles
   // in its own L2; each head carries the same work, which balances the XCDs.
   const int hsel = blockIdx.x, rank = blockIdx.y;
-  const int b = seq_by_work(a.cu_q, a.cu_k, a.batch, blockIdx.z);
+  const Sequence seq = seq_by_work(a.cu_q, a.cu_k, a.batch, blockIdx.z);
+  const int b = seq.b;
   // group 8: two slots per kv head (query heads 0-3 and 4-7), slot = half * Hkv
   // + kvh, so both halves of a kv head land on the same XCD
   const int kvh = G == 8 ? hsel % a.hkv : hsel;
   const int head = G == 8 ? kvh * 8 + (hsel / a.hkv) * 4 + wave : kvh * G + wave % GW;
-  const int q0 = a.cu_q[b], q_len = a.cu_q[b + 1] - q0;
-  const int k0 = a.cu_k[b], k_len = a.cu_k[b + 1] - k0;
+  const int q0 = seq.q0, q_len = seq.q_len, k0 = seq.k0, k_len = seq.k_len;
   // rank from the sequence's own end: the last (longest) block of the causal
   // triangle is dispatched first, then the next-to-last, ...
   const int qb0 = ((q_len + kBlockQ - 1) / kBlockQ - 1 - rank) * kBlockQ;
@@ -185,15 +201,27 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
     for (int r = 0; r < 16; ++r) o[n][r] = 0.f;
   float m_run = -INFINITY, l_run = 0.f;
 
-  // element offset of the 16 keys j .. j + 15 (a 16-aligned run inside one
-  // cache block of block_size tokens): block bt[j / BS], token j % BS
-  auto page_of = [&](int t) -> int64_t {
-    if (!PAGED) return 0;
+  // Where the wave's 16 keys of a tile (a 16-aligned run inside one cache block of block_size tokens) are: block, row in
+  // it.  Asked for tile after tile; the block id is not touched before the tile's loads, a tile later, so nothing waits
+  // for it.
+  const int step_blocks = PAGED ? kKeys / a.block_size : 0, step_rows = PAGED ? kKeys % a.block_size : 0;
+  int at_block = 0, at_row = 0;
+  auto page_of = [&](int t) {
+    if (!PAGED) return Page{0, 0};
     const int j = key_of(t) + 16 * wave;
-    if (j >= k_len || (WIN && j >= a.sinks && j + 16 <= blk_lo)) return 0;
-    const int blk = j / a.block_size;
-    const int64_t page = __builtin_amdgcn_readfirstlane(a.bt[(int64_t)b * a.bt_stride + blk]);
-    return page * a.page_stride + (int64_t)(j - blk * a.block_size) * a.tok_stride;
+    if (t == 0 || (WIN && t == sink_tiles)) {
+      at_block = j / a.block_size;
+      at_row = j - at_block * a.block_size;
+    } else {
+      at_block += step_blocks;
+      at_row += step_rows;
+      if (at_row >= a.block_size) {
+        at_row -= a.block_size;
+        ++at_block;
+      }
+    }
+    if (j >= k_len || (WIN && j >= a.sinks && j + 16 <= blk_lo)) return Page{0, 0};
+    return Page{load_index(a.bt + (int64_t)b * a.bt_stride + at_block), at_row};
   };
   const LdsAddr ad = lds_addr(lds, lane);
   // S^T of one tile from K buffer PAR
@@ -284,8 +312,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   // therefore runs a tile ahead of V: iteration t loads K(t+2) into the K
   // buffer S(t) used and V(t+1) into the V buffer P(t-1) V(t-1) used, both
   // freed by the barrier at its top.
-  int64_t pv_page = ntiles > 1 ? page_of(1) : 0, pk_page = ntiles > 2 ? page_of(2) : 0;
-  if (ntiles > 0) load_rows<PAGED, true, true, WIN>(lds, a, b, kvh, key_of(0), k0, k_len, page_of(0), blk_lo, wave, lane);
+  const Page page0 = page_of(0);
+  Page pv_page = ntiles > 1 ? page_of(1) : Page{0, 0}, pk_page = ntiles > 2 ? page_of(2) : Page{0, 0};
+  if (ntiles > 0) load_rows<PAGED, true, true, WIN>(lds, a, b, kvh, key_of(0), k0, k_len, page0, blk_lo, wave, lane);
   if (ntiles > 1)
     load_rows<PAGED, true, false, WIN>(lds + kBuf, a, b, kvh, key_of(1), k0, k_len, pv_page, blk_lo, wave, lane);
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");

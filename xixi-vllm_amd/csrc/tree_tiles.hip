@@ -190,11 +190,6 @@ XV_INLINE void finish_row(const RowsArgs& a, const TileState& st, int tok0, int 
   }
 }
 
-// Scalar load of a table entry at a wave-uniform index: it does not wait for the tiles in flight.
-XV_INLINE int load_index(const int32_t* p) {
-  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
-}
-
 // A workgroup barrier behind this wave's LDS accesses.  (A plain __syncthreads also waits for every tile in flight.)
 XV_INLINE void barrier() {
   __asm__ __volatile__("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -131,4 +131,9 @@ XV_INLINE bf16x8_t vt_operand(const short4_t (&t)[16], int n, int j) {
   return __builtin_bit_cast(bf16x8_t, r);
 }
 
+// Scalar load of a table entry at a wave-uniform index: it does not wait for the tiles in flight.
+XV_INLINE int load_index(const int32_t* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p));
+}
+
 }  // namespace
