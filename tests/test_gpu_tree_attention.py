@@ -56,6 +56,12 @@ def test_large_trees(dev, n, hq, hkv):
     _run(dev, [n, n + 700, 20 + n // 2], [n, n - 1, n // 2], hq, hkv, seed=n)
 
 
+@pytest.mark.parametrize("lens,nodes,hq", [([1024 + 900], [1024], 64), ([1003, 40, 900, 65], [1000, 3, 300, 65], 32), ([513] * 3, [513, 512, 257], 8)])
+def test_trees_of_many_rows(dev, lens, nodes, hq):
+    """More rows than a workgroup takes at once: each part of them has fewer ranges."""
+    _run(dev, lens, nodes, hq, 8, seed=len(nodes))
+
+
 @pytest.mark.parametrize("hq,hkv,nodes", [(32, 8, [20, 7]), (64, 8, [64]), (16, 8, [3, 30])])
 def test_long_contexts(dev, hq, hkv, nodes):
     _run(dev, [5000 + 777 * i for i in range(len(nodes))], nodes, hq, hkv, block=256, seed=4)

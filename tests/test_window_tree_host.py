@@ -70,6 +70,12 @@ def test_workspace_sizes(lib):
     assert size(0, 16, 32, 8) == size(4, 0, 32, 8) == size(4, 16, 12, 8) == 256
 
 
+def test_workspace_of_large_trees(lib):
+    """As many partial rows as fill the GPU, whatever the tree's size."""
+    for nodes, hq in ((33, 8), (128, 32), (300, 64), (1024, 64)):
+        assert lib.xv_tree_attention_workspace_size(256, nodes, hq, 8) < 80 << 20
+
+
 def _prefill(lib, **kw):
     a = dict(q=A, qst=4096, qsh=128, k=A, v=A, kvst=1024, kvsh=128, kc=None, vc=None, ps=0, ts=0, hs=0, bt=None, bts=0, cuq=A, cuk=A,
              out=A, ost=4096, B=4, maxq=512, Hq=32, Hkv=8, D=128, BS=16, window=100, sinks=4, scale=0.1)

@@ -579,7 +579,7 @@ constexpr int kWaveRows = 32;
 // Rows of a tree call from which on the merge takes four rows a wave: enough waves then without spreading a row's partials.
 constexpr int kManyRows = 8192;
 int slot_rows(int max_rows) { return max_rows <= 16 ? 16 : max_rows <= kWaveRows ? 32 : tile_rows(max_rows); }
-size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : kTileGroups); }
+size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : tile_ranges(max_rows)); }
 
 size_t al256(size_t x) { return (x + 255) / 256 * 256; }
 size_t seg_bytes(int batch, int hkv) { return al256((size_t)min(batch, kMaxBatch) * hkv * sizeof(int2)); }

@@ -377,19 +377,19 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
 }
 
 int tile_waves(int max_rows) { return max_rows <= 128 ? 4 : 8; }
+int tile_passes(int max_rows) { return (max_rows + 32 * tile_waves(max_rows) - 1) / (32 * tile_waves(max_rows)); }
 
 }  // namespace
 
-int xv_rows::tile_rows(int max_rows) {
-  const int per = 32 * tile_waves(max_rows);
-  return (max_rows + per - 1) / per * per;
-}
+int xv_rows::tile_rows(int max_rows) { return tile_passes(max_rows) * 32 * tile_waves(max_rows); }
+
+// As many as there are workgroups resident at once, two of four waves a CU or one of eight, shared among the passes: more
+// would only cut segments into more partials.
+int xv_rows::tile_ranges(int max_rows) { return max(8, 2048 / tile_waves(max_rows) / tile_passes(max_rows)); }
 
 int xv_rows::launch_tiles(const RowsArgs& a, int max_rows, hipStream_t stream) {
-  const int waves = tile_waves(max_rows);
-  const unsigned passes = (unsigned)(tile_rows(max_rows) / (32 * waves));
-  // as many workgroups as are resident at once: two of four waves a CU, one of eight
-  if (waves == 4) tree_tile_kernel<4, 2><<<dim3(kTileGroups, passes), 256, 0, stream>>>(a);
-  else tree_tile_kernel<8, 4><<<dim3(kTileGroups / 2, passes), 512, 0, stream>>>(a);
+  const dim3 grid((unsigned)tile_ranges(max_rows), (unsigned)tile_passes(max_rows));
+  if (tile_waves(max_rows) == 4) tree_tile_kernel<4, 2><<<grid, 256, 0, stream>>>(a);
+  else tree_tile_kernel<8, 4><<<grid, 512, 0, stream>>>(a);
   return (int)hipGetLastError();
 }
