@@ -310,9 +310,9 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
   __shared__ Sequences seqs;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (wave == 0)
-    load_sequences<TREE>(seqs, a, lane, [&](int ctx) { return units_of<TREE>(ctx, a.window, a.sinks); });
+    load_sequences<TREE, false>(seqs, a, lane, [&](int ctx) { return units_of<TREE>(ctx, a.window, a.sinks); });
   __syncthreads();
-  const Ranges rg = ranges_of(seqs, a, gridDim.x * kWaves, lane);
+  const Ranges rg = ranges_of<false>(seqs, a, gridDim.x * kWaves, lane);
   const int L = rg.len;
   const int id = wave * gridDim.x + blockIdx.x;  // short launches spread over the CUs first
   const int64_t f0 = (int64_t)id * L;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
   char* const idtab = mine + 2 * kUnitLds;
   const RowsLane offs = lane_offsets(a.ts, lane);
 
-  Cursor ic = cursor_at(seqs, a, f0), pc = ic;  // issue and process cursors
+  Cursor ic = cursor_at<false>(seqs, a, f0), pc = ic;  // issue and process cursors
   const __amdgpu_buffer_rsrc_t rbt =
       page_rsrc(reinterpret_cast<const bf16_t*>(a.bt), (uint32_t)((int64_t)a.batch * a.bt_stride * 4));
   load_window<TREE>(idtab, a, rbt, seqs, f0, 0, n, lane);
@@ -380,13 +380,13 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
   };
   issue(0);
   if (n > 1) {
-    advance(ic, seqs, a.hkv, a.batch);
+    advance<false>(ic, seqs, a);
     issue(1);
   }
   UnitRegs u;
   for (int x = 0; x < n; ++x) {
     const Cursor prev = pc;
-    if (x > 0) advance(pc, seqs, a.hkv, a.batch);
+    if (x > 0) advance<false>(pc, seqs, a);
     if (x == 0 || pc.u == 0) {
       if (x > 0) finish(prev);
       begin();
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(1, 
     else __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
     read_unit(u, mine + (x & 1) * kUnitLds, offs);
     if (x + 2 < n) {
-      advance(ic, seqs, a.hkv, a.batch);
+      advance<false>(ic, seqs, a);
       issue(x + 2);
     }
     const Pages p = pages_of<TREE>(pc.ctx, a.window, a.sinks);
@@ -440,10 +440,10 @@ __global__ __launch_bounds__(256) void rows_merge_kernel(RowsArgs a) {
   const int b = blockIdx.y;
   const int node = task / a.hq, h = task - node * a.hq;
   const int tok0 = TREE ? a.cu_q[b] : b;
-  if (node >= (TREE ? a.cu_q[b + 1] - tok0 : 1)) return;
+  if (node >= (TREE ? min(a.max_nodes, a.cu_q[b + 1] - tok0) : 1)) return;
   const int kvh = h >> a.glog, r0 = (node << a.glog) + (h & ((1 << a.glog) - 1));
   const int ctx = a.seqlens[b];
-  const int2 seg = a.ws_seg[b * a.hkv + kvh];  // stale when ctx <= 0: not used then
+  const int2 seg = a.ws_seg[seg_index(a, b, r0 / kPassRows, kvh)];  // stale when ctx <= 0: not used then
   bf16_t* orow = a.out + (int64_t)(tok0 + node) * a.out_st + (int64_t)h * kD;
   if (ctx <= 0) {
     *reinterpret_cast<uint32_t*>(orow + 2 * lane) = 0u;
@@ -451,7 +451,7 @@ __global__ __launch_bounds__(256) void rows_merge_kernel(RowsArgs a) {
   }
   const int n = seg.y;
   if (n <= 1) return;
-  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.rows + r0; };
+  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.rows + r0 % kPassRows; };
   const int g = lane >> 4, i = lane & 15;
   constexpr int kAhead = 4;  // partials in flight per lane row
   floatx4_t r[kAhead][2];
@@ -513,10 +513,10 @@ __global__ __launch_bounds__(256) void rows_merge4_kernel(RowsArgs a) {
   const int task = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 4 + (lane >> 4), b = blockIdx.y;
   const int node = task / a.hq, h = task - node * a.hq;
   const int tok0 = a.cu_q[b];
-  if (node >= a.cu_q[b + 1] - tok0) return;
+  if (node >= min(a.max_nodes, a.cu_q[b + 1] - tok0)) return;
   const int kvh = h >> a.glog, r0 = (node << a.glog) + (h & ((1 << a.glog) - 1));
   const int ctx = a.seqlens[b];
-  const int2 seg = a.ws_seg[b * a.hkv + kvh];  // stale when ctx <= 0: not used then
+  const int2 seg = a.ws_seg[seg_index(a, b, r0 / kPassRows, kvh)];  // stale when ctx <= 0: not used then
   uint32_t* orow = reinterpret_cast<uint32_t*>(a.out + (int64_t)(tok0 + node) * a.out_st + (int64_t)h * kD + 8 * i);
   if (ctx <= 0) {
 #pragma unroll
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(256) void rows_merge4_kernel(RowsArgs a) {
   }
   const int n = seg.y;
   if (n <= 1) return;
-  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.rows + r0; };
+  auto slot = [&](int j) { return (int64_t)(j == 0 ? 2 * seg.x + 1 : 2 * (seg.x + j)) * a.rows + r0 % kPassRows; };
   float mx = -INFINITY;
   for (int j = i; j < n; j += 16) mx = fmaxf(mx, a.ws_lse[slot(j)]);
   mx = row16_max(mx);
@@ -582,7 +582,10 @@ int slot_rows(int max_rows) { return max_rows <= 16 ? 16 : max_rows <= kWaveRows
 size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : tile_ranges(max_rows)); }
 
 size_t al256(size_t x) { return (x + 255) / 256 * 256; }
-size_t seg_bytes(int batch, int hkv) { return al256((size_t)min(batch, kMaxBatch) * hkv * sizeof(int2)); }
+int row_passes(int max_rows) { return max_rows <= kWaveRows ? 1 : tile_passes(max_rows); }
+size_t seg_bytes(int batch, int hkv, int max_rows) {
+  return al256((size_t)row_passes(max_rows) * min(batch, kMaxBatch) * hkv * sizeof(int2));
+}
 size_t lse_bytes(int max_rows) { return al256(slots(max_rows) * slot_rows(max_rows) * sizeof(float)); }
 
 bool valid_group(int hq, int hkv) {
@@ -596,8 +599,10 @@ int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* s
                 int batch, int max_nodes, void* workspace, hipStream_t stream) {
   const int max_rows = max_nodes << a.glog;
   a.rows = slot_rows(max_rows);
+  a.max_nodes = max_nodes;
+  a.passes = row_passes(max_rows);
   a.ws_seg = (int2*)workspace;
-  a.ws_lse = (float*)((char*)workspace + seg_bytes(batch, a.hkv));
+  a.ws_lse = (float*)((char*)workspace + seg_bytes(batch, a.hkv, max_rows));
   a.ws_o = (float*)((char*)a.ws_lse + lse_bytes(max_rows));
   // units that the widest visible list may hold
   const int64_t pages = TREE ? (a.max_ctx + kPage - 1) / kPage
@@ -636,10 +641,11 @@ int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* s
 // Checks shared by the two entries; fills the record's cache and table fields.
 bool rows_args(RowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const void* kc, const void* vc, int64_t ps, int64_t ts,
                int64_t hs, int64_t bt_stride, const void* out, int64_t out_st, int batch, int hq, int hkv, int head_dim,
-               int block_size, int max_blocks, float scale) {
+               int block_size, int max_blocks, int passes, float scale) {
   if (head_dim != kD || block_size <= 0 || block_size % kPage || batch < 0 || !valid_group(hq, hkv) || max_blocks <= 0) return false;
   const int64_t max_ctx = (int64_t)max_blocks * block_size;
-  if (max_ctx > (1 << 28)) return false;  // 256M tokens per sequence
+  // 256M tokens per sequence, and a launch's units (of 32 tokens, or of 64 as often as there are passes) in 31 bits
+  if (max_ctx > (1 << 28) || min(batch, kMaxBatch) * (max_ctx / 32 + 1) * max(1, (passes + 1) / 2) > INT32_MAX) return false;
   // rows move by 16-byte LDS-DMA at 32-bit offsets within a page
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15 || (q_st | q_sh | ps | ts | hs) & 7) return false;
   if (ts < kD || ts > (1 << 26) || ps < 0 || ps > UINT32_MAX || hs < 0 || bt_stride < max_blocks || min(batch, kMaxBatch) * bt_stride * 4 > INT32_MAX)
@@ -663,7 +669,7 @@ bool rows_args(RowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const voi
 extern "C" size_t xv_tree_attention_workspace_size(int batch, int max_nodes, int num_q_heads, int num_kv_heads) {
   if (batch <= 0 || max_nodes <= 0 || !valid_group(num_q_heads, num_kv_heads)) return 256;
   const int max_rows = max_nodes * (num_q_heads / num_kv_heads);
-  return seg_bytes(batch, num_kv_heads) + lse_bytes(max_rows) + slots(max_rows) * slot_rows(max_rows) * kD * sizeof(float);
+  return seg_bytes(batch, num_kv_heads, max_rows) + lse_bytes(max_rows) + slots(max_rows) * slot_rows(max_rows) * kD * sizeof(float);
 }
 
 extern "C" int xv_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,
@@ -676,7 +682,7 @@ extern "C" int xv_window_decode_attention(const void* q, int64_t q_stride_tok, i
   RowsArgs a{};
   if (window < 1 || sink_tokens < 0 ||
       !rows_args(a, q, q_stride_tok, q_stride_head, k_cache, v_cache, page_stride, tok_stride, head_stride, bt_stride, out,
-                 out_stride_tok, batch, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, scale))
+                 out_stride_tok, batch, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, 1, scale))
     return (int)hipErrorInvalidValue;
   if (batch == 0) return 0;
   if (workspace == nullptr || (uintptr_t)workspace & 15 ||
@@ -697,7 +703,8 @@ extern "C" int xv_tree_attention(const void* q, int64_t q_stride_tok, int64_t q_
   RowsArgs a{};
   if (max_nodes < 0 || max_nodes > 1024 || mask_words < 1 || max_nodes > 64 * (int64_t)mask_words || mask_stride < mask_words ||
       !rows_args(a, q, q_stride_tok, q_stride_head, k_cache, v_cache, page_stride, tok_stride, head_stride, bt_stride, out,
-                 out_stride_tok, batch, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, scale))
+                 out_stride_tok, batch, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                 valid_group(num_q_heads, num_kv_heads) ? row_passes(max_nodes * (num_q_heads / num_kv_heads)) : 1, scale))
     return (int)hipErrorInvalidValue;
   if (batch == 0 || max_nodes == 0) return 0;
   if (workspace == nullptr || (uintptr_t)workspace & 15 ||

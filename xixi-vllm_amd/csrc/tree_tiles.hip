@@ -4,7 +4,7 @@
 // The work split, partials and merge are those of xv_rows.h with 64-key tiles
 // as units and a workgroup per range: its waves take 32 rows each of the same
 // (sequence, kv head), so a K / V tile that is staged in LDS once serves up
-// to 32 WAVES rows (128 or 256; further ones are passes of the grid's y).
+// to 32 WAVES rows (128 or 256; further ones are further passes over the tiles).
 // Per tile and wave, on v_mfma_f32_32x32x16_bf16 as in prefill attention:
 // S^T = K Q^T, the softmax of a row in its lane pair, O^T += V^T P^T with P
 // straight from the scores' registers.  Tiles travel by LDS-DMA into a ring of
@@ -200,20 +200,21 @@ XV_INLINE void barrier() {
 template <int WAVES, int NB>
 __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
   constexpr int kRows = kKeys / WAVES;     // rows of a tile that a wave loads
+  static_assert(32 * WAVES <= kPassRows);
   constexpr int kOps = 2 * (kRows / 4);    // LDS-DMA instructions it takes for K and V
   __shared__ __attribute__((aligned(16))) char lds[NB * kBuf];
   __shared__ Sequences seqs;
   __shared__ uint64_t any[WAVES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
-  if (wave == 0) load_sequences<true>(seqs, a, lane, [](int ctx) { return (ctx + kKeys - 1) / kKeys; });
+  if (wave == 0) load_sequences<true, true>(seqs, a, lane, [](int ctx) { return (ctx + kKeys - 1) / kKeys; });
   __syncthreads();
-  const Ranges rg = ranges_of(seqs, a, gridDim.x, lane);
+  const Ranges rg = ranges_of<true>(seqs, a, gridDim.x, lane);
   const int id = blockIdx.x;
   const int64_t f0 = (int64_t)id * rg.len;
   const int n = (int)max((int64_t)0, min(f0 + rg.len, rg.total) - f0);
   if (n == 0) return;
-  const int row0 = (blockIdx.y * WAVES + wave) * 32, row = row0 + l32;  // this lane's row of every segment
+  const int row0 = wave * 32, row = row0 + l32;  // this lane's row of every segment
   const LdsAddr ad = lds_addr(lds, lane);
 
   // ---- The tiles' feed.  This wave loads rows r0 .. r0 + kRows - 1 of a tile, all in one cache block: row `r` on of block
@@ -222,7 +223,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
   const int r0 = kRows * wave;
   const int block = a.nsub * kPage;
   const int step_blocks = kKeys / block, step_rows = kKeys % block;
-  Cursor ic = cursor_at(seqs, a, f0);
+  Cursor ic = cursor_at<true>(seqs, a, f0);
   int issued = 0, idx = 0, r = 0, valid = 0, blk = 0;
   const int32_t* table = a.bt;
   auto fetch = [&] { blk = valid > 0 ? load_index(table + idx) : 0; };
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
       valid -= kKeys;
     } else {
       --ic.u;
-      advance(ic, seqs, a.hkv, a.batch);
+      advance<true>(ic, seqs, a);
       enter();
     }
     fetch();
@@ -267,11 +268,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
   enter();
   fetch();
 
-  // ---- Segments: the first row of q, the rows, and this lane's q
+  // ---- Segments: the first row of q, the rows (all from the pass's first on), and this lane's q
   Cursor pc = ic;  // tile x
-  auto rows_in = [&](int b, int& tok, int& rows) {
-    tok = lds_int(seqs.cq + b);
-    rows = (lds_int(seqs.cq + b + 1) - tok) << a.glog;
+  auto rows_in = [&](const Cursor& c, int& tok, int& rows) {
+    tok = lds_int(seqs.cq + c.b) + c.pass * (kPassRows >> a.glog);
+    rows = (lds_int(seqs.cq + c.b + 1) - tok) << a.glog;
   };
   Vec8 raw[8];
   auto load_q = [&](int kvh, int tok, int rows) {
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
   };
   // ---- Masks: a tile's first key as a node of its tree; where that is above -kKeys some row may not see every key.
   // This lane's words are loaded an iteration ahead.
-  auto node_of = [&](const Cursor& c, int rows) { return c.u * kKeys - (c.ctx - (rows >> a.glog)); };
+  auto node_of = [&](const Cursor& c, int rows) { return c.u * kKeys - c.ctx + ((rows + c.pass * kPassRows) >> a.glog); };
   uint64_t w0 = 0, w1 = 0;
   auto load_words = [&](int tok, int rows, int at) {
     const uint64_t* m = a.mask + (int64_t)(tok + (min(row, rows - 1) >> a.glog)) * a.mask_st;
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
     w1 = at > 0 && (at & 63) && w + 1 < a.words ? m[w + 1] : 0;
   };
   int tok, nrows;
-  rows_in(pc.b, tok, nrows);
+  rows_in(pc, tok, nrows);
   int at = node_of(pc, nrows);
   if (row0 < nrows) {
     load_q(pc.kvh, tok, nrows);
@@ -320,8 +321,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
     int tok1 = tok, nrows1 = nrows;
     const bool last = x + 1 == n, turn = pc.u + 1 == pc.nu || last;  // tile x ends its segment, or the range
     if (!last) {
-      advance(nc, seqs, a.hkv, a.batch);
-      if (turn) rows_in(nc.b, tok1, nrows1);
+      advance<true>(nc, seqs, a);
+      if (turn) rows_in(nc, tok1, nrows1);
     }
     const int at1 = node_of(nc, nrows1);
     if (row0 < nrows1) {  // ahead of the tiles: waiting for these does not wait for those
@@ -377,18 +378,17 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
 }
 
 int tile_waves(int max_rows) { return max_rows <= 128 ? 4 : 8; }
-int tile_passes(int max_rows) { return (max_rows + 32 * tile_waves(max_rows) - 1) / (32 * tile_waves(max_rows)); }
 
 }  // namespace
 
-int xv_rows::tile_rows(int max_rows) { return tile_passes(max_rows) * 32 * tile_waves(max_rows); }
-
-// As many as there are workgroups resident at once, two of four waves a CU or one of eight, shared among the passes: more
-// would only cut segments into more partials.
-int xv_rows::tile_ranges(int max_rows) { return max(8, 2048 / tile_waves(max_rows) / tile_passes(max_rows)); }
+int xv_rows::tile_rows(int max_rows) { return 32 * tile_waves(max_rows); }
+int xv_rows::tile_passes(int max_rows) { return (max_rows + kPassRows - 1) / kPassRows; }
+// As many as there are workgroups resident at once, two of four waves a CU or one of eight: more would only cut segments into
+// more partials.
+int xv_rows::tile_ranges(int max_rows) { return 2048 / tile_waves(max_rows); }
 
 int xv_rows::launch_tiles(const RowsArgs& a, int max_rows, hipStream_t stream) {
-  const dim3 grid((unsigned)tile_ranges(max_rows), (unsigned)tile_passes(max_rows));
+  const unsigned grid = (unsigned)tile_ranges(max_rows);
   if (tile_waves(max_rows) == 4) tree_tile_kernel<4, 2><<<grid, 256, 0, stream>>>(a);
   else tree_tile_kernel<8, 4><<<grid, 512, 0, stream>>>(a);
   return (int)hipGetLastError();

@@ -1,6 +1,6 @@
 // What the kernels of paged attention over a few rows per sequence share: their
 // arguments, and the flat (sequence, kv head, unit) space that is cut into
-// ranges.  A range's segments that it does not hold whole leave partials:
+// ranges; a sequence of many rows is in it once per pass over up to 256 of them.  A range's segments that it does not hold whole leave partials:
 // normalised fp32 rows and their log2-sum-exp, slot 2 * range for one that
 // started before the range, 2 * range + 1 for one that ends after it.
 #pragma once
@@ -20,7 +20,7 @@ struct RowsArgs {
   const int32_t* cu_q;                          // tree: first node of each sequence
   const uint64_t* mask; int64_t mask_st; int words;  // tree: visible nodes of each node
   bf16_t* out; int64_t out_st;
-  int2* ws_seg;     // (first range, partials) per (sequence, kv head)
+  int2* ws_seg;     // (first range, partials) per segment: seg_index
   float* ws_lse;    // log2-sum-exp of partial slot s, row r at s * rows + r
   float* ws_o;      // its rows, 128 values each
   int batch, hq, hkv, glog;  // query heads per kv head: 1 << glog
@@ -28,15 +28,20 @@ struct RowsArgs {
   int max_ctx;      // tokens the block table has room for
   int window, sinks;
   int rows;         // rows of a partial slot
+  int max_nodes;    // of a sequence; further ones are not looked at
+  int passes;       // of a sequence, at most
   // scale * log2(e); q is taken as (q & q_keep) ^ q_flip, so that the scale is positive: the sign of a negative
   // one goes to q, and a scale of 0 is 1 over a q of zeros
   float scale_log2;
   uint32_t q_keep, q_flip;
 };
 
+constexpr int kPassRows = 256;
+XV_INLINE int seg_index(const RowsArgs& a, int b, int pass, int kvh) { return (b * a.passes + pass) * a.hkv + kvh; }
+
 // Sequences of a launch, in LDS.
 struct Sequences {
-  int pref[kMaxBatch + 1];  // units of sequences 0 .. b - 1
+  int pref[kMaxBatch + 1];  // units of sequences 0 .. b - 1, all their passes
   int ctx[kMaxBatch];       // their tokens (0: no rows)
   int cq[kMaxBatch + 1];    // their first rows of q
 };
@@ -51,8 +56,14 @@ XV_INLINE int lds_int(const int* p) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+// Passes over n nodes, at least one.
+template <bool PASSES>
+XV_INLINE int passes_of(const RowsArgs& a, int n) {
+  return PASSES ? max(1, min(a.passes, (int)((((int64_t)n << a.glog) + kPassRows - 1) / kPassRows))) : 1;
+}
+
 // Fills `s` by one wave; units(ctx) > 0 for ctx > 0.
-template <bool TREE, typename F>
+template <bool TREE, bool PASSES, typename F>
 XV_INLINE void load_sequences(Sequences& s, const RowsArgs& a, int lane, F units) {
   int carry = 0;
   for (int c = 0; c < a.batch; c += 64) {
@@ -66,7 +77,7 @@ XV_INLINE void load_sequences(Sequences& s, const RowsArgs& a, int lane, F units
         if (q1 <= q0) ctx = 0;  // no rows: no units
       }
     }
-    int inc = ctx > 0 ? units(ctx) : 0;
+    int inc = ctx > 0 ? units(ctx) * passes_of<PASSES>(a, q1 - q0) : 0;
     inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xf, 0xf, true);  // inclusive scan: row_shr 1, 2, 4, 8,
     inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xf, 0xf, true);  // then the row sums across rows
     inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xf, 0xf, true);
@@ -90,9 +101,11 @@ struct Ranges {
   int64_t total;
   int len;
 };
+template <bool PASSES>
 XV_INLINE Ranges ranges_of(const Sequences& s, const RowsArgs& a, int nranges, int lane) {
   int longest = 0;
-  for (int b = lane; b < a.batch; b += 64) longest = max(longest, s.pref[b + 1] - s.pref[b]);
+  for (int b = lane; b < a.batch; b += 64)
+    longest = max(longest, (s.pref[b + 1] - s.pref[b]) / passes_of<PASSES>(a, s.cq[b + 1] - s.cq[b]));
   const int max_nu = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));  // exact in fp32 (below 2^24)
   Ranges r;
   r.total = (int64_t)a.hkv * __builtin_amdgcn_readfirstlane(s.pref[a.batch]);  // wave uniform, as all of this
@@ -102,29 +115,40 @@ XV_INLINE Ranges ranges_of(const Sequences& s, const RowsArgs& a, int nranges, i
 
 // A position in the flat space.
 struct Cursor {
-  int b, kvh, u;   // sequence, kv head, unit within the sequence
-  int nu, ctx;     // units and tokens of sequence b
+  int b, pass, kvh, u;  // sequence, pass over its rows, kv head, unit within the sequence
+  int np, nu, ctx;      // passes, units of one and tokens of sequence b
 };
+template <bool PASSES>
 XV_INLINE Cursor cursor_at(const Sequences& s, const RowsArgs& a, int64_t f) {
   Cursor c;
   c.b = __builtin_amdgcn_readfirstlane(seq_of(s.pref, a.batch, a.hkv, f));
-  c.nu = __builtin_amdgcn_readfirstlane(s.pref[c.b + 1] - s.pref[c.b]);
+  c.np = __builtin_amdgcn_readfirstlane(passes_of<PASSES>(a, s.cq[c.b + 1] - s.cq[c.b]));
+  c.nu = __builtin_amdgcn_readfirstlane((s.pref[c.b + 1] - s.pref[c.b]) / c.np);
   c.ctx = __builtin_amdgcn_readfirstlane(s.ctx[c.b]);
-  const int r = (int)(f - (int64_t)a.hkv * s.pref[c.b]);
-  c.kvh = __builtin_amdgcn_readfirstlane(r / c.nu);
-  c.u = __builtin_amdgcn_readfirstlane(r - c.kvh * c.nu);
+  const int64_t r = f - (int64_t)a.hkv * s.pref[c.b];
+  const int seg = __builtin_amdgcn_readfirstlane((int)(r / c.nu));
+  c.u = __builtin_amdgcn_readfirstlane((int)(r - (int64_t)seg * c.nu));
+  c.pass = PASSES ? __builtin_amdgcn_readfirstlane(seg / a.hkv) : 0;
+  c.kvh = seg - c.pass * a.hkv;
   return c;
 }
 // The next one.  Sequences without units are stepped over.
-XV_INLINE void advance(Cursor& c, const Sequences& s, int hkv, int batch) {
+template <bool PASSES>
+XV_INLINE void advance(Cursor& c, const Sequences& s, const RowsArgs& a) {
   if (++c.u < c.nu) return;
   c.u = 0;
-  if (++c.kvh < hkv) return;
+  if (++c.kvh < a.hkv) return;
   c.kvh = 0;
+  if (PASSES && ++c.pass < c.np) return;
+  c.pass = 0;
   do {
     ++c.b;
     c.nu = lds_int(s.pref + c.b + 1) - lds_int(s.pref + c.b);
-  } while (c.nu == 0 && c.b < batch - 1);
+  } while (c.nu == 0 && c.b < a.batch - 1);
+  if (PASSES) {
+    c.np = passes_of<PASSES>(a, lds_int(s.cq + c.b + 1) - lds_int(s.cq + c.b));
+    if (c.np > 1) c.nu /= c.np;
+  }
   c.ctx = lds_int(s.ctx + c.b);
 }
 
@@ -132,11 +156,11 @@ XV_INLINE void advance(Cursor& c, const Sequences& s, int hkv, int batch) {
 // -1 the output (the range holds all of it), else a partial slot.  `record`:
 // this caller also writes the segment's (first range, partials).
 XV_INLINE int finish_slot(const Sequences& s, const RowsArgs& a, const Cursor& c, int64_t f0, int n, int id, int len, bool record) {
-  const int64_t seg0 = (int64_t)a.hkv * lds_int(s.pref + c.b) + (int64_t)c.kvh * c.nu;
+  const int64_t seg0 = (int64_t)a.hkv * lds_int(s.pref + c.b) + (int64_t)(c.pass * a.hkv + c.kvh) * c.nu;
   const bool first = seg0 >= f0, last = seg0 + c.nu <= f0 + n;
   if (last && record) {
     const int w0 = (int)(seg0 / len);
-    a.ws_seg[c.b * a.hkv + c.kvh] = make_int2(w0, id - w0 + 1);
+    a.ws_seg[seg_index(a, c.b, c.pass, c.kvh)] = make_int2(w0, id - w0 + 1);
   }
   return first && last ? -1 : 2 * id + (first ? 1 : 0);
 }
@@ -148,6 +172,7 @@ XV_INLINE uint64_t low_bits64(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : 
 // Trees of more than 32 rows: tree_tiles.hip.  a: all but the workspace's slots, filled for `batch` sequences.
 int tile_ranges(int max_rows);     // ranges at most
 int tile_rows(int max_rows);       // rows of a partial slot
+int tile_passes(int max_rows);     // passes over a sequence's rows
 int launch_tiles(const RowsArgs& a, int max_rows, hipStream_t stream);
 
 }  // namespace xv_rows
