@@ -578,11 +578,11 @@ int rows_groups() {
 constexpr int kWaveRows = 32;
 // Rows of a tree call from which on the merge takes four rows a wave: enough waves then without spreading a row's partials.
 constexpr int kManyRows = 8192;
-int slot_rows(int max_rows) { return max_rows <= 16 ? 16 : max_rows <= kWaveRows ? 32 : tile_rows(max_rows); }
-size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : tile_ranges(max_rows)); }
+int slot_rows(int max_rows) { return max_rows <= 16 ? 16 : max_rows <= kWaveRows ? 32 : kPassRows; }
+size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : kTileGroups); }
 
 size_t al256(size_t x) { return (x + 255) / 256 * 256; }
-int row_passes(int max_rows) { return max_rows <= kWaveRows ? 1 : tile_passes(max_rows); }
+int row_passes(int max_rows) { return (max_rows + kPassRows - 1) / kPassRows; }
 size_t seg_bytes(int batch, int hkv, int max_rows) {
   return al256((size_t)row_passes(max_rows) * min(batch, kMaxBatch) * hkv * sizeof(int2));
 }
@@ -623,7 +623,7 @@ int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* s
       if (max_rows <= kWaveRows) {
         rows_kernel<2, TREE><<<groups, kWaves * 64, 0, stream>>>(a);
       } else {
-        const int e = launch_tiles(a, max_rows, stream);
+        const int e = launch_tiles(a, stream);
         if (e) return e;
       }
     }

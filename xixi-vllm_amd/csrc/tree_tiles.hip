@@ -4,11 +4,11 @@
 // The work split, partials and merge are those of xv_rows.h with 64-key tiles
 // as units and a workgroup per range: its waves take 32 rows each of the same
 // (sequence, kv head), so a K / V tile that is staged in LDS once serves up
-// to 32 WAVES rows (128 or 256; further ones are further passes over the tiles).
+// to 256 rows (further ones are further passes over the tiles).
 // Per tile and wave, on v_mfma_f32_32x32x16_bf16 as in prefill attention:
 // S^T = K Q^T, the softmax of a row in its lane pair, O^T += V^T P^T with P
 // straight from the scores' registers.  Tiles travel by LDS-DMA into a ring of
-// NB slots, one barrier per tile.
+// kRing slots, one barrier per tile.
 #include "xv_kernels.h"
 #include "xv_rows.h"
 #include "xv_tile.h"
@@ -17,6 +17,12 @@
 using namespace xv_rows;
 
 namespace {
+
+constexpr int kWaves = 8;
+constexpr int kRing = 4;                // tiles in LDS: 128 KB, a workgroup a CU
+constexpr int kRows = kKeys / kWaves;   // rows of a tile that a wave loads
+constexpr int kOps = 2 * (kRows / 4);   // LDS-DMA instructions it takes for K and V
+static_assert(32 * kWaves == kPassRows);
 
 const xv_bf16x2 kOnes = {(__bf16)1.0f, (__bf16)1.0f};
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -197,14 +203,10 @@ XV_INLINE void barrier() {
   __asm__ __volatile__("" ::: "memory");
 }
 
-template <int WAVES, int NB>
-__global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
-  constexpr int kRows = kKeys / WAVES;     // rows of a tile that a wave loads
-  static_assert(32 * WAVES <= kPassRows);
-  constexpr int kOps = 2 * (kRows / 4);    // LDS-DMA instructions it takes for K and V
-  __shared__ __attribute__((aligned(16))) char lds[NB * kBuf];
+__global__ __launch_bounds__(kWaves * 64, 2) void tree_tile_kernel(RowsArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[kRing * kBuf];
   __shared__ Sequences seqs;
-  __shared__ uint64_t any[WAVES];
+  __shared__ uint64_t any[kWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, h = lane >> 5;
   if (wave == 0) load_sequences<true, true>(seqs, a, lane, [](int ctx) { return (ctx + kKeys - 1) / kKeys; });
@@ -239,7 +241,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
                         (int64_t)ic.kvh * a.hs;
     const uint32_t bytes = valid > 0 ? (uint32_t)(((min(valid, kRows) - 1) * (int)a.ts + kD) * 2) : 0u;
     const __amdgpu_buffer_rsrc_t rk = page_rsrc(a.kc + off, bytes), rv = page_rsrc(a.vc + off, bytes);
-    char* const buf = lds + (issued % NB) * kBuf + r0 * 256;
+    char* const buf = lds + (issued % kRing) * kBuf + r0 * 256;
 #pragma unroll
     for (int s = 0; s < kRows / 4; ++s) {
       const int rr = 4 * s + (lane >> 4), R = r0 + rr;
@@ -309,12 +311,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
     if (at > -kKeys) load_words(tok, nrows, at);
   }
 #pragma unroll
-  for (int k = 0; k < NB - 1; ++k) issue();
+  for (int k = 0; k < kRing - 1; ++k) issue();
   if (row0 < nrows) take_q();
   TileState st;
   reset(st);
   for (int x = 0; x < n; ++x) {
-    __asm__ __volatile__("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * kOps) : "memory");
+    __asm__ __volatile__("s_waitcnt vmcnt(%0)" ::"n"((kRing - 2) * kOps) : "memory");
     barrier();  // tile x is in LDS; every wave is done with tile x - 1
     const uint64_t c0 = w0, c1 = w1;
     Cursor nc = pc;
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
       if (at1 > -kKeys) load_words(tok1, nrows1, at1);
     }
     issue();
-    const uint32_t slot = (uint32_t)(x % NB) * kBuf;
+    const uint32_t slot = (uint32_t)(x % kRing) * kBuf;
     uint64_t seen = 0;  // keys of the tile that this lane's row sees
     const bool edge = at > -kKeys;
     if (edge) {
@@ -343,7 +345,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
       barrier();
       uint64_t all = 0;
 #pragma unroll
-      for (int k = 0; k < WAVES; ++k) all |= any[k];
+      for (int k = 0; k < kWaves; ++k) all |= any[k];
 #pragma unroll
       for (int s = 0; s < kRows / 4; ++s) {
         const int R = r0 + 4 * s + (lane >> 4);
@@ -377,19 +379,9 @@ __global__ __launch_bounds__(WAVES * 64, 2) void tree_tile_kernel(RowsArgs a) {
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is on its way to LDS behind the wave's end
 }
 
-int tile_waves(int max_rows) { return max_rows <= 128 ? 4 : 8; }
-
 }  // namespace
 
-int xv_rows::tile_rows(int max_rows) { return 32 * tile_waves(max_rows); }
-int xv_rows::tile_passes(int max_rows) { return (max_rows + kPassRows - 1) / kPassRows; }
-// As many as there are workgroups resident at once, two of four waves a CU or one of eight: more would only cut segments into
-// more partials.
-int xv_rows::tile_ranges(int max_rows) { return 2048 / tile_waves(max_rows); }
-
-int xv_rows::launch_tiles(const RowsArgs& a, int max_rows, hipStream_t stream) {
-  const unsigned grid = (unsigned)tile_ranges(max_rows);
-  if (tile_waves(max_rows) == 4) tree_tile_kernel<4, 2><<<grid, 256, 0, stream>>>(a);
-  else tree_tile_kernel<8, 4><<<grid, 512, 0, stream>>>(a);
+int xv_rows::launch_tiles(const RowsArgs& a, hipStream_t stream) {
+  tree_tile_kernel<<<kTileGroups, kWaves * 64, 0, stream>>>(a);
   return (int)hipGetLastError();
 }

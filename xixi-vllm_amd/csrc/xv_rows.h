@@ -170,9 +170,7 @@ XV_INLINE uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u <<
 XV_INLINE uint64_t low_bits64(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; }
 
 // Trees of more than 32 rows: tree_tiles.hip.  a: all but the workspace's slots, filled for `batch` sequences.
-int tile_ranges(int max_rows);     // ranges at most
-int tile_rows(int max_rows);       // rows of a partial slot
-int tile_passes(int max_rows);     // passes over a sequence's rows
-int launch_tiles(const RowsArgs& a, int max_rows, hipStream_t stream);
+constexpr int kTileGroups = 256;   // ranges: as many as there are workgroups resident at once
+int launch_tiles(const RowsArgs& a, hipStream_t stream);
 
 }  // namespace xv_rows
