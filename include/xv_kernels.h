@@ -248,8 +248,9 @@ int xv_paged_decode_attention_fp4(const void* q, int64_t q_stride_tok, int64_t q
  * 1), itself among them, and the first `sink_tokens` (>= 0).  Block-table
  * entries that hold no visible token are not read; values that no query sees
  * may be anything.  bf16 pages.  A sequence is read up to max_blocks_per_seq *
- * block_size tokens at most (256M at most); the table rows of 256 sequences
- * (of all, where there are fewer) take 2 GB at most.  Layouts and supported
+ * block_size tokens at most (256M at most); for 256 sequences (or all, where
+ * there are fewer) these are below 64G together and the table rows take 2 GB at
+ * most.  Layouts and supported
  * shapes as xv_paged_decode_attention, any scale.
  * workspace: xv_tree_attention_workspace_size(batch, 1, ...) bytes, 16-byte
  * aligned, no initial contents.  Calls sharing one must be ordered on one stream.
@@ -275,7 +276,8 @@ int xv_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_st
  *   max_nodes  nodes of the largest tree at most, <= 64 * mask_words and <= 1024
  *   workspace  xv_tree_attention_workspace_size(...) bytes, 16-byte aligned, no
  *              initial contents.  Calls sharing one must be ordered on one stream.
- * Layouts, supported shapes and limits as xv_window_decode_attention.
+ * Layouts, supported shapes and limits as xv_window_decode_attention; the 64G
+ * are shared by the passes over a tree's rows (max_nodes * Hq / Hkv / 512).
  */
 size_t xv_tree_attention_workspace_size(int batch, int max_nodes, int num_q_heads, int num_kv_heads);
 int xv_tree_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,

@@ -150,6 +150,24 @@ def test_prefill_window_arguments():
             prefill_attention(q, kv, kv, cu, cu, 4, 4, 2, 128, **kw)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 4), (-1, 0), (5, -1), (1 << 31, 0), ((1 << 32) + 5, 0), (5, 1 << 32)])
+def test_window_sizes(window, sinks):
+    """Sizes that a 32-bit argument would wrap are refused too."""
+    from xvllm.layers.attention import Attention
+
+    with pytest.raises(ValueError, match="window"):
+        Attention(8, 128, 8, window=window, sink_tokens=sinks)
+
+
+@pytest.mark.parametrize("block,total", [(0, 4), ((1 << 32) + 16, 4), (16, -1), (16, (1 << 32) + 4)])
+def test_step_maps_sizes(block, total):
+    from xvllm.kv_ops import step_maps
+
+    x = torch.zeros(2, dtype=I32)
+    with pytest.raises(ValueError, match="block_size"):
+        step_maps(x, x, torch.zeros(2, 3, dtype=I32), x, block, total)
+
+
 def test_step_maps_needs_the_gpu():
     from xvllm.kv_ops import step_maps
 

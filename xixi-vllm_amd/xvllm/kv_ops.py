@@ -258,8 +258,10 @@ def step_maps(
       position seq_lens + depth instead of their index (tree_attention).
 
     The running sums stay below 2^31, and so do the pool's slots."""
+    if not 1 <= block_size <= 1 << 30 or not 0 <= total_tokens <= 1 << 30:
+        raise ValueError(f"block_size {block_size}, total_tokens {total_tokens}")
     dev = block_tables.get_device()
-    rows, i32 = seq_lens.shape[0], torch.int32
+    rows, i32 = seq_lens.numel(), torch.int32
     if dev < 0 or seq_lens.get_device() != dev or new_lens.get_device() != dev or free_pages.get_device() != dev:
         raise RuntimeError("xvllm ops run on the GPU only (HIP kernels), all operands on one device")
     if seq_lens.dtype != i32 or new_lens.dtype != i32 or free_pages.dtype != i32 or block_tables.dtype != i32:
@@ -276,8 +278,6 @@ def step_maps(
     if block_tables.shape[0] < rows or max_blocks < 1 or (inner != 1 and max_blocks > 1) or (bt_st < max_blocks and rows > 1):
         raise ValueError(f"block_tables {tuple(block_tables.shape)} of strides {block_tables.stride()} is not [{rows}, max_blocks] of "
                          "unit last stride")
-    if block_size < 1 or not 0 <= total_tokens <= 1 << 30:
-        raise ValueError(f"block_size {block_size}, total_tokens {total_tokens}")
     for name, t, n in (("free_head", free_head, 1), ("depths", depths, total_tokens), ("row_blocks", row_blocks, rows)):
         if t is not None:
             if t.dtype != i32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():

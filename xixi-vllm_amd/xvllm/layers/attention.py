@@ -193,9 +193,9 @@ def _windowed(window: int, sink_tokens: int) -> bool:
     """Whether a call has a sliding window (0: none), after checking its sizes."""
     if not window and not sink_tokens:
         return False
-    if window < 1 or sink_tokens < 0:
+    if not 1 <= window < 1 << 31 or not 0 <= sink_tokens < 1 << 31:
         raise ValueError(f"window {window}, sink_tokens {sink_tokens}: a window is at least 1, sinks go with one and are not "
-                         "negative")
+                         "negative, both below 2^31")
     return True
 
 
