@@ -644,8 +644,10 @@ bool rows_args(RowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const voi
                int block_size, int max_blocks, int passes, float scale) {
   if (head_dim != kD || block_size <= 0 || block_size % kPage || batch < 0 || !valid_group(hq, hkv) || max_blocks <= 0) return false;
   const int64_t max_ctx = (int64_t)max_blocks * block_size;
-  // 256M tokens per sequence, and a launch's units (of 32 tokens, or of 64 as often as there are passes) in 31 bits
-  if (max_ctx > (1 << 28) || min(batch, kMaxBatch) * (max_ctx / 32 + 1) * max(1, (passes + 1) / 2) > INT32_MAX) return false;
+  // 256M tokens per sequence, and the units (of 32 tokens, or of 64 as often as there are passes) of a launch's sequences,
+  // and of a sequence's kv heads, in 31 bits
+  if (max_ctx > (1 << 28) || max(hkv, min(batch, kMaxBatch)) * (max_ctx / 32 + 1) * max(1, (passes + 1) / 2) > INT32_MAX)
+    return false;
   // rows move by 16-byte LDS-DMA at 32-bit offsets within a page
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc) & 15 || (q_st | q_sh | ps | ts | hs) & 7) return false;
   if (ts < kD || ts > (1 << 26) || ps < 0 || ps > UINT32_MAX || hs < 0 || bt_stride < max_blocks || min(batch, kMaxBatch) * bt_stride * 4 > INT32_MAX)

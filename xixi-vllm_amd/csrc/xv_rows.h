@@ -104,8 +104,10 @@ struct Ranges {
 template <bool PASSES>
 XV_INLINE Ranges ranges_of(const Sequences& s, const RowsArgs& a, int nranges, int lane) {
   int longest = 0;
-  for (int b = lane; b < a.batch; b += 64)
-    longest = max(longest, (s.pref[b + 1] - s.pref[b]) / passes_of<PASSES>(a, s.cq[b + 1] - s.cq[b]));
+  for (int b = lane; b < a.batch; b += 64) {
+    const int nu = s.pref[b + 1] - s.pref[b];
+    longest = max(longest, a.passes > 1 ? nu / passes_of<PASSES>(a, s.cq[b + 1] - s.cq[b]) : nu);
+  }
   const int max_nu = __builtin_amdgcn_readfirstlane((int)wave_max((float)longest));  // exact in fp32 (below 2^24)
   Ranges r;
   r.total = (int64_t)a.hkv * __builtin_amdgcn_readfirstlane(s.pref[a.batch]);  // wave uniform, as all of this
@@ -123,12 +125,13 @@ XV_INLINE Cursor cursor_at(const Sequences& s, const RowsArgs& a, int64_t f) {
   Cursor c;
   c.b = __builtin_amdgcn_readfirstlane(seq_of(s.pref, a.batch, a.hkv, f));
   c.np = __builtin_amdgcn_readfirstlane(passes_of<PASSES>(a, s.cq[c.b + 1] - s.cq[c.b]));
-  c.nu = __builtin_amdgcn_readfirstlane((s.pref[c.b + 1] - s.pref[c.b]) / c.np);
+  c.nu = __builtin_amdgcn_readfirstlane(s.pref[c.b + 1] - s.pref[c.b]);
+  if (c.np > 1) c.nu /= c.np;
   c.ctx = __builtin_amdgcn_readfirstlane(s.ctx[c.b]);
-  const int64_t r = f - (int64_t)a.hkv * s.pref[c.b];
-  const int seg = __builtin_amdgcn_readfirstlane((int)(r / c.nu));
-  c.u = __builtin_amdgcn_readfirstlane((int)(r - (int64_t)seg * c.nu));
-  c.pass = PASSES ? __builtin_amdgcn_readfirstlane(seg / a.hkv) : 0;
+  const int r = (int)(f - (int64_t)a.hkv * s.pref[c.b]);
+  const int seg = __builtin_amdgcn_readfirstlane(r / c.nu);
+  c.u = __builtin_amdgcn_readfirstlane(r - seg * c.nu);
+  c.pass = PASSES && c.np > 1 ? seg / a.hkv : 0;
   c.kvh = seg - c.pass * a.hkv;
   return c;
 }
