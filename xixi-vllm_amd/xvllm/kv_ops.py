@@ -286,7 +286,7 @@ def step_maps(
                 raise RuntimeError(f"{name} must be on the block tables' device")
     # one allocation: positions (int64), slots, both running sums, the lengths, the rows' blocks, the list's head
     total_tokens = int(total_tokens)
-    buf = torch.empty(3 * total_tokens + total_tokens % 2 * 2 + 4 * rows + 3, dtype=i32, device=block_tables.device)
+    buf = block_tables.new_empty(3 * total_tokens + total_tokens % 2 * 2 + 4 * rows + 3)
     wide = 2 * total_tokens + total_tokens % 2 * 2  # the slots start 16-byte aligned
     pos, slots, cu_q, cu_k, ends, own, head = buf.split_with_sizes((wide, total_tokens, rows + 1, rows + 1, rows, rows, 1))
     base = buf.data_ptr()

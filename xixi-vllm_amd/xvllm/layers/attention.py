@@ -210,9 +210,13 @@ def _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, bs
     if k_cache.dim() != 4 or k_cache.shape[2:] != (hkv, d) or v_cache.shape != k_cache.shape or v_cache.stride() != st or st[3] != 1:
         raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} are not pages [NB, BS, {hkv}, {d}] of one "
                          "layout")
-    q3, qs0, qs1 = _q_view(q, hq, d)
-    if q3.dim() != 3 or q3.shape[1:] != (hq, d):
-        raise ValueError(f"q {tuple(q.shape)} is not rows of {hq} heads of {d}")
+    rows, qs = q.shape[0], q.stride()
+    if q.dim() == 2 and q.shape[1] == hq * d and qs[1] == 1 and not (qs[0] | d) % 8 and aligned16(q):
+        q3, qs0, qs1 = q, qs[0], d  # the usual rows, without the cost of a view
+    else:
+        q3, qs0, qs1 = _q_view(q, hq, d)
+        if q3.dim() != 3 or q3.shape[1:] != (hq, d):
+            raise ValueError(f"q {tuple(q.shape)} is not rows of {hq} heads of {d}")
     if block_tables.dim() != 2 or block_tables.shape[0] < bsz or cache_seqlens.dim() != 1 or cache_seqlens.shape[0] < bsz:
         raise ValueError(f"block_tables {tuple(block_tables.shape)}, cache_seqlens {tuple(cache_seqlens.shape)}: not a row and a "
                          f"length for each of {bsz} sequences")
@@ -227,9 +231,8 @@ def _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, bs
         bt = bt.contiguous()
         bt_st = max_blocks
     sl = as_int32(cache_seqlens).contiguous()
-    rows = q3.shape[0]
     if out is None:
-        out = torch.empty((rows, hq * d), dtype=q.dtype, device=q.device)
+        out = q.new_empty((rows, hq * d))
         out_st = hq * d
     elif out.shape != (rows, hq * d) or out.dtype != q.dtype or out.get_device() != dev or out.stride(-1) != 1:
         raise ValueError(f"out must be bf16 [{rows}, {hq * d}] of unit last stride on the cache's device")
@@ -248,7 +251,7 @@ def _window_decode(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d,
     if bsz == 0:
         return out
     ws_bytes = _C.lib().xv_tree_attention_workspace_size(bsz, 1, hq, hkv)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
     call("xv_window_decode_attention", dev, *head, out.data_ptr(), out_st, ws.data_ptr(), ws_bytes, bsz, hq, hkv, d, bs,
          max_blocks, window, sink_tokens, scale)
@@ -322,7 +325,7 @@ def tree_attention(
         mask = mask.contiguous()
     cu = as_int32(cu_seqlens_q).contiguous()
     ws_bytes = _C.lib().xv_tree_attention_workspace_size(bsz, max_seqlen_q, num_qo_heads, num_kv_heads)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
     call("xv_tree_attention", dev, *head, cu.data_ptr(), mask.data_ptr(), max(mask.stride(0), words), words, out.data_ptr(), out_st,
          ws.data_ptr(), ws_bytes, bsz, max_seqlen_q, num_qo_heads, num_kv_heads, head_dim, bs, max_blocks, scale)
