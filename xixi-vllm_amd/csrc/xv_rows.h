@@ -36,6 +36,8 @@ struct RowsArgs {
   uint32_t q_keep, q_flip;
 };
 
+// Passes are segments of the flat space: equal ranges over them balance a large tree among small ones (one of 1024 nodes
+// among 31 of 20: 178 us, 1065 with the same number of workgroups for every pass).
 constexpr int kPassRows = 256;
 XV_INLINE int seg_index(const RowsArgs& a, int b, int pass, int kvh) { return (b * a.passes + pass) * a.hkv + kvh; }
 
