@@ -30,9 +30,9 @@
 // passes over those that none of its queries sees.  Bound by the softmax beside
 // the products, as without a window (products busy 52 % of the time, vector work
 // 44 %): one document of 16001 with a window of 4096, 16 / 8 heads, 474 GFLOP,
-// 494 us (960 TFLOP/s); 16 chunks of up to 512 over up to 12000 cached tokens,
-// window 2000, 64 / 8 heads, 379 GFLOP, 485 us (781); 12 prompts of 40 to 2500,
-// window 512, 32 / 8 heads, 97 GFLOP, 182 us (534: short lists of tiles, each
+// 480 us (989 TFLOP/s); 16 chunks of up to 512 over up to 12000 cached tokens,
+// window 2000, 64 / 8 heads, 379 GFLOP, 473 us (800); 12 prompts of 40 to 2500,
+// window 512, 32 / 8 heads, 97 GFLOP, 180 us (540: short lists of tiles, each
 // with a start and two masked edges).
 #include "xv_common.h"
 #include "xv_kernels.h"
