@@ -1,7 +1,7 @@
 """``vllm::attention`` custom op (reference ``src/compute/layers/attention.py:13-143``):
 stores this step's K/V at ``slot_mapping`` (kv_ops.store_kvcache), then runs
 paged GQA decode attention or varlen causal prefill attention, both as gfx950
-HIP kernels.  Same signature (and one optional argument more), same module-global ``attention_context`` pool
+HIP kernels.  Same signature (and three optional arguments more), same module-global ``attention_context`` pool
 handle, same ``AttnInputs`` record.
 """
 from __future__ import annotations
@@ -9,6 +9,7 @@ from __future__ import annotations
 import math
 from contextlib import contextmanager
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -206,18 +207,20 @@ def _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, bs
     require_bf16(q)
     if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
         raise TypeError(f"{what} reads bf16 pages, got {k_cache.dtype} and {v_cache.dtype}")
-    st = k_cache.stride()
-    if k_cache.dim() != 4 or k_cache.shape[2:] != (hkv, d) or v_cache.shape != k_cache.shape or v_cache.stride() != st or st[3] != 1:
+    ks, st = k_cache.shape, k_cache.stride()
+    if len(ks) != 4 or ks[2] != hkv or ks[3] != d or v_cache.shape != ks or v_cache.stride() != st or st[3] != 1:
         raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} are not pages [NB, BS, {hkv}, {d}] of one "
                          "layout")
-    rows, qs = q.shape[0], q.stride()
-    if q.dim() == 2 and q.shape[1] == hq * d and qs[1] == 1 and not (qs[0] | d) % 8 and aligned16(q):
-        q3, qs0, qs1 = q, qs[0], d  # the usual rows, without the cost of a view
+    shape, qs = q.shape, q.stride()
+    usual = len(shape) == 2 and shape[1] == hq * d and qs[1] == 1 and not (qs[0] | d) % 8 and aligned16(q)
+    if usual:
+        q3, qs0, qs1 = q, qs[0], d  # without the cost of a view
     else:
         q3, qs0, qs1 = _q_view(q, hq, d)
         if q3.dim() != 3 or q3.shape[1:] != (hq, d):
             raise ValueError(f"q {tuple(q.shape)} is not rows of {hq} heads of {d}")
-    if block_tables.dim() != 2 or block_tables.shape[0] < bsz or cache_seqlens.dim() != 1 or cache_seqlens.shape[0] < bsz:
+    tables = block_tables.shape
+    if len(tables) != 2 or tables[0] < bsz or cache_seqlens.dim() != 1 or cache_seqlens.shape[0] < bsz:
         raise ValueError(f"block_tables {tuple(block_tables.shape)}, cache_seqlens {tuple(cache_seqlens.shape)}: not a row and a "
                          f"length for each of {bsz} sequences")
     dev = k_cache.get_device()
@@ -225,22 +228,27 @@ def _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, bs
             or cache_seqlens.get_device() != dev):
         raise RuntimeError("xvllm ops run on the GPU only (HIP kernels), q, the cache, block_tables and cache_seqlens on one device")
     bt = as_int32(block_tables)
-    max_blocks = bt.shape[1]
+    max_blocks = tables[1]
     bt_st, inner = bt.stride()
     if inner != 1 or (bsz > 1 and bt_st < max_blocks):
         bt = bt.contiguous()
         bt_st = max_blocks
     sl = as_int32(cache_seqlens).contiguous()
     if out is None:
-        out = q.new_empty((rows, hq * d))
+        out = torch.empty_like(q) if usual and qs[0] == hq * d else q.new_empty((shape[0], hq * d))
         out_st = hq * d
-    elif out.shape != (rows, hq * d) or out.dtype != q.dtype or out.get_device() != dev or out.stride(-1) != 1:
-        raise ValueError(f"out must be bf16 [{rows}, {hq * d}] of unit last stride on the cache's device")
+    elif out.shape != (shape[0], hq * d) or out.dtype != q.dtype or out.get_device() != dev or out.stride(-1) != 1:
+        raise ValueError(f"out must be bf16 [{shape[0]}, {hq * d}] of unit last stride on the cache's device")
     else:
         out_st = out.stride(0)
     head = (q3.data_ptr(), qs0, qs1, k_cache.data_ptr(), v_cache.data_ptr(), *st[:3], bt.data_ptr(), max(bt_st, max_blocks),
             sl.data_ptr())
-    return dev, head, (q3, bt, sl), out, out_st, k_cache.shape[1], max_blocks
+    return dev, head, (q3, bt, sl), out, out_st, ks[1], max_blocks
+
+
+@lru_cache(maxsize=1024)
+def _rows_workspace_size(batch: int, max_nodes: int, hq: int, hkv: int) -> int:
+    return _C.lib().xv_tree_attention_workspace_size(batch, max_nodes, hq, hkv)
 
 
 def _window_decode(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, softmax_scale, out, window,
@@ -250,7 +258,7 @@ def _window_decode(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d,
                                                                out, "a windowed decode")
     if bsz == 0:
         return out
-    ws_bytes = _C.lib().xv_tree_attention_workspace_size(bsz, 1, hq, hkv)
+    ws_bytes = _rows_workspace_size(bsz, 1, hq, hkv)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
     call("xv_window_decode_attention", dev, *head, out.data_ptr(), out_st, ws.data_ptr(), ws_bytes, bsz, hq, hkv, d, bs,
@@ -324,7 +332,7 @@ def tree_attention(
     if (words > 1 and mask.stride(1) != 1) or mask.stride(0) < words:
         mask = mask.contiguous()
     cu = as_int32(cu_seqlens_q).contiguous()
-    ws_bytes = _C.lib().xv_tree_attention_workspace_size(bsz, max_seqlen_q, num_qo_heads, num_kv_heads)
+    ws_bytes = _rows_workspace_size(bsz, max_seqlen_q, num_qo_heads, num_kv_heads)
     ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
     call("xv_tree_attention", dev, *head, cu.data_ptr(), mask.data_ptr(), max(mask.stride(0), words), words, out.data_ptr(), out_st,
