@@ -75,15 +75,14 @@ struct Page {
   int row;
 };
 
-// Wave w moves keys key0+16w .. +15 of the tile (one cache page when paged):
-// 4 LDS-DMA instructions for K and/or 4 for V, each 4 whole rows.
+// Wave w moves the 16 keys from j0 on (one cache page when paged), rows 16w .. +15
+// of the tile: 4 LDS-DMA instructions for K and/or 4 for V, each 4 whole rows.
 // WIN: keys sinks .. lo - 1 are seen by no query of the workgroup: their V
 // reads as zeros (whatever the cache holds there), and 16 keys that are all
 // such are not read at all (their block-table entry may be gone).
 template <bool PAGED, bool DO_K, bool DO_V, bool WIN>
-XV_INLINE void load_rows(char* buf, const PrefillArgs& a, int b, int kvh, int key0, int k0, int k_len,
+XV_INLINE void load_rows(char* buf, const PrefillArgs& a, int b, int kvh, int j0, int k0, int k_len,
                          Page page, int lo, int wave, int lane) {
-  const int j0 = key0 + 16 * wave;
   const int valid = WIN && j0 >= a.sinks && j0 + 16 <= lo ? 0 : min(16, k_len - j0);
   const bf16_t *kb, *vb;
   int64_t rs;  // row stride (elements)
@@ -175,12 +174,16 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   const int qw0 = qb0 + (wave / GW) * 32;  // the wave's first query
   const int my_q = qw0 + l32;
   const int kv_end = min(k_len, shift + min(qb0 + kBlockQ, q_len));  // keys the block needs
-  // WIN: the tiles of the block are those of the sinks, then those from its first query's window on
+  // The keys that the block needs, 16 at a time: all of them; WIN: the sinks', then those from its first query's window on.
+  // Four sixteens are a tile.
   const int blk_lo = WIN ? max(0, shift + qb0 + 1 - a.window) : 0;
-  const int sink_tiles = WIN ? (min(a.sinks, blk_lo) + kKeys - 1) / kKeys : 0;
-  const int skip = WIN ? max(0, blk_lo / kKeys - sink_tiles) : 0;
-  const int ntiles = max(0, (kv_end + kKeys - 1) / kKeys - skip);
-  auto key_of = [&](int t) { return (WIN && t >= sink_tiles ? t + skip : t) * kKeys; };  // first key of tile t
+  const int sink_16 = WIN ? (min(a.sinks, blk_lo) + 15) / 16 : 0;
+  const int skip = WIN ? max(0, blk_lo / 16 - sink_16) : 0;
+  const int ntiles = WIN ? max(0, (kv_end + 15) / 16 - skip + 3) / 4 : max(0, (kv_end + kKeys - 1) / kKeys);
+  auto key_of = [&](int t, int g) {  // first key of tile t's sixteen g
+    const int i = 4 * t + g;
+    return 16 * (WIN && i >= sink_16 ? i + skip : i);
+  };
   const bool active = qw0 < q_len;
   const int wave_kend = active ? min(k_len, shift + min(qw0 + 32, q_len)) : 0;  // keys any query of the wave sees
   const int wave_kfull = shift + qw0 + 1;  // keys every query of the wave sees
@@ -189,8 +192,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   const int wave_lo = WIN ? wave_kfull - a.window : 0;       // of the wave's first query's, and of its last one's
   const int wave_lo_last = WIN ? wave_lo + 31 : 0;
   auto needed = [&](int t) {  // whether any query of the wave sees a key of tile t
-    const int key0 = key_of(t);
-    return key0 < wave_kend && (!WIN || key0 + kKeys > wave_lo || key0 < a.sinks);
+    const int key0 = key_of(t, 0);
+    return key0 < wave_kend && (!WIN || key_of(t, 3) + 16 > wave_lo || key0 < a.sinks);
   };
 
   // Q^T B-operands: lane holds query my_q, d = 16s + 8(l/32) .. +7
@@ -218,8 +221,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   int at_block = 0, at_row = 0;
   auto page_of = [&](int t) {
     if (!PAGED) return Page{0, 0};
-    const int j = key_of(t) + 16 * wave;
-    if (t == 0 || (WIN && t == sink_tiles)) {
+    const int j = key_of(t, wave);
+    if (t == 0 || (WIN && 4 * t + wave < sink_16 + 4)) {  // not 64 keys behind the last ones, or maybe not
       at_block = j / a.block_size;
       at_row = j - at_block * a.block_size;
     } else {
@@ -250,15 +253,15 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   };
   // online softmax of tile t's scores s -> P (bf16), O and l rescaled as needed
   auto softmax = [&](int t, floatx16_t (&s)[2], bf16x8_t (&pb)[2][2]) {
-    const int key0 = key_of(t);
+    const int key0 = key_of(t, 0), key3 = key_of(t, 3);
     // (on raw scores: scale > 0 keeps the order; p = exp2(s*scale - m*scale))
     // the tile crosses some query's diagonal, or the first key of some query's window
-    if (key0 + kKeys > wave_kfull || (WIN && key0 < wave_lo_last && key0 + kKeys > a.sinks)) {
+    if (key3 + 16 > wave_kfull || (WIN && key0 < wave_lo_last && key3 + 16 > a.sinks)) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = key0 + 32 * mt + 8 * (r >> 2) + 4 * h + (r & 3);
+          const int key = key_of(t, 2 * mt + (r >> 3)) + 8 * ((r >> 2) & 1) + 4 * h + (r & 3);
           s[mt][r] = key < my_kend && (!WIN || key >= my_lo || key < a.sinks) ? s[mt][r] : -INFINITY;
         }
     }
@@ -324,9 +327,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   // freed by the barrier at its top.
   const Page page0 = page_of(0);
   Page pv_page = ntiles > 1 ? page_of(1) : Page{0, 0}, pk_page = ntiles > 2 ? page_of(2) : Page{0, 0};
-  if (ntiles > 0) load_rows<PAGED, true, true, WIN>(lds, a, b, kvh, key_of(0), k0, k_len, page0, blk_lo, wave, lane);
+  if (ntiles > 0) load_rows<PAGED, true, true, WIN>(lds, a, b, kvh, key_of(0, wave), k0, k_len, page0, blk_lo, wave, lane);
   if (ntiles > 1)
-    load_rows<PAGED, true, false, WIN>(lds + kBuf, a, b, kvh, key_of(1), k0, k_len, pv_page, blk_lo, wave, lane);
+    load_rows<PAGED, true, false, WIN>(lds + kBuf, a, b, kvh, key_of(1, wave), k0, k_len, pv_page, blk_lo, wave, lane);
   __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   // scores of even tiles in s_even, of odd tiles in s_odd (no copies)
@@ -337,9 +340,9 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
     __asm__ __volatile__("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // K(t+1) and V(t) are in LDS; every wave is done with iteration t-1
     if (t + 2 < ntiles)
-      load_rows<PAGED, true, false, WIN>(lds + PAR * kBuf, a, b, kvh, key_of(t + 2), k0, k_len, pk_page, blk_lo, wave, lane);
+      load_rows<PAGED, true, false, WIN>(lds + PAR * kBuf, a, b, kvh, key_of(t + 2, wave), k0, k_len, pk_page, blk_lo, wave, lane);
     if (t + 1 < ntiles)
-      load_rows<PAGED, false, true, WIN>(lds + (1 - PAR) * kBuf, a, b, kvh, key_of(t + 1), k0, k_len, pv_page, blk_lo, wave, lane);
+      load_rows<PAGED, false, true, WIN>(lds + (1 - PAR) * kBuf, a, b, kvh, key_of(t + 1, wave), k0, k_len, pv_page, blk_lo, wave, lane);
     pv_page = pk_page;
     if (t + 3 < ntiles) pk_page = page_of(t + 3);
     if (t + 1 < ntiles && needed(t + 1)) s_tile(std::integral_constant<int, 1 - PAR>{}, sn);
