@@ -406,8 +406,8 @@ int xv_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_h
  * xv_prefill_attention with a sliding window and sinks: the query at position p
  * of its sequence sees keys j <= p with j > p - window (>= 1) or j < sink_tokens
  * (>= 0).  No counterpart in the reference.  Block-table entries that hold no
- * key that a query of the call sees are not read.  scale > 0; the rest as
- * xv_prefill_attention.
+ * key that a query of the call sees are not read.  total_q: cu_seqlens_q[batch]
+ * or more.  scale > 0; the rest as xv_prefill_attention.
  */
 int xv_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                                 const void* k, const void* v, int64_t kv_stride_tok, int64_t kv_stride_head,
@@ -416,7 +416,7 @@ int xv_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_s
                                 const int32_t* block_tables, int64_t bt_stride,
                                 const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                                 void* out, int64_t out_stride_tok,
-                                int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+                                int batch, int max_seqlen_q, int64_t total_q, int num_q_heads, int num_kv_heads,
                                 int head_dim, int block_size, int window, int sink_tokens, float scale,
                                 hipStream_t stream);
 

@@ -78,7 +78,7 @@ def test_workspace_of_large_trees(lib):
 
 def _prefill(lib, **kw):
     a = dict(q=A, qst=4096, qsh=128, k=A, v=A, kvst=1024, kvsh=128, kc=None, vc=None, ps=0, ts=0, hs=0, bt=None, bts=0, cuq=A, cuk=A,
-             out=A, ost=4096, B=4, maxq=512, Hq=32, Hkv=8, D=128, BS=16, window=100, sinks=4, scale=0.1)
+             out=A, ost=4096, B=4, maxq=512, total=900, Hq=32, Hkv=8, D=128, BS=16, window=100, sinks=4, scale=0.1)
     a.update(kw)
     return lib.xv_window_prefill_attention(*a.values(), None)
 
@@ -87,9 +87,9 @@ def test_window_prefill_refusals(lib):
     for kw in (dict(window=0), dict(sinks=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(D=64), dict(Hq=24),
                dict(k=None), dict(k=A + 8), dict(kvst=1020), dict(q=A + 8), dict(qsh=130), dict(out=A + 4), dict(ost=4098),
                dict(bt=A, kc=A, vc=A, BS=40), dict(bt=A, kc=None, vc=A), dict(bt=A, kc=A + 8, vc=A), dict(maxq=32 * 65536),
-               dict(B=70000), dict(B=-1)):
+               dict(B=70000), dict(B=-1), dict(total=-1), dict(total=1 << 31)):
         assert _prefill(lib, **kw) == INVALID, kw
-    assert _prefill(lib, B=0) == 0 and _prefill(lib, maxq=0) == 0
+    assert _prefill(lib, B=0) == 0 and _prefill(lib, maxq=0) == 0 and _prefill(lib, total=0) == 0
 
 
 def _maps(lib, **kw):

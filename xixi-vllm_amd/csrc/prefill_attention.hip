@@ -146,6 +146,48 @@ XV_INLINE Sequence seq_by_work(const int* cu_q, const int* cu_k, int batch, int 
                   __builtin_amdgcn_readlane(kl, b)};
 }
 
+// Block `flat` of the sequences' blocks of BQ queries one after the other, in the
+// order above: its sequence, and its rank in it (-1: there is none).  For a grid
+// without the places of blocks that shorter sequences do not have.
+struct Block {
+  Sequence seq;
+  int rank;
+};
+template <int BQ>
+XV_INLINE Block block_by_work(const int* cu_q, const int* cu_k, int batch, int flat) {
+  const int lane = threadIdx.x & 63;
+  for (int c = 0; c < batch; c += 64) {
+    const int i = c + lane;
+    int q0 = 0, ql = 0, k0 = 0, kl = 0;
+    if (i < batch) {
+      q0 = cu_q[i];
+      k0 = cu_k[i];
+      ql = cu_q[i + 1] - q0;
+      kl = cu_k[i + 1] - k0;
+    }
+    const int64_t w = (int64_t)ql * (kl - ql) + (int64_t)ql * (ql + 1) / 2;
+    const int blocks = max(0, (ql + BQ - 1) / BQ);
+    int before = 0, all = 0;  // blocks of the sequences dispatched before this lane's, and of all 64
+    for (int t = 0; t < min(64, batch - c); ++t) {
+      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)w, t);
+      const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)w >> 32), t);
+      const int64_t wt = (int64_t)(((uint64_t)hi << 32) | lo);
+      const int bt = __builtin_amdgcn_readlane(blocks, t);
+      before += wt > w || (wt == w && t < lane) ? bt : 0;
+      all += bt;
+    }
+    const uint64_t m = __ballot(flat >= before && flat < before + blocks);
+    if (m) {
+      const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(m));
+      return Block{Sequence{c + l, __builtin_amdgcn_readlane(q0, l), __builtin_amdgcn_readlane(ql, l),
+                            __builtin_amdgcn_readlane(k0, l), __builtin_amdgcn_readlane(kl, l)},
+                   flat - __builtin_amdgcn_readlane(before, l)};
+    }
+    flat -= all;
+  }
+  return Block{Sequence{0, 0, 0, 0, 0}, -1};
+}
+
 template <int G, bool PAGED, bool WIN>
 __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   constexpr int GW = G < 4 ? G : 4;   // query heads per workgroup
@@ -158,8 +200,12 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   // XCD-aware order: workgroups go round-robin to the 8 XCDs, so with the head
   // slot fastest every XCD serves the same kv head(s) and keeps their K/V tiles
   // in its own L2; each head carries the same work, which balances the XCDs.
-  const int hsel = blockIdx.x, rank = blockIdx.y;
-  const Sequence seq = seq_by_work(a.cu_q, a.cu_k, a.batch, blockIdx.z);
+  const int hsel = blockIdx.x;
+  const Block blk = WIN ? block_by_work<kBlockQ>(a.cu_q, a.cu_k, a.batch, (int)(blockIdx.z * gridDim.y + blockIdx.y))
+                        : Block{seq_by_work(a.cu_q, a.cu_k, a.batch, blockIdx.z), (int)blockIdx.y};
+  if (WIN && blk.rank < 0) return;
+  const Sequence seq = blk.seq;
+  const int rank = blk.rank;
   const int b = seq.b;
   // group 8: two slots per kv head (query heads 0-3 and 4-7), slot = half * Hkv
   // + kvh, so both halves of a kv head land on the same XCD
@@ -387,7 +433,7 @@ void launch(const PrefillArgs& a, dim3 grid, hipStream_t stream) {
   }
 }
 
-// window 0: every query sees all keys up to itself
+// window 0: every query sees all keys up to itself (total_q is not looked at)
 int prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
             const void* k, const void* v, int64_t kv_stride_tok, int64_t kv_stride_head,
             const void* k_cache, const void* v_cache,
@@ -395,10 +441,10 @@ int prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
             const int32_t* block_tables, int64_t bt_stride,
             const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
             void* out, int64_t out_stride_tok,
-            int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+            int batch, int max_seqlen_q, int64_t total_q, int num_q_heads, int num_kv_heads,
             int head_dim, int block_size, int window, int sink_tokens, float scale,
             hipStream_t stream) {
-  if (head_dim != kD || batch < 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
+  if (head_dim != kD || batch < 0 || total_q < 0 || total_q > INT32_MAX || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
     return (int)hipErrorInvalidValue;
   const int group = num_q_heads / num_kv_heads;
   if (group != 1 && group != 2 && group != 4 && group != 8) return (int)hipErrorInvalidValue;
@@ -430,7 +476,13 @@ int prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   const int block_q = 32 * (4 / gw);
   a.qblocks = (max_seqlen_q + block_q - 1) / block_q;
   if (a.qblocks > 65535 || batch > 65535) return (int)hipErrorInvalidValue;  // grid y / z limits
-  const dim3 grid((unsigned)(num_kv_heads * (group == 8 ? 2 : 1)), (unsigned)a.qblocks, (unsigned)batch);
+  dim3 grid((unsigned)(num_kv_heads * (group == 8 ? 2 : 1)), (unsigned)a.qblocks, (unsigned)batch);
+  if (window > 0) {
+    if (total_q == 0) return 0;
+    const int64_t blocks = min((int64_t)a.qblocks * batch, total_q / block_q + batch);
+    grid.y = (unsigned)min(blocks, (int64_t)32768);
+    grid.z = (unsigned)((blocks + 32767) / 32768);
+  }
   switch (group) {
     case 1: launch<1>(a, grid, stream); break;
     case 2: launch<2>(a, grid, stream); break;
@@ -454,7 +506,7 @@ extern "C" int xv_prefill_attention(const void* q, int64_t q_stride_tok, int64_t
                                     int head_dim, int block_size, float scale, hipStream_t stream) {
   return prefill(q, q_stride_tok, q_stride_head, k, v, kv_stride_tok, kv_stride_head, k_cache, v_cache, page_stride,
                  tok_stride, head_stride, block_tables, bt_stride, cu_seqlens_q, cu_seqlens_k, out, out_stride_tok, batch,
-                 max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, 0, 0, scale, stream);
+                 max_seqlen_q, 0, num_q_heads, num_kv_heads, head_dim, block_size, 0, 0, scale, stream);
 }
 
 extern "C" int xv_window_prefill_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
@@ -464,11 +516,11 @@ extern "C" int xv_window_prefill_attention(const void* q, int64_t q_stride_tok, 
                                            const int32_t* block_tables, int64_t bt_stride,
                                            const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                                            void* out, int64_t out_stride_tok,
-                                           int batch, int max_seqlen_q, int num_q_heads, int num_kv_heads,
+                                           int batch, int max_seqlen_q, int64_t total_q, int num_q_heads, int num_kv_heads,
                                            int head_dim, int block_size, int window, int sink_tokens, float scale,
                                            hipStream_t stream) {
   if (window < 1 || sink_tokens < 0 || !(scale > 0.f)) return (int)hipErrorInvalidValue;
   return prefill(q, q_stride_tok, q_stride_head, k, v, kv_stride_tok, kv_stride_head, k_cache, v_cache, page_stride,
                  tok_stride, head_stride, block_tables, bt_stride, cu_seqlens_q, cu_seqlens_k, out, out_stride_tok, batch,
-                 max_seqlen_q, num_q_heads, num_kv_heads, head_dim, block_size, window, sink_tokens, scale, stream);
+                 max_seqlen_q, total_q, num_q_heads, num_kv_heads, head_dim, block_size, window, sink_tokens, scale, stream);
 }

@@ -100,7 +100,7 @@ SIGNATURES: dict[str, tuple] = {
     "xv_window_prefill_attention": (
         i32,
         [vp, i64, i64, vp, vp, i64, i64, vp, vp, i64, i64, i64, vp, i64, vp, vp, vp, i64,
-         i32, i32, i32, i32, i32, i32, i32, i32, f32, vp],
+         i32, i32, i64, i32, i32, i32, i32, i32, i32, f32, vp],
     ),
     "xv_step_maps": (
         i32, [vp, vp, vp, i32, vp, i64, i32, i32, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp]

@@ -593,7 +593,7 @@ def prefill_attention(
         page = 16
     if windowed:
         call("xv_window_prefill_attention", q3.get_device(), ptr(q3), qs0, qs1, ptr(kd), ptr(vd), kvs0, kvs1, ptr(kc), ptr(vc), ps,
-             ts, hs, ptr(bt), bts, ptr(cuq), ptr(cuk), ptr(out), out.stride(0), bsz, int(max_seqlen_q), num_qo_heads,
+             ts, hs, ptr(bt), bts, ptr(cuq), ptr(cuk), ptr(out), out.stride(0), bsz, int(max_seqlen_q), q3.shape[0], num_qo_heads,
              num_kv_heads, head_dim, page, int(window), int(sink_tokens), float(scale))
         return out
     _C.check(
