@@ -165,15 +165,16 @@ XV_INLINE Block block_by_work(const int* cu_q, const int* cu_k, int batch, int f
       ql = cu_q[i + 1] - q0;
       kl = cu_k[i + 1] - k0;
     }
+    // the work to 17 bits, the lane behind it: no two are alike, and one comparison of 32 bits a sequence
     const int64_t w = (int64_t)ql * (kl - ql) + (int64_t)ql * (ql + 1) / 2;
+    const uint32_t key = (__builtin_bit_cast(uint32_t, (float)max((int64_t)0, w)) & ~63u) | (63 - lane);
     const int blocks = max(0, (ql + BQ - 1) / BQ);
     int before = 0, all = 0;  // blocks of the sequences dispatched before this lane's, and of all 64
-    for (int t = 0; t < min(64, batch - c); ++t) {
-      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)w, t);
-      const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)w >> 32), t);
-      const int64_t wt = (int64_t)(((uint64_t)hi << 32) | lo);
+    const int n = min(64, batch - c);
+#pragma unroll 4
+    for (int t = 0; t < n; ++t) {
       const int bt = __builtin_amdgcn_readlane(blocks, t);
-      before += wt > w || (wt == w && t < lane) ? bt : 0;
+      before += (uint32_t)__builtin_amdgcn_readlane((int)key, t) > key ? bt : 0;
       all += bt;
     }
     const uint64_t m = __ballot(flat >= before && flat < before + blocks);
@@ -409,17 +410,34 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
   }
   // ---- normalise and write: lane holds O[my_q][32n + 8j + 4(l/32) + r] ----
   const float lsum = xor32_sum(l_run);
-  if (!active || my_q >= q_len) return;
+  if (!active) return;
   const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
-  bf16_t* op = a.out + (int64_t)(q0 + my_q) * a.out_st + (int64_t)head * kD + 4 * h;
+  // By way of LDS, so that a store instruction takes four whole rows and not a piece of all 32: 8 KB of the K buffers, which
+  // nobody reads from the last iteration's barrier on.  16-byte chunk c of row r is at slot c ^ r % 16.
+  char* const mine = lds + (wave >> 1) * kBuf + (wave & 1) * (kTile / 2);
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint2 w = make_uint2(pack_bf16x2(o[n][4 * j] * inv, o[n][4 * j + 1] * inv),
                                  pack_bf16x2(o[n][4 * j + 2] * inv, o[n][4 * j + 3] * inv));
-      *reinterpret_cast<uint2*>(op + 32 * n + 8 * j) = w;
+      *reinterpret_cast<uint2*>(mine + l32 * 256 + (((4 * n + j) ^ (l32 & 15)) << 4) + 8 * h) = w;
     }
+  __asm__ __volatile__("" ::: "memory");  // a wave's LDS accesses stay in this order
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef u32x4 __attribute__((aligned(8))) u32x4_a8;  // the caller's rows are 8-byte aligned
+  bf16_t* const op = a.out + (int64_t)(q0 + qw0) * a.out_st + (int64_t)head * kD + 8 * (lane & 15);
+  u32x4 rows[8];
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const int r = 4 * s + (lane >> 4);
+    rows[s] = *reinterpret_cast<const u32x4*>(mine + r * 256 + (((lane & 15) ^ (r & 15)) << 4));
+  }
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const int r = 4 * s + (lane >> 4);
+    if (qw0 + r < q_len) *reinterpret_cast<u32x4_a8*>(op + (int64_t)r * a.out_st) = rows[s];
+  }
 }
 
 template <int G>
