@@ -131,3 +131,30 @@ def test_graph_replays(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, body())
+
+
+@pytest.mark.parametrize("block", [0, 16])
+def test_many_sequences(dev, block):
+    """More than 64 and more than 128 sequences, some without queries, one of them long."""
+    new = [600 if i == 133 else (11 * i) % 47 for i in range(150)]
+    lens = [n + (17 * i) % 60 for i, n in enumerate(new)]
+    _case(dev, lens, new, 2, 2, 30, 3, block, seed=9)
+
+
+def test_rows_of_eight_byte_alignment(dev):
+    """The C entry's output rows need only 8 bytes, and what is around them stays."""
+    from xvllm._torch_glue import call
+    from xvllm.layers.attention import prefill_attention
+
+    hq, lens = 2, [90, 37]
+    q, k, v = (torch.randn(sum(lens), hq * D, generator=torch.Generator().manual_seed(s)).to(torch.bfloat16).to(dev) for s in range(3))
+    cu = torch.tensor([0, 90, 127], dtype=torch.int32, device=dev)
+    want = prefill_attention(q, k, v, cu, cu, 90, hq, hq, D, window=20, sink_tokens=1)
+    wide = torch.full((sum(lens) + 1, hq * D + 12), 7.0, dtype=torch.bfloat16, device=dev)
+    out = wide[:-1, 4 : 4 + hq * D]
+    assert out.data_ptr() % 16 == 8
+    call("xv_window_prefill_attention", 0, q.data_ptr(), hq * D, D, k.data_ptr(), v.data_ptr(), hq * D, D, None, None, 0, 0, 0, None, 0,
+         cu.data_ptr(), cu.data_ptr(), out.data_ptr(), out.stride(0), 2, 90, sum(lens), hq, hq, D, 16, 20, 1, D ** -0.5)
+    assert torch.equal(out, want)
+    out.fill_(7.0)
+    assert (wide == 7).all()
