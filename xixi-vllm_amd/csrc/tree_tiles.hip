@@ -14,14 +14,15 @@
 // heads, 317 MB and 37 GFLOP, 104 us (3.0 TB/s, 356 TFLOP/s); 4 of 40 to 90 over
 // up to 90000, 16 / 8 heads, 1013 MB and 128 GFLOP, 232 us (4.4 TB/s, 554
 // TFLOP/s).  Neither stream nor products alone bound it: without the products it
-// takes two thirds of that, without the loads three quarters.  Of 4700 cycles a
-// tile a wave computes 2200 (the 32 products are 1056; the softmax between them
-// waits for one and is waited for by the other), stands 580 at its LDS-DMA (all
-// waves issue theirs behind the barrier), spends 350 on where the next tile is and
-// 800 on the barrier and on data; a segment's start and end take 6500 more.
-// Scores a tile ahead of the softmax, loads issued later or by some of the waves,
-// the halves of a tile on two waves where half of them have no rows: each took
-// from one of these what it gave another, 0 to 10 % slower in all.
+// takes two thirds of that, without the loads three quarters.  Of 3900 to 4700
+// cycles a tile the first wave computes 2200 (the 32 products are 1056; the softmax
+// between them waits for one and is waited for by the other), stands 580 at its
+// LDS-DMA (all waves issue theirs behind the barrier), spends 350 on where the next
+// tile is and 500 to 800 on the barrier and on data; a segment's ends take 6500.
+// Above 128 rows some SIMDs have two waves of rows, and the others wait for them.
+// Scores a tile ahead of the softmax, loads issued later or by four of the waves,
+// two tiles a barrier, halves of a tile or a tile each on two waves where half of
+// them have no rows: 0 to 10 % slower in all.
 //
 // Workgroups of four waves and a ring of two, two a CU, for up to 128 rows:
 // slower on most (32 trees of 32 nodes over 2000 tokens 77 against 63 us, 16 of
