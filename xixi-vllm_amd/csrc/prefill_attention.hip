@@ -30,7 +30,7 @@
 // masked, and a wave passes over those that none of its queries sees.  Bound by the
 // softmax beside the products, as without a window (products busy 52 % of the time,
 // vector work 44 %): one document of 16001 with a window of 4096, 16 / 8 heads, 474
-// GFLOP, 470 to 516 us (up to 1010 TFLOP/s); 16 chunks of up to 512 over up to
+// GFLOP, 487 to 516 us (up to 974 TFLOP/s); 16 chunks of up to 512 over up to
 // 12000 cached tokens, window 2000, 64 / 8 heads, 379 GFLOP, 473 us (801); 12
 // prompts of 40 to 2500, window 512, 32 / 8 heads, 97 GFLOP, 165 us (591: seven
 // tiles a workgroup, a third of whose time is start and end).
