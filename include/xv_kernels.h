@@ -464,7 +464,9 @@ int xv_fused_add_rmsnorm_parts(const float* parts, int64_t part_stride, int64_t 
  * build_cos_sin_cache, src/compute/layers/rotary.py:7-20.
  *   o[:D/2] = x1*cos - x2*sin;  o[D/2:] = x2*cos + x1*sin
  * q element (t, h, d) at t*q_stride_tok + h*q_stride_head + d; k likewise;
- * q_out [T, Hq, D] and k_out [T, Hkv, D] contiguous.  positions int64 [T].
+ * q_out [T, Hq, D] and k_out [T, Hkv, D] contiguous.  positions int64 [T],
+ * each a row of the table (0 .. max_pos - 1: nothing checks it), here and in
+ * the entries below.
  */
 int xv_rotary_embedding(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                         const void* k, int64_t k_stride_tok, int64_t k_stride_head,

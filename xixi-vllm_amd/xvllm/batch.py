@@ -54,10 +54,12 @@ class Batch:
                  device: torch.device, block_size: int, num_blocks: int | None = None,
                  cascade_groups: int = 0, cascade_max_prefix_blocks: int = 0, cascade_min_blocks: int = 16,
                  cascade_max_rows: int = 16, cascade_token_bytes: int = 0,
-                 cascade_min_shared_bytes: int | None = None) -> None:
+                 cascade_min_shared_bytes: int | None = None, max_positions: int | None = None) -> None:
         """`num_blocks`: pages in the KV pool; when given, every page id and
         slot staged for the device is checked against it on the host (a bad
         one raises ValueError instead of reaching a kernel).
+        `max_positions`: rows of the model's rotary table; when given, a
+        position past it raises ValueError too.
         `cascade_groups` > 0: decode builds also stage the batch's
         shared-prefix groups (at most that many, of at most cascade_max_rows
         rows, prefixes of cascade_min_blocks .. cascade_max_prefix_blocks
@@ -65,7 +67,7 @@ class Batch:
         cascade_min_shared_bytes of KV per layer (prefix tokens x
         cascade_token_bytes; default prefix_cache.CASCADE_MIN_SHARED_BYTES);
         otherwise the build stages no groups and cascade_rows is 0."""
-        self.num_blocks = num_blocks
+        self.num_blocks, self.max_positions = num_blocks, max_positions
         self.max_bs, self.max_tokens, self.max_blocks = max_bs, max_tokens, max_blocks
         self.vocab_size, self.device, self.block_size = vocab_size, device, block_size
         gpu = lambda shape, dt, fill=0: torch.full(shape, fill, dtype=dt, device=device)
@@ -219,6 +221,8 @@ class Batch:
             raise ValueError(f"sequence {seqs[i].seq_id}: position {int(pos[i])} has no page in its block table")
         if ((ids < 0) | (ids >= self.vocab_size)).any():
             raise ValueError(f"decode input id outside [0, {self.vocab_size})")
+        if self.max_positions is not None and (pos >= self.max_positions).any():
+            raise ValueError(f"position {int(pos.max())} is past the {self.max_positions} that the model's rotary table holds")
         rows = np.arange(n)
         slot = self._bt_np[rows, pos // self.block_size].astype(np.int64) * self.block_size + pos % self.block_size
         self._h_ids.numpy()[:n] = ids
@@ -284,6 +288,9 @@ class Batch:
             pos[nt : nt + n] = np.arange(start, end)
             if (end + self.block_size - 1) // self.block_size > len(s.block_table):
                 raise ValueError(f"sequence {s.seq_id}: positions up to {end} need more pages than its block table")
+            if self.max_positions is not None and end > self.max_positions:
+                raise ValueError(f"sequence {s.seq_id}: position {end - 1} is past the {self.max_positions} that the model's "
+                                 "rotary table holds")
             slot[nt : nt + n] = slots_for_range(s.block_table, start, end, self.block_size)
             self._check_pages(s.seq_id, np.asarray(s.block_table[: (end + self.block_size - 1) // self.block_size]))
             cuq[i + 1], cuk[i + 1] = cuq[i] + n, cuk[i] + end

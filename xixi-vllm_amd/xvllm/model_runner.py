@@ -22,6 +22,7 @@ from .cuda_graph import HipGraphRunner
 from .kv_ops import FP4_PAGES
 from .kv_pool import KVPool
 from .layers.attention import Attention, AttnInputs, AttnMetadata, attention_context
+from .layers.rotary import RotaryEmbedding
 from .sampler import Sampler, reserve_workspace, sample
 
 
@@ -45,6 +46,15 @@ def sample_mode(batch: Batch) -> int:
     if batch.use_min_p:
         f |= _C.XV_SAMPLE_USE_MIN_P
     return f
+
+
+def reserve_positions(model, positions: int) -> int | None:
+    """Make every rotary table of `model` hold `positions` positions; how many
+    all of them hold then, None for a model without such tables."""
+    tables = [m for m in model.modules() if isinstance(m, RotaryEmbedding)] if hasattr(model, "modules") else []
+    for m in tables:
+        m.reserve(positions)
+    return min((m.cos_sin_cache.shape[0] for m in tables), default=None)
 
 
 class ModelRunner:
@@ -108,7 +118,9 @@ class ModelRunner:
                            cascade_max_prefix_blocks=cascade_max_prefix_blocks, cascade_min_blocks=cascade_min_blocks,
                            cascade_max_rows=max(1, 128 // (cfg.num_attention_heads // cfg.num_key_value_heads)),
                            cascade_token_bytes=cfg.num_key_value_heads * _head_dim(cfg) * 2 * kv.dtype.itemsize,
-                           cascade_min_shared_bytes=cascade_min_shared_bytes)
+                           cascade_min_shared_bytes=cascade_min_shared_bytes,
+                           # every position that a block table's row has room for, also past max_position_embeddings
+                           max_positions=reserve_positions(model, max_blocks * self.block_size))
         self.vocab_size = cfg.vocab_size
         act_dtype = torch.bfloat16 if kv.dtype in (torch.float8_e4m3fn, FP4_PAGES) else kv.dtype  # activations stay bf16
         self._decode_out = torch.zeros(self.max_bs, self.hidden_size, dtype=act_dtype, device=self.device)
