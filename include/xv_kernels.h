@@ -174,6 +174,15 @@ int xv_gather_kv_fp8(const void* k_cache, const void* v_cache, int64_t cache_pag
                      int64_t bt_stride, int block_size, const int32_t* cu_seqlens_k, int batch,
                      int max_seqlen_k, int num_kv_heads, int head_dim, float k_scale, float v_scale,
                      void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream);
+/* The same for xv_window_prefill_attention: the rows of keys that no query of
+ * sequence b (its last cu_seqlens_q[b + 1] - cu_seqlens_q[b] tokens) sees are
+ * left as they are, and block-table entries of such keys alone are not read. */
+int xv_window_gather_kv_fp8(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
+                            int64_t cache_tok_stride, int64_t cache_head_stride, const int32_t* block_tables,
+                            int64_t bt_stride, int block_size, const int32_t* cu_seqlens_q,
+                            const int32_t* cu_seqlens_k, int batch, int max_seqlen_k, int num_kv_heads, int head_dim,
+                            int window, int sink_tokens, float k_scale, float v_scale, void* k_out, void* v_out,
+                            int64_t out_stride_tok, hipStream_t stream);
 
 /*
  * KV store into a 4-bit cache (OCP MXFP4).  No counterpart in the reference,
@@ -215,6 +224,14 @@ int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_pag
                      const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
                      const int32_t* cu_seqlens_k, int batch, int64_t total_tokens, int num_kv_heads, int head_dim,
                      void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream);
+/* The same for xv_window_prefill_attention, as xv_window_gather_kv_fp8. */
+int xv_window_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
+                            int64_t cache_tok_stride, int64_t cache_head_stride, const void* k_scale,
+                            const void* v_scale, int64_t scale_page_stride, int64_t scale_tok_stride,
+                            int64_t scale_head_stride, int block_size, const int32_t* block_tables, int64_t bt_stride,
+                            int max_blocks_per_seq, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch,
+                            int64_t total_tokens, int num_kv_heads, int head_dim, int window, int sink_tokens,
+                            void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream);
 
 /*
  * xv_paged_decode_attention over a 4-bit (MXFP4) cache written by

@@ -217,17 +217,22 @@ extern "C" int xv_store_kvcache_fp8(const void* key, int64_t key_stride_tok, int
 // Chunked prefill over fp8 pages: every sequence's keys (cached prefix and
 // this chunk, already stored) dequantized into bf16 rows at cu_seqlens_k[b]
 // + t, the varlen k/v layout xv_prefill_attention reads: bf16(value * scale).
-// One thread per 8-value piece of one (token, kv head).
+// One thread per 8-value piece of one (token, kv head).  WIN: the rows of keys
+// that no query sees (of a prefill with a window and sinks, and cu_q its
+// queries) stay as they are, and their block-table entries are not read.
+template <bool WIN>
 __global__ __launch_bounds__(256) void gather_kv_fp8_kernel(
     const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, int64_t ps, int64_t ts, int64_t hs,
     const int32_t* __restrict__ bt, int64_t bt_stride, int block_size, const int32_t* __restrict__ cu_k, int hkv,
-    float k_scale, float v_scale, bf16_t* __restrict__ ko, bf16_t* __restrict__ vo, int64_t o_st) {
+    float k_scale, float v_scale, bf16_t* __restrict__ ko, bf16_t* __restrict__ vo, int64_t o_st,
+    const int32_t* __restrict__ cu_q, int window, int sinks) {
   const int b = blockIdx.y;
   const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per_tok = hkv * 16;  // 8-value pieces of a token (D = 128)
   const int t = (int)(idx / per_tok);
   const int k0 = cu_k[b];
   if (t >= cu_k[b + 1] - k0) return;
+  if (WIN && window_hides(t, cu_k[b + 1] - k0, cu_q[b + 1] - cu_q[b], window, sinks)) return;
   const int rem = (int)(idx - (int64_t)t * per_tok), h = rem >> 4, c = rem & 15;
   const int64_t blk = bt[(int64_t)b * bt_stride + t / block_size];
   const int64_t src = blk * ps + (int64_t)(t % block_size) * ts + (int64_t)h * hs + c * 8;
@@ -249,11 +254,12 @@ __global__ __launch_bounds__(256) void gather_kv_fp8_kernel(
   store_vec8(vo + dst, dq(vq, v_scale));
 }
 
-extern "C" int xv_gather_kv_fp8(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
-                                int64_t cache_tok_stride, int64_t cache_head_stride, const int32_t* block_tables,
-                                int64_t bt_stride, int block_size, const int32_t* cu_seqlens_k, int batch,
-                                int max_seqlen_k, int num_kv_heads, int head_dim, float k_scale, float v_scale,
-                                void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream) {
+// window 0: all keys (cu_seqlens_q is not looked at)
+static int gather_kv_fp8(const void* k_cache, const void* v_cache, int64_t cache_page_stride, int64_t cache_tok_stride,
+                         int64_t cache_head_stride, const int32_t* block_tables, int64_t bt_stride, int block_size,
+                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch, int max_seqlen_k,
+                         int num_kv_heads, int head_dim, int window, int sink_tokens, float k_scale, float v_scale,
+                         void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream) {
   if (head_dim != 128 || batch < 0 || max_seqlen_k < 0 || num_kv_heads <= 0 || block_size <= 0 ||
       batch > 65535 || !(k_scale > 0.0f) || !(v_scale > 0.0f))
     return (int)hipErrorInvalidValue;
@@ -263,12 +269,35 @@ extern "C" int xv_gather_kv_fp8(const void* k_cache, const void* v_cache, int64_
   if (batch == 0 || max_seqlen_k == 0) return 0;
   const int64_t pieces = (int64_t)max_seqlen_k * num_kv_heads * 16;
   if ((pieces + 255) / 256 > 0x7fffffff) return (int)hipErrorInvalidValue;
-  gather_kv_fp8_kernel<<<dim3((unsigned)((pieces + 255) / 256), (unsigned)batch), 256, 0, stream>>>(
+  (window > 0 ? gather_kv_fp8_kernel<true> : gather_kv_fp8_kernel<false>)<<<
+      dim3((unsigned)((pieces + 255) / 256), (unsigned)batch), 256, 0, stream>>>(
       (const uint8_t*)k_cache, (const uint8_t*)v_cache, cache_page_stride, cache_tok_stride, cache_head_stride,
       block_tables, bt_stride, block_size, cu_seqlens_k, num_kv_heads, k_scale, v_scale, (bf16_t*)k_out,
-      (bf16_t*)v_out, out_stride_tok);
+      (bf16_t*)v_out, out_stride_tok, cu_seqlens_q, window, sink_tokens);
   XV_CHECK_LAUNCH();
   return 0;
+}
+
+extern "C" int xv_gather_kv_fp8(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
+                                int64_t cache_tok_stride, int64_t cache_head_stride, const int32_t* block_tables,
+                                int64_t bt_stride, int block_size, const int32_t* cu_seqlens_k, int batch,
+                                int max_seqlen_k, int num_kv_heads, int head_dim, float k_scale, float v_scale,
+                                void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream) {
+  return gather_kv_fp8(k_cache, v_cache, cache_page_stride, cache_tok_stride, cache_head_stride, block_tables, bt_stride,
+                       block_size, nullptr, cu_seqlens_k, batch, max_seqlen_k, num_kv_heads, head_dim, 0, 0, k_scale, v_scale,
+                       k_out, v_out, out_stride_tok, stream);
+}
+
+extern "C" int xv_window_gather_kv_fp8(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
+                                       int64_t cache_tok_stride, int64_t cache_head_stride, const int32_t* block_tables,
+                                       int64_t bt_stride, int block_size, const int32_t* cu_seqlens_q,
+                                       const int32_t* cu_seqlens_k, int batch, int max_seqlen_k, int num_kv_heads,
+                                       int head_dim, int window, int sink_tokens, float k_scale, float v_scale,
+                                       void* k_out, void* v_out, int64_t out_stride_tok, hipStream_t stream) {
+  if (window < 1 || sink_tokens < 0 || (!cu_seqlens_q && batch > 0)) return (int)hipErrorInvalidValue;
+  return gather_kv_fp8(k_cache, v_cache, cache_page_stride, cache_tok_stride, cache_head_stride, block_tables, bt_stride,
+                       block_size, cu_seqlens_q, cu_seqlens_k, batch, max_seqlen_k, num_kv_heads, head_dim, window,
+                       sink_tokens, k_scale, v_scale, k_out, v_out, out_stride_tok, stream);
 }
 
 // --------------------------------------------------------------------------

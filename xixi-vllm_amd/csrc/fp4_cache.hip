@@ -94,7 +94,8 @@ extern "C" int xv_store_kvcache_fp4(const void* key, int64_t key_stride_tok, int
 // sequence by bisection, the block id), then 16 lanes widen a head row of 128
 // values, 8 of K and of V each (4 bytes in, 16 out), the heads' loads in
 // flight together.  Rows past the last sequence (or of blocks past the table's
-// width) are left as they are.
+// width) are left as they are; WIN: those of keys that no query sees (of a prefill
+// with a window and sinks, and cu_q its queries) too, their block ids not read.
 // Bound by the rows it writes: 16 sequences of 1229 tokens on average, 8 heads
 // (81 MB out), with the store of their last 512 before it 28.8 us, of which this
 // about 19; three of 20000 to 35000 (306 MB out) 79 us, 6.1 TB/s, in a replayed
@@ -108,11 +109,11 @@ extern "C" int xv_store_kvcache_fp4(const void* key, int64_t key_stride_tok, int
 // 104, though with its prefill 2594 against 2575).
 constexpr int kGatherHeads = 2;
 constexpr int64_t kCached = 256ll << 20;
-template <bool NT>
+template <bool NT, bool WIN>
 __global__ __launch_bounds__(256) void gather_kv_fp4_kernel(
     Fp4Cache cd, const int32_t* __restrict__ bt, int64_t bt_stride, int max_blocks, const int32_t* __restrict__ cu,
     int batch, int total_rows, int heads, int chunks_per_head, bf16_t* __restrict__ ko, bf16_t* __restrict__ vo,
-    int64_t o_st) {
+    int64_t o_st, const int32_t* __restrict__ cu_q, int window, int sinks) {
   __shared__ int64_t src[kTokens], ssrc[kTokens];  // a row's codes and scales in the cache, -1: not written
   const int row0 = blockIdx.x * kTokens, h0 = blockIdx.y * kGatherHeads;
   if (threadIdx.x < kTokens) {
@@ -126,7 +127,8 @@ __global__ __launch_bounds__(256) void gather_kv_fp4_kernel(
       }
       const int t = row - cu[lo];
       const int blk = t / cd.block_size;
-      if (t >= 0 && blk < max_blocks) {
+      const bool hidden = WIN && window_hides(t, cu[lo + 1] - cu[lo], cu_q[lo + 1] - cu_q[lo], window, sinks);
+      if (t >= 0 && blk < max_blocks && !hidden) {
         const int64_t page = bt[(int64_t)lo * bt_stride + blk];
         const int r = t - blk * cd.block_size;
         at = page * cd.ps + (int64_t)r * cd.ts;
@@ -169,16 +171,13 @@ __global__ __launch_bounds__(256) void gather_kv_fp4_kernel(
   }
 }
 
-extern "C" int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
-                                int64_t cache_tok_stride, int64_t cache_head_stride, const void* k_scale,
-                                const void* v_scale, int64_t scale_page_stride, int64_t scale_tok_stride,
-                                int64_t scale_head_stride, int block_size, const int32_t* block_tables,
-                                int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_k, int batch,
-                                int64_t total_tokens, int num_kv_heads, int head_dim, void* k_out, void* v_out,
-                                int64_t out_stride_tok, hipStream_t stream) {
-  const Fp4Cache cd = {(uint8_t*)k_cache, (uint8_t*)v_cache, cache_page_stride, cache_tok_stride, cache_head_stride,
-                       (uint8_t*)k_scale, (uint8_t*)v_scale, scale_page_stride, scale_tok_stride, scale_head_stride,
-                       block_size};
+namespace {
+
+// window 0: all keys (cu_seqlens_q is not looked at)
+int gather_kv_fp4(const Fp4Cache& cd, const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                  const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int batch, int64_t total_tokens,
+                  int num_kv_heads, int head_dim, int window, int sink_tokens, void* k_out, void* v_out,
+                  int64_t out_stride_tok, hipStream_t stream) {
   if (batch < 0 || total_tokens < 0 || total_tokens > INT32_MAX || num_kv_heads <= 0 || head_dim <= 0 ||
       head_dim % kFp4Block || max_blocks_per_seq < 0 || !cache_ok(cd))
     return (int)hipErrorInvalidValue;
@@ -189,9 +188,43 @@ extern "C" int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_
   if (num_kv_heads > 65535 * kGatherHeads || (int64_t)num_kv_heads * head_dim > INT32_MAX) return (int)hipErrorInvalidValue;
   const dim3 grid((unsigned)((total_tokens + kTokens - 1) / kTokens), (unsigned)((num_kv_heads + kGatherHeads - 1) / kGatherHeads));
   const bool large = total_tokens * num_kv_heads * head_dim * 4 > kCached;
-  (large ? gather_kv_fp4_kernel<true> : gather_kv_fp4_kernel<false>)<<<grid, 256, 0, stream>>>(
-      cd, block_tables, bt_stride, max_blocks_per_seq, cu_seqlens_k, batch, (int)total_tokens, num_kv_heads, head_dim / 8,
-      (bf16_t*)k_out, (bf16_t*)v_out, out_stride_tok);
+  const auto kernel = window > 0 ? (large ? gather_kv_fp4_kernel<true, true> : gather_kv_fp4_kernel<false, true>)
+                                 : (large ? gather_kv_fp4_kernel<true, false> : gather_kv_fp4_kernel<false, false>);
+  kernel<<<grid, 256, 0, stream>>>(cd, block_tables, bt_stride, max_blocks_per_seq, cu_seqlens_k, batch, (int)total_tokens,
+                                   num_kv_heads, head_dim / 8, (bf16_t*)k_out, (bf16_t*)v_out, out_stride_tok, cu_seqlens_q,
+                                   window, sink_tokens);
   XV_CHECK_LAUNCH();
   return 0;
+}
+
+}  // namespace
+
+extern "C" int xv_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
+                                int64_t cache_tok_stride, int64_t cache_head_stride, const void* k_scale,
+                                const void* v_scale, int64_t scale_page_stride, int64_t scale_tok_stride,
+                                int64_t scale_head_stride, int block_size, const int32_t* block_tables,
+                                int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_k, int batch,
+                                int64_t total_tokens, int num_kv_heads, int head_dim, void* k_out, void* v_out,
+                                int64_t out_stride_tok, hipStream_t stream) {
+  const Fp4Cache cd = {(uint8_t*)k_cache, (uint8_t*)v_cache, cache_page_stride, cache_tok_stride, cache_head_stride,
+                       (uint8_t*)k_scale, (uint8_t*)v_scale, scale_page_stride, scale_tok_stride, scale_head_stride,
+                       block_size};
+  return gather_kv_fp4(cd, block_tables, bt_stride, max_blocks_per_seq, nullptr, cu_seqlens_k, batch, total_tokens,
+                       num_kv_heads, head_dim, 0, 0, k_out, v_out, out_stride_tok, stream);
+}
+
+extern "C" int xv_window_gather_kv_fp4(const void* k_cache, const void* v_cache, int64_t cache_page_stride,
+                                       int64_t cache_tok_stride, int64_t cache_head_stride, const void* k_scale,
+                                       const void* v_scale, int64_t scale_page_stride, int64_t scale_tok_stride,
+                                       int64_t scale_head_stride, int block_size, const int32_t* block_tables,
+                                       int64_t bt_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_q,
+                                       const int32_t* cu_seqlens_k, int batch, int64_t total_tokens, int num_kv_heads,
+                                       int head_dim, int window, int sink_tokens, void* k_out, void* v_out,
+                                       int64_t out_stride_tok, hipStream_t stream) {
+  if (window < 1 || sink_tokens < 0 || (!cu_seqlens_q && batch > 0)) return (int)hipErrorInvalidValue;
+  const Fp4Cache cd = {(uint8_t*)k_cache, (uint8_t*)v_cache, cache_page_stride, cache_tok_stride, cache_head_stride,
+                       (uint8_t*)k_scale, (uint8_t*)v_scale, scale_page_stride, scale_tok_stride, scale_head_stride,
+                       block_size};
+  return gather_kv_fp4(cd, block_tables, bt_stride, max_blocks_per_seq, cu_seqlens_q, cu_seqlens_k, batch, total_tokens,
+                       num_kv_heads, head_dim, window, sink_tokens, k_out, v_out, out_stride_tok, stream);
 }

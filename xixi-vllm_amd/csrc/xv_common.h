@@ -125,4 +125,10 @@ XV_INLINE float row_bcast(float x) {
 XV_INLINE float wave_sum(float x) { return xor32_sum(xor16_sum(row16_sum(x))); }
 XV_INLINE float wave_max(float x) { return xor32_max(xor16_max(row16_max(x))); }
 
+// Whether no query of a windowed prefill sees key t of its k_len keys: the first of its q_len queries (the last tokens)
+// sees those from k_len - q_len + 1 - window on and the sinks, later ones nothing before that.
+XV_INLINE bool window_hides(int t, int k_len, int q_len, int window, int sinks) {
+  return q_len <= 0 || (t >= sinks && t <= (int64_t)k_len - q_len - window);
+}
+
 #define XV_CHECK_LAUNCH() do { hipError_t e_ = hipGetLastError(); if (e_ != hipSuccess) return (int)e_; } while (0)

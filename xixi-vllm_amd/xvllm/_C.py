@@ -74,11 +74,17 @@ SIGNATURES: dict[str, tuple] = {
     "xv_gather_kv_fp8": (
         i32, [vp, vp, i64, i64, i64, vp, i64, i32, vp, i32, i32, i32, i32, f32, f32, vp, vp, i64, vp]
     ),
+    "xv_window_gather_kv_fp8": (
+        i32, [vp, vp, i64, i64, i64, vp, i64, i32, vp, vp, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp, i64, vp]
+    ),
     "xv_store_kvcache_fp4": (
         i32, [vp, i64, i64, vp, i64, i64, vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i32, vp, i64, i32, i32, vp]
     ),
     "xv_gather_kv_fp4": (
         i32, [vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i32, vp, i64, i32, vp, i32, i64, i32, i32, vp, vp, i64, vp]
+    ),
+    "xv_window_gather_kv_fp4": (
+        i32, [vp, vp, i64, i64, i64, vp, vp, i64, i64, i64, i32, vp, i64, i32, vp, vp, i32, i64, i32, i32, i32, i32, vp, vp, i64, vp]
     ),
     "xv_paged_decode_fp4_workspace_size": (sz, [i32, i32, i32]),
     "xv_paged_decode_attention_fp4": (

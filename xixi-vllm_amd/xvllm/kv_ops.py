@@ -162,6 +162,9 @@ def gather_kvcache(
     k_block_scale: torch.Tensor,
     v_block_scale: torch.Tensor,
     out: tuple[torch.Tensor, torch.Tensor] | None = None,
+    cu_seqlens_q: torch.Tensor | None = None,
+    window: int = 0,
+    sink_tokens: int = 0,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values of whole sequences out of 4-bit pages: rows
     cu_seqlens_k[b] .. cu_seqlens_k[b+1] of the two bf16 [total_tokens, Hkv, D]
@@ -172,7 +175,12 @@ def gather_kvcache(
     The cache as store_kvcache writes it, [NB, BS, Hkv, D/2] with its scales;
     block_tables int32 [B, max_blocks]; total_tokens = cu_seqlens_k[B], as the
     host knows it.  Rows from cu_seqlens_k[B] on are left as they were (out:
-    the two outputs to write into, of total_tokens rows)."""
+    the two outputs to write into, of total_tokens rows).
+
+    window > 0: for prefill_attention with this window and sink_tokens, whose
+    queries are sequence b's last cu_seqlens_q[b+1] - cu_seqlens_q[b] tokens:
+    rows of keys that none of them sees are left as they were, and block-table
+    entries that hold only such keys are not read."""
     require_cuda(k_cache, v_cache, block_tables, cu_seqlens_k)
     if k_cache.dtype != FP4_PAGES:
         raise TypeError(f"gather_kvcache reads 4-bit pages ({FP4_PAGES}), got {k_cache.dtype}")
@@ -188,6 +196,14 @@ def gather_kvcache(
                          "are not [B + 1] and [B, max_blocks]")
     if total_tokens < 0:
         raise ValueError("total_tokens must not be negative")
+    if window or sink_tokens or cu_seqlens_q is not None:
+        if not 1 <= window < 1 << 31 or not 0 <= sink_tokens < 1 << 31:
+            raise ValueError(f"window {window}, sink_tokens {sink_tokens}: a window is at least 1, sinks and cu_seqlens_q go with "
+                             "one, sinks are not negative, both below 2^31")
+        if cu_seqlens_q is None or cu_seqlens_q.shape != cu_seqlens_k.shape:
+            raise ValueError("a windowed read back needs cu_seqlens_q, as long as cu_seqlens_k")
+        if cu_seqlens_q.get_device() != dev:
+            raise RuntimeError("cu_seqlens_q must be on the cache's device")
     if out is None:
         ko, vo = torch.empty((2, total_tokens, hkv, d), dtype=torch.bfloat16, device=k_cache.device).unbind(0)
         row = hkv * d
@@ -205,6 +221,11 @@ def gather_kvcache(
     if bt.stride(-1) != 1:
         bt = bt.contiguous()
     cu = as_int32(cu_seqlens_k).contiguous()
+    if window:
+        cuq = as_int32(cu_seqlens_q).contiguous()
+        call("xv_window_gather_kv_fp4", dev, *codes, *scales, bs, ptr(bt), bt.stride(0), bt.shape[1], ptr(cuq), ptr(cu), bsz,
+             int(total_tokens), hkv, d, int(window), int(sink_tokens), ptr(ko), ptr(vo), row)
+        return ko, vo
     call("xv_gather_kv_fp4", dev, *codes, *scales, bs, ptr(bt), bt.stride(0), bt.shape[1], ptr(cu), bsz,
          int(total_tokens), hkv, d, ptr(ko), ptr(vo), row)
     return ko, vo

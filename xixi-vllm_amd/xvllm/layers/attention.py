@@ -520,7 +520,7 @@ def prefill_attention(
 
     window > 0: a query sees the last `window` keys up to itself and the
     sequence's first sink_tokens (softmax_scale > 0); block-table entries that
-    hold no key some query sees are not read from bf16 pages."""
+    hold no key some query sees are not read."""
     windowed = _windowed(window, sink_tokens)
     if windowed and softmax_scale is not None and not softmax_scale > 0:
         raise ValueError(f"a windowed prefill needs softmax_scale > 0, got {softmax_scale}")
@@ -541,8 +541,9 @@ def prefill_attention(
             raise ValueError(f"total_seqlen_k {total_seqlen_k} is not the keys of {bsz} sequences of up to {max_seqlen_k}")
         if k_cache.dim() != 4 or k_cache.shape[2] != num_kv_heads or k_cache.shape[3] * 2 != head_dim:
             raise ValueError(f"cache {tuple(k_cache.shape)} is not 4-bit pages [NB, BS, {num_kv_heads}, {head_dim} / 2]")
+        seen = dict(cu_seqlens_q=cuq, window=window, sink_tokens=sink_tokens) if windowed else {}
         kd, vd = gather_kvcache(k_cache, v_cache, block_tables, cuk, int(total_seqlen_k) or bsz * int(max_seqlen_k),
-                                k_block_scale=k_block_scale, v_block_scale=v_block_scale)
+                                k_block_scale=k_block_scale, v_block_scale=v_block_scale, **seen)
         return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
                                  head_dim, softmax_scale=softmax_scale, window=window, sink_tokens=sink_tokens)
     if block_tables is not None and k_cache is not None and k_cache.dtype == torch.float8_e4m3fn:
@@ -557,14 +558,15 @@ def prefill_attention(
         rows = bsz * int(max_seqlen_k)
         kd = torch.empty((max(rows, 1), hkv, head_dim), dtype=torch.bfloat16, device=q.device)
         vd = torch.empty_like(kd)
-        _C.check(
-            _C.lib().xv_gather_kv_fp8(
-                ptr(k_cache), ptr(v_cache), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), ptr(bt),
-                bt.stride(0), k_cache.shape[1], ptr(cuk), bsz, int(max_seqlen_k), hkv, head_dim, float(k_scale),
-                float(v_scale), ptr(kd), ptr(vd), kd.stride(0), stream_of(q),
-            ),
-            "xv_gather_kv_fp8",
-        )
+        pages = (ptr(k_cache), ptr(v_cache), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), ptr(bt), bt.stride(0),
+                 k_cache.shape[1])
+        rows_out = (float(k_scale), float(v_scale), ptr(kd), ptr(vd), kd.stride(0))
+        if windowed:
+            call("xv_window_gather_kv_fp8", q3.get_device(), *pages, ptr(cuq), ptr(cuk), bsz, int(max_seqlen_k), hkv, head_dim,
+                 int(window), int(sink_tokens), *rows_out)
+        else:
+            _C.check(_C.lib().xv_gather_kv_fp8(*pages, ptr(cuk), bsz, int(max_seqlen_k), hkv, head_dim, *rows_out,
+                                               stream_of(q)), "xv_gather_kv_fp8")
         return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
                                  head_dim, softmax_scale=softmax_scale, window=window, sink_tokens=sink_tokens)
     if block_tables is not None:
