@@ -200,6 +200,11 @@ def _windowed(window: int, sink_tokens: int) -> bool:
     return True
 
 
+def _hides(window: int, block_tables: torch.Tensor | None, k_cache: torch.Tensor) -> bool:
+    """Whether a window (0: none) may hide a token: one as long as all that a table row has room for hides none."""
+    return window > 0 and (block_tables is None or window < block_tables.shape[-1] * k_cache.shape[1])
+
+
 def _paged_rows(q, k_cache, v_cache, block_tables, cache_seqlens, hq, hkv, d, bsz, out, what):
     """Operands of the attention kernels that take bf16 pages and a workspace
     per call: the C ABI's q, cache, table and length arguments, the output and
@@ -367,13 +372,14 @@ def paged_decode_attention(
     (torch.float4_e2m1fn_x2 [NB, BS, Hkv, D/2]) to its codes times the block
     scales k_block_scale / v_block_scale [NB, BS, Hkv, D/32].
 
-    window > 0 (bf16 caches): the query sees the last `window` tokens of its
-    sequence, itself among them, and the first sink_tokens; block-table entries
-    that hold none of these are not read.
+    window > 0: the query sees the last `window` tokens of its sequence, itself
+    among them, and the first sink_tokens; block-table entries that hold none of
+    these are not read.  Caches are bf16, unless the window is as long as all
+    that the table has room for and so hides nothing.
 
     The 4-bit and the windowed form take a workspace of their own per call; the
     others share one per device (decode_workspace)."""
-    if _windowed(window, sink_tokens):
+    if _windowed(window, sink_tokens) and (k_cache.dtype == torch.bfloat16 or _hides(window, block_tables, k_cache)):
         return _window_decode(q, k_cache, v_cache, block_tables, cache_seqlens, num_qo_heads, num_kv_heads, head_dim,
                               softmax_scale, out, window, sink_tokens)
     if k_cache.dtype == FP4_PAGES:
@@ -687,9 +693,9 @@ class Attention(nn.Module):
             raise ValueError("a prefill step takes no tree plan")
         if not attn.is_prefill and (attn.cascade is not None or attn.tree is not None):
             # shared-prefix decode, or trees of drafted tokens: the plan does not fit the vllm::attention schema
-            if self.window or (attn.cascade is not None and attn.tree is not None):
-                raise ValueError("a sliding window, a shared-prefix plan and a tree plan exclude each other")
             k_cache, v_cache = _layer_caches(self.layer_id)
+            if _hides(self.window, attn.block_tables, k_cache) or (attn.cascade is not None and attn.tree is not None):
+                raise ValueError("a sliding window, a shared-prefix plan and a tree plan exclude each other")
             if attn.tree is None:
                 _refuse_cascade(k_cache)
             scales = _layer_scales(self.layer_id)

@@ -88,8 +88,10 @@ class ModelRunner:
         read them), and every runner of the model then uses them."""
         if cascade_groups > 0 and kv.dtype == FP4_PAGES:
             raise ValueError("no cascade decode over a 4-bit KV pool: cascade_groups must be 0")
-        windowed = [m for m in model.modules() if isinstance(m, Attention) and m.window] if hasattr(model, "modules") else []
-        if windowed:
+        # a window as long as all that a block table's row has room for hides nothing
+        bs = getattr(kv, "block_size", 1)
+        reach = (context_len + bs - 1) // bs * bs
+        if hasattr(model, "modules") and any(isinstance(m, Attention) and 0 < m.window < reach for m in model.modules()):
             if cascade_groups > 0:
                 raise ValueError("no cascade decode with a sliding window: cascade_groups must be 0")
             if kv.dtype in (torch.float8_e4m3fn, FP4_PAGES):
