@@ -3,7 +3,7 @@
 // tokens (one row per node and query head).
 //
 //   out[r] = sum_t softmax_t(scale * q[r] . K[t]) V[t] over the tokens t row r sees
-//   window: row at position p = ctx - 1 sees t > p - window and t < sinks
+//   window: row at position p = ctx - 1 sees t > p - window, and t < sinks
 //   tree:   node i of n, token ctx - n + i, sees t < ctx - n and the nodes of its mask
 //
 // Work split: a sequence's visible 16-token pages in order (the sinks' pages,
@@ -11,8 +11,8 @@
 // unit) space is flattened in that order and cut into equal contiguous ranges;
 // a range cut inside a segment leaves partials (normalised fp32 rows and their
 // log2-sum-exp) for a merge kernel, two partial slots per range at most.
-// A wave takes NT tiles of 16 rows, 1 or 2; sequences of more rows (large
-// trees) are the matter of tree_tiles.hip.
+// A wave takes NT tiles of 16 rows, 1 or 2; trees of more rows, and few ones of
+// more than 16, are the matter of tree_tiles.hip.
 //
 // A unit (32 tokens), all on v_mfma_f32_16x16x32_bf16:
 //   K and V rows go HBM -> LDS by LDS-DMA, two units in flight per wave.
@@ -579,26 +579,36 @@ int rows_groups() {
   return cached;
 }
 
-// Calls of up to 32 rows per sequence and kv head (query heads per kv head times
-// the nodes of the largest tree) run here, a wave on its own; larger trees share
-// their tiles among the waves of a workgroup (tree_tiles.hip), of which up to 32
-// rows would keep one busy.  Trees of 32 rows here and there: 256 of 700 tokens
-// 134 and 174 us, 32 of 4000 108 and 106, 4 of 60000 178 and 180, 1 of 4000 25.6
-// and 20.6.  Up to 16 rows one tile of rows does.
+// Trees of up to 16 rows per sequence and kv head (nodes times query heads per kv head) run here, a wave on its own; those
+// of more than 32 share their tiles among the waves of a workgroup (tree_tiles.hip).  Between the two it goes by the
+// (sequence, kv head) segments: no more than the workgroups there, and a segment is cut into more ranges here, which
+// the merge then joins.  Captured calls of 32 rows, 8 kv heads (here, there, us):
+//   sequences        1           4           32          64          128         256
+//   300 tokens     9.6, 10.6  12.5, 11.6   28.4, 18.1  30.3, 27.5  36.8, 45.4   73, 92
+//   1000          11.4, 11.1  21.7, 13.7   36.7, 31.8  57.7, 55.2    91, 113   186, 222
+//   4000          24.6, 15.4  30.9, 24.9  103.2, 100.3  177, 192
+//   16000         32.5, 25.0  59.6, 55.4
+//   60000         59.3, 52.8   175, 194
+// So up to 32 sequences of 8 kv heads go there (20 rows: as these).  What that costs is 5 to 11 % where they hold more than
+// 100000 tokens together: the host knows the tables' width, not their lengths.
 constexpr int kWaveRows = 32;
+bool by_tiles(int batch, int hkv, int max_rows) {
+  return max_rows > kWaveRows || (max_rows > 16 && (int64_t)batch * hkv <= kTileGroups);
+}
 // Rows of a tree call from which on the merge takes four rows a wave: enough waves then without spreading a row's partials.
-// Four and one a wave, the whole call: 256 rows in many partials 46 and 26 us, 8192 rows 47.5 and 46.5 (1 us less for four
-// where the contexts are long), 16384 rows 57 and 61, 65536 rows 96 and 103.
+// Four and one a wave, the whole call, captured: 2048 rows 37.9 and 34.8 us, 17.6 and 16.7; 4096 44.4 and 44.0, 25.5 and
+// 25.8; 8192 35.8 and 37.6, 102.4 and 104.2 (60.8 and 59.3 in the one case that is the other way); 16384 48.0 and 49.4;
+// 65536 34.2 and 41.0.
 constexpr int kManyRows = 8192;
-int slot_rows(int max_rows) { return max_rows <= 16 ? 16 : max_rows <= kWaveRows ? 32 : kPassRows; }
-size_t slots(int max_rows) { return 2 * (size_t)(max_rows <= kWaveRows ? kMaxGroups * kWaves : kTileGroups); }
+int slot_rows(int max_rows, bool tiles) { return tiles ? kPassRows : max_rows <= 16 ? 16 : 32; }
+size_t slots(bool tiles) { return 2 * (size_t)(tiles ? kTileGroups : kMaxGroups * kWaves); }
 
 size_t al256(size_t x) { return (x + 255) / 256 * 256; }
 int row_passes(int max_rows) { return (max_rows + kPassRows - 1) / kPassRows; }
 size_t seg_bytes(int batch, int hkv, int max_rows) {
   return al256((size_t)row_passes(max_rows) * min(batch, kMaxBatch) * hkv * sizeof(int2));
 }
-size_t lse_bytes(int max_rows) { return al256(slots(max_rows) * slot_rows(max_rows) * sizeof(float)); }
+size_t lse_bytes(int max_rows, bool tiles) { return al256(slots(tiles) * slot_rows(max_rows, tiles) * sizeof(float)); }
 
 bool valid_group(int hq, int hkv) {
   if (hkv <= 0 || hq <= 0 || hq % hkv) return false;
@@ -610,12 +620,13 @@ template <bool TREE>
 int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* seqlens, const int32_t* cu_q, bf16_t* out,
                 int batch, int max_nodes, void* workspace, hipStream_t stream) {
   const int max_rows = max_nodes << a.glog;
-  a.rows = slot_rows(max_rows);
+  const bool tiles = TREE && by_tiles(batch, a.hkv, max_rows);
+  a.rows = slot_rows(max_rows, tiles);
   a.max_nodes = max_nodes;
   a.passes = row_passes(max_rows);
   a.ws_seg = (int2*)workspace;
   a.ws_lse = (float*)((char*)workspace + seg_bytes(batch, a.hkv, max_rows));
-  a.ws_o = (float*)((char*)a.ws_lse + lse_bytes(max_rows));
+  a.ws_o = (float*)((char*)a.ws_lse + lse_bytes(max_rows, tiles));
   // units that the widest visible list may hold
   const int64_t pages = TREE ? (a.max_ctx + kPage - 1) / kPage
                              : min((int64_t)(a.max_ctx + kPage - 1) / kPage,
@@ -632,7 +643,7 @@ int launch_rows(RowsArgs a, const bf16_t* q, const int32_t* bt, const int32_t* s
     if (max_rows <= 16) {
       rows_kernel<1, TREE><<<groups, kWaves * 64, 0, stream>>>(a);
     } else if constexpr (TREE) {
-      if (max_rows <= kWaveRows) {
+      if (!tiles) {
         rows_kernel<2, TREE><<<groups, kWaves * 64, 0, stream>>>(a);
       } else {
         const int e = launch_tiles(a, stream);
@@ -683,7 +694,8 @@ bool rows_args(RowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const voi
 extern "C" size_t xv_tree_attention_workspace_size(int batch, int max_nodes, int num_q_heads, int num_kv_heads) {
   if (batch <= 0 || max_nodes <= 0 || !valid_group(num_q_heads, num_kv_heads)) return 256;
   const int max_rows = max_nodes * (num_q_heads / num_kv_heads);
-  return seg_bytes(batch, num_kv_heads, max_rows) + lse_bytes(max_rows) + slots(max_rows) * slot_rows(max_rows) * kD * sizeof(float);
+  const bool tiles = max_rows > 16;  // of either kernel, so that a smaller batch never needs more
+  return seg_bytes(batch, num_kv_heads, max_rows) + lse_bytes(max_rows, tiles) + slots(tiles) * slot_rows(max_rows, tiles) * kD * sizeof(float);
 }
 
 extern "C" int xv_window_decode_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k_cache,

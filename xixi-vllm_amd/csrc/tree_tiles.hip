@@ -1,5 +1,6 @@
 // Attention of trees of drafted tokens with more than 32 rows (nodes times query
-// heads per kv head) over the paged cache, for gfx950.
+// heads per kv head), or few trees with more than 16, over the paged cache, for
+// gfx950.
 //
 // The work split, partials and merge are those of xv_rows.h with 64-key tiles
 // as units and a workgroup per range: its waves take 32 rows each of the same

@@ -174,7 +174,7 @@ XV_INLINE int finish_slot(const Sequences& s, const RowsArgs& a, const Cursor& c
 XV_INLINE uint32_t low_bits(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 XV_INLINE uint64_t low_bits64(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull; }
 
-// Trees of more than 32 rows: tree_tiles.hip.  a: all but the workspace's slots, filled for `batch` sequences.
+// Trees of more than 32 rows, and few of more than 16: tree_tiles.hip.  a: all but the workspace's slots, filled for `batch` sequences.
 constexpr int kTileGroups = 256;   // ranges: as many as there are workgroups resident at once
 int launch_tiles(const RowsArgs& a, hipStream_t stream);
 
