@@ -30,10 +30,11 @@
 // masked, and a wave passes over those that none of its queries sees.  Bound by the
 // softmax beside the products, as without a window (products busy 52 % of the time,
 // vector work 44 %): one document of 16001 with a window of 4096, 16 / 8 heads, 474
-// GFLOP, 487 to 516 us (up to 974 TFLOP/s); 16 chunks of up to 512 over up to
-// 12000 cached tokens, window 2000, 64 / 8 heads, 379 GFLOP, 473 us (801); 12
-// prompts of 40 to 2500, window 512, 32 / 8 heads, 97 GFLOP, 165 us (591: seven
-// tiles a workgroup, a third of whose time is start and end).
+// GFLOP, 516 us a call (919 TFLOP/s); 16 chunks of up to 512 over up to 12000
+// cached tokens, window 2000, 64 / 8 heads, 379 GFLOP, 471 us (803); 12 prompts of
+// 40 to 2500, window 512, 32 / 8 heads, 97 GFLOP, 165 us (589: seven tiles a
+// workgroup, a third of whose time is start and end).  Under a profiler the kernels
+// alone take 580, 545 and 194 us (medians; 527, 490 and 172 at best).
 #include "xv_common.h"
 #include "xv_kernels.h"
 #include "xv_tile.h"
@@ -338,7 +339,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PrefillArgs a) {
           const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][8 * kk + 2 * e], a.scale_log2, nm));
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][8 * kk + 2 * e + 1], a.scale_log2, nm));
           w[e] = pack_bf16x2(p0, p1);
-          // the row sum takes the bf16 values P.V multiplies
+          // the row sum takes the bf16 values P.V multiplies: their rounding (2^-8 of a weight at most, as in the other
+          // kernels over bf16 pages) moves the output by that share of the values' spread only
           l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(xv_bf16x2, w[e]), kOnes, l_run, false);
         }
         __builtin_memcpy(&pb[mt][kk], w, 16);

@@ -206,7 +206,7 @@ XV_INLINE void unit_math(RowsState<NT>& st, const UnitRegs& u, const bf16x8_t (&
       const float p0 = __builtin_amdgcn_exp2f(fmaf(a[t][p][r], scale_log2, nm));
       const float p1 = __builtin_amdgcn_exp2f(fmaf(a[t][p][r + 1], scale_log2, nm));
       w[e] = pack_bf16x2(p0, p1);
-      // the row sum takes the bf16 weights that the product multiplies: their rounding (2^-9 of a weight) moves
+      // the row sum takes the bf16 weights that the product multiplies: their rounding (2^-8 of a weight at most) moves
       // the output by that share of the values' spread only, and a row of one heavy token is exact
       st.l[t] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(xv_bf16x2, w[e]),
                                                 (xv_bf16x2){(__bf16)1.0f, (__bf16)1.0f}, st.l[t], false);

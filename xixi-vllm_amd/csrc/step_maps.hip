@@ -8,14 +8,20 @@
 //   token t      the i-th new one of row b: position old + i (old + depth[t]
 //                for a drafted tree), slot page * BS + (old + i) % BS
 //
-// Bound by latency: a launch, the lengths, then the pages, two trips to memory
-// one after the other.  So it is one launch: every workgroup runs the prefix
+// Bound by latency.  So it is one launch: every workgroup runs the prefix
 // sums over the rows itself (into LDS: they cost it less than a second launch
 // would), then takes its share of the tokens or of the new pages, each found
 // by a binary search there.  A token in a new page takes the page from the free
 // list, not from the table, so nothing written here is read here and
-// workgroups need no order.  2.6 us for one request, 6.7 for 180 that decode and
-// 20 chunks of up to 400 tokens, 7.5 for 256 drafted trees of up to 64 nodes.
+// workgroups need no order.
+//
+// 2.5 us for one request, 6.7 for 180 that decode and 20 chunks of up to 400
+// tokens, 7.5 for 256 drafted trees of up to 64 nodes.  The lengths, then the pages
+// are two trips to memory in all of them; what the larger ones add are the sums (200
+// requests of which one has a token 3.2) and above all the searches, chains of
+// dependent LDS reads: a thread makes one for each row that its four tokens lie in,
+// one after the other (200 requests of four new tokens each, one search a thread,
+// 3.9; of one token each, four searches, 5.3; 16 of them 3.3 and 4.2).
 #include "xv_common.h"
 #include "xv_kernels.h"
 

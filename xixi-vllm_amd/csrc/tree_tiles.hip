@@ -11,11 +11,12 @@
 // straight from the scores' registers.  Tiles travel by LDS-DMA into a ring of
 // kRing slots, one barrier per tile.
 //
-// Measured (kernel): 32 trees of 5 to 64 nodes over up to 4096 tokens, 32 / 8
-// heads, 317 MB and 37 GFLOP, 104 us (3.0 TB/s, 356 TFLOP/s); 4 of 40 to 90 over
-// up to 90000, 16 / 8 heads, 1013 MB and 128 GFLOP, 232 us (4.4 TB/s, 554
-// TFLOP/s).  Neither stream nor products alone bound it: without the products it
-// takes two thirds of that, without the loads three quarters.  Of 3900 to 4700
+// Measured (a call with its merge): 32 trees of 5 to 64 nodes over up to 4096
+// tokens, 32 / 8 heads, 317 MB and 37 GFLOP, 113 us (2.8 TB/s, 327 TFLOP/s); 4 of
+// 40 to 90 over up to 90000, 16 / 8 heads, 1013 MB and 128 GFLOP, 257 us (3.9 TB/s,
+// 500 TFLOP/s).  Under a profiler the kernel alone takes 111 and 321 us (medians;
+// 109 and 249 at best).  Neither stream nor products alone bound it: without the
+// products it takes two thirds of that, without the loads three quarters.  Of 3900 to 4700
 // cycles a tile the first wave computes 2200 (the 32 products are 1056; the softmax
 // between them waits for one and is waited for by the other), stands 580 at its
 // LDS-DMA (all waves issue theirs behind the barrier), spends 350 on where the next
@@ -142,7 +143,8 @@ XV_INLINE void softmax_tile(TileState& st, const floatx16_t (&s)[2], bf16x8_t (&
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r], scale_log2, nm));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][r + 1], scale_log2, nm));
         w[e] = pack_bf16x2(p0, p1);
-        // the row sum takes the bf16 weights that the product multiplies
+        // the row sum takes the bf16 weights that the product multiplies: their rounding (2^-8 of a weight at most) moves
+        // the output by that share of the values' spread only
         st.l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(xv_bf16x2, w[e]), kOnes, st.l, false);
       }
       __builtin_memcpy(&pb[mt][kk], w, 16);
