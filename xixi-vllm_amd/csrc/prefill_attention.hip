@@ -477,6 +477,9 @@ int prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
     if (!k || !v) return (int)hipErrorInvalidValue;
     if (((uintptr_t)k | (uintptr_t)v) & 15 || (kv_stride_tok | kv_stride_head) & 7) return (int)hipErrorInvalidValue;
   }
+  // 32-bit offsets within 16 tokens
+  const int64_t row = block_tables ? tok_stride : kv_stride_tok;
+  if (row < 0 || row > (1 << 26)) return (int)hipErrorInvalidValue;
   // q rows are read as 16-byte vectors, out is written as 8-byte pieces
   if ((uintptr_t)q & 15 || (q_stride_tok | q_stride_head) & 7 || (uintptr_t)out & 7 || out_stride_tok & 3)
     return (int)hipErrorInvalidValue;

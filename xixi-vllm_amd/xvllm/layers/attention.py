@@ -493,6 +493,29 @@ def cascade_decode_attention(
     return out
 
 
+def _check_prefill(q3, cu_seqlens_q, cu_seqlens_k, hq, hkv, d, k, v, k_cache, v_cache, block_tables) -> None:
+    """What the prefill kernels take on trust: one device, a length for every sequence, rows of hq and hkv heads, and
+    caches of one layout (they are given one set of strides)."""
+    if q3.dim() != 3 or q3.shape[1:] != (hq, d):
+        raise ValueError(f"q {tuple(q3.shape)} is not rows of {hq} heads of {d}")
+    if cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] < 1 or cu_seqlens_k.dim() != 1 or cu_seqlens_k.shape[0] < cu_seqlens_q.shape[0]:
+        raise ValueError(f"cu_seqlens_q {tuple(cu_seqlens_q.shape)} and cu_seqlens_k {tuple(cu_seqlens_k.shape)} are not [B + 1]")
+    dev, bsz = q3.get_device(), cu_seqlens_q.shape[0] - 1
+    operands = (k, v) if block_tables is None else (k_cache, v_cache, block_tables)
+    if any(t is None for t in operands):
+        raise ValueError("prefill needs k and v, or k_cache, v_cache and block_tables")
+    if any(t.get_device() != dev for t in (cu_seqlens_q, cu_seqlens_k, *operands)):
+        raise RuntimeError("xvllm ops run on the GPU only (HIP kernels), all operands on one device")
+    if block_tables is None:
+        return
+    if block_tables.dim() != 2 or block_tables.shape[0] < bsz:
+        raise ValueError(f"block_tables {tuple(block_tables.shape)} has no row for each of {bsz} sequences")
+    if k_cache.dtype != FP4_PAGES:
+        ks, st = k_cache.shape, k_cache.stride()
+        if len(ks) != 4 or ks[2] != hkv or ks[3] != d or st[3] != 1 or v_cache.shape != ks or v_cache.stride() != st or v_cache.dtype != k_cache.dtype:
+            raise ValueError(f"caches {tuple(ks)} and {tuple(v_cache.shape)} are not pages [NB, BS, {hkv}, {d}] of one type and layout")
+
+
 def prefill_attention(
     q: torch.Tensor,
     k: torch.Tensor | None,
@@ -533,6 +556,7 @@ def prefill_attention(
     q3, qs0, qs1 = _q_view(q, num_qo_heads, head_dim)
     require_cuda(q3, cu_seqlens_q, cu_seqlens_k)
     require_bf16(q3)
+    _check_prefill(q3, cu_seqlens_q, cu_seqlens_k, num_qo_heads, num_kv_heads, head_dim, k, v, k_cache, v_cache, block_tables)
     bsz = cu_seqlens_q.shape[0] - 1
     cuq = cu_seqlens_q.to(torch.int32).contiguous()
     cuk = cu_seqlens_k.to(torch.int32).contiguous()
@@ -576,7 +600,6 @@ def prefill_attention(
         return prefill_attention(q, kd, vd, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, num_qo_heads, num_kv_heads,
                                  head_dim, softmax_scale=softmax_scale, window=window, sink_tokens=sink_tokens)
     if block_tables is not None:
-        assert k_cache is not None and v_cache is not None
         require_bf16(k_cache, v_cache)
         bt = block_tables.to(torch.int32)
         if bt.stride(-1) != 1:
@@ -592,8 +615,11 @@ def prefill_attention(
         v3 = v.view(v.shape[0], num_kv_heads, head_dim) if v.dim() == 2 else v
         if (k3.stride() != v3.stride() or k3.stride(-1) != 1 or k3.stride(0) % 8 or k3.stride(1) % 8
                 or not aligned16(k3) or not aligned16(v3)):
-            k3, v3 = k3.contiguous(), v3.contiguous()
+            # whole rows may be unaligned too: fresh allocations
+            k3, v3 = (t.clone(memory_format=torch.contiguous_format) for t in (k3, v3))
         require_bf16(k3, v3)
+        if k3.shape != v3.shape or k3.dim() != 3 or k3.shape[1:] != (num_kv_heads, head_dim):
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are not rows of {num_kv_heads} heads of {head_dim}")
         kd, vd = k3, v3
         kvs0, kvs1 = k3.stride(0), k3.stride(1)
         kc = vc = bt = None
