@@ -102,3 +102,17 @@ def test_rows_that_no_query_sees_stay(dev, fmt, window, sinks, block):
         assert got[0].data_ptr() == out.data_ptr()
     seen = torch.cat(_seen(window, sinks)).to(dev)
     assert torch.equal(out[:, seen], want[:, seen]) and (out[:, ~seen] == 7.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+@pytest.mark.parametrize("window", [0, 30])
+def test_lengths_in_a_larger_batch_s_buffer(dev, fmt, window):
+    """cu_seqlens_k may be longer than the sequences there are."""
+    from xvllm.layers.attention import prefill_attention
+
+    hq, hkv = 8, 4
+    pool, bt, kw = _pool(dev, fmt, 16, hkv, seed=4)
+    q = torch.randn(sum(NEW), hq * D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(dev)
+    run = lambda cu_k: prefill_attention(q, None, None, _cu(NEW, dev), cu_k, max(NEW), hq, hkv, D, k_cache=pool[0], v_cache=pool[1],
+                                         block_tables=bt.to(dev), window=window, **kw)
+    assert torch.equal(run(_cu(LENS + [7, 7], dev)), run(_cu(LENS, dev)))

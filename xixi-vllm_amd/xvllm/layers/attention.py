@@ -559,7 +559,7 @@ def prefill_attention(
     _check_prefill(q3, cu_seqlens_q, cu_seqlens_k, num_qo_heads, num_kv_heads, head_dim, k, v, k_cache, v_cache, block_tables)
     bsz = cu_seqlens_q.shape[0] - 1
     cuq = cu_seqlens_q.to(torch.int32).contiguous()
-    cuk = cu_seqlens_k.to(torch.int32).contiguous()
+    cuk = cu_seqlens_k[: bsz + 1].to(torch.int32).contiguous()  # it may be a larger batch's buffer
     out = torch.empty((q3.shape[0], num_qo_heads * head_dim), dtype=q.dtype, device=q.device)
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else softmax_scale
     if block_tables is not None and k_cache is not None and k_cache.dtype == FP4_PAGES:
